@@ -375,6 +375,141 @@ B2SQ_API b2sq_status b2sq_gemm_i8_grouped(uint32_t groups, uint32_t rows, uint32
                                           b2sq_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* MoE: a whole layer for a few tokens                                      */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * The experts' side of a mixture-of-experts layer for decode-sized batches,
+ * from the router's choice to the combined output (the reference runs such a
+ * layer only on whole prompts, piece by piece).  For token t and slot k with
+ * expert e = topk_ids[t*topk+k]:
+ *   xq, rs1  = smoothquant(x[t], smooth1[e])              as b2sq_smoothquant
+ *   [g | u]  = float(w13[e] xq) * (rs1 * s13[e])          exact int32 sums
+ *   h        = g / (1 + exp(-g)) * u * smooth2[e]
+ *   hq, rs2  = max|h| / quant_max and its int8 rounding, as above
+ *   d        = float(w2[e] hq) * (rs2 * s2[e])
+ *   out[t]   = cvt_rn(sum over k of topk_weights[t*topk+k] * d)   fp32, in slot order
+ * A slot whose id is outside [0, experts) adds nothing; an expert may be named
+ * twice by one token.  Everything between the int8 products is fp32.
+ *   x        fp16 or bf16 (x_type) [tokens, hidden], row pitch ldx elements
+ *   smooth1  [experts, hidden], smooth2 [experts, inter]
+ *   w13      int8 [experts][2 * inter][hidden]: gate rows, then up rows
+ *   s13      [experts, 2 * inter]
+ *   w2       int8 [experts][hidden][inter], s2 [experts, hidden]
+ *   out      x_type [tokens, hidden], contiguous
+ * Requirements (else UNSUPPORTED): hidden and inter multiples of 16 and at
+ * most 131072, x, w13, w2 and out 16-byte aligned, ldx a multiple of 8,
+ * tokens * topk <= 4096 (larger batches: b2sq_moe_sorting and
+ * b2sq_gemm_i8_grouped).  experts <= 1024.
+ * workspace: b2sq_moe_layer_workspace_size bytes, 256-byte aligned, contents
+ * arbitrary and not kept; calls that may overlap need separate ones.
+ */
+B2SQ_API b2sq_status b2sq_moe_layer(const void* x, b2sq_dtype x_type, uint32_t ldx,
+                                    const float* topk_weights, const int32_t* topk_ids,
+                                    const float* smooth1, const int8_t* w13, const float* s13,
+                                    const float* smooth2, const int8_t* w2, const float* s2,
+                                    void* out, uint32_t tokens, uint32_t hidden, uint32_t inter,
+                                    uint32_t experts, uint32_t topk, float quant_max,
+                                    void* workspace, size_t workspace_bytes,
+                                    b2sq_stream_t stream);
+B2SQ_API b2sq_status b2sq_moe_layer_workspace_size(uint32_t tokens, uint32_t hidden, uint32_t inter,
+                                                   uint32_t experts, uint32_t topk, size_t* bytes);
+
+/* ------------------------------------------------------------------------ */
+/* Key/value cache in 4 bits: append, attention, eviction                   */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * A paged cache of keys and values, quantised per token and head in groups of
+ * 64 channels with a step s and a base z each (value = q * s + z, q in 0..15):
+ *   k, v              uint8 [pages][kv_heads][page_size][head_dim / 2],
+ *                     channel 2i in the low nibble of byte i
+ *   k_scale, v_scale  fp16 [pages][kv_heads][page_size][head_dim / 64][2]: s, z
+ *   weight            fp32 [pages][kv_heads][page_size], the attention weight
+ *                     each token has gathered; NULL where it is not kept
+ * head_dim 64, 128 or 256; page_size a multiple of 16; all buffers 16-byte
+ * aligned.  Position p of sequence b is slot p % page_size of page
+ * page_table[b * max_pages + p / page_size].  The table, the lengths and the
+ * token offsets live on the device; a page id outside [0, pages) stands for
+ * tokens that are not there (never written, never seen), and so do positions
+ * at or past max_pages * page_size.
+ *
+ * The tokens of a call are packed: rows token_start[b] .. token_start[b+1] - 1
+ * belong to sequence b and are its last ones: row i of n has position
+ * seq_lens[b] - n + i, and seq_lens counts them.  Offsets lie in 0 .. tokens
+ * and do not decrease (where they do, rows may be left out).  Rows behind the
+ * last sequence are left alone.
+ */
+typedef struct {
+    uint8_t* k;
+    uint8_t* v;
+    void* k_scale;
+    void* v_scale;
+    float* weight;
+    uint32_t pages, kv_heads, page_size, head_dim;
+} b2sq_kv4_cache;
+
+/*
+ * Quantises new keys and values ([tokens, kv_heads, head_dim], fp16 or bf16,
+ * token pitch k_stride / v_stride elements, heads contiguous) into the cache:
+ *   z = fp16(min), s = fp16((max - min) / 15) over the group, inputs saturated
+ *   to +-65504;  q = clamp(rint((v - z) / s), 0, 15), ties to even (0 if s = 0)
+ * and sets their weight to 0.  A NaN makes s and z of its group NaN.
+ * k_out / v_out (nullable, contiguous, same type) receive the values that the
+ * cache now stands for.  A token without a place in the table is skipped.
+ * Requirements (else UNSUPPORTED): 16-byte aligned rows (pitches multiples of 8).
+ */
+B2SQ_API b2sq_status b2sq_kv4_append(const void* k, const void* v, b2sq_dtype type, uint32_t tokens,
+                                     uint32_t k_stride, uint32_t v_stride, const b2sq_kv4_cache* cache,
+                                     const int32_t* page_table, uint32_t batch, uint32_t max_pages,
+                                     const int32_t* seq_lens, const int32_t* token_start,
+                                     void* k_out, void* v_out, b2sq_stream_t stream);
+
+/*
+ * Attention of new query tokens over the cache, each sequence's own keys (append
+ * them first): query i of n sees the positions below seq_lens[b] - n + i + 1.
+ *   s = scale * q . K,  p = softmax(s),  out = p V
+ * q: [tokens, heads, head_dim] fp16 or bf16, token pitch q_stride elements;
+ * heads a multiple of kv_heads (query head j reads key head j / (heads /
+ * kv_heads)).  out: the same type, contiguous.  A query that sees nothing gives
+ * 0.  No sequence has more than max_queries rows (rows past it are not
+ * written).  Statistics and sums are fp32.
+ * accumulate_weight: adds to cache->weight, for every key head and position, the
+ * sum of p over the head's query heads and the call's queries; a page that two
+ * sequences of the call share would be added to by both at once, so it must
+ * belong to one.
+ * workspace: b2sq_kv4_attention_workspace_size bytes, 256-byte aligned, contents
+ * arbitrary and not kept; calls that may overlap need separate ones.
+ */
+B2SQ_API b2sq_status b2sq_kv4_attention(const void* q, b2sq_dtype type, uint32_t tokens, uint32_t heads,
+                                        uint32_t q_stride, const b2sq_kv4_cache* cache,
+                                        const int32_t* page_table, uint32_t batch, uint32_t max_pages,
+                                        const int32_t* seq_lens, const int32_t* token_start,
+                                        uint32_t max_queries, float scale, void* out, int accumulate_weight,
+                                        void* workspace, size_t workspace_bytes, b2sq_stream_t stream);
+B2SQ_API b2sq_status b2sq_kv4_attention_workspace_size(uint32_t batch, uint32_t heads, uint32_t kv_heads,
+                                                       uint32_t head_dim, uint32_t page_size,
+                                                       uint32_t max_pages, uint32_t max_queries,
+                                                       int accumulate_weight, size_t* bytes);
+
+/*
+ * Thins sequences out by the attention weight their tokens have gathered.  A
+ * sequence of more than `budget` tokens keeps, in every key head by itself, its
+ * newest `recent` tokens and the budget - recent others of the largest weight
+ * (equal weights: the lower position; -0 equals 0; a NaN counts as the
+ * largest); a shorter one keeps all.  Kept tokens are copied in order, with
+ * their weights, to positions 0, 1, ... of new_page_table, and new_lens[b]
+ * receives their number, min(seq_lens[b], budget) (less where the new table
+ * holds fewer).  The old pages are only read: they may be shared with other
+ * sequences, but no page may stand in both tables.  recent <= budget; the
+ * cache keeps weights; budget 0 empties every sequence.
+ */
+B2SQ_API b2sq_status b2sq_kv4_evict(const b2sq_kv4_cache* cache, const int32_t* page_table, uint32_t batch,
+                                    uint32_t max_pages, const int32_t* seq_lens, const int32_t* new_page_table,
+                                    uint32_t new_max_pages, uint32_t budget, uint32_t recent,
+                                    int32_t* new_lens, b2sq_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Diagnostics                                                              */
 /* ------------------------------------------------------------------------ */
 

@@ -6,6 +6,7 @@ The compute lives in ``libb2sq.so`` (CUDA kernels behind the C ABI of
 from .api import (  # noqa: F401
     B2sqError,
     COL_MAJOR,
+    KV4Cache,
     ROW_MAJOR,
     Workspace,
     debug_bounded_wait,
@@ -16,6 +17,10 @@ from .api import (  # noqa: F401
     kernel_smoothquant,
     last_device_error,
     gemm_grouped,
+    kv4_append,
+    kv4_attention,
+    kv4_evict,
+    moe_layer,
     moe_smoothquant,
     moe_sorting,
     plan,

@@ -43,6 +43,20 @@ class GemmPlan(C.Structure):
     ]
 
 
+class Kv4CacheStruct(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("pages", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("page_size", C.c_uint32),
+        ("head_dim", C.c_uint32),
+    ]
+
+
 class B2sqError(RuntimeError):
     """A libb2sq call returned a non-OK status."""
 
@@ -79,6 +93,14 @@ SIGNATURES = {
     "b2sq_moe_sorting": (_i, [_vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp]),
     "b2sq_gemm_i8_grouped": (_i, [_u32, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _i, _u32, _vp, _vp,
                                   _f32, _f32, _vp, _vp, _vp]),
+    "b2sq_moe_layer": (_i, [_vp, _i, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32,
+                            _f32, _vp, _sz, _vp]),
+    "b2sq_moe_layer_workspace_size": (_i, [_u32, _u32, _u32, _u32, _u32, C.POINTER(_sz)]),
+    "b2sq_kv4_append": (_i, [_vp, _vp, _i, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp]),
+    "b2sq_kv4_attention": (_i, [_vp, _i, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _vp, _vp, _u32, _f32, _vp, _i, _vp, _sz,
+                                _vp]),
+    "b2sq_kv4_attention_workspace_size": (_i, [_u32, _u32, _u32, _u32, _u32, _u32, _u32, _i, C.POINTER(_sz)]),
+    "b2sq_kv4_evict": (_i, [_vp, _vp, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _vp, _vp]),
     "b2sq_status_string": (C.c_char_p, [_i]),
     "b2sq_last_error_message": (C.c_char_p, []),
     "b2sq_last_device_error": (_i, [_vp, C.POINTER(_u32)]),

@@ -14,6 +14,10 @@ this module                reference operator (file:line)
 ``moe_sorting``            kernel_moe_sorting_*, rocwmma_moe_sorting.cpp:53-125
 =========================  ===================================================
 
+Without a counterpart there: the decode step's ``moe_layer`` (a whole
+mixture-of-experts layer for a few tokens) and the 4-bit key/value cache
+(``KV4Cache``, ``kv4_append``, ``kv4_attention``, ``kv4_evict``).
+
 Errors: the reference exits on a HIP error (CHECK_HIP, common.hpp:33-46) and
 prints-and-returns on unsupported GEMM shapes (rocwmma_gemm_quantized.cpp:199-203);
 here both raise :class:`B2sqError` carrying the library's status code.
@@ -21,6 +25,8 @@ here both raise :class:`B2sqError` carrying the library's status code.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -457,3 +463,224 @@ def smoothquant_gemm(x: torch.Tensor, smooth_scale: torch.Tensor, w_nk: torch.Te
 
 
 kernel_topk_softmax = topk_softmax
+
+
+# ----------------------------------------------------------------------------- decode step
+def _on(dev: torch.device):
+    """The library launches on the current device: makes it the tensors' own."""
+    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _new(make, shape, dtype: torch.dtype, dev: torch.device, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
+    """A tensor made (and filled) on the stream that the call runs on."""
+    if stream is None:
+        return make(shape, dtype=dtype, device=dev)
+    with torch.cuda.stream(stream):
+        return make(shape, dtype=dtype, device=dev)
+
+
+def _scratch(given: Optional[torch.Tensor], nbytes: int, dev: torch.device, stream: Optional[torch.cuda.Stream]):
+    """Workspace of a call: the caller's, or one of its own from the allocator (ordered on the call's stream, so calls
+    on several streams and captured graphs never share one)."""
+    if given is not None:
+        if given.device != dev or not given.is_contiguous():
+            raise ValueError("workspace must be a contiguous tensor on the operands' device")
+        return given.data_ptr(), given.numel() * given.element_size(), given
+    if nbytes == 0:
+        return None, 0, None
+    t = _new(torch.empty, nbytes, torch.uint8, dev, stream)
+    return t.data_ptr(), nbytes, t
+
+
+def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, dev: torch.device) -> int:
+    """Address of a contiguous tensor of this type, shape and device."""
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {dev}")
+    return t.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _moe_layer_ws(device: int, *sizes: int) -> int:
+    out = C.c_size_t(0)
+    _lib.check(_lib.load().b2sq_moe_layer_workspace_size(*sizes, C.byref(out)), "b2sq_moe_layer_workspace_size")
+    return out.value
+
+
+def moe_layer(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor, smooth1: torch.Tensor,
+              w13: torch.Tensor, s13: torch.Tensor, smooth2: torch.Tensor, w2: torch.Tensor, s2: torch.Tensor,
+              quant_max: float = 127.0, out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+              stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """A mixture-of-experts layer for a few tokens, after the router (``topk_softmax``): smoothquant, the experts'
+    gate and up products, SwiGLU, the second quantisation, the down products and the weighted sum.
+
+    x fp16 / bf16 [T, H]; topk_weights fp32 and topk_ids int32 [T, topk]; smooth1 fp32 [E, H]; w13 int8 [E, 2I, H]
+    (gate rows, then up rows) with s13 fp32 [E, 2I]; smooth2 fp32 [E, I]; w2 int8 [E, H, I] with s2 fp32 [E, H].
+    Returns out [T, H] in x's type.  T * topk <= 4096; H and I multiples of 16."""
+    code = _DTYPE_CODE.get(x.dtype)
+    if code is None or x.dtype == torch.int32 or x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError("x must be a row-major fp16 or bf16 [tokens, hidden] tensor")
+    dev = _need_cuda(x)
+    T, H = x.shape
+    if w2.dim() != 3 or topk_ids.dim() != 2:
+        raise ValueError("w2 must be int8 [experts, hidden, inter] and topk_ids int32 [tokens, topk]")
+    E, I, K = w2.shape[0], w2.shape[2], topk_ids.shape[1]
+    f32 = torch.float32
+    if out is None:
+        out = _new(torch.empty, (T, H), x.dtype, dev, stream)
+    args = (_want(topk_weights, "topk_weights", f32, (T, K), dev), _want(topk_ids, "topk_ids", torch.int32, (T, K), dev),
+            _want(smooth1, "smooth1", f32, (E, H), dev), _want(w13, "w13", torch.int8, (E, 2 * I, H), dev),
+            _want(s13, "s13", f32, (E, 2 * I), dev), _want(smooth2, "smooth2", f32, (E, I), dev),
+            _want(w2, "w2", torch.int8, (E, H, I), dev), _want(s2, "s2", f32, (E, H), dev),
+            _want(out, "out", x.dtype, (T, H), dev))
+    with _on(dev):
+        ws, ws_bytes, hold = _scratch(workspace, _moe_layer_ws(dev.index, T, H, I, E, K), dev, stream)
+        st = _lib.load().b2sq_moe_layer(x.data_ptr(), code, x.stride(0) if T > 1 else H, *args, T, H, I, E, K,
+                                        float(quant_max), ws, ws_bytes, _stream_ptr(stream, dev))
+    _lib.check(st, "b2sq_moe_layer")
+    return out
+
+
+class KV4Cache:
+    """A paged key/value cache in 4 bits: groups of 64 channels with a step and a base each (value = q * step + base).
+
+    k, v             uint8 [pages, kv_heads, page_size, head_dim / 2], channel 2i in the low nibble of byte i
+    k_scale, v_scale fp16 [pages, kv_heads, page_size, head_dim / 64, 2]: step, base
+    weight           fp32 [pages, kv_heads, page_size] or None: the attention weight each token has gathered
+
+    ``KV4Cache.empty`` allocates one.  The buffers belong to the object: replace the object, not its tensors."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 weight: Optional[torch.Tensor] = None):
+        if k.dim() != 4:
+            raise ValueError("k must be uint8 [pages, kv_heads, page_size, head_dim / 2]")
+        pages, heads, size, half = k.shape
+        dev = _need_cuda(k)
+        scales = (pages, heads, size, half // 32, 2)
+        _want(k, "k", torch.uint8, (pages, heads, size, half), dev)
+        _want(v, "v", torch.uint8, (pages, heads, size, half), dev)
+        _want(k_scale, "k_scale", torch.float16, scales, dev)
+        _want(v_scale, "v_scale", torch.float16, scales, dev)
+        if weight is not None:
+            _want(weight, "weight", torch.float32, (pages, heads, size), dev)
+        self.k, self.v, self.k_scale, self.v_scale, self.weight = k, v, k_scale, v_scale, weight
+        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, 2 * half
+        self.device = dev
+        self._struct = _lib.Kv4CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                           _ptr(weight), pages, heads, size, 2 * half)
+        self._ref = C.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, weights: bool = False,
+              device: Optional[torch.device] = None) -> "KV4Cache":
+        """A cache of zeros; ``weights``: with room for the attention weights that ``kv4_evict`` goes by."""
+        dev = device if device is not None else torch.device("cuda", torch.cuda.current_device())
+        data = [torch.zeros((pages, kv_heads, page_size, head_dim // 2), dtype=torch.uint8, device=dev) for _ in range(2)]
+        scale = [torch.zeros((pages, kv_heads, page_size, head_dim // 64, 2), dtype=torch.float16, device=dev)
+                 for _ in range(2)]
+        w = torch.zeros((pages, kv_heads, page_size), dtype=torch.float32, device=dev) if weights else None
+        return cls(*data, *scale, w)
+
+
+def _kv4_rows(t: torch.Tensor, name: str, dev: torch.device):
+    """(tokens, heads, token pitch) of a [tokens, heads, head_dim] tensor whose heads lie side by side."""
+    if t.dim() != 3 or t.device != dev or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous heads on {dev}")
+    return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _kv4_seqs(page_table: torch.Tensor, seq_lens: torch.Tensor, token_start: Optional[torch.Tensor], dev: torch.device):
+    """(page table, batch, pages a sequence, lengths[, offsets]) for the library."""
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be int32 [batch, pages]")
+    B, P = page_table.shape
+    args = (_want(page_table, "page_table", torch.int32, (B, P), dev), B, P,
+            _want(seq_lens, "seq_lens", torch.int32, (B,), dev))
+    return args if token_start is None else args + (_want(token_start, "token_start", torch.int32, (B + 1,), dev),)
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, seq_lens: torch.Tensor,
+               token_start: torch.Tensor, k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None,
+               stream: Optional[torch.cuda.Stream] = None) -> None:
+    """Quantises new keys and values (fp16 / bf16 [tokens, kv_heads, head_dim], slices of a joint projection allowed)
+    into the cache.  Rows token_start[b] .. token_start[b+1] - 1 are the last tokens of sequence b, whose length
+    seq_lens[b] counts them.  k_out / v_out receive the values that the cache now stands for.  page_table int32
+    [batch, pages], seq_lens int32 [batch], token_start int32 [batch + 1], all on the device."""
+    dev = cache.device
+    code = _DTYPE_CODE.get(k.dtype)
+    if code is None or k.dtype == torch.int32 or v.dtype != k.dtype:
+        raise ValueError("k and v must both be fp16 or bf16")
+    T, heads, ks = _kv4_rows(k, "k", dev)
+    _, _, vs = _kv4_rows(v, "v", dev)
+    shape = (T, cache.kv_heads, cache.head_dim)
+    if tuple(k.shape) != shape or tuple(v.shape) != shape:
+        raise ValueError(f"k and v must be {shape} for this cache")
+    ko = None if k_out is None else _want(k_out, "k_out", k.dtype, shape, dev)
+    vo = None if v_out is None else _want(v_out, "v_out", k.dtype, shape, dev)
+    seqs = _kv4_seqs(page_table, seq_lens, token_start, dev)
+    with _on(dev):
+        st = _lib.load().b2sq_kv4_append(k.data_ptr(), v.data_ptr(), code, T, ks, vs, cache._ref, *seqs, ko, vo,
+                                         _stream_ptr(stream, dev))
+    _lib.check(st, "b2sq_kv4_append")
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv4_attention_ws(device: int, *sizes: int) -> int:
+    out = C.c_size_t(0)
+    _lib.check(_lib.load().b2sq_kv4_attention_workspace_size(*sizes, C.byref(out)), "b2sq_kv4_attention_workspace_size")
+    return out.value
+
+
+def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                  token_start: torch.Tensor, max_queries: int = 1, scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None, accumulate_weight: bool = False,
+                  workspace: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """Attention of new query tokens over the 4-bit cache; q fp16 / bf16 [tokens, heads, head_dim], heads a multiple of
+    the cache's.  Rows token_start[b] .. token_start[b+1] - 1 (at most max_queries) are the last tokens of sequence b,
+    and each sees itself and what came before it.  scale defaults to head_dim ** -0.5.  accumulate_weight adds the
+    softmax weights each cached token received to cache.weight.  Rows of a new ``out`` that belong to no sequence are
+    zero; those of a given one are left as they were."""
+    dev = cache.device
+    code = _DTYPE_CODE.get(q.dtype)
+    if code is None or q.dtype == torch.int32:
+        raise ValueError("q must be fp16 or bf16")
+    T, heads, qs = _kv4_rows(q, "q", dev)
+    if q.shape[2] != cache.head_dim:
+        raise ValueError(f"q must have head_dim {cache.head_dim}")
+    if max_queries < 0:
+        raise ValueError("max_queries must not be negative")
+    if out is None:
+        out = _new(torch.zeros, q.shape, q.dtype, dev, stream)
+    o = _want(out, "out", q.dtype, tuple(q.shape), dev)
+    seqs = _kv4_seqs(page_table, seq_lens, token_start, dev)
+    sc = cache.head_dim ** -0.5 if scale is None else float(scale)
+    acc = int(accumulate_weight)
+    with _on(dev):
+        need = _kv4_attention_ws(dev.index, seqs[1], heads, cache.kv_heads, cache.head_dim, cache.page_size, seqs[2],
+                                 max_queries, acc)
+        ws, ws_bytes, hold = _scratch(workspace, need, dev, stream)
+        st = _lib.load().b2sq_kv4_attention(q.data_ptr(), code, T, heads, qs, cache._ref, *seqs, max_queries, sc, o, acc,
+                                            ws, ws_bytes, _stream_ptr(stream, dev))
+    _lib.check(st, "b2sq_kv4_attention")
+    return out
+
+
+def kv4_evict(cache: KV4Cache, page_table: torch.Tensor, seq_lens: torch.Tensor, new_page_table: torch.Tensor,
+              budget: int, recent: int = 0, new_lens: Optional[torch.Tensor] = None,
+              stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """Thins each sequence out to ``budget`` tokens: in every key head the newest ``recent`` ones and those that
+    gathered the most attention weight, copied in order to the pages of new_page_table (pages that page_table does not
+    name).  Returns the new lengths int32 [batch]; the old pages are left as they are."""
+    dev = cache.device
+    table, B, P, lens = _kv4_seqs(page_table, seq_lens, None, dev)
+    if new_page_table.dim() != 2 or budget < 0 or recent < 0:
+        raise ValueError("new_page_table must be int32 [batch, pages], budget and recent must not be negative")
+    NP = new_page_table.shape[1]
+    new_table = _want(new_page_table, "new_page_table", torch.int32, (B, NP), dev)
+    if new_lens is None:
+        new_lens = _new(torch.empty, (B,), torch.int32, dev, stream)
+    nl = _want(new_lens, "new_lens", torch.int32, (B,), dev)
+    with _on(dev):
+        st = _lib.load().b2sq_kv4_evict(cache._ref, table, B, P, lens, new_table, NP, budget, recent, nl,
+                                        _stream_ptr(stream, dev))
+    _lib.check(st, "b2sq_kv4_evict")
+    return new_lens

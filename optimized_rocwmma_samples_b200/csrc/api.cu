@@ -558,6 +558,221 @@ b2sq_status b2sq_gemm_i8_grouped(uint32_t groups, uint32_t rows, uint32_t n, uin
     return ok();
 }
 
+}  // extern "C"
+
+namespace {
+constexpr uint32_t kMaxMoeRoutes = 4096;
+constexpr uint32_t kMaxMoeDepth = 131072;  // 127 * 127 * depth fits in int32
+
+b2sq_status validate_moe_layer(const char* fn, uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t experts,
+                               uint32_t topk)
+{
+    if (experts == 0 || experts > 1024) return fail(B2SQ_ERR_INVALID_ARG, "%s: experts must be in [1, 1024]", fn);
+    if (topk == 0) return fail(B2SQ_ERR_INVALID_ARG, "%s: topk must be >= 1", fn);
+    if (hidden == 0 || inter == 0) return fail(B2SQ_ERR_INVALID_ARG, "%s: hidden and inter must be >= 1", fn);
+    if (hidden % 16 || inter % 16 || hidden > kMaxMoeDepth || inter > kMaxMoeDepth)
+        return fail(B2SQ_ERR_UNSUPPORTED, "%s: hidden and inter must be multiples of 16 up to %u", fn, kMaxMoeDepth);
+    if ((uint64_t)tokens * topk > kMaxMoeRoutes)
+        return fail(B2SQ_ERR_UNSUPPORTED, "%s: tokens * topk above %u (use moe_sorting and gemm_i8_grouped)", fn,
+                    kMaxMoeRoutes);
+    return ok();
+}
+
+b2sq_status validate_kv4_cache(const char* fn, const b2sq_kv4_cache* c, uint32_t max_pages)
+{
+    if (!c) return fail(B2SQ_ERR_INVALID_ARG, "%s: cache is null", fn);
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(B2SQ_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256", fn);
+    if (c->page_size == 0 || c->page_size % 16)
+        return fail(B2SQ_ERR_UNSUPPORTED, "%s: page_size must be a multiple of 16", fn);
+    if (c->kv_heads == 0 || c->kv_heads > 65535)
+        return fail(B2SQ_ERR_INVALID_ARG, "%s: kv_heads must be in [1, 65535]", fn);
+    if ((uint64_t)max_pages * c->page_size > 0x7fffffffull)
+        return fail(B2SQ_ERR_INVALID_ARG, "%s: max_pages * page_size overflows 31 bits", fn);
+    if (c->pages > 0x7fffffffu) return fail(B2SQ_ERR_INVALID_ARG, "%s: too many pages", fn);
+    if (c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale))
+        return fail(B2SQ_ERR_INVALID_ARG, "%s: null cache buffer", fn);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16) ||
+        !aligned(c->weight, 16))
+        return fail(B2SQ_ERR_UNSUPPORTED, "%s: cache buffers must be 16-byte aligned", fn);
+    return ok();
+}
+
+b2sq_status validate_kv4_seqs(const char* fn, const int32_t* table, uint32_t batch, uint32_t max_pages,
+                              const int32_t* lens, const int32_t* start)
+{
+    if (batch > 65535) return fail(B2SQ_ERR_INVALID_ARG, "%s: batch must be <= 65535", fn);
+    if ((max_pages > 0 && !table) || !lens || !start) return fail(B2SQ_ERR_INVALID_ARG, "%s: null pointer", fn);
+    if (!aligned(table, 4) || !aligned(lens, 4) || !aligned(start, 4))
+        return fail(B2SQ_ERR_INVALID_ARG, "%s: misaligned pointer", fn);
+    return ok();
+}
+
+b2sq::Kv4Cache kv4_cache_of(const b2sq_kv4_cache* c)
+{
+    return {c->k, c->v, c->k_scale, c->v_scale, c->weight, c->pages, c->kv_heads, c->page_size, c->head_dim};
+}
+}  // namespace
+
+extern "C" {
+
+b2sq_status b2sq_moe_layer_workspace_size(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t experts,
+                                          uint32_t topk, size_t* bytes)
+{
+    if (!bytes) return fail(B2SQ_ERR_INVALID_ARG, "moe_layer_workspace_size: bytes is null");
+    *bytes = 0;
+    b2sq_status st = validate_moe_layer("moe_layer_workspace_size", tokens, hidden, inter, experts, topk);
+    if (st != B2SQ_OK || tokens == 0) return st;
+    uint32_t sms = 0;
+    cudaError_t e = current_sm_count(&sms);
+    if (e != cudaSuccess) return cuda_fail(e, "moe_layer_workspace_size: SM count");
+    *bytes = b2sq::moe_layer_workspace(tokens, hidden, inter, experts, topk, sms);
+    return ok();
+}
+
+b2sq_status b2sq_moe_layer(const void* x, b2sq_dtype x_type, uint32_t ldx, const float* topk_weights,
+                           const int32_t* topk_ids, const float* smooth1, const int8_t* w13, const float* s13,
+                           const float* smooth2, const int8_t* w2, const float* s2, void* out, uint32_t tokens,
+                           uint32_t hidden, uint32_t inter, uint32_t experts, uint32_t topk, float quant_max,
+                           void* workspace, size_t workspace_bytes, b2sq_stream_t stream)
+{
+    if (x_type != B2SQ_F16 && x_type != B2SQ_BF16)
+        return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: x must be f16 or bf16");
+    if (!qmax_ok(quant_max)) return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: quant_max must be in (0, 127]");
+    b2sq_status st = validate_moe_layer("moe_layer", tokens, hidden, inter, experts, topk);
+    if (st != B2SQ_OK || tokens == 0) return st;
+    if (!x || !topk_weights || !topk_ids || !smooth1 || !w13 || !s13 || !smooth2 || !w2 || !s2 || !out)
+        return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: null pointer");
+    if (ldx < hidden) return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: ldx %u < hidden %u", ldx, hidden);
+    if (!aligned(topk_weights, 4) || !aligned(topk_ids, 4) || !aligned(smooth1, 4) || !aligned(s13, 4) ||
+        !aligned(smooth2, 4) || !aligned(s2, 4))
+        return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: misaligned pointer");
+    if (!aligned(x, 16) || !aligned(w13, 16) || !aligned(w2, 16) || !aligned(out, 16) || ldx % 8)
+        return fail(B2SQ_ERR_UNSUPPORTED, "moe_layer: x, w13, w2, out 16-byte aligned and ldx a multiple of 8");
+    uint32_t sms = 0;
+    cudaError_t e = current_sm_count(&sms);
+    if (e != cudaSuccess) return cuda_fail(e, "moe_layer: SM count");
+    const size_t need = b2sq::moe_layer_workspace(tokens, hidden, inter, experts, topk, sms);
+    if (!workspace || workspace_bytes < need)
+        return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: workspace of %zu bytes needed", need);
+    if (!aligned(workspace, 256)) return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: workspace must be 256-byte aligned");
+    const b2sq::MoeLayer m{x,  x_type == B2SQ_BF16, ldx, topk_weights, topk_ids, smooth1, w13,  s13,      smooth2,
+                           w2, s2,                  out, tokens,       hidden,   inter,   experts, topk, quant_max};
+    e = b2sq::launch_moe_layer(m, workspace, sms, reinterpret_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "moe_layer launch");
+    return ok();
+}
+
+b2sq_status b2sq_kv4_append(const void* k, const void* v, b2sq_dtype type, uint32_t tokens, uint32_t k_stride,
+                            uint32_t v_stride, const b2sq_kv4_cache* cache, const int32_t* page_table, uint32_t batch,
+                            uint32_t max_pages, const int32_t* seq_lens, const int32_t* token_start, void* k_out,
+                            void* v_out, b2sq_stream_t stream)
+{
+    if (type != B2SQ_F16 && type != B2SQ_BF16) return fail(B2SQ_ERR_INVALID_ARG, "kv4_append: k, v must be f16 or bf16");
+    b2sq_status st = validate_kv4_cache("kv4_append", cache, max_pages);
+    if (st != B2SQ_OK || tokens == 0 || batch == 0) return st;
+    st = validate_kv4_seqs("kv4_append", page_table, batch, max_pages, seq_lens, token_start);
+    if (st != B2SQ_OK) return st;
+    if (!k || !v) return fail(B2SQ_ERR_INVALID_ARG, "kv4_append: null pointer");
+    const uint64_t row = (uint64_t)cache->kv_heads * cache->head_dim;
+    if (k_stride < row || v_stride < row) return fail(B2SQ_ERR_INVALID_ARG, "kv4_append: token pitch below kv_heads * head_dim");
+    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_out, 16) || !aligned(v_out, 16) || k_stride % 8 || v_stride % 8)
+        return fail(B2SQ_ERR_UNSUPPORTED, "kv4_append: rows must be 16-byte aligned");
+    if (tokens > 0x7fffffffu || tokens * row / 2048 >= 0x7fffffffull)
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_append: too many tokens for one launch");
+    cudaError_t e = b2sq::launch_kv4_append(kv4_cache_of(cache),
+                                            {page_table, seq_lens, token_start, batch, max_pages, tokens}, k, v,
+                                            type == B2SQ_BF16, k_stride, v_stride, k_out, v_out,
+                                            reinterpret_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kv4_append launch");
+    return ok();
+}
+
+b2sq_status b2sq_kv4_attention_workspace_size(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                                              uint32_t page_size, uint32_t max_pages, uint32_t max_queries,
+                                              int accumulate_weight, size_t* bytes)
+{
+    if (!bytes) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention_workspace_size: bytes is null");
+    *bytes = 0;
+    if (kv_heads == 0 || heads == 0 || heads % kv_heads)
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention_workspace_size: heads must be a multiple of kv_heads");
+    if ((uint64_t)max_pages * page_size > 0x7fffffffull)
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention_workspace_size: max_pages * page_size overflows 31 bits");
+    uint32_t sms = 0;
+    cudaError_t e = current_sm_count(&sms);
+    if (e != cudaSuccess) return cuda_fail(e, "kv4_attention_workspace_size: SM count");
+    *bytes = b2sq::kv4_attention_workspace(batch, heads, kv_heads, head_dim, max_queries, max_pages * page_size,
+                                           accumulate_weight != 0, sms);
+    return ok();
+}
+
+b2sq_status b2sq_kv4_attention(const void* q, b2sq_dtype type, uint32_t tokens, uint32_t heads, uint32_t q_stride,
+                               const b2sq_kv4_cache* cache, const int32_t* page_table, uint32_t batch,
+                               uint32_t max_pages, const int32_t* seq_lens, const int32_t* token_start,
+                               uint32_t max_queries, float scale, void* out, int accumulate_weight, void* workspace,
+                               size_t workspace_bytes, b2sq_stream_t stream)
+{
+    if (type != B2SQ_F16 && type != B2SQ_BF16) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: q must be f16 or bf16");
+    if (!std::isfinite(scale)) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: scale must be finite");
+    b2sq_status st = validate_kv4_cache("kv4_attention", cache, max_pages);
+    if (st != B2SQ_OK) return st;
+    if (heads == 0 || heads % cache->kv_heads)
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: heads (%u) must be a multiple of kv_heads (%u)", heads,
+                    cache->kv_heads);
+    if (accumulate_weight && !cache->weight)
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: the cache keeps no weights");
+    if (tokens == 0 || batch == 0 || max_queries == 0) return ok();
+    st = validate_kv4_seqs("kv4_attention", page_table, batch, max_pages, seq_lens, token_start);
+    if (st != B2SQ_OK) return st;
+    if (!q || !out) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: null pointer");
+    const uint64_t row = (uint64_t)heads * cache->head_dim;
+    if (q_stride < row) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: token pitch below heads * head_dim");
+    if (!aligned(q, 16) || !aligned(out, 16) || q_stride % 8)
+        return fail(B2SQ_ERR_UNSUPPORTED, "kv4_attention: q and out rows must be 16-byte aligned");
+    if (tokens > 0x7fffffffu || (uint64_t)max_queries * heads > 0x7fffffffull)
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: too many query rows for one launch");
+    uint32_t sms = 0;
+    cudaError_t e = current_sm_count(&sms);
+    if (e != cudaSuccess) return cuda_fail(e, "kv4_attention: SM count");
+    const size_t need = b2sq::kv4_attention_workspace(batch, heads, cache->kv_heads, cache->head_dim, max_queries,
+                                                      max_pages * cache->page_size, accumulate_weight != 0, sms);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: workspace of %zu bytes needed", need);
+    if (!aligned(workspace, 256)) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: workspace must be 256-byte aligned");
+    const b2sq::Kv4Attention a{kv4_cache_of(cache),
+                               {page_table, seq_lens, token_start, batch, max_pages, tokens},
+                               q, out, type == B2SQ_BF16, heads, max_queries, q_stride, scale, accumulate_weight != 0};
+    e = b2sq::launch_kv4_attention(a, workspace, sms, reinterpret_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kv4_attention launch");
+    return ok();
+}
+
+b2sq_status b2sq_kv4_evict(const b2sq_kv4_cache* cache, const int32_t* page_table, uint32_t batch, uint32_t max_pages,
+                           const int32_t* seq_lens, const int32_t* new_page_table, uint32_t new_max_pages,
+                           uint32_t budget, uint32_t recent, int32_t* new_lens, b2sq_stream_t stream)
+{
+    b2sq_status st = validate_kv4_cache("kv4_evict", cache, max_pages);
+    if (st == B2SQ_OK) st = validate_kv4_cache("kv4_evict", cache, new_max_pages);
+    if (st != B2SQ_OK) return st;
+    if (recent > budget) return fail(B2SQ_ERR_INVALID_ARG, "kv4_evict: recent (%u) above budget (%u)", recent, budget);
+    if (!cache->weight) return fail(B2SQ_ERR_INVALID_ARG, "kv4_evict: the cache keeps no weights");
+    if (batch == 0) return ok();
+    st = validate_kv4_seqs("kv4_evict", page_table, batch, max_pages, seq_lens, seq_lens);
+    if (st != B2SQ_OK) return st;
+    if ((new_max_pages > 0 && !new_page_table) || !new_lens) return fail(B2SQ_ERR_INVALID_ARG, "kv4_evict: null pointer");
+    if (!aligned(new_page_table, 4) || !aligned(new_lens, 4))
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_evict: misaligned pointer");
+    if (new_page_table && new_page_table == page_table)
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_evict: the new table must name other pages than the old one");
+    uint32_t sms = 0;
+    cudaError_t e = current_sm_count(&sms);
+    if (e != cudaSuccess) return cuda_fail(e, "kv4_evict: SM count");
+    e = b2sq::launch_kv4_evict(kv4_cache_of(cache), page_table, max_pages, seq_lens, new_page_table, new_max_pages, batch,
+                               budget, recent, new_lens, sms, reinterpret_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kv4_evict launch");
+    return ok();
+}
+
 b2sq_status b2sq_last_device_error(b2sq_stream_t stream, uint32_t* where)
 {
     uint32_t v = 0;

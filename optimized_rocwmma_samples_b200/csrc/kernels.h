@@ -116,6 +116,62 @@ cudaError_t launch_moe_sort(const int32_t* ids, uint32_t tokens, uint32_t topk, 
 cudaError_t launch_topk_softmax(const void* logits, float* topk_w, int32_t* topk_i, uint32_t tokens,
                                 uint32_t experts, uint32_t topk, cudaStream_t st);
 
+// The 4-bit paged key/value cache (layout: kv4.cuh) and the sequences of a call.
+struct Kv4Cache {
+    uint8_t *k, *v;
+    void *k_scale, *v_scale;  // fp16 pairs
+    float* weight;            // nullable
+    uint32_t pages, kv_heads, page_size, head_dim;
+};
+struct Kv4Seqs {
+    const int32_t* page_table;   // [batch][max_pages]
+    const int32_t* seq_lens;     // [batch], with this call's tokens
+    const int32_t* token_start;  // [batch + 1] offsets into the packed tokens
+    uint32_t batch, max_pages, tokens;
+};
+cudaError_t launch_kv4_append(const Kv4Cache& c, const Kv4Seqs& s, const void* k, const void* v, bool bf16,
+                              uint64_t k_stride, uint64_t v_stride, void* k_out, void* v_out, cudaStream_t st);
+
+struct Kv4Attention {
+    Kv4Cache cache;
+    Kv4Seqs seqs;
+    const void* q;
+    void* out;
+    bool bf16;
+    uint32_t heads, max_queries;
+    uint64_t q_stride;
+    float scale;
+    bool accumulate;
+};
+size_t kv4_attention_workspace(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                               uint32_t max_queries, uint32_t max_len, bool accumulate, uint32_t num_sms);
+cudaError_t launch_kv4_attention(const Kv4Attention& a, void* workspace, uint32_t num_sms, cudaStream_t st);
+
+cudaError_t launch_kv4_evict(const Kv4Cache& c, const int32_t* page_table, uint32_t max_pages, const int32_t* seq_lens,
+                             const int32_t* new_table, uint32_t new_max_pages, uint32_t batch, uint32_t budget,
+                             uint32_t recent, int32_t* new_lens, uint32_t num_sms, cudaStream_t st);
+
+// Mixture-of-experts layer for a few tokens (moe_layer.cu).
+struct MoeLayer {
+    const void* x;
+    bool bf16;
+    uint64_t x_stride;
+    const float* topk_w;
+    const int32_t* topk_ids;
+    const float* smooth1;
+    const int8_t* w13;
+    const float* s13;
+    const float* smooth2;
+    const int8_t* w2;
+    const float* s2;
+    void* out;
+    uint32_t tokens, hidden, inter, experts, topk;
+    float qmax;
+};
+size_t moe_layer_workspace(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t experts, uint32_t topk,
+                           uint32_t num_sms);
+cudaError_t launch_moe_layer(const MoeLayer& m, void* workspace, uint32_t num_sms, cudaStream_t st);
+
 // Debug: a kernel that waits for an mbarrier nobody arrives on, with a limit.
 cudaError_t launch_debug_bounded_wait(uint64_t limit_ns, cudaStream_t st);
 

@@ -1,0 +1,212 @@
+// kv4_evict.cu — thins sequences of the 4-bit cache out to a budget of tokens.
+//
+// A sequence of n > budget tokens keeps, in every head by itself, its newest
+// `recent` tokens and of the others the budget - recent with the largest
+// accumulated attention weight (equal weights: the lower position; a NaN
+// counts as the largest).  Kept tokens stay in order and are copied, with
+// their weights, to the pages of a second table; shorter sequences are copied
+// whole.
+//
+// The threshold is found by a radix search over the weights' sortable bits
+// (four passes of 8 bits over keys in shared memory), places by ballots and
+// one prefix sum over the warps.  Every block of a head repeats that search
+// and copies its own share of the kept rows, so no block waits for another.
+#include "kv4.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace b2sq {
+
+namespace {
+
+constexpr uint32_t kEvictThreads = 512;
+constexpr uint32_t kEvictWarps = kEvictThreads / 32;
+constexpr uint32_t kEvictKeys = 40960;  // keys held in shared memory (160 KB); longer sequences re-read theirs
+constexpr uint32_t kEvictRows = 4096;   // kept rows one block lists at a time
+
+// Bits that order as the weights do; -0 equals +0, NaN is above infinity.
+__device__ __forceinline__ uint32_t weight_key(float w)
+{
+    if (w != w) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(w + 0.f);
+    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kEvictThreads)
+    kv4_evict_kernel(Kv4Cache c, const int32_t* __restrict__ page_table, uint32_t max_pages,
+                     const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ new_table,
+                     uint32_t new_max_pages, uint32_t budget, uint32_t recent, int32_t* __restrict__ new_lens,
+                     uint32_t key_slots, uint32_t row_slots)
+{
+    extern __shared__ uint32_t ev_smem[];
+    uint32_t* keys = ev_smem;              // [key_slots]
+    uint32_t* rows = ev_smem + key_slots;  // [row_slots]
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t warp_gt[kEvictWarps], warp_eq[kEvictWarps];
+    __shared__ uint32_t sel_digit, sel_above;
+
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint32_t b = blockIdx.z, head = blockIdx.y;
+    const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const int32_t* table = page_table + (uint64_t)b * max_pages;
+    const int32_t* dst_table = new_table + (uint64_t)b * new_max_pages;
+    const uint32_t n = min((uint32_t)max(__ldg(seq_lens + b), 0), max_pages * c.page_size);
+    const uint32_t kept = min(min(n, budget), new_max_pages * c.page_size);
+    if (blockIdx.x == 0 && head == 0 && tid == 0) new_lens[b] = (int32_t)kept;
+    // this block's share of the kept rows
+    const uint32_t d0 = (uint32_t)((uint64_t)kept * blockIdx.x / gridDim.x);
+    const uint32_t d1 = (uint32_t)((uint64_t)kept * (blockIdx.x + 1) / gridDim.x);
+    if (d0 == d1) return;
+
+    const bool all = n <= kept;
+    const uint32_t newest = min(recent, kept);
+    const uint32_t old = all ? 0 : n - newest;      // candidates
+    const uint32_t want = all ? 0 : kept - newest;  // of them kept
+
+    auto key_of = [&](uint32_t i) -> uint32_t {
+        const int64_t r = kv4_row(c, table, i, head);
+        return r < 0 ? 0u : weight_key(c.weight[r]);
+    };
+    const bool held = old <= key_slots;
+    if (held)
+        for (uint32_t i = tid; i < old; i += kEvictThreads) keys[i] = key_of(i);
+    auto key_at = [&](uint32_t i) { return held ? keys[i] : key_of(i); };
+
+    // the want-th largest key: `prefix` gathers its digits, `above` counts larger ones
+    uint32_t prefix = 0, above = 0;
+    if (want > 0 && want < old) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            for (uint32_t i = tid; i < 256; i += kEvictThreads) hist[i] = 0;
+            __syncthreads();
+            for (uint32_t i = tid; i < (old + 31) / 32 * 32; i += kEvictThreads) {  // whole warps
+                const uint32_t key = i < old ? key_at(i) : 0;
+                const bool mine = i < old && (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
+                const uint32_t digit = mine ? (key >> shift) & 255u : 256u;
+                // lanes of the same digit add once (weights of one size share their upper digits)
+                const uint32_t same = __match_any_sync(0xffffffffu, digit);
+                if (mine && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+            }
+            __syncthreads();
+            if (warp == 0) {
+                uint32_t mine[8], sum = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {  // lane l holds digits 255 - 8 l downwards
+                    mine[j] = hist[255 - (lane * 8 + j)];
+                    sum += mine[j];
+                }
+                uint32_t incl = sum;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const uint32_t t = __shfl_up_sync(0xffffffffu, incl, off);
+                    if (lane >= (uint32_t)off) incl += t;
+                }
+                uint32_t run = above + incl - sum;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (run < want && run + mine[j] >= want) {
+                        sel_digit = 255 - (lane * 8 + j);
+                        sel_above = run;
+                    }
+                    run += mine[j];
+                }
+            }
+            __syncthreads();
+            prefix |= sel_digit << shift;
+            above = sel_above;
+        }
+    }
+    const uint32_t ties = want - above;  // of the keys equal to `prefix`, the first ones
+    const bool take_all_old = want == old, take_none = want == 0;
+
+    // each warp walks a run of positions: first its counts, then the places
+    const uint32_t run = (old + kEvictWarps * 32 - 1) / (kEvictWarps * 32) * 32;
+    const uint32_t w0 = min(warp * run, old), w1 = min(w0 + run, old);
+    uint32_t gt = 0, eq = 0;
+    if (!take_none)
+        for (uint32_t i = w0 + lane; i < w0 + run; i += 32) {
+            const uint32_t key = i < w1 ? key_at(i) : 0;
+            gt += __popc(__ballot_sync(0xffffffffu, i < w1 && (take_all_old || key > prefix)));
+            eq += __popc(__ballot_sync(0xffffffffu, i < w1 && !take_all_old && key == prefix));
+        }
+    if (lane == 0) {
+        warp_gt[warp] = gt;
+        warp_eq[warp] = eq;
+    }
+    __syncthreads();
+    uint32_t gt0 = 0, eq0 = 0;
+    for (uint32_t i = 0; i < warp; ++i) {
+        gt0 += warp_gt[i];
+        eq0 += warp_eq[i];
+    }
+
+    const uint32_t ng = c.head_dim / kKv4Group;
+    const uint32_t quads = c.head_dim / 32;  // 16-byte pieces of a row's keys (and of its values)
+    for (uint32_t r0 = d0; r0 < d1; r0 += row_slots) {
+        const uint32_t r1 = min(r0 + row_slots, d1);
+        if (!take_none) {
+            uint32_t g = gt0, e = eq0;
+            for (uint32_t i = w0 + lane; i < w0 + run; i += 32) {
+                const uint32_t key = i < w1 ? key_at(i) : 0;
+                const bool is_gt = i < w1 && (take_all_old || key > prefix);
+                const bool is_eq = i < w1 && !take_all_old && key == prefix;
+                const uint32_t mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
+                const uint32_t below = (1u << lane) - 1;
+                const uint32_t eq_rank = e + __popc(me & below);
+                if (is_gt || (is_eq && eq_rank < ties)) {
+                    const uint32_t to = g + __popc(mg & below) + min(eq_rank, ties);
+                    if (to >= r0 && to < r1) rows[to - r0] = i;
+                }
+                g += __popc(mg);
+                e += __popc(me);
+            }
+        }
+        for (uint32_t to = max(r0, want) + tid; to < r1; to += kEvictThreads) rows[to - r0] = all ? to : n - kept + to;
+        __syncthreads();
+        for (uint32_t u = tid; u < (r1 - r0) * 2 * quads; u += kEvictThreads) {
+            const uint32_t j = u / (2 * quads), piece = u % (2 * quads);
+            const int64_t src = kv4_row(c, table, rows[j], head), dst = kv4_row(c, dst_table, r0 + j, head);
+            if (src < 0 || dst < 0) continue;
+            uint8_t* base = piece < quads ? c.k : c.v;
+            const uint32_t q = piece < quads ? piece : piece - quads;
+            reinterpret_cast<uint4*>(base)[dst * quads + q] = reinterpret_cast<const uint4*>(base)[src * quads + q];
+        }
+        for (uint32_t u = tid; u < (r1 - r0) * (2 * ng + 1); u += kEvictThreads) {
+            const uint32_t j = u / (2 * ng + 1), piece = u % (2 * ng + 1);
+            const int64_t src = kv4_row(c, table, rows[j], head), dst = kv4_row(c, dst_table, r0 + j, head);
+            if (src < 0 || dst < 0) continue;
+            if (piece == 2 * ng) {
+                c.weight[dst] = c.weight[src];
+            } else {
+                uint32_t* base = static_cast<uint32_t*>(piece < ng ? c.k_scale : c.v_scale);
+                const uint32_t q = piece < ng ? piece : piece - ng;
+                base[dst * ng + q] = base[src * ng + q];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_kv4_evict(const Kv4Cache& c, const int32_t* page_table, uint32_t max_pages, const int32_t* seq_lens,
+                             const int32_t* new_table, uint32_t new_max_pages, uint32_t batch, uint32_t budget,
+                             uint32_t recent, int32_t* new_lens, uint32_t num_sms, cudaStream_t st)
+{
+    const uint64_t heads = (uint64_t)batch * c.kv_heads;
+    // about two blocks an SM; a block copies at least 64 rows
+    const uint32_t split = (uint32_t)std::max<uint64_t>(
+        1, std::min<uint64_t>((2 * num_sms + heads - 1) / heads, std::min<uint64_t>(16, (budget + 63) / 64)));
+    const uint32_t cap = max_pages * c.page_size;
+    const uint32_t key_slots = cap <= kEvictKeys ? (cap + 3) / 4 * 4 : 0;
+    const uint32_t row_slots = std::min(kEvictRows, (budget + split - 1) / split + 1);
+    const size_t smem = (size_t)(key_slots + row_slots) * 4;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(kv4_evict_kernel, (kEvictKeys + kEvictRows) * 4, done);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kv4_evict_kernel, dim3(split, c.kv_heads, batch), dim3(kEvictThreads), smem, st, c, page_table,
+                      max_pages, seq_lens, new_table, new_max_pages, budget, recent, new_lens, key_slots, row_slots);
+}
+
+}  // namespace b2sq
