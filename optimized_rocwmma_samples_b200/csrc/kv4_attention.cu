@@ -6,8 +6,32 @@
 // and, where asked, weight[head][position] += sum of p over the head's query
 // heads and the queries.  A row that sees nothing gives 0.
 //
-// One warp per query row, positions in turn; the row's maximum and sum go to
-// the workspace for the weights, which a second kernel adds up per position.
+// What bounds it is reading the cache (D/2 + D/16 bytes for a token's keys, as
+// many for its values), so all query rows of a key head (its query heads times
+// the queries) share one pass, 8 NT rows at a time, and nibbles become matrix
+// operands with as few instructions as possible:
+//  * A nibble masked out of a 16-bit word, q or 16 q, is the fp16 subnormal
+//    q 2^-24 or q 2^-20.  mma.m16n8k16 takes subnormals as they are, so one AND
+//    turns two nibbles into two operands (and a shift by 8 serves the word's
+//    upper half).  The powers of two, the group's step and its base are applied
+//    to the sums: q.K over a group = s * sum(q4 q) + z * sum(q).
+//  * Scores: K is the 16 x 16 operand (16 tokens, 16 channels of one word
+//    position), the query rows are the 8 columns, prepared once in that order
+//    as fp16 scaled by a power of two to [2^9, 2^10) (exact for both types).
+//  * Output: V^T is the 16 x 16 operand; ldmatrix.trans moves whole 16-bit
+//    words (4 channels of a token), which is the transposition needed.  The
+//    probabilities, times the token's step over a running power of two of the
+//    group, are rounded to fp16 (11 bits; the result has 8 or 11) and turned
+//    into the other operand by movmatrix.  sum(p z) is kept apart in fp32.
+//
+// Work is split evenly over the grid in chunks of 16 tokens, whatever the
+// lengths: the (sequence, head, row block) items lie one after another on a
+// line of chunks and every block takes an equal piece of it.  Blocks that get
+// part of an item leave their maxima, sums and outputs in the workspace, and a
+// second kernel joins them in a fixed order (and adds up the weights from the
+// scores that the first one left there).  In a block each of the four warps
+// streams its own chunks through a ring of cp.async stages, with no barrier
+// until the item's end.
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -16,123 +40,801 @@ namespace b2sq {
 
 namespace {
 
-struct KvAttnParams {
+constexpr uint32_t kWarps = 4;
+constexpr uint32_t kThreads = kWarps * 32;
+constexpr uint32_t kChunk = 16;     // tokens a warp takes at a time
+constexpr uint32_t kMinChunks = 4;  // a block gets at least one for each warp
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnParams {
     Kv4Cache c;
     Kv4Seqs s;
-    uint32_t heads, max_queries;
+    const void* q;
+    void* out;
     uint64_t q_stride;
-    float scale;
+    uint32_t heads, group, max_queries, row_pad;  // row_pad: group * max_queries rounded up to 8
+    float scale_log2;
+    uint32_t* unit_start;  // [batch + 1] first chunk of each sequence on the line
+    float2* stats;         // [batch * kv_heads][row_pad] (max, sum) of items that one block did whole
+    float* part_o;         // [2 * blocks][8 NT][D]
+    float2* part_ml;       // [2 * blocks][8 NT]
+    float* scores;         // [batch * kv_heads][positions][row_pad], for the weights
 };
 
-__device__ __forceinline__ float kv4_value(const uint8_t* data, const __half* sz, int64_t row, uint32_t d, uint32_t ng,
-                                           uint32_t ch)
+// Blocks a SM that registers (and shared memory) leave room for.
+template <int D, int NT>
+constexpr uint32_t attn_blocks()
 {
-    const uint32_t byte = data[row * (d / 2) + ch / 2];
-    const uint32_t q = (ch & 1) ? byte >> 4 : byte & 15u;
-    const __half* g = sz + (row * ng + ch / kKv4Group) * 2;
-    return fmaf((float)q, __half2float(g[0]), __half2float(g[1]));
+    return D == 64 ? (NT == 1 ? 6 : NT == 2 ? 4 : 3) : D == 128 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (NT == 1 ? 3 : 2);
+}
+constexpr uint32_t kMaxBlocks = 6;
+
+template <int D, int NT>
+struct AttnSmem {
+    static constexpr uint32_t rows = 8 * NT;
+    static constexpr uint32_t data = kChunk * D / 2;                // a chunk's key nibbles
+    static constexpr uint32_t scales = kChunk * (D / 64) * 4;       // and their steps and bases
+    static constexpr uint32_t stage = 2 * (data + scales);
+    static constexpr uint32_t stages = D == 64 ? 6 : D == 128 ? 4 : 3;
+    static constexpr uint32_t ring = kWarps * stages * stage;
+    static constexpr uint32_t q = rows * D * 2;
+    static constexpr uint32_t pitch = D + 2;
+    static constexpr uint32_t merge = rows * pitch * 4;
+    static constexpr uint32_t fixed = ring + q + merge;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x)
+{
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+    return d;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Words j of four nibbles each become fp16 subnormals: nibbles 0 and 2 stand for q 2^-24, 1 and 3 for q 2^-20.
+template <int J>
+__device__ __forceinline__ uint32_t nibbles(uint32_t w)
+{
+    return (J < 2 ? w : w >> 8) & ((J & 1) ? 0x00f000f0u : 0x000f000fu);
 }
 
-// grid (max_queries * heads, batch), one warp a block; lane holds channels lane, lane + 32, ...
-template <typename T, int D>
-__global__ void __launch_bounds__(32) kv4_rows_kernel(KvAttnParams a, const T* __restrict__ q, T* __restrict__ out,
-                                                      float2* __restrict__ stats)
+struct SeqShape {
+    uint32_t len, n, start, vis, chunks, blocks;
+};
+// vis: positions with a place in the table; an empty sequence has one chunk in which nothing is seen
+__device__ __forceinline__ SeqShape seq_shape(const AttnParams& a, uint32_t b, uint32_t rows)
 {
-    griddep_wait();
-    griddep_launch_dependents();
-    const uint32_t b = blockIdx.y, i = blockIdx.x / a.heads, head = blockIdx.x % a.heads, lane = threadIdx.x;
-    uint32_t start;
-    const uint32_t n = kv4_new_rows(a.s, b, start);
-    if (i >= n) return;
-    const uint32_t kvh = head / (a.heads / a.c.kv_heads);
-    const int64_t vis = (int64_t)kv4_len(a.s, b) - n + i + 1;
-    const uint32_t see = (uint32_t)max((int64_t)0, min(vis, (int64_t)kv4_cap(a.c, a.s)));
-    float qf[D / 32], o[D / 32];
-    for (int j = 0; j < D / 32; ++j) {
-        qf[j] = (float)q[(uint64_t)(start + i) * a.q_stride + (uint64_t)head * D + lane + 32 * j];
-        o[j] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    const int32_t* table = a.s.page_table + (uint64_t)b * a.s.max_pages;
-    for (uint32_t t = 0; t < see; ++t) {
-        const int64_t row = kv4_row(a.c, table, t, kvh);
-        if (row < 0) continue;
-        float dot = 0.f;
-        for (int j = 0; j < D / 32; ++j)
-            dot = fmaf(qf[j], kv4_value(a.c.k, (const __half*)a.c.k_scale, row, D, D / 64, lane + 32 * j), dot);
-        for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-        const float s = dot * a.scale;
-        const float mn = fmaxf(m, s), f = m == -INFINITY ? 0.f : expf(m - mn), p = s == -INFINITY ? 0.f : expf(s - mn);
-        for (int j = 0; j < D / 32; ++j)
-            o[j] = o[j] * f + p * kv4_value(a.c.v, (const __half*)a.c.v_scale, row, D, D / 64, lane + 32 * j);
-        l = l * f + p;
-        m = mn;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int j = 0; j < D / 32; ++j)
-        out[((uint64_t)(start + i) * a.heads + head) * D + lane + 32 * j] = (T)(o[j] * inv);
-    if (stats && lane == 0) stats[((uint64_t)b * a.max_queries + i) * a.heads + head] = make_float2(m, inv);
+    SeqShape s;
+    s.len = kv4_len(a.s, b);
+    s.n = kv4_new_rows(a.s, b, s.start);
+    s.vis = min(s.len, kv4_cap(a.c, a.s));
+    s.chunks = max(1u, (s.vis + kChunk - 1) / kChunk);
+    s.blocks = (min(s.n, a.max_queries) * a.group + rows - 1) / rows;
+    return s;
 }
 
-// grid (positions / 8, kv_heads, batch), a warp a position
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_weights_kernel(KvAttnParams a, const T* __restrict__ q,
-                                                          const float2* __restrict__ stats)
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_kernel(AttnParams a)
 {
+    using S = AttnSmem<D, NT>;
+    constexpr uint32_t NG = D / 64, CPR = D / 32, ROWS = 8 * NT, STAGES = S::stages;
+    extern __shared__ __align__(16) uint8_t at_smem[];
+    uint8_t* ring = at_smem;
+    __half* q_frag = reinterpret_cast<__half*>(at_smem + S::ring);  // [NT][NG][2][32 lanes] x 16 bytes
+    float* merge = reinterpret_cast<float*>(at_smem + S::ring + S::q);
+    uint32_t* ustart = reinterpret_cast<uint32_t*>(at_smem + S::fixed);  // [batch + 1]
+    __shared__ float row_mul[ROWS], row_sum[ROWS][NG];
+    __shared__ int row_vis[ROWS];
+    __shared__ float2 warp_ml[kWarps][ROWS];
+    __shared__ uint32_t scan_part[kWarps];
+
+    const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, tig = lane & 3;
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t b = blockIdx.z, kvh = blockIdx.y, t = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
-    uint32_t start;
-    const uint32_t n = kv4_new_rows(a.s, b, start);
-    if (t >= kv4_cap(a.c, a.s)) return;
-    const int64_t row = kv4_row(a.c, a.s.page_table + (uint64_t)b * a.s.max_pages, t, kvh);
-    const uint32_t group = a.heads / a.c.kv_heads;
-    float sum = 0.f;
-    bool any = false;
-    for (uint32_t i = 0; i < min(n, a.max_queries); ++i) {
-        if ((int64_t)t >= (int64_t)kv4_len(a.s, b) - n + i + 1 || row < 0) continue;
-        any = true;
-        for (uint32_t g = 0; g < group; ++g) {
-            const uint32_t head = kvh * group + g;
-            float dot = 0.f;
-            for (int j = 0; j < D / 32; ++j)
-                dot = fmaf((float)q[(uint64_t)(start + i) * a.q_stride + (uint64_t)head * D + lane + 32 * j],
-                           kv4_value(a.c.k, (const __half*)a.c.k_scale, row, D, D / 64, lane + 32 * j), dot);
-            for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-            const float2 st = stats[((uint64_t)b * a.max_queries + i) * a.heads + head];
-            sum += expf(dot * a.scale - st.x) * st.y;
+
+    // the line of chunks: first chunk of every sequence
+    {
+        uint32_t carry = 0;
+        for (uint32_t base = 0; base < a.s.batch; base += kThreads) {
+            const uint32_t b = base + tid;
+            uint32_t v = 0;
+            if (b < a.s.batch) {
+                const SeqShape sh = seq_shape(a, b, ROWS);
+                v = sh.chunks * sh.blocks * a.c.kv_heads;
+            }
+            uint32_t incl = v;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const uint32_t t = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= (uint32_t)off) incl += t;
+            }
+            if (lane == 31) scan_part[warp] = incl;
+            __syncthreads();
+            uint32_t before = carry;
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                if (w < warp) before += scan_part[w];
+                carry += scan_part[w];
+            }
+            if (b < a.s.batch) ustart[b] = before + incl - v;
+            __syncthreads();
         }
+        if (tid == 0) ustart[a.s.batch] = carry;
+        __syncthreads();
+        if (blockIdx.x == 0)
+            for (uint32_t b = tid; b <= a.s.batch; b += kThreads) a.unit_start[b] = ustart[b];
     }
-    if (lane == 0 && any) a.c.weight[row] += sum;
+    const uint32_t total = ustart[a.s.batch];
+    const uint32_t blocks = max(1u, min(gridDim.x, total / kMinChunks));
+    if (blockIdx.x >= blocks || total == 0) return;
+    const uint32_t begin = (uint32_t)((uint64_t)total * blockIdx.x / blocks);
+    const uint32_t end = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / blocks);
+
+    const uint32_t ring_base = smem_u32(ring) + warp * STAGES * S::stage;
+    uint32_t unit = begin;
+    uint32_t b = 0;
+    {  // the last sequence that starts at or before `unit` (empty ones share their start with the next)
+        uint32_t lo = 0, hi = a.s.batch;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (ustart[mid] <= unit)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        b = lo;
+    }
+    while (unit < end) {
+        while (ustart[b + 1] <= unit) ++b;
+        const SeqShape sh = seq_shape(a, b, ROWS);
+        const uint32_t in_seq = unit - ustart[b];
+        const uint32_t item = in_seq / sh.chunks, c0 = in_seq % sh.chunks;
+        const uint32_t head = item / sh.blocks, block = item % sh.blocks;
+        const uint32_t c1 = min(sh.chunks, c0 + (end - unit));
+        const bool whole = c0 == 0 && c1 == sh.chunks;
+        const int32_t* table = a.s.page_table + (uint64_t)b * a.s.max_pages;
+        const uint32_t all_rows = min(sh.n, a.max_queries) * a.group;
+
+        // stage loads: chunk c of the item into ring slot `slot` of this warp
+        auto page_row = [&](uint32_t c) -> int64_t {  // cache row of the chunk's first token, -1 if it has none
+            return c * kChunk < sh.vis ? kv4_row(a.c, table, c * kChunk, head) : -1;
+        };
+        auto load = [&](uint32_t c, uint32_t slot) {
+            const int64_t row = c < c1 ? page_row(c) : -1;
+            if (row >= 0) {
+                const uint32_t dst = ring_base + slot * S::stage;
+                const uint8_t* ks = a.c.k + row * (D / 2);
+                const uint8_t* vs = a.c.v + row * (D / 2);
+#pragma unroll
+                for (uint32_t i = 0; i < S::data / 512; ++i) {
+                    const uint32_t u = i * 32 + lane, r = u / CPR, ch = u % CPR;
+                    const uint32_t to = r * CPR + (ch ^ ((r / (8 / CPR)) & (CPR - 1)));
+                    cp_async16(dst + to * 16, ks + u * 16);
+                    cp_async16(dst + S::data + to * 16, vs + u * 16);
+                }
+                constexpr uint32_t SC = S::scales / 16;
+                if (lane < SC)
+                    cp_async16(dst + 2 * S::data + lane * 16,
+                               static_cast<const uint8_t*>(a.c.k_scale) + row * (NG * 4) + lane * 16);
+                else if (lane < 2 * SC)
+                    cp_async16(dst + 2 * S::data + lane * 16,
+                               static_cast<const uint8_t*>(a.c.v_scale) + row * (NG * 4) + (lane - SC) * 16);
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < STAGES - 1; ++i) load(c0 + warp + i * kWarps, i);
+
+        // the item's query rows, as operands
+        for (uint32_t r = warp; r < ROWS; r += kWarps) {
+            const uint32_t row = block * ROWS + r;
+            float v[D / 32], mx = 0.f;
+            const bool there = row < all_rows;
+            const uint32_t qi = row / a.group, qh = head * a.group + row % a.group;
+            const T* src = static_cast<const T*>(a.q) + (uint64_t)(sh.start + qi) * a.q_stride + (uint64_t)qh * D;
+#pragma unroll
+            for (uint32_t i = 0; i < D / 32; ++i) {
+                v[i] = there ? (float)src[lane + 32 * i] : 0.f;
+                mx = fmaxf(mx, fabsf(v[i]));
+            }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            // 2^(9 - exponent of the largest); none for rows of zeros or with an infinity
+            const int ex = (int)(__float_as_uint(mx) >> 23);
+            const int shift = (ex == 0 || ex == 255) ? 0 : min(max(136 - ex, -100), 100);
+            const float f = __uint_as_float((uint32_t)(127 + shift) << 23);
+#pragma unroll
+            for (uint32_t i = 0; i < D / 32; ++i) {
+                // channel 32 i + lane: word position j, k half, operand register and lane
+                const uint32_t gr = i / 2, cb = i & 1, t4 = lane / 8, y = lane & 7, j = y & 3, hi = y >> 2;
+                const uint32_t at = ((((r / 8) * NG + gr) * 2 + j / 2) * 32 + (r & 7) * 4 + t4) * 8 + (j & 1) * 4 + cb * 2 + hi;
+                q_frag[at] = __float2half_rn(v[i] * ((j & 1) ? f * 0.0625f : f));
+            }
+#pragma unroll
+            for (uint32_t gr = 0; gr < NG; ++gr) {
+                float sum = v[2 * gr] + v[2 * gr + 1];
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                if (lane == 0) row_sum[r][gr] = sum * a.scale_log2;
+            }
+            if (lane == 0) {
+                row_mul[r] = a.scale_log2 * (16777216.f / f);
+                // rows that are not there see everything (their columns are not used), so that they mask nothing
+                row_vis[r] = there ? (int)max((int64_t)0, min((int64_t)sh.vis, (int64_t)sh.len - sh.n + qi + 1)) : (int)sh.vis;
+            }
+        }
+        __syncthreads();
+        float mul[NT][2], qsum[NT][2][NG];
+        int vis[NT][2];
+        int least = 0x7fffffff;  // positions that all rows see
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t r = nt * 8 + 2 * tig + x;
+                mul[nt][x] = row_mul[r];
+                vis[nt][x] = row_vis[r];
+#pragma unroll
+                for (uint32_t gr = 0; gr < NG; ++gr) qsum[nt][x][gr] = row_sum[r][gr];
+            }
+        for (uint32_t r = 0; r < ROWS; ++r) least = min(least, row_vis[r]);
+
+        float o[NG][4][NT][4] = {};
+        float m[NT][2], l[NT][2], zs[NT][2][NG];
+        float inv_ref[NG];  // 1 / the power of two that steps of a group are taken over
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                m[nt][x] = -INFINITY;
+                l[nt][x] = 0.f;
+#pragma unroll
+                for (uint32_t gr = 0; gr < NG; ++gr) zs[nt][x][gr] = 0.f;
+            }
+#pragma unroll
+        for (uint32_t gr = 0; gr < NG; ++gr) inv_ref[gr] = 16777216.f;
+
+        uint32_t slot = 0;
+        for (uint32_t c = c0 + warp; c < c1; c += kWarps) {
+            {
+                uint32_t next = slot + STAGES - 1;
+                if (next >= STAGES) next -= STAGES;
+                __syncwarp();
+                load(c + (STAGES - 1) * kWarps, next);
+            }
+            cp_async_wait<STAGES - 1>();
+            __syncwarp();
+            const uint32_t base = ring_base + slot * S::stage;
+            const uint8_t* stage = ring + (warp * STAGES + slot) * S::stage;
+            if (++slot == STAGES) slot = 0;
+            if (page_row(c) < 0) {  // no such page: nothing of this chunk is seen
+                if (a.scores) {
+                    for (uint32_t i = lane; i < kChunk * ROWS; i += 32) {
+                        const uint32_t row = block * ROWS + i % ROWS;
+                        const uint64_t t = c * kChunk + i / ROWS;
+                        if (row < a.row_pad && t < kv4_cap(a.c, a.s))
+                            a.scores[(((uint64_t)b * a.c.kv_heads + head) * kv4_cap(a.c, a.s) + t) * a.row_pad + row] =
+                                -INFINITY;
+                    }
+                }
+                continue;
+            }
+
+            // scores of 16 tokens
+            float acc[NG][NT][4] = {};
+            const uint32_t tok = (lane & 7) + ((lane >> 3) & 1) * 8;  // ldmatrix row of this lane
+            const uint32_t sw = (tok / (8 / CPR)) & (CPR - 1);
+#pragma unroll
+            for (uint32_t gr = 0; gr < NG; ++gr) {
+                uint32_t w[4];
+                ldsm4(base + (tok * CPR + ((gr * 2 + (lane >> 4)) ^ sw)) * 16, w);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint4* qf = reinterpret_cast<const uint4*>(q_frag) + ((nt * NG + gr) * 2) * 32 + lane;
+                    const uint4 q0 = qf[0], q1 = qf[32];
+                    mma_f16(acc[gr][nt], nibbles<0>(w[0]), nibbles<0>(w[1]), nibbles<0>(w[2]), nibbles<0>(w[3]), q0.x, q0.y);
+                    mma_f16(acc[gr][nt], nibbles<1>(w[0]), nibbles<1>(w[1]), nibbles<1>(w[2]), nibbles<1>(w[3]), q0.z, q0.w);
+                    mma_f16(acc[gr][nt], nibbles<2>(w[0]), nibbles<2>(w[1]), nibbles<2>(w[2]), nibbles<2>(w[3]), q1.x, q1.y);
+                    mma_f16(acc[gr][nt], nibbles<3>(w[0]), nibbles<3>(w[1]), nibbles<3>(w[2]), nibbles<3>(w[3]), q1.z, q1.w);
+                }
+            }
+            // thread: tokens g and g + 8, rows 2 tig and 2 tig + 1 of every eight
+            float2 ksz[2][NG], vsz[2][NG];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const __half2* kp = reinterpret_cast<const __half2*>(stage + 2 * S::data) + (g + 8 * h) * NG;
+                const __half2* vp = reinterpret_cast<const __half2*>(stage + 2 * S::data + S::scales) + (g + 8 * h) * NG;
+#pragma unroll
+                for (uint32_t gr = 0; gr < NG; ++gr) {
+                    ksz[h][gr] = __half22float2(kp[gr]);
+                    vsz[h][gr] = __half22float2(vp[gr]);
+                }
+            }
+            const int t0 = (int)(c * kChunk + g);
+            const bool full = (int)(c * kChunk + kChunk) <= least;
+            float s[NT][4];
+            bool grow = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int h = i >> 1, x = i & 1;
+                    float dot = 0.f, off = 0.f;
+#pragma unroll
+                    for (uint32_t gr = 0; gr < NG; ++gr) {
+                        dot = fmaf(acc[gr][nt][i], ksz[h][gr].x, dot);
+                        off = fmaf(qsum[nt][x][gr], ksz[h][gr].y, off);
+                    }
+                    const float v = fmaf(dot, mul[nt][x], off);
+                    s[nt][i] = full || t0 + 8 * h < vis[nt][x] ? v : -INFINITY;
+                    grow |= s[nt][i] > m[nt][x] + 6.f;  // p may reach 2^6 before the maximum is moved
+                }
+            if (a.scores) {
+                float* sp = a.scores + ((((uint64_t)b * a.c.kv_heads + head) * kv4_cap(a.c, a.s)) + t0) * a.row_pad +
+                            block * ROWS + 2 * tig;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    if (block * ROWS + nt * 8 < a.row_pad) {
+                        *reinterpret_cast<float2*>(sp + nt * 8) = make_float2(s[nt][0], s[nt][1]);
+                        *reinterpret_cast<float2*>(sp + 8 * a.row_pad + nt * 8) = make_float2(s[nt][2], s[nt][3]);
+                    }
+            }
+#pragma unroll
+            for (uint32_t gr = 0; gr < NG; ++gr)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) grow |= fabsf(vsz[h][gr].x) * inv_ref[gr] > 2.f;
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float mx = fmaxf(s[nt][x], s[nt][2 + x]);
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                        if (mx > m[nt][x]) {
+                            const float f = mx == INFINITY ? 0.f : ex2(m[nt][x] - mx);
+                            m[nt][x] = mx;
+                            l[nt][x] *= f;
+#pragma unroll
+                            for (uint32_t gr = 0; gr < NG; ++gr) {
+                                zs[nt][x][gr] *= f;
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    o[gr][j][nt][x] *= f;
+                                    o[gr][j][nt][2 + x] *= f;
+                                }
+                            }
+                        }
+                    }
+                // steps: a new power of two for groups whose steps have grown past twice the old one
+#pragma unroll
+                for (uint32_t gr = 0; gr < NG; ++gr) {
+                    float mx = 0.f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float st = fabsf(vsz[h][gr].x);
+                        if (t0 + 8 * h < (int)sh.vis && st < INFINITY) mx = fmaxf(mx, st);
+                    }
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                    if (mx * inv_ref[gr] > 2.f) {
+                        const float fresh = __uint_as_float((254u - (__float_as_uint(mx) >> 23)) << 23);
+                        const float f = fresh / inv_ref[gr];
+                        inv_ref[gr] = fresh;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) o[gr][j][nt][i] *= f;
+                    }
+                }
+            }
+            // probabilities
+            uint32_t pb[NG][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float p[4];
+                bool see[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int h = i >> 1, x = i & 1;
+                    see[i] = full || t0 + 8 * h < vis[nt][x];
+                    p[i] = see[i] ? ex2(s[nt][i] - (m[nt][x] == -INFINITY ? 0.f : m[nt][x])) : 0.f;
+                    l[nt][x] += p[i];
+                }
+#pragma unroll
+                for (uint32_t gr = 0; gr < NG; ++gr) {
+                    float pv[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int h = i >> 1, x = i & 1;
+                        // unseen tokens may hold anything, NaN too
+                        if (see[i]) zs[nt][x][gr] = fmaf(p[i], vsz[h][gr].y, zs[nt][x][gr]);
+                        pv[i] = see[i] ? p[i] * (vsz[h][gr].x * (inv_ref[gr] * 256.f)) : 0.f;
+                    }
+                    pb[gr][nt][0] = movmatrix(f2_to_pair<__half>(pv[0], pv[1]));
+                    pb[gr][nt][1] = movmatrix(f2_to_pair<__half>(pv[2], pv[3]));
+                }
+            }
+            // outputs
+#pragma unroll
+            for (uint32_t gr = 0; gr < NG; ++gr) {
+                uint32_t w[4];
+                ldsm4_trans(base + S::data + (tok * CPR + ((gr * 2 + (lane >> 4)) ^ sw)) * 16, w);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma_f16(o[gr][0][nt], nibbles<0>(w[0]), nibbles<0>(w[2]), nibbles<0>(w[1]), nibbles<0>(w[3]),
+                            pb[gr][nt][0], pb[gr][nt][1]);
+                    mma_f16(o[gr][1][nt], nibbles<1>(w[0]), nibbles<1>(w[2]), nibbles<1>(w[1]), nibbles<1>(w[3]),
+                            pb[gr][nt][0], pb[gr][nt][1]);
+                    mma_f16(o[gr][2][nt], nibbles<2>(w[0]), nibbles<2>(w[2]), nibbles<2>(w[1]), nibbles<2>(w[3]),
+                            pb[gr][nt][0], pb[gr][nt][1]);
+                    mma_f16(o[gr][3][nt], nibbles<3>(w[0]), nibbles<3>(w[2]), nibbles<3>(w[1]), nibbles<3>(w[3]),
+                            pb[gr][nt][0], pb[gr][nt][1]);
+                }
+            }
+        }
+        cp_async_wait<0>();
+
+        // the warps' sums become the block's
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+                    l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], off);
+#pragma unroll
+                    for (uint32_t gr = 0; gr < NG; ++gr)
+                        zs[nt][x][gr] += __shfl_xor_sync(0xffffffffu, zs[nt][x][gr], off);
+                }
+                if (g == 0) warp_ml[warp][nt * 8 + 2 * tig + x] = make_float2(m[nt][x], l[nt][x]);
+            }
+        __syncthreads();
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            if (warp == w) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t r = nt * 8 + 2 * tig + x;
+                        float top = -INFINITY;
+                        for (uint32_t v = 0; v < kWarps; ++v) top = fmaxf(top, warp_ml[v][r].x);
+                        // a warp that saw nothing has l = 0, or a NaN that has to stay
+                        const float f = m[nt][x] == -INFINITY ? l[nt][x] : m[nt][x] == top ? 1.f : ex2(m[nt][x] - top);
+#pragma unroll
+                        for (uint32_t gr = 0; gr < NG; ++gr)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                for (int cb = 0; cb < 2; ++cb) {
+                                    // 2^24 or 2^20 of the nibble, 2^-8 of p, the group's power of two
+                                    const float back = ((j & 1) ? 4096.f : 65536.f) / inv_ref[gr];
+                                    const float v = fmaf(o[gr][j][nt][cb * 2 + x], back, zs[nt][x][gr]) * f;
+                                    float* at = merge + r * S::pitch + gr * 64 + cb * 32 + 4 * g + j;
+                                    *at = w == 0 ? v : *at + v;
+                                }
+                    }
+            }
+            __syncthreads();
+        }
+        const uint32_t seg = unit == begin ? 0 : 1;
+        for (uint32_t r = warp; r < ROWS; r += kWarps) {
+            float top = -INFINITY, sum = 0.f;
+            for (uint32_t v = 0; v < kWarps; ++v) top = fmaxf(top, warp_ml[v][r].x);
+            for (uint32_t v = 0; v < kWarps; ++v) {
+                const float2 ml = warp_ml[v][r];
+                sum += ml.x == -INFINITY ? ml.y : ml.x == top ? ml.y : ml.y * ex2(ml.x - top);
+            }
+            const uint32_t row = block * ROWS + r;
+            if (whole) {
+                if (row < all_rows) {
+                    const uint32_t qi = row / a.group, qh = head * a.group + row % a.group;
+                    T* dst = static_cast<T*>(a.out) + ((uint64_t)(sh.start + qi) * a.heads + qh) * D;
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    for (uint32_t ch = lane * 2; ch < D; ch += 64)
+                        *reinterpret_cast<uint32_t*>(dst + ch) =
+                            f2_to_pair<T>(merge[r * S::pitch + ch] * inv, merge[r * S::pitch + ch + 1] * inv);
+                    if (a.scores && lane == 0)
+                        a.stats[((uint64_t)b * a.c.kv_heads + head) * a.row_pad + row] = make_float2(top, sum);
+                }
+            } else {
+                const uint64_t slot_at = (uint64_t)(2 * blockIdx.x + seg) * ROWS + r;
+                for (uint32_t ch = lane * 2; ch < D; ch += 64)
+                    *reinterpret_cast<float2*>(a.part_o + slot_at * D + ch) =
+                        make_float2(merge[r * S::pitch + ch], merge[r * S::pitch + ch + 1]);
+                if (lane == 0) a.part_ml[slot_at] = make_float2(top, sum);
+            }
+        }
+        __syncthreads();
+        unit += c1 - c0;
+    }
+}
+
+// Pieces of an item that blocks left in the workspace: slots of blocks `first` .. `last`.
+struct Pieces {
+    uint32_t first, last, first_slot;
+};
+__device__ __forceinline__ Pieces pieces_of(uint32_t unit0, uint32_t chunks, uint32_t total, uint32_t blocks)
+{
+    Pieces p;
+    p.first = (uint32_t)((((uint64_t)unit0 + 1) * blocks - 1) / total);
+    p.last = (uint32_t)((((uint64_t)unit0 + chunks) * blocks - 1) / total);
+    const uint32_t begin = (uint32_t)((uint64_t)total * p.first / blocks);
+    p.first_slot = 2 * p.first + (unit0 == begin ? 0 : 1);
+    return p;
+}
+__device__ __forceinline__ uint32_t piece_slot(const Pieces& p, uint32_t i) { return i == 0 ? p.first_slot : 2 * (p.first + i); }
+
+constexpr uint32_t kJoinThreads = 256;
+
+// Blocks below join_blocks: a warp a query row joins the pieces of its item.
+// The others: weights of an equal piece of all positions, from the scores.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, uint32_t rows_per_item, uint32_t grid1,
+                                                                uint32_t join_blocks)
+{
+    __shared__ float2 row_ml[kJoinThreads];
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const uint32_t total = a.unit_start[a.s.batch];
+    if (total == 0) return;
+    const uint32_t blocks = max(1u, min(grid1, total / kMinChunks));
+    if (blockIdx.x < join_blocks) {
+        const uint64_t id = (uint64_t)blockIdx.x * (kJoinThreads / 32) + warp;
+        if (id >= (uint64_t)a.s.tokens * a.heads) return;
+        const uint32_t token = (uint32_t)(id / a.heads), qh = (uint32_t)(id % a.heads);
+        uint32_t lo = 0, hi = a.s.batch;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (__ldg(a.s.token_start + mid + 1) <= (int32_t)token)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        if (lo == a.s.batch) return;
+        const SeqShape sh = seq_shape(a, lo, rows_per_item);
+        if (token < sh.start || token - sh.start >= min(sh.n, a.max_queries)) return;
+        const uint32_t head = qh / a.group, row = (token - sh.start) * a.group + qh % a.group;
+        const uint32_t block = row / rows_per_item, r = row % rows_per_item;
+        const Pieces p =
+            pieces_of(a.unit_start[lo] + (head * sh.blocks + block) * sh.chunks, sh.chunks, total, blocks);
+        if (p.first == p.last) return;  // written whole
+        const uint32_t count = p.last - p.first + 1;
+        float top = -INFINITY;
+        for (uint32_t i = lane; i < count; i += 32)
+            top = fmaxf(top, a.part_ml[(uint64_t)piece_slot(p, i) * rows_per_item + r].x);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        constexpr uint32_t V = D / 64;  // pairs of channels a lane holds
+        float2 o[V] = {};
+        float sum = 0.f;
+        for (uint32_t i0 = 0; i0 < count; i0 += 32) {
+            float f = 0.f, ls = 0.f;
+            if (i0 + lane < count) {
+                const float2 ml = a.part_ml[(uint64_t)piece_slot(p, i0 + lane) * rows_per_item + r];
+                f = ml.x == -INFINITY ? 0.f : ml.x == top ? 1.f : ex2(ml.x - top);
+                ls = ml.x == -INFINITY ? ml.y : ml.y * f;  // a NaN stays
+            }
+            const uint32_t here = min(32u, count - i0);
+#pragma unroll 4
+            for (uint32_t i = 0; i < here; ++i) {
+                const float fi = __shfl_sync(0xffffffffu, f, i);
+                sum += __shfl_sync(0xffffffffu, ls, i);
+                const float* src = a.part_o + ((uint64_t)piece_slot(p, i0 + i) * rows_per_item + r) * D;
+#pragma unroll
+                for (uint32_t v = 0; v < V; ++v) {
+                    const float2 x = *reinterpret_cast<const float2*>(src + v * 64 + lane * 2);
+                    o[v].x = fmaf(x.x, fi, o[v].x);
+                    o[v].y = fmaf(x.y, fi, o[v].y);
+                }
+            }
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        T* dst = static_cast<T*>(a.out) + ((uint64_t)token * a.heads + qh) * D;
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v)
+            *reinterpret_cast<uint32_t*>(dst + v * 64 + lane * 2) = f2_to_pair<T>(o[v].x * inv, o[v].y * inv);
+        return;
+    }
+    // weights: the line again, where each item of a sequence's first row block stands for its head
+    const uint32_t wb = blockIdx.x - join_blocks, wblocks = gridDim.x - join_blocks;
+    const uint32_t begin = (uint32_t)((uint64_t)total * wb / wblocks), end = (uint32_t)((uint64_t)total * (wb + 1) / wblocks);
+    uint32_t lo = 0, hi = a.s.batch;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (a.unit_start[mid] <= begin)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    uint32_t b = lo, unit = begin;
+    while (unit < end) {
+        while (a.unit_start[b + 1] <= unit) ++b;
+        const SeqShape sh = seq_shape(a, b, rows_per_item);
+        const uint32_t in_seq = unit - a.unit_start[b];
+        // a head's row blocks make one run of blocks * chunks units; its positions are spread over that run
+        const uint32_t run = sh.blocks * sh.chunks, head = in_seq / run, u0 = in_seq % run, u1 = min(run, u0 + (end - unit));
+        const uint32_t p0 = (uint32_t)((uint64_t)sh.vis * u0 / run), p1 = (uint32_t)((uint64_t)sh.vis * u1 / run);
+        const uint32_t all_rows = min(sh.n, a.max_queries) * a.group;
+        const float* scores = a.scores + ((uint64_t)b * a.c.kv_heads + head) * kv4_cap(a.c, a.s) * a.row_pad;
+        const int32_t* table = a.s.page_table + (uint64_t)b * a.s.max_pages;
+        for (uint32_t r0 = 0; r0 < all_rows; r0 += kJoinThreads) {
+            const uint32_t rows = min(kJoinThreads, all_rows - r0);
+            __syncthreads();
+            if (tid < rows) {
+                const uint32_t row = r0 + tid, block = row / rows_per_item, r = row % rows_per_item;
+                const Pieces p =
+                    pieces_of(a.unit_start[b] + (head * sh.blocks + block) * sh.chunks, sh.chunks, total, blocks);
+                float2 ml;
+                if (p.first == p.last) {
+                    ml = a.stats[((uint64_t)b * a.c.kv_heads + head) * a.row_pad + row];
+                } else {
+                    const uint32_t count = p.last - p.first + 1;
+                    ml = make_float2(-INFINITY, 0.f);
+                    for (uint32_t i = 0; i < count; ++i)
+                        ml.x = fmaxf(ml.x, a.part_ml[(uint64_t)piece_slot(p, i) * rows_per_item + r].x);
+                    for (uint32_t i = 0; i < count; ++i) {
+                        const float2 x = a.part_ml[(uint64_t)piece_slot(p, i) * rows_per_item + r];
+                        ml.y += x.x == -INFINITY ? x.y : x.x == ml.x ? x.y : x.y * ex2(x.x - ml.x);
+                    }
+                }
+                row_ml[tid] = make_float2(ml.x == -INFINITY ? 0.f : ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y);
+            }
+            __syncthreads();
+            for (uint32_t t = p0 + tid; t < p1; t += kJoinThreads) {
+                const int64_t at = kv4_row(a.c, table, t, head);
+                if (at < 0) continue;
+                const float* sp = scores + (uint64_t)t * a.row_pad + r0;
+                float sum = 0.f;
+                for (uint32_t r = 0; r < rows; r += 4) {  // row_pad is a multiple of 8
+                    const float4 s = *reinterpret_cast<const float4*>(sp + r);
+                    const float sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (r + i < rows) {
+                            const float2 ml = row_ml[r + i];
+                            sum = fmaf(sv[i] == -INFINITY ? 0.f : ex2(sv[i] - ml.x), ml.y, sum);
+                        }
+                }
+                a.c.weight[at] += sum;
+            }
+        }
+        unit += u1 - u0;
+    }
+}
+
+struct AttnWs {
+    size_t unit_start, stats, part_o, part_ml, scores, bytes;
+};
+uint32_t tiles_of(uint32_t rows, uint32_t dim) { return rows <= 8 ? 1 : rows <= 16 || dim == 256 ? 2 : 4; }
+
+AttnWs layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t max_queries, uint32_t max_len,
+              bool accumulate, uint32_t num_sms)
+{
+    const uint64_t rows = (uint64_t)(heads / kv_heads) * max_queries;
+    const uint64_t pad = (rows + 7) / 8 * 8;
+    const uint64_t slots = 2ull * num_sms * kMaxBlocks * 8 * tiles_of((uint32_t)std::min<uint64_t>(rows, 1u << 20), dim);
+    AttnWs w;
+    size_t at = 0;
+    auto take = [&](uint64_t n) {
+        const size_t here = at;
+        at += (n + 255) / 256 * 256;
+        return here;
+    };
+    w.unit_start = take((batch + 1ull) * 4);
+    w.part_ml = take(slots * 8);
+    w.part_o = take(slots * dim * 4);
+    w.stats = take(accumulate ? (uint64_t)batch * kv_heads * pad * 8 : 0);
+    w.scores = take(accumulate ? (uint64_t)batch * kv_heads * max_len * pad * 4 : 0);
+    w.bytes = at;
+    return w;
+}
+
+template <typename T, int D, int NT>
+cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t st)
+{
+    using S = AttnSmem<D, NT>;
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(kv4_attention_kernel<T, D, NT>, S::fixed + (kMaxAttnBatch + 1) * 4, done);
+    if (e != cudaSuccess) return e;
+    const uint32_t grid = num_sms * attn_blocks<D, NT>();
+    e = launch_pdl(kv4_attention_kernel<T, D, NT>, dim3(grid), dim3(kThreads), S::fixed + (p.s.batch + 1) * 4, st, p);
+    if (e != cudaSuccess) return e;
+    const uint64_t rows = (uint64_t)p.s.tokens * p.heads;
+    const uint32_t join = (uint32_t)((rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+    return launch_pdl(kv4_join_kernel<T, D>, dim3(join + (accumulate ? 4 * num_sms : 0)), dim3(kJoinThreads), 0, st, p,
+                      8u * NT, grid, join);
 }
 
 template <typename T, int D>
-cudaError_t run(const Kv4Attention& a, void* workspace, cudaStream_t st)
+cudaError_t run_dim(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t st)
 {
-    const KvAttnParams p{a.cache, a.seqs, a.heads, a.max_queries, a.q_stride, a.scale};
-    float2* stats = a.accumulate ? static_cast<float2*>(workspace) : nullptr;
-    cudaError_t e = launch_pdl(kv4_rows_kernel<T, D>, dim3(a.max_queries * a.heads, a.seqs.batch), dim3(32), 0, st, p,
-                               static_cast<const T*>(a.q), static_cast<T*>(a.out), stats);
-    if (e != cudaSuccess || !a.accumulate) return e;
-    const uint32_t cap = a.seqs.max_pages * a.cache.page_size;
-    return launch_pdl(kv4_weights_kernel<T, D>, dim3((cap + 7) / 8, a.cache.kv_heads, a.seqs.batch), dim3(256), 0, st,
-                      p, static_cast<const T*>(a.q), static_cast<const float2*>(stats));
+    switch (tiles_of(std::min(p.group * p.max_queries, 1u << 20), D)) {
+        case 1: return run<T, D, 1>(p, accumulate, num_sms, st);
+        case 2: return run<T, D, 2>(p, accumulate, num_sms, st);
+        default:
+            if constexpr (D < 256) return run<T, D, 4>(p, accumulate, num_sms, st);
+            return cudaErrorInvalidValue;
+    }
 }
 
 }  // namespace
 
-size_t kv4_attention_workspace(uint32_t batch, uint32_t heads, uint32_t, uint32_t, uint32_t max_queries, uint32_t,
-                               bool accumulate, uint32_t)
+size_t kv4_attention_workspace(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                               uint32_t max_queries, uint32_t max_len, bool accumulate, uint32_t num_sms)
 {
-    return accumulate ? (size_t)batch * heads * max_queries * sizeof(float2) : 0;
+    return layout(batch, heads, kv_heads, head_dim, max_queries, max_len, accumulate, num_sms).bytes;
 }
 
-cudaError_t launch_kv4_attention(const Kv4Attention& a, void* workspace, uint32_t, cudaStream_t st)
+cudaError_t launch_kv4_attention(const Kv4Attention& a, void* workspace, uint32_t num_sms, cudaStream_t st)
 {
+    const uint32_t cap = a.seqs.max_pages * a.cache.page_size;
+    const AttnWs w = layout(a.seqs.batch, a.heads, a.cache.kv_heads, a.cache.head_dim, a.max_queries, cap, a.accumulate,
+                            num_sms);
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    AttnParams p{};
+    p.c = a.cache;
+    p.s = a.seqs;
+    p.q = a.q;
+    p.out = a.out;
+    p.q_stride = a.q_stride;
+    p.heads = a.heads;
+    p.group = a.heads / a.cache.kv_heads;
+    p.max_queries = a.max_queries;
+    p.row_pad = (p.group * a.max_queries + 7) / 8 * 8;
+    p.scale_log2 = a.scale * kLog2e;
+    p.unit_start = reinterpret_cast<uint32_t*>(base + w.unit_start);
+    p.stats = reinterpret_cast<float2*>(base + w.stats);
+    p.part_o = reinterpret_cast<float*>(base + w.part_o);
+    p.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
+    p.scores = a.accumulate ? reinterpret_cast<float*>(base + w.scores) : nullptr;
     switch (a.cache.head_dim) {
-        case 64: return a.bf16 ? run<__nv_bfloat16, 64>(a, workspace, st) : run<__half, 64>(a, workspace, st);
-        case 128: return a.bf16 ? run<__nv_bfloat16, 128>(a, workspace, st) : run<__half, 128>(a, workspace, st);
-        default: return a.bf16 ? run<__nv_bfloat16, 256>(a, workspace, st) : run<__half, 256>(a, workspace, st);
+        case 64:
+            return a.bf16 ? run_dim<__nv_bfloat16, 64>(p, a.accumulate, num_sms, st)
+                          : run_dim<__half, 64>(p, a.accumulate, num_sms, st);
+        case 128:
+            return a.bf16 ? run_dim<__nv_bfloat16, 128>(p, a.accumulate, num_sms, st)
+                          : run_dim<__half, 128>(p, a.accumulate, num_sms, st);
+        default:
+            return a.bf16 ? run_dim<__nv_bfloat16, 256>(p, a.accumulate, num_sms, st)
+                          : run_dim<__half, 256>(p, a.accumulate, num_sms, st);
     }
 }
 
