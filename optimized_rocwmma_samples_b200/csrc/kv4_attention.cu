@@ -35,6 +35,7 @@
 #include "kv4.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b2sq {
 
@@ -123,8 +124,21 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 __device__ __forceinline__ float ex2(float x)
 {
     float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+template <uint32_t N>
+__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N])
+{
+    if constexpr (N == 1) {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
 }
 // Words j of four nibbles each become fp16 subnormals: nibbles 0 and 2 stand for q 2^-24, 1 and 3 for q 2^-20.
 template <int J>
@@ -152,7 +166,9 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_kernel(AttnParams a)
 {
     using S = AttnSmem<D, NT>;
-    constexpr uint32_t NG = D / 64, CPR = D / 32, ROWS = 8 * NT, STAGES = S::stages;
+    constexpr uint32_t NG = D / 64, CPR = D / 32, ROWS = 8 * NT, STAGES = S::stages, SC = S::scales / 16;
+    // fp16 results want more bits of the probabilities than fp16 has: a second operand holds what the first leaves
+    constexpr bool SPLIT = std::is_same<T, __half>::value;
     extern __shared__ __align__(16) uint8_t at_smem[];
     uint8_t* ring = at_smem;
     __half* q_frag = reinterpret_cast<__half*>(at_smem + S::ring);  // [NT][NG][2][32 lanes] x 16 bytes
@@ -204,6 +220,7 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
     const uint32_t begin = (uint32_t)((uint64_t)total * blockIdx.x / blocks);
     const uint32_t end = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / blocks);
 
+    const uint32_t page_chunks = a.c.page_size / kChunk;
     const uint32_t ring_base = smem_u32(ring) + warp * STAGES * S::stage;
     uint32_t unit = begin;
     uint32_t b = 0;
@@ -229,35 +246,54 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
         const int32_t* table = a.s.page_table + (uint64_t)b * a.s.max_pages;
         const uint32_t all_rows = min(sh.n, a.max_queries) * a.group;
 
-        // stage loads: chunk c of the item into ring slot `slot` of this warp
-        auto page_row = [&](uint32_t c) -> int64_t {  // cache row of the chunk's first token, -1 if it has none
-            return c * kChunk < sh.vis ? kv4_row(a.c, table, c * kChunk, head) : -1;
-        };
-        auto load = [&](uint32_t c, uint32_t slot) {
-            const int64_t row = c < c1 ? page_row(c) : -1;
-            if (row >= 0) {
-                const uint32_t dst = ring_base + slot * S::stage;
-                const uint8_t* ks = a.c.k + row * (D / 2);
-                const uint8_t* vs = a.c.v + row * (D / 2);
-#pragma unroll
-                for (uint32_t i = 0; i < S::data / 512; ++i) {
-                    const uint32_t u = i * 32 + lane, r = u / CPR, ch = u % CPR;
-                    const uint32_t to = r * CPR + (ch ^ ((r / (8 / CPR)) & (CPR - 1)));
-                    cp_async16(dst + to * 16, ks + u * 16);
-                    cp_async16(dst + S::data + to * 16, vs + u * 16);
+        // this warp's chunks: an even share of the block's, one after another
+        const uint32_t wc0 = c0 + (uint32_t)((uint64_t)(c1 - c0) * warp / kWarps);
+        const uint32_t wc1 = c0 + (uint32_t)((uint64_t)(c1 - c0) * (warp + 1) / kWarps);
+        // loads run ahead of the computation by STAGES - 1 chunks, and page ids by one page
+        uint32_t lc = wc0, lslot = 0, left = 0;  // next chunk, its ring slot, chunks left on its page
+        uint32_t valid = 0;                      // bit i: the chunk loaded i loads ago has a page
+        uint32_t page_at = wc0 / page_chunks;
+        const uint32_t page_end = sh.vis == 0 ? 0 : (sh.vis - 1) / a.c.page_size + 1;
+        int32_t page = page_at < page_end ? __ldg(table + page_at) : -1, next_page = page;
+        const uint8_t *kp = nullptr, *vp = nullptr, *sp = nullptr;
+        auto load = [&]() {
+            valid <<= 1;
+            if (lc < wc1) {
+                if (left == 0) {
+                    const uint32_t skip = lc == wc0 ? wc0 % page_chunks : 0;
+                    left = page_chunks - skip;
+                    page = next_page;
+                    ++page_at;
+                    next_page = page_at < page_end ? __ldg(table + page_at) : -1;
+                    const int64_t row = ((int64_t)page * a.c.kv_heads + head) * a.c.page_size + skip * kChunk;
+                    kp = a.c.k + row * (D / 2) + lane * 16;
+                    vp = a.c.v + row * (D / 2) + lane * 16;
+                    sp = static_cast<const uint8_t*>(lane < SC ? a.c.k_scale : a.c.v_scale) + row * (NG * 4) +
+                         (lane < SC ? lane : lane - SC) * 16;
                 }
-                constexpr uint32_t SC = S::scales / 16;
-                if (lane < SC)
-                    cp_async16(dst + 2 * S::data + lane * 16,
-                               static_cast<const uint8_t*>(a.c.k_scale) + row * (NG * 4) + lane * 16);
-                else if (lane < 2 * SC)
-                    cp_async16(dst + 2 * S::data + lane * 16,
-                               static_cast<const uint8_t*>(a.c.v_scale) + row * (NG * 4) + (lane - SC) * 16);
+                if ((uint32_t)page < a.c.pages) {
+                    valid |= 1;
+                    const uint32_t dst = ring_base + lslot * S::stage;
+#pragma unroll
+                    for (uint32_t i = 0; i < S::data / 512; ++i) {
+                        const uint32_t u = i * 32 + lane, r = u / CPR, ch = u % CPR;
+                        const uint32_t to = r * CPR + (ch ^ ((r / (8 / CPR)) & (CPR - 1)));
+                        cp_async16(dst + to * 16, kp + i * 512);
+                        cp_async16(dst + S::data + to * 16, vp + i * 512);
+                    }
+                    if (lane < 2 * SC) cp_async16(dst + 2 * S::data + lane * 16, sp);
+                }
+                kp += S::data;
+                vp += S::data;
+                sp += S::scales;
+                --left;
+                ++lc;
             }
             cp_async_commit();
+            if (++lslot == STAGES) lslot = 0;
         };
 #pragma unroll
-        for (uint32_t i = 0; i < STAGES - 1; ++i) load(c0 + warp + i * kWarps, i);
+        for (uint32_t i = 0; i < STAGES - 1; ++i) load();
 
         // the item's query rows, as operands
         for (uint32_t r = warp; r < ROWS; r += kWarps) {
@@ -314,54 +350,38 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
         for (uint32_t r = 0; r < ROWS; ++r) least = min(least, row_vis[r]);
 
         float o[NG][4][NT][4] = {};
-        float m[NT][2], l[NT][2], zs[NT][2][NG];
-        float inv_ref[NG];  // 1 / the power of two that steps of a group are taken over
+        float m[NT][2], l[NT][2], zs[NT][2][NG];  // m: 0 until the row has seen a token
+        float ref[NG];                            // 2^8 / the power of two that a group's steps are taken over
+        uint32_t seen = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                m[nt][x] = -INFINITY;
+                m[nt][x] = 0.f;
                 l[nt][x] = 0.f;
 #pragma unroll
                 for (uint32_t gr = 0; gr < NG; ++gr) zs[nt][x][gr] = 0.f;
             }
 #pragma unroll
-        for (uint32_t gr = 0; gr < NG; ++gr) inv_ref[gr] = 16777216.f;
+        for (uint32_t gr = 0; gr < NG; ++gr) ref[gr] = 4294967296.f;
 
-        uint32_t slot = 0;
-        for (uint32_t c = c0 + warp; c < c1; c += kWarps) {
-            {
-                uint32_t next = slot + STAGES - 1;
-                if (next >= STAGES) next -= STAGES;
-                __syncwarp();
-                load(c + (STAGES - 1) * kWarps, next);
-            }
-            cp_async_wait<STAGES - 1>();
-            __syncwarp();
-            const uint32_t base = ring_base + slot * S::stage;
+        const uint32_t tok = (lane & 7) + ((lane >> 3) & 1) * 8;  // ldmatrix row of this lane
+        const uint32_t sw = (tok / (8 / CPR)) & (CPR - 1);
+        const uint32_t mat = ring_base + tok * CPR * 16;
+        float* score_at = a.scores ? a.scores + (((uint64_t)b * a.c.kv_heads + head) * kv4_cap(a.c, a.s) + wc0 * kChunk + g) * a.row_pad + block * ROWS + 2 * tig
+                                   : nullptr;
+
+        // one chunk of 16 tokens; FULL: every row sees all of them
+        auto step = [&](uint32_t c, uint32_t slot, auto full_tag) {
+            constexpr bool FULL = decltype(full_tag)::value;
+            const uint32_t base = mat + slot * S::stage;
             const uint8_t* stage = ring + (warp * STAGES + slot) * S::stage;
-            if (++slot == STAGES) slot = 0;
-            if (page_row(c) < 0) {  // no such page: nothing of this chunk is seen
-                if (a.scores) {
-                    for (uint32_t i = lane; i < kChunk * ROWS; i += 32) {
-                        const uint32_t row = block * ROWS + i % ROWS;
-                        const uint64_t t = c * kChunk + i / ROWS;
-                        if (row < a.row_pad && t < kv4_cap(a.c, a.s))
-                            a.scores[(((uint64_t)b * a.c.kv_heads + head) * kv4_cap(a.c, a.s) + t) * a.row_pad + row] =
-                                -INFINITY;
-                    }
-                }
-                continue;
-            }
-
-            // scores of 16 tokens
+            // scores
             float acc[NG][NT][4] = {};
-            const uint32_t tok = (lane & 7) + ((lane >> 3) & 1) * 8;  // ldmatrix row of this lane
-            const uint32_t sw = (tok / (8 / CPR)) & (CPR - 1);
 #pragma unroll
             for (uint32_t gr = 0; gr < NG; ++gr) {
                 uint32_t w[4];
-                ldsm4(base + (tok * CPR + ((gr * 2 + (lane >> 4)) ^ sw)) * 16, w);
+                ldsm4(base + ((gr * 2 + (lane >> 4)) ^ sw) * 16, w);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const uint4* qf = reinterpret_cast<const uint4*>(q_frag) + ((nt * NG + gr) * 2) * 32 + lane;
@@ -373,51 +393,60 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                 }
             }
             // thread: tokens g and g + 8, rows 2 tig and 2 tig + 1 of every eight
-            float2 ksz[2][NG], vsz[2][NG];
+            float2 ksz[2][NG];
+            float vs[2][NG], vz[2][NG];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const __half2* kp = reinterpret_cast<const __half2*>(stage + 2 * S::data) + (g + 8 * h) * NG;
-                const __half2* vp = reinterpret_cast<const __half2*>(stage + 2 * S::data + S::scales) + (g + 8 * h) * NG;
+                uint32_t kw[NG], vw[NG];
+                lds_words<NG>(stage + 2 * S::data + (g + 8 * h) * NG * 4, kw);
+                lds_words<NG>(stage + 2 * S::data + S::scales + (g + 8 * h) * NG * 4, vw);
 #pragma unroll
                 for (uint32_t gr = 0; gr < NG; ++gr) {
-                    ksz[h][gr] = __half22float2(kp[gr]);
-                    vsz[h][gr] = __half22float2(vp[gr]);
+                    ksz[h][gr] = pair_to_f2<__half>(kw[gr]);
+                    const float2 v = pair_to_f2<__half>(vw[gr]);
+                    vs[h][gr] = v.x;
+                    vz[h][gr] = v.y;
                 }
             }
             const int t0 = (int)(c * kChunk + g);
-            const bool full = (int)(c * kChunk + kChunk) <= least;
-            float s[NT][4];
-            bool grow = false;
+            bool see[NT][4];
+            float s[NT][4];  // score - m
+            float top = -INFINITY, step_top = 0.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int h = i >> 1, x = i & 1;
-                    float dot = 0.f, off = 0.f;
+                    float dot = acc[0][nt][i] * ksz[h][0].x, off = fmaf(qsum[nt][x][0], ksz[h][0].y, -m[nt][x]);
 #pragma unroll
-                    for (uint32_t gr = 0; gr < NG; ++gr) {
+                    for (uint32_t gr = 1; gr < NG; ++gr) {
                         dot = fmaf(acc[gr][nt][i], ksz[h][gr].x, dot);
                         off = fmaf(qsum[nt][x][gr], ksz[h][gr].y, off);
                     }
-                    const float v = fmaf(dot, mul[nt][x], off);
-                    s[nt][i] = full || t0 + 8 * h < vis[nt][x] ? v : -INFINITY;
-                    grow |= s[nt][i] > m[nt][x] + 6.f;  // p may reach 2^6 before the maximum is moved
+                    see[nt][i] = FULL || t0 + 8 * h < vis[nt][x];
+                    s[nt][i] = see[nt][i] ? fmaf(dot, mul[nt][x], off) : -INFINITY;
+                    top = fmaxf(top, s[nt][i]);
                 }
-            if (a.scores) {
-                float* sp = a.scores + ((((uint64_t)b * a.c.kv_heads + head) * kv4_cap(a.c, a.s)) + t0) * a.row_pad +
-                            block * ROWS + 2 * tig;
+            if (score_at) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                     if (block * ROWS + nt * 8 < a.row_pad) {
-                        *reinterpret_cast<float2*>(sp + nt * 8) = make_float2(s[nt][0], s[nt][1]);
-                        *reinterpret_cast<float2*>(sp + 8 * a.row_pad + nt * 8) = make_float2(s[nt][2], s[nt][3]);
+                        *reinterpret_cast<float2*>(score_at + nt * 8) = make_float2(s[nt][0] + m[nt][0], s[nt][1] + m[nt][1]);
+                        *reinterpret_cast<float2*>(score_at + 8 * a.row_pad + nt * 8) =
+                            make_float2(s[nt][2] + m[nt][0], s[nt][3] + m[nt][1]);
                     }
             }
+            // the steps over the group's power of two (unseen tokens may hold anything: only read where see[])
+            float pw[2][NG];
 #pragma unroll
             for (uint32_t gr = 0; gr < NG; ++gr)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) grow |= fabsf(vsz[h][gr].x) * inv_ref[gr] > 2.f;
-            if (__any_sync(0xffffffffu, grow)) {
+                for (int h = 0; h < 2; ++h) {
+                    pw[h][gr] = vs[h][gr] * ref[gr];
+                    step_top = fmaxf(step_top, fabsf(pw[h][gr]));
+                }
+            // p may reach 2^6 and a step twice its power of two before the references are moved
+            if (__any_sync(0xffffffffu, top > 6.f || step_top > 512.f || seen != (1u << (2 * NT)) - 1)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -425,9 +454,13 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                         float mx = fmaxf(s[nt][x], s[nt][2 + x]);
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                        if (mx > m[nt][x]) {
-                            const float f = mx == INFINITY ? 0.f : ex2(m[nt][x] - mx);
-                            m[nt][x] = mx;
+                        const uint32_t bit = 1u << (nt * 2 + x);
+                        if (mx > 0.f || (!(seen & bit) && mx > -INFINITY)) {
+                            const float f = (seen & bit) ? ex2(-mx) : 0.f;
+                            seen |= bit;
+                            m[nt][x] += mx;
+                            s[nt][x] -= mx;
+                            s[nt][2 + x] -= mx;
                             l[nt][x] *= f;
 #pragma unroll
                             for (uint32_t gr = 0; gr < NG; ++gr) {
@@ -440,21 +473,22 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                             }
                         }
                     }
-                // steps: a new power of two for groups whose steps have grown past twice the old one
 #pragma unroll
                 for (uint32_t gr = 0; gr < NG; ++gr) {
                     float mx = 0.f;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float st = fabsf(vsz[h][gr].x);
+                        const float st = fabsf(vs[h][gr]);
                         if (t0 + 8 * h < (int)sh.vis && st < INFINITY) mx = fmaxf(mx, st);
                     }
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                    if (mx * inv_ref[gr] > 2.f) {
-                        const float fresh = __uint_as_float((254u - (__float_as_uint(mx) >> 23)) << 23);
-                        const float f = fresh / inv_ref[gr];
-                        inv_ref[gr] = fresh;
+                    if (mx * ref[gr] > 512.f) {
+                        const float fresh = __uint_as_float((262u - (__float_as_uint(mx) >> 23)) << 23);
+                        const float f = fresh / ref[gr];
+                        ref[gr] = fresh;
+                        pw[0][gr] = vs[0][gr] * fresh;
+                        pw[1][gr] = vs[1][gr] * fresh;
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -466,16 +500,14 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
             }
             // probabilities
             uint32_t pb[NG][NT][2];
+            [[maybe_unused]] uint32_t pb2[SPLIT ? NG : 1][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float p[4];
-                bool see[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int h = i >> 1, x = i & 1;
-                    see[i] = full || t0 + 8 * h < vis[nt][x];
-                    p[i] = see[i] ? ex2(s[nt][i] - (m[nt][x] == -INFINITY ? 0.f : m[nt][x])) : 0.f;
-                    l[nt][x] += p[i];
+                    p[i] = ex2(s[nt][i]);  // 0 where unseen
+                    l[nt][i & 1] += p[i];
                 }
 #pragma unroll
                 for (uint32_t gr = 0; gr < NG; ++gr) {
@@ -483,31 +515,59 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int h = i >> 1, x = i & 1;
-                        // unseen tokens may hold anything, NaN too
-                        if (see[i]) zs[nt][x][gr] = fmaf(p[i], vsz[h][gr].y, zs[nt][x][gr]);
-                        pv[i] = see[i] ? p[i] * (vsz[h][gr].x * (inv_ref[gr] * 256.f)) : 0.f;
+                        if (FULL || see[nt][i]) zs[nt][x][gr] = fmaf(p[i], vz[h][gr], zs[nt][x][gr]);
+                        pv[i] = FULL || see[nt][i] ? p[i] * pw[h][gr] : 0.f;
                     }
-                    pb[gr][nt][0] = movmatrix(f2_to_pair<__half>(pv[0], pv[1]));
-                    pb[gr][nt][1] = movmatrix(f2_to_pair<__half>(pv[2], pv[3]));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t w = f2_to_pair<__half>(pv[2 * h], pv[2 * h + 1]);
+                        pb[gr][nt][h] = movmatrix(w);
+                        if constexpr (SPLIT) {
+                            const float2 r = pair_to_f2<__half>(w);
+                            pb2[gr][nt][h] = movmatrix(f2_to_pair<__half>(pv[2 * h] - r.x, pv[2 * h + 1] - r.y));
+                        }
+                    }
                 }
             }
             // outputs
 #pragma unroll
             for (uint32_t gr = 0; gr < NG; ++gr) {
                 uint32_t w[4];
-                ldsm4_trans(base + S::data + (tok * CPR + ((gr * 2 + (lane >> 4)) ^ sw)) * 16, w);
+                ldsm4_trans(base + S::data + ((gr * 2 + (lane >> 4)) ^ sw) * 16, w);
+                auto word = [&](auto j_tag) {
+                    constexpr int J = decltype(j_tag)::value;
+                    const uint32_t a0 = nibbles<J>(w[0]), a1 = nibbles<J>(w[2]), a2 = nibbles<J>(w[1]), a3 = nibbles<J>(w[3]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma_f16(o[gr][0][nt], nibbles<0>(w[0]), nibbles<0>(w[2]), nibbles<0>(w[1]), nibbles<0>(w[3]),
-                            pb[gr][nt][0], pb[gr][nt][1]);
-                    mma_f16(o[gr][1][nt], nibbles<1>(w[0]), nibbles<1>(w[2]), nibbles<1>(w[1]), nibbles<1>(w[3]),
-                            pb[gr][nt][0], pb[gr][nt][1]);
-                    mma_f16(o[gr][2][nt], nibbles<2>(w[0]), nibbles<2>(w[2]), nibbles<2>(w[1]), nibbles<2>(w[3]),
-                            pb[gr][nt][0], pb[gr][nt][1]);
-                    mma_f16(o[gr][3][nt], nibbles<3>(w[0]), nibbles<3>(w[2]), nibbles<3>(w[1]), nibbles<3>(w[3]),
-                            pb[gr][nt][0], pb[gr][nt][1]);
-                }
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_f16(o[gr][J][nt], a0, a1, a2, a3, pb[gr][nt][0], pb[gr][nt][1]);
+                        if constexpr (SPLIT) mma_f16(o[gr][J][nt], a0, a1, a2, a3, pb2[gr][nt][0], pb2[gr][nt][1]);
+                    }
+                };
+                word(std::integral_constant<int, 0>());
+                word(std::integral_constant<int, 1>());
+                word(std::integral_constant<int, 2>());
+                word(std::integral_constant<int, 3>());
             }
+        };
+
+        uint32_t slot = 0;
+        for (uint32_t c = wc0; c < wc1; ++c) {
+            __syncwarp();
+            load();
+            cp_async_wait<STAGES - 1>();
+            __syncwarp();
+            if ((valid >> (STAGES - 1)) & 1) {
+                if ((int)(c * kChunk + kChunk) <= least)
+                    step(c, slot, std::true_type());
+                else
+                    step(c, slot, std::false_type());
+            } else if (score_at) {  // no such page: nothing of this chunk is seen
+                const uint32_t rows = min(ROWS, a.row_pad - block * ROWS);
+                for (uint32_t i = lane; i < kChunk * rows && c * kChunk < sh.vis; i += 32)
+                    score_at[((int64_t)(i / rows) - g) * a.row_pad + (int64_t)(i % rows) - 2 * tig] = -INFINITY;
+            }
+            if (score_at) score_at += kChunk * a.row_pad;
+            if (++slot == STAGES) slot = 0;
         }
         cp_async_wait<0>();
 
@@ -523,6 +583,7 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                     for (uint32_t gr = 0; gr < NG; ++gr)
                         zs[nt][x][gr] += __shfl_xor_sync(0xffffffffu, zs[nt][x][gr], off);
                 }
+                if (!((seen >> (nt * 2 + x)) & 1)) m[nt][x] = -INFINITY;
                 if (g == 0) warp_ml[warp][nt * 8 + 2 * tig + x] = make_float2(m[nt][x], l[nt][x]);
             }
         __syncthreads();
@@ -543,8 +604,8 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                             for (int j = 0; j < 4; ++j)
 #pragma unroll
                                 for (int cb = 0; cb < 2; ++cb) {
-                                    // 2^24 or 2^20 of the nibble, 2^-8 of p, the group's power of two
-                                    const float back = ((j & 1) ? 4096.f : 65536.f) / inv_ref[gr];
+                                    // 2^24 or 2^20 of the nibble, the group's power of two
+                                    const float back = ((j & 1) ? 1048576.f : 16777216.f) / ref[gr];
                                     const float v = fmaf(o[gr][j][nt][cb * 2 + x], back, zs[nt][x][gr]) * f;
                                     float* at = merge + r * S::pitch + gr * 64 + cb * 32 + 4 * g + j;
                                     *at = w == 0 ? v : *at + v;
