@@ -53,9 +53,8 @@ struct AttnParams {
     const void* q;
     void* out;
     uint64_t q_stride;
-    uint32_t heads, group, max_queries, row_pad;  // row_pad: group * max_queries rounded up to 8
+    uint32_t heads, group, max_queries, row_pad;  // row_pad: group * max_queries rounded up to 4
     float scale_log2;
-    uint32_t* unit_start;  // [batch + 1] first chunk of each sequence on the line
     float2* stats;         // [batch * kv_heads][row_pad] (max, sum) of items that one block did whole
     float* part_o;         // [2 * blocks][8 NT][D]
     float2* part_ml;       // [2 * blocks][8 NT]
@@ -79,9 +78,9 @@ struct AttnSmem {
     static constexpr uint32_t stages = D == 64 ? 6 : D == 128 ? 4 : 3;
     static constexpr uint32_t ring = kWarps * stages * stage;
     static constexpr uint32_t q = rows * D * 2;
-    static constexpr uint32_t pitch = D + 2;
-    static constexpr uint32_t merge = rows * pitch * 4;
-    static constexpr uint32_t fixed = ring + q + merge;
+    static constexpr uint32_t pitch = D + 2;  // of a row in the join of the warps, which uses the drained ring
+    static_assert(kWarps * 8 * pitch * 4 <= ring, "ring too small for the join");
+    static constexpr uint32_t fixed = ring + q;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src)
@@ -120,6 +119,13 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ float ex2(float x)
 {
@@ -162,6 +168,69 @@ __device__ __forceinline__ SeqShape seq_shape(const AttnParams& a, uint32_t b, u
     return s;
 }
 
+// Equal pieces of `total` chunks for `blocks` blocks: the first `rest` get one more.
+struct Split {
+    uint32_t blocks, each, rest;
+    __device__ __forceinline__ Split(uint32_t total, uint32_t grid)
+    {
+        blocks = max(1u, min(grid, total / kMinChunks));
+        each = total / blocks;
+        rest = total - each * blocks;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * each + min(i, rest); }
+    __device__ __forceinline__ uint32_t block_of(uint32_t unit) const
+    {
+        const uint32_t big = rest * (each + 1);
+        return unit < big ? unit / (each + 1) : rest + (unit - big) / each;
+    }
+};
+
+// First chunk of every sequence on the line, into shared memory [batch + 1]; all threads of the block.
+template <uint32_t THREADS>
+__device__ __forceinline__ void lay_out(const AttnParams& a, uint32_t rows, uint32_t* ustart, uint32_t* part)
+{
+    const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    uint32_t carry = 0;
+    for (uint32_t base = 0; base < a.s.batch; base += THREADS) {
+        const uint32_t b = base + tid;
+        uint32_t v = 0;
+        if (b < a.s.batch) {
+            const SeqShape sh = seq_shape(a, b, rows);
+            v = sh.chunks * sh.blocks * a.c.kv_heads;
+        }
+        uint32_t incl = v;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= (uint32_t)off) incl += t;
+        }
+        if (lane == 31) part[warp] = incl;
+        __syncthreads();
+        uint32_t before = carry;
+        for (uint32_t w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) before += part[w];
+            carry += part[w];
+        }
+        if (b < a.s.batch) ustart[b] = before + incl - v;
+        __syncthreads();
+    }
+    if (tid == 0) ustart[a.s.batch] = carry;
+    __syncthreads();
+}
+// The last sequence that starts at or before `unit` (empty ones share their start with the next).
+__device__ __forceinline__ uint32_t seq_of(const uint32_t* ustart, uint32_t batch, uint32_t unit)
+{
+    uint32_t lo = 0, hi = batch;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (ustart[mid] <= unit)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_kernel(AttnParams a)
 {
@@ -172,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
     extern __shared__ __align__(16) uint8_t at_smem[];
     uint8_t* ring = at_smem;
     __half* q_frag = reinterpret_cast<__half*>(at_smem + S::ring);  // [NT][NG][2][32 lanes] x 16 bytes
-    float* merge = reinterpret_cast<float*>(at_smem + S::ring + S::q);
+    float* merge = reinterpret_cast<float*>(ring);  // [kWarps][8][pitch]
     uint32_t* ustart = reinterpret_cast<uint32_t*>(at_smem + S::fixed);  // [batch + 1]
     __shared__ float row_mul[ROWS], row_sum[ROWS][NG];
     __shared__ int row_vis[ROWS];
@@ -183,58 +252,16 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
     griddep_wait();
     griddep_launch_dependents();
 
-    // the line of chunks: first chunk of every sequence
-    {
-        uint32_t carry = 0;
-        for (uint32_t base = 0; base < a.s.batch; base += kThreads) {
-            const uint32_t b = base + tid;
-            uint32_t v = 0;
-            if (b < a.s.batch) {
-                const SeqShape sh = seq_shape(a, b, ROWS);
-                v = sh.chunks * sh.blocks * a.c.kv_heads;
-            }
-            uint32_t incl = v;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const uint32_t t = __shfl_up_sync(0xffffffffu, incl, off);
-                if (lane >= (uint32_t)off) incl += t;
-            }
-            if (lane == 31) scan_part[warp] = incl;
-            __syncthreads();
-            uint32_t before = carry;
-            for (uint32_t w = 0; w < kWarps; ++w) {
-                if (w < warp) before += scan_part[w];
-                carry += scan_part[w];
-            }
-            if (b < a.s.batch) ustart[b] = before + incl - v;
-            __syncthreads();
-        }
-        if (tid == 0) ustart[a.s.batch] = carry;
-        __syncthreads();
-        if (blockIdx.x == 0)
-            for (uint32_t b = tid; b <= a.s.batch; b += kThreads) a.unit_start[b] = ustart[b];
-    }
+    lay_out<kThreads>(a, ROWS, ustart, scan_part);
     const uint32_t total = ustart[a.s.batch];
-    const uint32_t blocks = max(1u, min(gridDim.x, total / kMinChunks));
-    if (blockIdx.x >= blocks || total == 0) return;
-    const uint32_t begin = (uint32_t)((uint64_t)total * blockIdx.x / blocks);
-    const uint32_t end = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / blocks);
+    const Split split(total, gridDim.x);
+    if (blockIdx.x >= split.blocks || total == 0) return;
+    const uint32_t begin = split.begin(blockIdx.x), end = split.begin(blockIdx.x + 1);
 
     const uint32_t page_chunks = a.c.page_size / kChunk;
     const uint32_t ring_base = smem_u32(ring) + warp * STAGES * S::stage;
     uint32_t unit = begin;
-    uint32_t b = 0;
-    {  // the last sequence that starts at or before `unit` (empty ones share their start with the next)
-        uint32_t lo = 0, hi = a.s.batch;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (ustart[mid] <= unit)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        b = lo;
-    }
+    uint32_t b = seq_of(ustart, a.s.batch, unit);
     while (unit < end) {
         while (ustart[b + 1] <= unit) ++b;
         const SeqShape sh = seq_shape(a, b, ROWS);
@@ -377,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
             const uint32_t base = mat + slot * S::stage;
             const uint8_t* stage = ring + (warp * STAGES + slot) * S::stage;
             // scores
-            float acc[NG][NT][4] = {};
+            float acc[NG][NT][4];
 #pragma unroll
             for (uint32_t gr = 0; gr < NG; ++gr) {
                 uint32_t w[4];
@@ -386,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                 for (int nt = 0; nt < NT; ++nt) {
                     const uint4* qf = reinterpret_cast<const uint4*>(q_frag) + ((nt * NG + gr) * 2) * 32 + lane;
                     const uint4 q0 = qf[0], q1 = qf[32];
-                    mma_f16(acc[gr][nt], nibbles<0>(w[0]), nibbles<0>(w[1]), nibbles<0>(w[2]), nibbles<0>(w[3]), q0.x, q0.y);
+                    mma_f16_first(acc[gr][nt], nibbles<0>(w[0]), nibbles<0>(w[1]), nibbles<0>(w[2]), nibbles<0>(w[3]), q0.x, q0.y);
                     mma_f16(acc[gr][nt], nibbles<1>(w[0]), nibbles<1>(w[1]), nibbles<1>(w[2]), nibbles<1>(w[3]), q0.z, q0.w);
                     mma_f16(acc[gr][nt], nibbles<2>(w[0]), nibbles<2>(w[1]), nibbles<2>(w[2]), nibbles<2>(w[3]), q1.x, q1.y);
                     mma_f16(acc[gr][nt], nibbles<3>(w[0]), nibbles<3>(w[1]), nibbles<3>(w[2]), nibbles<3>(w[3]), q1.z, q1.w);
@@ -430,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
             if (score_at) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                    if (block * ROWS + nt * 8 < a.row_pad) {
+                    if (block * ROWS + nt * 8 + 2 * tig < a.row_pad) {
                         *reinterpret_cast<float2*>(score_at + nt * 8) = make_float2(s[nt][0] + m[nt][0], s[nt][1] + m[nt][1]);
                         *reinterpret_cast<float2*>(score_at + 8 * a.row_pad + nt * 8) =
                             make_float2(s[nt][2] + m[nt][0], s[nt][3] + m[nt][1]);
@@ -586,60 +613,69 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                 if (!((seen >> (nt * 2 + x)) & 1)) m[nt][x] = -INFINITY;
                 if (g == 0) warp_ml[warp][nt * 8 + 2 * tig + x] = make_float2(m[nt][x], l[nt][x]);
             }
-        __syncthreads();
-        for (uint32_t w = 0; w < kWarps; ++w) {
-            if (warp == w) {
+        __syncthreads();  // every warp's ring is drained, its maxima and sums are there
+        const uint32_t seg = unit == begin ? 0 : 1;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+            if (nt > 0) __syncthreads();
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t r = nt * 8 + 2 * tig + x;
-                        float top = -INFINITY;
-                        for (uint32_t v = 0; v < kWarps; ++v) top = fmaxf(top, warp_ml[v][r].x);
-                        // a warp that saw nothing has l = 0, or a NaN that has to stay
-                        const float f = m[nt][x] == -INFINITY ? l[nt][x] : m[nt][x] == top ? 1.f : ex2(m[nt][x] - top);
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t r = nt * 8 + 2 * tig + x;
+                float top = -INFINITY;
 #pragma unroll
-                        for (uint32_t gr = 0; gr < NG; ++gr)
+                for (uint32_t v = 0; v < kWarps; ++v) top = fmaxf(top, warp_ml[v][r].x);
+                // a warp that saw nothing has l = 0, or a NaN that has to stay
+                const float f = m[nt][x] == -INFINITY ? l[nt][x] : m[nt][x] == top ? 1.f : ex2(m[nt][x] - top);
+                float* at = merge + (warp * 8 + 2 * tig + x) * S::pitch + 4 * g;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
+                for (uint32_t gr = 0; gr < NG; ++gr) {
+                    // the group's power of two (exactly inverted), and 2^24 or 2^20 of the nibble
+                    const float back = __uint_as_float((254u << 23) - __float_as_uint(ref[gr])) * 1048576.f;
 #pragma unroll
-                                for (int cb = 0; cb < 2; ++cb) {
-                                    // 2^24 or 2^20 of the nibble, the group's power of two
-                                    const float back = ((j & 1) ? 1048576.f : 16777216.f) / ref[gr];
-                                    const float v = fmaf(o[gr][j][nt][cb * 2 + x], back, zs[nt][x][gr]) * f;
-                                    float* at = merge + r * S::pitch + gr * 64 + cb * 32 + 4 * g + j;
-                                    *at = w == 0 ? v : *at + v;
-                                }
-                    }
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int cb = 0; cb < 2; ++cb)
+                            at[gr * 64 + cb * 32 + j] =
+                                fmaf(o[gr][j][nt][cb * 2 + x], (j & 1) ? back : back * 16.f, zs[nt][x][gr]) * f;
+                }
             }
             __syncthreads();
-        }
-        const uint32_t seg = unit == begin ? 0 : 1;
-        for (uint32_t r = warp; r < ROWS; r += kWarps) {
-            float top = -INFINITY, sum = 0.f;
-            for (uint32_t v = 0; v < kWarps; ++v) top = fmaxf(top, warp_ml[v][r].x);
-            for (uint32_t v = 0; v < kWarps; ++v) {
-                const float2 ml = warp_ml[v][r];
-                sum += ml.x == -INFINITY ? ml.y : ml.x == top ? ml.y : ml.y * ex2(ml.x - top);
-            }
-            const uint32_t row = block * ROWS + r;
-            if (whole) {
-                if (row < all_rows) {
-                    const uint32_t qi = row / a.group, qh = head * a.group + row % a.group;
-                    T* dst = static_cast<T*>(a.out) + ((uint64_t)(sh.start + qi) * a.heads + qh) * D;
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                    for (uint32_t ch = lane * 2; ch < D; ch += 64)
-                        *reinterpret_cast<uint32_t*>(dst + ch) =
-                            f2_to_pair<T>(merge[r * S::pitch + ch] * inv, merge[r * S::pitch + ch + 1] * inv);
-                    if (a.scores && lane == 0)
+#pragma unroll
+            for (uint32_t r8 = warp; r8 < 8; r8 += kWarps) {
+                const uint32_t r = nt * 8 + r8, row = block * ROWS + r;
+                if (row >= all_rows) continue;
+                float top = -INFINITY, sum = 0.f;
+#pragma unroll
+                for (uint32_t v = 0; v < kWarps; ++v) top = fmaxf(top, warp_ml[v][r].x);
+#pragma unroll
+                for (uint32_t v = 0; v < kWarps; ++v) {
+                    const float2 ml = warp_ml[v][r];
+                    sum += ml.x == -INFINITY || ml.x == top ? ml.y : ml.y * ex2(ml.x - top);
+                }
+                const uint32_t qi = row / a.group, qh = head * a.group + row % a.group;
+                T* dst = static_cast<T*>(a.out) + ((uint64_t)(sh.start + qi) * a.heads + qh) * D;
+                const uint64_t slot_at = (uint64_t)(2 * blockIdx.x + seg) * ROWS + r;
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                for (uint32_t ch = lane * 2; ch < D; ch += 64) {
+                    float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (uint32_t w = 0; w < kWarps; ++w) {
+                        const float2 t = *reinterpret_cast<const float2*>(merge + (w * 8 + r8) * S::pitch + ch);
+                        v.x += t.x;
+                        v.y += t.y;
+                    }
+                    if (whole)
+                        *reinterpret_cast<uint32_t*>(dst + ch) = f2_to_pair<T>(v.x * inv, v.y * inv);
+                    else
+                        *reinterpret_cast<float2*>(a.part_o + slot_at * D + ch) = v;
+                }
+                if (lane == 0) {
+                    if (!whole)
+                        a.part_ml[slot_at] = make_float2(top, sum);
+                    else if (a.scores)
                         a.stats[((uint64_t)b * a.c.kv_heads + head) * a.row_pad + row] = make_float2(top, sum);
                 }
-            } else {
-                const uint64_t slot_at = (uint64_t)(2 * blockIdx.x + seg) * ROWS + r;
-                for (uint32_t ch = lane * 2; ch < D; ch += 64)
-                    *reinterpret_cast<float2*>(a.part_o + slot_at * D + ch) =
-                        make_float2(merge[r * S::pitch + ch], merge[r * S::pitch + ch + 1]);
-                if (lane == 0) a.part_ml[slot_at] = make_float2(top, sum);
             }
         }
         __syncthreads();
@@ -650,37 +686,43 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
 // Pieces of an item that blocks left in the workspace: slots of blocks `first` .. `last`.
 struct Pieces {
     uint32_t first, last, first_slot;
+    __device__ __forceinline__ Pieces(const Split& split, uint32_t unit0, uint32_t chunks)
+    {
+        first = split.block_of(unit0);
+        last = split.block_of(unit0 + chunks - 1);
+        first_slot = 2 * first + (unit0 == split.begin(first) ? 0 : 1);
+    }
+    __device__ __forceinline__ uint32_t count() const { return last - first + 1; }
+    __device__ __forceinline__ uint32_t slot(uint32_t i) const { return i == 0 ? first_slot : 2 * (first + i); }
 };
-__device__ __forceinline__ Pieces pieces_of(uint32_t unit0, uint32_t chunks, uint32_t total, uint32_t blocks)
-{
-    Pieces p;
-    p.first = (uint32_t)((((uint64_t)unit0 + 1) * blocks - 1) / total);
-    p.last = (uint32_t)((((uint64_t)unit0 + chunks) * blocks - 1) / total);
-    const uint32_t begin = (uint32_t)((uint64_t)total * p.first / blocks);
-    p.first_slot = 2 * p.first + (unit0 == begin ? 0 : 1);
-    return p;
-}
-__device__ __forceinline__ uint32_t piece_slot(const Pieces& p, uint32_t i) { return i == 0 ? p.first_slot : 2 * (p.first + i); }
 
 constexpr uint32_t kJoinThreads = 256;
 
-// Blocks below join_blocks: a warp a query row joins the pieces of its item.
+// Blocks below join_blocks: WPR warps a query row join the pieces of its item.
 // The others: weights of an equal piece of all positions, from the scores.
-template <typename T, int D>
+// What depends on the call's inputs alone is worked out before the wait for
+// the first kernel, which has waited for the inputs itself.
+template <typename T, int D, uint32_t WPR>
 __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, uint32_t rows_per_item, uint32_t grid1,
                                                                 uint32_t join_blocks)
 {
+    constexpr uint32_t WARPS = kJoinThreads / 32, V = D / 64;  // V: pairs of channels a lane holds
+    extern __shared__ uint32_t ustart[];
     __shared__ float2 row_ml[kJoinThreads];
-    griddep_wait();
-    griddep_launch_dependents();
+    __shared__ float2 part[WPR > 1 ? WARPS : 1][V * 32];
+    __shared__ float part_l[WARPS];
+    __shared__ uint32_t scan_part[WARPS];
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    const uint32_t total = a.unit_start[a.s.batch];
-    if (total == 0) return;
-    const uint32_t blocks = max(1u, min(grid1, total / kMinChunks));
+    lay_out<kJoinThreads>(a, rows_per_item, ustart, scan_part);
+    const uint32_t total = ustart[a.s.batch];
+    if (total == 0) {
+        griddep_wait();
+        return;
+    }
+    const Split split(total, grid1);
     if (blockIdx.x < join_blocks) {
-        const uint64_t id = (uint64_t)blockIdx.x * (kJoinThreads / 32) + warp;
-        if (id >= (uint64_t)a.s.tokens * a.heads) return;
-        const uint32_t token = (uint32_t)(id / a.heads), qh = (uint32_t)(id % a.heads);
+        const uint64_t id = (uint64_t)blockIdx.x * (WARPS / WPR) + warp / WPR;
+        const uint32_t token = (uint32_t)min(id / a.heads, (uint64_t)a.s.tokens), qh = (uint32_t)(id % a.heads);
         uint32_t lo = 0, hi = a.s.batch;
         while (lo < hi) {
             const uint32_t mid = (lo + hi) / 2;
@@ -689,44 +731,73 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, ui
             else
                 hi = mid;
         }
-        if (lo == a.s.batch) return;
-        const SeqShape sh = seq_shape(a, lo, rows_per_item);
-        if (token < sh.start || token - sh.start >= min(sh.n, a.max_queries)) return;
-        const uint32_t head = qh / a.group, row = (token - sh.start) * a.group + qh % a.group;
-        const uint32_t block = row / rows_per_item, r = row % rows_per_item;
-        const Pieces p =
-            pieces_of(a.unit_start[lo] + (head * sh.blocks + block) * sh.chunks, sh.chunks, total, blocks);
-        if (p.first == p.last) return;  // written whole
-        const uint32_t count = p.last - p.first + 1;
+        bool mine = token < a.s.tokens && lo < a.s.batch;
+        uint32_t count = 0, r = 0;
+        Pieces p(split, 0, 1);
+        if (mine) {
+            const SeqShape sh = seq_shape(a, lo, rows_per_item);
+            mine = token >= sh.start && token - sh.start < min(sh.n, a.max_queries);
+            if (mine) {
+                const uint32_t head = qh / a.group, row = (token - sh.start) * a.group + qh % a.group;
+                r = row % rows_per_item;
+                p = Pieces(split, ustart[lo] + (head * sh.blocks + row / rows_per_item) * sh.chunks, sh.chunks);
+                count = p.count();
+                mine = count > 1;  // otherwise written whole
+            }
+        }
+        griddep_wait();
+        griddep_launch_dependents();
         float top = -INFINITY;
-        for (uint32_t i = lane; i < count; i += 32)
-            top = fmaxf(top, a.part_ml[(uint64_t)piece_slot(p, i) * rows_per_item + r].x);
+        if (mine)
+            for (uint32_t i = lane; i < count; i += 32)
+                top = fmaxf(top, a.part_ml[(uint64_t)p.slot(i) * rows_per_item + r].x);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        constexpr uint32_t V = D / 64;  // pairs of channels a lane holds
         float2 o[V] = {};
         float sum = 0.f;
-        for (uint32_t i0 = 0; i0 < count; i0 += 32) {
-            float f = 0.f, ls = 0.f;
-            if (i0 + lane < count) {
-                const float2 ml = a.part_ml[(uint64_t)piece_slot(p, i0 + lane) * rows_per_item + r];
-                f = ml.x == -INFINITY ? 0.f : ml.x == top ? 1.f : ex2(ml.x - top);
-                ls = ml.x == -INFINITY ? ml.y : ml.y * f;  // a NaN stays
+        // this warp's pieces: every WPR-th
+        if (mine)
+            for (uint32_t i0 = warp % WPR; i0 < count; i0 += 32 * WPR) {
+                float f = 0.f;
+                const uint32_t i_lane = i0 + lane * WPR;
+                if (i_lane < count) {
+                    const float2 ml = a.part_ml[(uint64_t)p.slot(i_lane) * rows_per_item + r];
+                    f = ml.x == -INFINITY ? 0.f : ml.x == top ? 1.f : ex2(ml.x - top);
+                    sum += ml.x == -INFINITY ? ml.y : ml.y * f;  // a NaN stays
+                }
+                const uint32_t here = min(32u, (count - i0 + WPR - 1) / WPR);
+#pragma unroll 8
+                for (uint32_t i = 0; i < here; ++i) {
+                    const float fi = __shfl_sync(0xffffffffu, f, i);
+                    const float* src = a.part_o + ((uint64_t)p.slot(i0 + i * WPR) * rows_per_item + r) * D;
+#pragma unroll
+                    for (uint32_t v = 0; v < V; ++v) {
+                        const float2 x = *reinterpret_cast<const float2*>(src + v * 64 + lane * 2);
+                        o[v].x = fmaf(x.x, fi, o[v].x);
+                        o[v].y = fmaf(x.y, fi, o[v].y);
+                    }
+                }
             }
-            const uint32_t here = min(32u, count - i0);
-#pragma unroll 4
-            for (uint32_t i = 0; i < here; ++i) {
-                const float fi = __shfl_sync(0xffffffffu, f, i);
-                sum += __shfl_sync(0xffffffffu, ls, i);
-                const float* src = a.part_o + ((uint64_t)piece_slot(p, i0 + i) * rows_per_item + r) * D;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if constexpr (WPR > 1) {
+#pragma unroll
+            for (uint32_t v = 0; v < V; ++v) part[warp][v * 32 + lane] = o[v];
+            if (lane == 0) part_l[warp] = sum;
+            __syncthreads();
+            if (warp % WPR != 0) return;
+#pragma unroll
+            for (uint32_t w = 1; w < WPR; ++w) {
+                sum += part_l[warp + w];
 #pragma unroll
                 for (uint32_t v = 0; v < V; ++v) {
-                    const float2 x = *reinterpret_cast<const float2*>(src + v * 64 + lane * 2);
-                    o[v].x = fmaf(x.x, fi, o[v].x);
-                    o[v].y = fmaf(x.y, fi, o[v].y);
+                    const float2 x = part[warp + w][v * 32 + lane];
+                    o[v].x += x.x;
+                    o[v].y += x.y;
                 }
             }
         }
+        if (!mine) return;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         T* dst = static_cast<T*>(a.out) + ((uint64_t)token * a.heads + qh) * D;
 #pragma unroll
@@ -734,23 +805,17 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, ui
             *reinterpret_cast<uint32_t*>(dst + v * 64 + lane * 2) = f2_to_pair<T>(o[v].x * inv, o[v].y * inv);
         return;
     }
-    // weights: the line again, where each item of a sequence's first row block stands for its head
+    // weights: the line again; a head's row blocks make one run of blocks * chunks units, over which its positions
+    // are spread evenly
     const uint32_t wb = blockIdx.x - join_blocks, wblocks = gridDim.x - join_blocks;
     const uint32_t begin = (uint32_t)((uint64_t)total * wb / wblocks), end = (uint32_t)((uint64_t)total * (wb + 1) / wblocks);
-    uint32_t lo = 0, hi = a.s.batch;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (a.unit_start[mid] <= begin)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    uint32_t b = lo, unit = begin;
+    uint32_t unit = begin, b = seq_of(ustart, a.s.batch, unit);
+    griddep_wait();
+    griddep_launch_dependents();
     while (unit < end) {
-        while (a.unit_start[b + 1] <= unit) ++b;
+        while (ustart[b + 1] <= unit) ++b;
         const SeqShape sh = seq_shape(a, b, rows_per_item);
-        const uint32_t in_seq = unit - a.unit_start[b];
-        // a head's row blocks make one run of blocks * chunks units; its positions are spread over that run
+        const uint32_t in_seq = unit - ustart[b];
         const uint32_t run = sh.blocks * sh.chunks, head = in_seq / run, u0 = in_seq % run, u1 = min(run, u0 + (end - unit));
         const uint32_t p0 = (uint32_t)((uint64_t)sh.vis * u0 / run), p1 = (uint32_t)((uint64_t)sh.vis * u1 / run);
         const uint32_t all_rows = min(sh.n, a.max_queries) * a.group;
@@ -759,42 +824,47 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, ui
         for (uint32_t r0 = 0; r0 < all_rows; r0 += kJoinThreads) {
             const uint32_t rows = min(kJoinThreads, all_rows - r0);
             __syncthreads();
-            if (tid < rows) {
-                const uint32_t row = r0 + tid, block = row / rows_per_item, r = row % rows_per_item;
-                const Pieces p =
-                    pieces_of(a.unit_start[b] + (head * sh.blocks + block) * sh.chunks, sh.chunks, total, blocks);
-                float2 ml;
-                if (p.first == p.last) {
+            // eight lanes a row gather its maximum and sum
+            for (uint32_t i = tid / 8; i < (rows + 3) / 4 * 4; i += kJoinThreads / 8) {
+                const uint32_t row = min(r0 + i, all_rows - 1), r = row % rows_per_item, l8 = tid & 7;
+                const uint32_t lanes = 0xffu << (tid & 24);
+                const Pieces p(split, ustart[b] + (head * sh.blocks + row / rows_per_item) * sh.chunks, sh.chunks);
+                const uint32_t count = p.count();
+                float2 ml = make_float2(-INFINITY, 0.f);
+                if (count == 1) {
                     ml = a.stats[((uint64_t)b * a.c.kv_heads + head) * a.row_pad + row];
                 } else {
-                    const uint32_t count = p.last - p.first + 1;
-                    ml = make_float2(-INFINITY, 0.f);
-                    for (uint32_t i = 0; i < count; ++i)
-                        ml.x = fmaxf(ml.x, a.part_ml[(uint64_t)piece_slot(p, i) * rows_per_item + r].x);
-                    for (uint32_t i = 0; i < count; ++i) {
-                        const float2 x = a.part_ml[(uint64_t)piece_slot(p, i) * rows_per_item + r];
-                        ml.y += x.x == -INFINITY ? x.y : x.x == ml.x ? x.y : x.y * ex2(x.x - ml.x);
+                    for (uint32_t k = l8; k < count; k += 8)
+                        ml.x = fmaxf(ml.x, a.part_ml[(uint64_t)p.slot(k) * rows_per_item + r].x);
+#pragma unroll
+                    for (int off = 4; off > 0; off >>= 1) ml.x = fmaxf(ml.x, __shfl_xor_sync(lanes, ml.x, off));
+                    for (uint32_t k = l8; k < count; k += 8) {
+                        const float2 x = a.part_ml[(uint64_t)p.slot(k) * rows_per_item + r];
+                        ml.y += x.x == -INFINITY || x.x == ml.x ? x.y : x.y * ex2(x.x - ml.x);
                     }
+#pragma unroll
+                    for (int off = 4; off > 0; off >>= 1) ml.y += __shfl_xor_sync(lanes, ml.y, off);
                 }
-                row_ml[tid] = make_float2(ml.x == -INFINITY ? 0.f : ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y);
+                if (l8 == 0 && i < kJoinThreads)
+                    row_ml[i] = i < rows ? make_float2(ml.x == -INFINITY ? 0.f : ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y)
+                                         : make_float2(0.f, 0.f);
             }
             __syncthreads();
+#pragma unroll 4
             for (uint32_t t = p0 + tid; t < p1; t += kJoinThreads) {
                 const int64_t at = kv4_row(a.c, table, t, head);
-                if (at < 0) continue;
                 const float* sp = scores + (uint64_t)t * a.row_pad + r0;
                 float sum = 0.f;
-                for (uint32_t r = 0; r < rows; r += 4) {  // row_pad is a multiple of 8
+                for (uint32_t r = 0; r < rows; r += 4) {  // row_pad is a multiple of 4
                     const float4 s = *reinterpret_cast<const float4*>(sp + r);
                     const float sv[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (r + i < rows) {
-                            const float2 ml = row_ml[r + i];
-                            sum = fmaf(sv[i] == -INFINITY ? 0.f : ex2(sv[i] - ml.x), ml.y, sum);
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 ml = row_ml[r + i];
+                        if (r + i < rows) sum = fmaf(ex2(sv[i] - ml.x), ml.y, sum);
+                    }
                 }
-                a.c.weight[at] += sum;
+                if (at >= 0) a.c.weight[at] += sum;
             }
         }
         unit += u1 - u0;
@@ -802,7 +872,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, ui
 }
 
 struct AttnWs {
-    size_t unit_start, stats, part_o, part_ml, scores, bytes;
+    size_t stats, part_o, part_ml, scores, bytes;
 };
 uint32_t tiles_of(uint32_t rows, uint32_t dim) { return rows <= 8 ? 1 : rows <= 16 || dim == 256 ? 2 : 4; }
 
@@ -810,7 +880,7 @@ AttnWs layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, u
               bool accumulate, uint32_t num_sms)
 {
     const uint64_t rows = (uint64_t)(heads / kv_heads) * max_queries;
-    const uint64_t pad = (rows + 7) / 8 * 8;
+    const uint64_t pad = (rows + 3) / 4 * 4;
     const uint64_t slots = 2ull * num_sms * kMaxBlocks * 8 * tiles_of((uint32_t)std::min<uint64_t>(rows, 1u << 20), dim);
     AttnWs w;
     size_t at = 0;
@@ -819,7 +889,6 @@ AttnWs layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, u
         at += (n + 255) / 256 * 256;
         return here;
     };
-    w.unit_start = take((batch + 1ull) * 4);
     w.part_ml = take(slots * 8);
     w.part_o = take(slots * dim * 4);
     w.stats = take(accumulate ? (uint64_t)batch * kv_heads * pad * 8 : 0);
@@ -828,6 +897,8 @@ AttnWs layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, u
     return w;
 }
 
+uint64_t kv4_chunks(const AttnParams& p) { return (uint64_t)p.s.max_pages * p.c.page_size / kChunk; }
+
 template <typename T, int D, int NT>
 cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t st)
 {
@@ -835,13 +906,23 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(kv4_attention_kernel<T, D, NT>, S::fixed + (kMaxAttnBatch + 1) * 4, done);
     if (e != cudaSuccess) return e;
-    const uint32_t grid = num_sms * attn_blocks<D, NT>();
-    e = launch_pdl(kv4_attention_kernel<T, D, NT>, dim3(grid), dim3(kThreads), S::fixed + (p.s.batch + 1) * 4, st, p);
+    // no more blocks than the page tables have room for chunks
+    const uint64_t items = (uint64_t)p.s.batch * p.c.kv_heads * ((p.group * p.max_queries + 8 * NT - 1) / (8 * NT));
+    const uint64_t most = items * (kv4_chunks(p) + 1) / kMinChunks + 1;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(most, num_sms * attn_blocks<D, NT>());
+    const uint32_t line = (p.s.batch + 1) * 4;
+    e = launch_pdl(kv4_attention_kernel<T, D, NT>, dim3(grid), dim3(kThreads), S::fixed + line, st, p);
     if (e != cudaSuccess) return e;
     const uint64_t rows = (uint64_t)p.s.tokens * p.heads;
-    const uint32_t join = (uint32_t)((rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
-    return launch_pdl(kv4_join_kernel<T, D>, dim3(join + (accumulate ? 4 * num_sms : 0)), dim3(kJoinThreads), 0, st, p,
-                      8u * NT, grid, join);
+    const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 4 * num_sms) : 0;
+    constexpr uint32_t kJoinWarps = kJoinThreads / 32;
+    // few rows: four warps each, for the latency; many: one
+    if (rows <= 16 * num_sms) {
+        const uint32_t join = (uint32_t)((rows * 4 + kJoinWarps - 1) / kJoinWarps);
+        return launch_pdl(kv4_join_kernel<T, D, 4>, dim3(join + weights), dim3(kJoinThreads), line, st, p, 8u * NT, grid, join);
+    }
+    const uint32_t join = (uint32_t)((rows + kJoinWarps - 1) / kJoinWarps);
+    return launch_pdl(kv4_join_kernel<T, D, 1>, dim3(join + weights), dim3(kJoinThreads), line, st, p, 8u * NT, grid, join);
 }
 
 template <typename T, int D>
@@ -879,9 +960,8 @@ cudaError_t launch_kv4_attention(const Kv4Attention& a, void* workspace, uint32_
     p.heads = a.heads;
     p.group = a.heads / a.cache.kv_heads;
     p.max_queries = a.max_queries;
-    p.row_pad = (p.group * a.max_queries + 7) / 8 * 8;
+    p.row_pad = (p.group * a.max_queries + 3) / 4 * 4;
     p.scale_log2 = a.scale * kLog2e;
-    p.unit_start = reinterpret_cast<uint32_t*>(base + w.unit_start);
     p.stats = reinterpret_cast<float2*>(base + w.stats);
     p.part_o = reinterpret_cast<float*>(base + w.part_o);
     p.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
