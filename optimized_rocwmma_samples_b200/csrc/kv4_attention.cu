@@ -33,6 +33,7 @@
 // streams its own chunks through a ring of cp.async stages, with no barrier
 // until the item's end.
 #include "kv4.cuh"
+#include "sq_math.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -43,8 +44,7 @@ namespace {
 
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = kWarps * 32;
-constexpr uint32_t kChunk = 16;     // tokens a warp takes at a time
-constexpr uint32_t kMinChunks = 4;  // a block gets at least one for each warp
+constexpr uint32_t kMinTokens = 64;  // of a block's share: fewer leave too little to do between its start and its join
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -55,6 +55,7 @@ struct AttnParams {
     uint64_t q_stride;
     uint32_t heads, group, max_queries, row_pad;  // row_pad: group * max_queries rounded up to 4
     float scale_log2;
+    uint32_t chunk;  // tokens a warp takes at a time: 16 or 32
     float2* stats;         // [batch * kv_heads][row_pad] (max, sum) of items that one block did whole
     float* part_o;         // [2 * blocks][8 NT][D]
     float2* part_ml;       // [2 * blocks][8 NT]
@@ -62,20 +63,21 @@ struct AttnParams {
 };
 
 // Blocks a SM that registers (and shared memory) leave room for.
-template <int D, int NT>
+template <int D, int NT, int CH>
 constexpr uint32_t attn_blocks()
 {
+    if (CH == 2) return D == 64 ? 5 : 3;
     return D == 64 ? (NT == 1 ? 6 : NT == 2 ? 4 : 3) : D == 128 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (NT == 1 ? 3 : 2);
 }
 constexpr uint32_t kMaxBlocks = 6;
 
-template <int D, int NT>
+template <int D, int NT, int CH>
 struct AttnSmem {
     static constexpr uint32_t rows = 8 * NT;
-    static constexpr uint32_t data = kChunk * D / 2;                // a chunk's key nibbles
-    static constexpr uint32_t scales = kChunk * (D / 64) * 4;       // and their steps and bases
+    static constexpr uint32_t data = CH * 16 * D / 2;               // a chunk's key nibbles
+    static constexpr uint32_t scales = CH * 16 * (D / 64) * 4;      // and their steps and bases
     static constexpr uint32_t stage = 2 * (data + scales);
-    static constexpr uint32_t stages = D == 64 ? 6 : D == 128 ? 4 : 3;
+    static constexpr uint32_t stages = D == 64 ? (CH == 2 ? 4 : 6) : D == 128 ? (CH == 2 ? 3 : 4) : 3;
     static constexpr uint32_t ring = kWarps * stages * stage;
     static constexpr uint32_t q = rows * D * 2;
     static constexpr uint32_t pitch = D + 2;  // of a row in the join of the warps, which uses the drained ring
@@ -163,7 +165,7 @@ __device__ __forceinline__ SeqShape seq_shape(const AttnParams& a, uint32_t b, u
     s.len = kv4_len(a.s, b);
     s.n = kv4_new_rows(a.s, b, s.start);
     s.vis = min(s.len, kv4_cap(a.c, a.s));
-    s.chunks = max(1u, (s.vis + kChunk - 1) / kChunk);
+    s.chunks = max(1u, (s.vis + a.chunk - 1) / a.chunk);
     s.blocks = (min(s.n, a.max_queries) * a.group + rows - 1) / rows;
     return s;
 }
@@ -171,9 +173,9 @@ __device__ __forceinline__ SeqShape seq_shape(const AttnParams& a, uint32_t b, u
 // Equal pieces of `total` chunks for `blocks` blocks: the first `rest` get one more.
 struct Split {
     uint32_t blocks, each, rest;
-    __device__ __forceinline__ Split(uint32_t total, uint32_t grid)
+    __device__ __forceinline__ Split(uint32_t total, uint32_t grid, uint32_t chunk)
     {
-        blocks = max(1u, min(grid, total / kMinChunks));
+        blocks = max(1u, min(grid, total / (kMinTokens / chunk)));
         each = total / blocks;
         rest = total - each * blocks;
     }
@@ -231,11 +233,11 @@ __device__ __forceinline__ uint32_t seq_of(const uint32_t* ustart, uint32_t batc
     return lo;
 }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_kernel(AttnParams a)
+template <typename T, int D, int NT, int CH>
+__global__ void __launch_bounds__(kThreads, attn_blocks<D, NT, CH>()) kv4_attention_kernel(AttnParams a)
 {
-    using S = AttnSmem<D, NT>;
-    constexpr uint32_t NG = D / 64, CPR = D / 32, ROWS = 8 * NT, STAGES = S::stages, SC = S::scales / 16;
+    using S = AttnSmem<D, NT, CH>;
+    constexpr uint32_t CHUNK = 16 * CH, NG = D / 64, CPR = D / 32, ROWS = 8 * NT, STAGES = S::stages, SC = S::scales / 16;
     // fp16 results want more bits of the probabilities than fp16 has: a second operand holds what the first leaves
     constexpr bool SPLIT = std::is_same<T, __half>::value;
     extern __shared__ __align__(16) uint8_t at_smem[];
@@ -254,11 +256,11 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
 
     lay_out<kThreads>(a, ROWS, ustart, scan_part);
     const uint32_t total = ustart[a.s.batch];
-    const Split split(total, gridDim.x);
+    const Split split(total, gridDim.x, CHUNK);
     if (blockIdx.x >= split.blocks || total == 0) return;
     const uint32_t begin = split.begin(blockIdx.x), end = split.begin(blockIdx.x + 1);
 
-    const uint32_t page_chunks = a.c.page_size / kChunk;
+    const uint32_t page_chunks = a.c.page_size / CHUNK;
     const uint32_t ring_base = smem_u32(ring) + warp * STAGES * S::stage;
     uint32_t unit = begin;
     uint32_t b = seq_of(ustart, a.s.batch, unit);
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                     page = next_page;
                     ++page_at;
                     next_page = page_at < page_end ? __ldg(table + page_at) : -1;
-                    const int64_t row = ((int64_t)page * a.c.kv_heads + head) * a.c.page_size + skip * kChunk;
+                    const int64_t row = ((int64_t)page * a.c.kv_heads + head) * a.c.page_size + skip * CHUNK;
                     kp = a.c.k + row * (D / 2) + lane * 16;
                     vp = a.c.v + row * (D / 2) + lane * 16;
                     sp = static_cast<const uint8_t*>(lane < SC ? a.c.k_scale : a.c.v_scale) + row * (NG * 4) +
@@ -395,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
         const uint32_t tok = (lane & 7) + ((lane >> 3) & 1) * 8;  // ldmatrix row of this lane
         const uint32_t sw = (tok / (8 / CPR)) & (CPR - 1);
         const uint32_t mat = ring_base + tok * CPR * 16;
-        float* score_at = a.scores ? a.scores + (((uint64_t)b * a.c.kv_heads + head) * kv4_cap(a.c, a.s) + wc0 * kChunk + g) * a.row_pad + block * ROWS + 2 * tig
+        float* score_at = a.scores ? a.scores + (((uint64_t)b * a.c.kv_heads + head) * kv4_cap(a.c, a.s) + wc0 * CHUNK + g) * a.row_pad + block * ROWS + 2 * tig
                                    : nullptr;
 
         // one chunk of 16 tokens; FULL: every row sees all of them
@@ -403,82 +405,93 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
             constexpr bool FULL = decltype(full_tag)::value;
             const uint32_t base = mat + slot * S::stage;
             const uint8_t* stage = ring + (warp * STAGES + slot) * S::stage;
-            // scores
-            float acc[NG][NT][4];
-#pragma unroll
-            for (uint32_t gr = 0; gr < NG; ++gr) {
-                uint32_t w[4];
-                ldsm4(base + ((gr * 2 + (lane >> 4)) ^ sw) * 16, w);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const uint4* qf = reinterpret_cast<const uint4*>(q_frag) + ((nt * NG + gr) * 2) * 32 + lane;
-                    const uint4 q0 = qf[0], q1 = qf[32];
-                    mma_f16_first(acc[gr][nt], nibbles<0>(w[0]), nibbles<0>(w[1]), nibbles<0>(w[2]), nibbles<0>(w[3]), q0.x, q0.y);
-                    mma_f16(acc[gr][nt], nibbles<1>(w[0]), nibbles<1>(w[1]), nibbles<1>(w[2]), nibbles<1>(w[3]), q0.z, q0.w);
-                    mma_f16(acc[gr][nt], nibbles<2>(w[0]), nibbles<2>(w[1]), nibbles<2>(w[2]), nibbles<2>(w[3]), q1.x, q1.y);
-                    mma_f16(acc[gr][nt], nibbles<3>(w[0]), nibbles<3>(w[1]), nibbles<3>(w[2]), nibbles<3>(w[3]), q1.z, q1.w);
-                }
-            }
-            // thread: tokens g and g + 8, rows 2 tig and 2 tig + 1 of every eight
-            float2 ksz[2][NG];
-            float vs[2][NG], vz[2][NG];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t kw[NG], vw[NG];
-                lds_words<NG>(stage + 2 * S::data + (g + 8 * h) * NG * 4, kw);
-                lds_words<NG>(stage + 2 * S::data + S::scales + (g + 8 * h) * NG * 4, vw);
-#pragma unroll
-                for (uint32_t gr = 0; gr < NG; ++gr) {
-                    ksz[h][gr] = pair_to_f2<__half>(kw[gr]);
-                    const float2 v = pair_to_f2<__half>(vw[gr]);
-                    vs[h][gr] = v.x;
-                    vz[h][gr] = v.y;
-                }
-            }
-            const int t0 = (int)(c * kChunk + g);
-            bool see[NT][4];
-            float s[NT][4];  // score - m
+            const int t0 = (int)(c * CHUNK + g);
+            bool see[CH][NT][4];
+            float s[CH][NT][4];  // score - m
+            float vs[CH][2][NG], vz[CH][2][NG];
             float top = -INFINITY, step_top = 0.f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int ch = 0; ch < CH; ++ch) {
+                float acc[NG][NT][4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int h = i >> 1, x = i & 1;
-                    float dot = acc[0][nt][i] * ksz[h][0].x, off = fmaf(qsum[nt][x][0], ksz[h][0].y, -m[nt][x]);
+                for (uint32_t gr = 0; gr < NG; ++gr) {
+                    uint32_t w[4];
+                    ldsm4(base + ch * 8 * D + ((gr * 2 + (lane >> 4)) ^ sw) * 16, w);
 #pragma unroll
-                    for (uint32_t gr = 1; gr < NG; ++gr) {
-                        dot = fmaf(acc[gr][nt][i], ksz[h][gr].x, dot);
-                        off = fmaf(qsum[nt][x][gr], ksz[h][gr].y, off);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint4* qf = reinterpret_cast<const uint4*>(q_frag) + ((nt * NG + gr) * 2) * 32 + lane;
+                        const uint4 q0 = qf[0], q1 = qf[32];
+                        mma_f16_first(acc[gr][nt], nibbles<0>(w[0]), nibbles<0>(w[1]), nibbles<0>(w[2]), nibbles<0>(w[3]),
+                                      q0.x, q0.y);
+                        mma_f16(acc[gr][nt], nibbles<1>(w[0]), nibbles<1>(w[1]), nibbles<1>(w[2]), nibbles<1>(w[3]), q0.z,
+                                q0.w);
+                        mma_f16(acc[gr][nt], nibbles<2>(w[0]), nibbles<2>(w[1]), nibbles<2>(w[2]), nibbles<2>(w[3]), q1.x,
+                                q1.y);
+                        mma_f16(acc[gr][nt], nibbles<3>(w[0]), nibbles<3>(w[1]), nibbles<3>(w[2]), nibbles<3>(w[3]), q1.z,
+                                q1.w);
                     }
-                    see[nt][i] = FULL || t0 + 8 * h < vis[nt][x];
-                    s[nt][i] = see[nt][i] ? fmaf(dot, mul[nt][x], off) : -INFINITY;
-                    top = fmaxf(top, s[nt][i]);
                 }
-            if (score_at) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    if (block * ROWS + nt * 8 + 2 * tig < a.row_pad) {
-                        *reinterpret_cast<float2*>(score_at + nt * 8) = make_float2(s[nt][0] + m[nt][0], s[nt][1] + m[nt][1]);
-                        *reinterpret_cast<float2*>(score_at + 8 * a.row_pad + nt * 8) =
-                            make_float2(s[nt][2] + m[nt][0], s[nt][3] + m[nt][1]);
-                    }
-            }
-            // the steps over the group's power of two (unseen tokens may hold anything: only read where see[])
-            float pw[2][NG];
-#pragma unroll
-            for (uint32_t gr = 0; gr < NG; ++gr)
+                // thread: tokens g and g + 8, rows 2 tig and 2 tig + 1 of every eight
+                float2 ksz[2][NG];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    pw[h][gr] = vs[h][gr] * ref[gr];
-                    step_top = fmaxf(step_top, fabsf(pw[h][gr]));
+                    uint32_t kw[NG], vw[NG];
+                    lds_words<NG>(stage + 2 * S::data + (ch * 16 + g + 8 * h) * NG * 4, kw);
+                    lds_words<NG>(stage + 2 * S::data + S::scales + (ch * 16 + g + 8 * h) * NG * 4, vw);
+#pragma unroll
+                    for (uint32_t gr = 0; gr < NG; ++gr) {
+                        h2_to_f2(kw[gr], ksz[h][gr].x, ksz[h][gr].y);
+                        h2_to_f2(vw[gr], vs[ch][h][gr], vz[ch][h][gr]);
+                    }
                 }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int h = i >> 1, x = i & 1;
+                        float dot = acc[0][nt][i] * ksz[h][0].x, off = fmaf(qsum[nt][x][0], ksz[h][0].y, -m[nt][x]);
+#pragma unroll
+                        for (uint32_t gr = 1; gr < NG; ++gr) {
+                            dot = fmaf(acc[gr][nt][i], ksz[h][gr].x, dot);
+                            off = fmaf(qsum[nt][x][gr], ksz[h][gr].y, off);
+                        }
+                        see[ch][nt][i] = FULL || t0 + 16 * ch + 8 * h < vis[nt][x];
+                        s[ch][nt][i] = see[ch][nt][i] ? fmaf(dot, mul[nt][x], off) : -INFINITY;
+                        top = fmaxf(top, s[ch][nt][i]);
+                    }
+                if (score_at) {
+                    float* sp_at = score_at + ch * 16 * a.row_pad;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        // (the last chunk may reach past the table by its second half)
+                        if (block * ROWS + nt * 8 + 2 * tig < a.row_pad && (CH == 1 || c * CHUNK + ch * 16 < sh.vis)) {
+                            *reinterpret_cast<float2*>(sp_at + nt * 8) =
+                                make_float2(s[ch][nt][0] + m[nt][0], s[ch][nt][1] + m[nt][1]);
+                            *reinterpret_cast<float2*>(sp_at + 8 * a.row_pad + nt * 8) =
+                                make_float2(s[ch][nt][2] + m[nt][0], s[ch][nt][3] + m[nt][1]);
+                        }
+                }
+            }
+            // the steps over the group's power of two (unseen tokens may hold anything: only read where see[])
+            float pw[CH][2][NG];
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+                for (uint32_t gr = 0; gr < NG; ++gr)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        pw[ch][h][gr] = vs[ch][h][gr] * ref[gr];
+                        step_top = fmaxf(step_top, fabsf(pw[ch][h][gr]));
+                    }
             // p may reach 2^6 and a step twice its power of two before the references are moved
             if (__any_sync(0xffffffffu, top > 6.f || step_top > 512.f || seen != (1u << (2 * NT)) - 1)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        float mx = fmaxf(s[nt][x], s[nt][2 + x]);
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int ch = 0; ch < CH; ++ch) mx = fmaxf(mx, fmaxf(s[ch][nt][x], s[ch][nt][2 + x]));
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
                         const uint32_t bit = 1u << (nt * 2 + x);
@@ -486,8 +499,11 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                             const float f = (seen & bit) ? ex2(-mx) : 0.f;
                             seen |= bit;
                             m[nt][x] += mx;
-                            s[nt][x] -= mx;
-                            s[nt][2 + x] -= mx;
+#pragma unroll
+                            for (int ch = 0; ch < CH; ++ch) {
+                                s[ch][nt][x] -= mx;
+                                s[ch][nt][2 + x] -= mx;
+                            }
                             l[nt][x] *= f;
 #pragma unroll
                             for (uint32_t gr = 0; gr < NG; ++gr) {
@@ -504,18 +520,22 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                 for (uint32_t gr = 0; gr < NG; ++gr) {
                     float mx = 0.f;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float st = fabsf(vs[h][gr]);
-                        if (t0 + 8 * h < (int)sh.vis && st < INFINITY) mx = fmaxf(mx, st);
-                    }
+                    for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float st = fabsf(vs[ch][h][gr]);
+                            if (t0 + 16 * ch + 8 * h < (int)sh.vis && st < INFINITY) mx = fmaxf(mx, st);
+                        }
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
                     if (mx * ref[gr] > 512.f) {
                         const float fresh = __uint_as_float((262u - (__float_as_uint(mx) >> 23)) << 23);
                         const float f = fresh / ref[gr];
                         ref[gr] = fresh;
-                        pw[0][gr] = vs[0][gr] * fresh;
-                        pw[1][gr] = vs[1][gr] * fresh;
+#pragma unroll
+                        for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) pw[ch][h][gr] = vs[ch][h][gr] * fresh;
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -525,55 +545,59 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
                     }
                 }
             }
-            // probabilities
-            uint32_t pb[NG][NT][2];
-            [[maybe_unused]] uint32_t pb2[SPLIT ? NG : 1][NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float p[4];
+            for (int ch = 0; ch < CH; ++ch) {
+                // probabilities
+                uint32_t pb[NG][NT][2];
+                [[maybe_unused]] uint32_t pb2[SPLIT ? NG : 1][NT][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[i] = ex2(s[nt][i]);  // 0 where unseen
-                    l[nt][i & 1] += p[i];
-                }
-#pragma unroll
-                for (uint32_t gr = 0; gr < NG; ++gr) {
-                    float pv[4];
+                for (int nt = 0; nt < NT; ++nt) {
+                    float p[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int h = i >> 1, x = i & 1;
-                        if (FULL || see[nt][i]) zs[nt][x][gr] = fmaf(p[i], vz[h][gr], zs[nt][x][gr]);
-                        pv[i] = FULL || see[nt][i] ? p[i] * pw[h][gr] : 0.f;
+                        p[i] = ex2(s[ch][nt][i]);  // 0 where unseen
+                        l[nt][i & 1] += p[i];
                     }
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t w = f2_to_pair<__half>(pv[2 * h], pv[2 * h + 1]);
-                        pb[gr][nt][h] = movmatrix(w);
-                        if constexpr (SPLIT) {
-                            const float2 r = pair_to_f2<__half>(w);
-                            pb2[gr][nt][h] = movmatrix(f2_to_pair<__half>(pv[2 * h] - r.x, pv[2 * h + 1] - r.y));
+                    for (uint32_t gr = 0; gr < NG; ++gr) {
+                        float pv[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int h = i >> 1, x = i & 1;
+                            if (FULL || see[ch][nt][i]) zs[nt][x][gr] = fmaf(p[i], vz[ch][h][gr], zs[nt][x][gr]);
+                            pv[i] = FULL || see[ch][nt][i] ? p[i] * pw[ch][h][gr] : 0.f;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t w = f2_to_pair<__half>(pv[2 * h], pv[2 * h + 1]);
+                            pb[gr][nt][h] = movmatrix(w);
+                            if constexpr (SPLIT) {
+                                const float2 r = pair_to_f2<__half>(w);
+                                pb2[gr][nt][h] = movmatrix(f2_to_pair<__half>(pv[2 * h] - r.x, pv[2 * h + 1] - r.y));
+                            }
                         }
                     }
                 }
-            }
-            // outputs
+                // outputs
 #pragma unroll
-            for (uint32_t gr = 0; gr < NG; ++gr) {
-                uint32_t w[4];
-                ldsm4_trans(base + S::data + ((gr * 2 + (lane >> 4)) ^ sw) * 16, w);
-                auto word = [&](auto j_tag) {
-                    constexpr int J = decltype(j_tag)::value;
-                    const uint32_t a0 = nibbles<J>(w[0]), a1 = nibbles<J>(w[2]), a2 = nibbles<J>(w[1]), a3 = nibbles<J>(w[3]);
+                for (uint32_t gr = 0; gr < NG; ++gr) {
+                    uint32_t w[4];
+                    ldsm4_trans(base + S::data + ch * 8 * D + ((gr * 2 + (lane >> 4)) ^ sw) * 16, w);
+                    auto word = [&](auto j_tag) {
+                        constexpr int J = decltype(j_tag)::value;
+                        const uint32_t a0 = nibbles<J>(w[0]), a1 = nibbles<J>(w[2]), a2 = nibbles<J>(w[1]),
+                                       a3 = nibbles<J>(w[3]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_f16(o[gr][J][nt], a0, a1, a2, a3, pb[gr][nt][0], pb[gr][nt][1]);
-                        if constexpr (SPLIT) mma_f16(o[gr][J][nt], a0, a1, a2, a3, pb2[gr][nt][0], pb2[gr][nt][1]);
-                    }
-                };
-                word(std::integral_constant<int, 0>());
-                word(std::integral_constant<int, 1>());
-                word(std::integral_constant<int, 2>());
-                word(std::integral_constant<int, 3>());
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_f16(o[gr][J][nt], a0, a1, a2, a3, pb[gr][nt][0], pb[gr][nt][1]);
+                            if constexpr (SPLIT) mma_f16(o[gr][J][nt], a0, a1, a2, a3, pb2[gr][nt][0], pb2[gr][nt][1]);
+                        }
+                    };
+                    word(std::integral_constant<int, 0>());
+                    word(std::integral_constant<int, 1>());
+                    word(std::integral_constant<int, 2>());
+                    word(std::integral_constant<int, 3>());
+                }
             }
         };
 
@@ -584,16 +608,16 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT>()) kv4_attention_
             cp_async_wait<STAGES - 1>();
             __syncwarp();
             if ((valid >> (STAGES - 1)) & 1) {
-                if ((int)(c * kChunk + kChunk) <= least)
+                if ((int)(c * CHUNK + CHUNK) <= least)
                     step(c, slot, std::true_type());
                 else
                     step(c, slot, std::false_type());
             } else if (score_at) {  // no such page: nothing of this chunk is seen
                 const uint32_t rows = min(ROWS, a.row_pad - block * ROWS);
-                for (uint32_t i = lane; i < kChunk * rows && c * kChunk < sh.vis; i += 32)
+                for (uint32_t i = lane; i < CHUNK * rows && c * CHUNK + i / rows < sh.vis; i += 32)
                     score_at[((int64_t)(i / rows) - g) * a.row_pad + (int64_t)(i % rows) - 2 * tig] = -INFINITY;
             }
-            if (score_at) score_at += kChunk * a.row_pad;
+            if (score_at) score_at += CHUNK * a.row_pad;
             if (++slot == STAGES) slot = 0;
         }
         cp_async_wait<0>();
@@ -719,7 +743,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, ui
         griddep_wait();
         return;
     }
-    const Split split(total, grid1);
+    const Split split(total, grid1, a.chunk);
     if (blockIdx.x < join_blocks) {
         const uint64_t id = (uint64_t)blockIdx.x * (WARPS / WPR) + warp / WPR;
         const uint32_t token = (uint32_t)min(id / a.heads, (uint64_t)a.s.tokens), qh = (uint32_t)(id % a.heads);
@@ -897,21 +921,20 @@ AttnWs layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, u
     return w;
 }
 
-uint64_t kv4_chunks(const AttnParams& p) { return (uint64_t)p.s.max_pages * p.c.page_size / kChunk; }
-
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int CH>
 cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t st)
 {
-    using S = AttnSmem<D, NT>;
+    using S = AttnSmem<D, NT, CH>;
+    p.chunk = 16 * CH;
     static std::atomic<uint64_t> done{0};
-    cudaError_t e = allow_smem(kv4_attention_kernel<T, D, NT>, S::fixed + (kMaxAttnBatch + 1) * 4, done);
+    cudaError_t e = allow_smem(kv4_attention_kernel<T, D, NT, CH>, S::fixed + (kMaxAttnBatch + 1) * 4, done);
     if (e != cudaSuccess) return e;
     // no more blocks than the page tables have room for chunks
     const uint64_t items = (uint64_t)p.s.batch * p.c.kv_heads * ((p.group * p.max_queries + 8 * NT - 1) / (8 * NT));
-    const uint64_t most = items * (kv4_chunks(p) + 1) / kMinChunks + 1;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(most, num_sms * attn_blocks<D, NT>());
+    const uint64_t most = items * ((uint64_t)p.s.max_pages * p.c.page_size + p.chunk) / kMinTokens + 1;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(most, num_sms * attn_blocks<D, NT, CH>());
     const uint32_t line = (p.s.batch + 1) * 4;
-    e = launch_pdl(kv4_attention_kernel<T, D, NT>, dim3(grid), dim3(kThreads), S::fixed + line, st, p);
+    e = launch_pdl(kv4_attention_kernel<T, D, NT, CH>, dim3(grid), dim3(kThreads), S::fixed + line, st, p);
     if (e != cudaSuccess) return e;
     const uint64_t rows = (uint64_t)p.s.tokens * p.heads;
     const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 4 * num_sms) : 0;
@@ -929,10 +952,14 @@ template <typename T, int D>
 cudaError_t run_dim(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t st)
 {
     switch (tiles_of(std::min(p.group * p.max_queries, 1u << 20), D)) {
-        case 1: return run<T, D, 1>(p, accumulate, num_sms, st);
-        case 2: return run<T, D, 2>(p, accumulate, num_sms, st);
+        case 1:
+            // chunks of 32 tokens, where pages hold whole ones: half the steps, and two chains of products to overlap
+            if constexpr (D < 256)
+                if (p.c.page_size % 32 == 0) return run<T, D, 1, 2>(p, accumulate, num_sms, st);
+            return run<T, D, 1, 1>(p, accumulate, num_sms, st);
+        case 2: return run<T, D, 2, 1>(p, accumulate, num_sms, st);
         default:
-            if constexpr (D < 256) return run<T, D, 4>(p, accumulate, num_sms, st);
+            if constexpr (D < 256) return run<T, D, 4, 1>(p, accumulate, num_sms, st);
             return cudaErrorInvalidValue;
     }
 }
