@@ -42,8 +42,6 @@ namespace b2sq {
 
 namespace {
 
-constexpr uint32_t kWarps = 4;
-constexpr uint32_t kThreads = kWarps * 32;
 constexpr uint32_t kMinTokens = 64;  // of a block's share: fewer leave too little to do between its start and its join
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -62,7 +60,12 @@ struct AttnParams {
     float* scores;         // [batch * kv_heads][positions][row_pad], for the weights
 };
 
-// Blocks a SM that registers (and shared memory) leave room for.
+// Warps of a block, and blocks a SM that registers and shared memory leave room for.
+template <int D, int NT, int CH>
+constexpr uint32_t attn_warps()
+{
+    return 4;  // one a scheduler: five were slower (60.5 us against 57.5 at 2 x 100001 tokens)
+}
 template <int D, int NT, int CH>
 constexpr uint32_t attn_blocks()
 {
@@ -74,14 +77,15 @@ constexpr uint32_t kMaxBlocks = 6;
 template <int D, int NT, int CH>
 struct AttnSmem {
     static constexpr uint32_t rows = 8 * NT;
+    static constexpr uint32_t warps = attn_warps<D, NT, CH>();
     static constexpr uint32_t data = CH * 16 * D / 2;               // a chunk's key nibbles
     static constexpr uint32_t scales = CH * 16 * (D / 64) * 4;      // and their steps and bases
     static constexpr uint32_t stage = 2 * (data + scales);
     static constexpr uint32_t stages = D == 64 ? (CH == 2 ? 4 : 6) : D == 128 ? (CH == 2 ? 3 : 4) : 3;
-    static constexpr uint32_t ring = kWarps * stages * stage;
+    static constexpr uint32_t ring = warps * stages * stage;
     static constexpr uint32_t q = rows * D * 2;
     static constexpr uint32_t pitch = D + 2;  // of a row in the join of the warps, which uses the drained ring
-    static_assert(kWarps * 8 * pitch * 4 <= ring, "ring too small for the join");
+    static_assert(warps * 8 * pitch * 4 <= ring, "ring too small for the join");
     static constexpr uint32_t fixed = ring + q;
 };
 
@@ -234,9 +238,10 @@ __device__ __forceinline__ uint32_t seq_of(const uint32_t* ustart, uint32_t batc
 }
 
 template <typename T, int D, int NT, int CH>
-__global__ void __launch_bounds__(kThreads, attn_blocks<D, NT, CH>()) kv4_attention_kernel(AttnParams a)
+__global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, NT, CH>()) kv4_attention_kernel(AttnParams a)
 {
     using S = AttnSmem<D, NT, CH>;
+    constexpr uint32_t kWarps = S::warps, kThreads = kWarps * 32;
     constexpr uint32_t CHUNK = 16 * CH, NG = D / 64, CPR = D / 32, ROWS = 8 * NT, STAGES = S::stages, SC = S::scales / 16;
     // fp16 results want more bits of the probabilities than fp16 has: a second operand holds what the first leaves
     constexpr bool SPLIT = std::is_same<T, __half>::value;
@@ -408,51 +413,50 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT, CH>()) kv4_attent
             const int t0 = (int)(c * CHUNK + g);
             bool see[CH][NT][4];
             float s[CH][NT][4];  // score - m
-            float vs[CH][2][NG], vz[CH][2][NG];
-            float top = -INFINITY, step_top = 0.f;
+            uint32_t vw[CH][2][NG];  // the values' steps and bases
+            float top = -INFINITY;
+            float acc[CH][NG][NT][4];
 #pragma unroll
-            for (int ch = 0; ch < CH; ++ch) {
-                float acc[NG][NT][4];
+            for (uint32_t gr = 0; gr < NG; ++gr) {
+                uint32_t w[CH][4];
 #pragma unroll
-                for (uint32_t gr = 0; gr < NG; ++gr) {
-                    uint32_t w[4];
-                    ldsm4(base + ch * 8 * D + ((gr * 2 + (lane >> 4)) ^ sw) * 16, w);
+                for (int ch = 0; ch < CH; ++ch) ldsm4(base + ch * 8 * D + ((gr * 2 + (lane >> 4)) ^ sw) * 16, w[ch]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const uint4* qf = reinterpret_cast<const uint4*>(q_frag) + ((nt * NG + gr) * 2) * 32 + lane;
-                        const uint4 q0 = qf[0], q1 = qf[32];
-                        mma_f16_first(acc[gr][nt], nibbles<0>(w[0]), nibbles<0>(w[1]), nibbles<0>(w[2]), nibbles<0>(w[3]),
-                                      q0.x, q0.y);
-                        mma_f16(acc[gr][nt], nibbles<1>(w[0]), nibbles<1>(w[1]), nibbles<1>(w[2]), nibbles<1>(w[3]), q0.z,
-                                q0.w);
-                        mma_f16(acc[gr][nt], nibbles<2>(w[0]), nibbles<2>(w[1]), nibbles<2>(w[2]), nibbles<2>(w[3]), q1.x,
-                                q1.y);
-                        mma_f16(acc[gr][nt], nibbles<3>(w[0]), nibbles<3>(w[1]), nibbles<3>(w[2]), nibbles<3>(w[3]), q1.z,
-                                q1.w);
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint4* qf = reinterpret_cast<const uint4*>(q_frag) + ((nt * NG + gr) * 2) * 32 + lane;
+                    const uint4 q0 = qf[0], q1 = qf[32];
+#pragma unroll
+                    for (int ch = 0; ch < CH; ++ch) {
+                        const uint32_t(&k)[4] = w[ch];
+                        float(&d)[4] = acc[ch][gr][nt];
+                        mma_f16_first(d, nibbles<0>(k[0]), nibbles<0>(k[1]), nibbles<0>(k[2]), nibbles<0>(k[3]), q0.x, q0.y);
+                        mma_f16(d, nibbles<1>(k[0]), nibbles<1>(k[1]), nibbles<1>(k[2]), nibbles<1>(k[3]), q0.z, q0.w);
+                        mma_f16(d, nibbles<2>(k[0]), nibbles<2>(k[1]), nibbles<2>(k[2]), nibbles<2>(k[3]), q1.x, q1.y);
+                        mma_f16(d, nibbles<3>(k[0]), nibbles<3>(k[1]), nibbles<3>(k[2]), nibbles<3>(k[3]), q1.z, q1.w);
                     }
                 }
+            }
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch) {
                 // thread: tokens g and g + 8, rows 2 tig and 2 tig + 1 of every eight
                 float2 ksz[2][NG];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t kw[NG], vw[NG];
+                    uint32_t kw[NG];
                     lds_words<NG>(stage + 2 * S::data + (ch * 16 + g + 8 * h) * NG * 4, kw);
-                    lds_words<NG>(stage + 2 * S::data + S::scales + (ch * 16 + g + 8 * h) * NG * 4, vw);
+                    lds_words<NG>(stage + 2 * S::data + S::scales + (ch * 16 + g + 8 * h) * NG * 4, vw[ch][h]);
 #pragma unroll
-                    for (uint32_t gr = 0; gr < NG; ++gr) {
-                        h2_to_f2(kw[gr], ksz[h][gr].x, ksz[h][gr].y);
-                        h2_to_f2(vw[gr], vs[ch][h][gr], vz[ch][h][gr]);
-                    }
+                    for (uint32_t gr = 0; gr < NG; ++gr) h2_to_f2(kw[gr], ksz[h][gr].x, ksz[h][gr].y);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int h = i >> 1, x = i & 1;
-                        float dot = acc[0][nt][i] * ksz[h][0].x, off = fmaf(qsum[nt][x][0], ksz[h][0].y, -m[nt][x]);
+                        float dot = acc[ch][0][nt][i] * ksz[h][0].x, off = fmaf(qsum[nt][x][0], ksz[h][0].y, -m[nt][x]);
 #pragma unroll
                         for (uint32_t gr = 1; gr < NG; ++gr) {
-                            dot = fmaf(acc[gr][nt][i], ksz[h][gr].x, dot);
+                            dot = fmaf(acc[ch][gr][nt][i], ksz[h][gr].x, dot);
                             off = fmaf(qsum[nt][x][gr], ksz[h][gr].y, off);
                         }
                         see[ch][nt][i] = FULL || t0 + 16 * ch + 8 * h < vis[nt][x];
@@ -472,19 +476,18 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT, CH>()) kv4_attent
                         }
                 }
             }
-            // the steps over the group's power of two (unseen tokens may hold anything: only read where see[])
-            float pw[CH][2][NG];
+            // largest steps of the groups (unseen tokens may hold anything; a NaN drops out)
+            bool wide = false;
 #pragma unroll
-            for (int ch = 0; ch < CH; ++ch)
+            for (uint32_t gr = 0; gr < NG; ++gr) {
+                __half2 hm = __habs2(*reinterpret_cast<const __half2*>(&vw[0][0][gr]));
 #pragma unroll
-                for (uint32_t gr = 0; gr < NG; ++gr)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        pw[ch][h][gr] = vs[ch][h][gr] * ref[gr];
-                        step_top = fmaxf(step_top, fabsf(pw[ch][h][gr]));
-                    }
+                for (int i = 1; i < 2 * CH; ++i)
+                    hm = __hmax2(hm, __habs2(*reinterpret_cast<const __half2*>(&vw[i / 2][i & 1][gr])));
+                wide |= __low2float(hm) * ref[gr] > 512.f;
+            }
             // p may reach 2^6 and a step twice its power of two before the references are moved
-            if (__any_sync(0xffffffffu, top > 6.f || step_top > 512.f || seen != (1u << (2 * NT)) - 1)) {
+            if (__any_sync(0xffffffffu, top > 6.f || wide || seen != (1u << (2 * NT)) - 1)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT, CH>()) kv4_attent
                     for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float st = fabsf(vs[ch][h][gr]);
+                            const float st = fabsf(__low2float(*reinterpret_cast<const __half2*>(&vw[ch][h][gr])));
                             if (t0 + 16 * ch + 8 * h < (int)sh.vis && st < INFINITY) mx = fmaxf(mx, st);
                         }
 #pragma unroll
@@ -532,10 +535,6 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT, CH>()) kv4_attent
                         const float fresh = __uint_as_float((262u - (__float_as_uint(mx) >> 23)) << 23);
                         const float f = fresh / ref[gr];
                         ref[gr] = fresh;
-#pragma unroll
-                        for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) pw[ch][h][gr] = vs[ch][h][gr] * fresh;
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -548,6 +547,15 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT, CH>()) kv4_attent
 #pragma unroll
             for (int ch = 0; ch < CH; ++ch) {
                 // probabilities
+                float pw[2][NG], vz[2][NG];  // steps over the group's power of two, and bases
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (uint32_t gr = 0; gr < NG; ++gr) {
+                        float st;
+                        h2_to_f2(vw[ch][h][gr], st, vz[h][gr]);
+                        pw[h][gr] = st * ref[gr];
+                    }
                 uint32_t pb[NG][NT][2];
                 [[maybe_unused]] uint32_t pb2[SPLIT ? NG : 1][NT][2];
 #pragma unroll
@@ -564,8 +572,8 @@ __global__ void __launch_bounds__(kThreads, attn_blocks<D, NT, CH>()) kv4_attent
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int h = i >> 1, x = i & 1;
-                            if (FULL || see[ch][nt][i]) zs[nt][x][gr] = fmaf(p[i], vz[ch][h][gr], zs[nt][x][gr]);
-                            pv[i] = FULL || see[ch][nt][i] ? p[i] * pw[ch][h][gr] : 0.f;
+                            if (FULL || see[ch][nt][i]) zs[nt][x][gr] = fmaf(p[i], vz[h][gr], zs[nt][x][gr]);
+                            pv[i] = FULL || see[ch][nt][i] ? p[i] * pw[h][gr] : 0.f;
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -934,7 +942,7 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
     const uint64_t most = items * ((uint64_t)p.s.max_pages * p.c.page_size + p.chunk) / kMinTokens + 1;
     const uint32_t grid = (uint32_t)std::min<uint64_t>(most, num_sms * attn_blocks<D, NT, CH>());
     const uint32_t line = (p.s.batch + 1) * 4;
-    e = launch_pdl(kv4_attention_kernel<T, D, NT, CH>, dim3(grid), dim3(kThreads), S::fixed + line, st, p);
+    e = launch_pdl(kv4_attention_kernel<T, D, NT, CH>, dim3(grid), dim3(S::warps * 32), S::fixed + line, st, p);
     if (e != cudaSuccess) return e;
     const uint64_t rows = (uint64_t)p.s.tokens * p.heads;
     const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 4 * num_sms) : 0;
