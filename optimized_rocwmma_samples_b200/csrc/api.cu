@@ -562,7 +562,8 @@ b2sq_status b2sq_gemm_i8_grouped(uint32_t groups, uint32_t rows, uint32_t n, uin
 
 namespace {
 constexpr uint32_t kMaxMoeRoutes = 4096;
-constexpr uint32_t kMaxMoeDepth = 131072;  // 127 * 127 * depth fits in int32
+constexpr uint32_t kMaxMoeHidden = 16384;  // eight int8 rows of it fit in shared memory beside the ring
+constexpr uint32_t kMaxMoeInter = 131072;  // 127 * 127 * inter fits in int32
 
 b2sq_status validate_moe_layer(const char* fn, uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t experts,
                                uint32_t topk)
@@ -570,8 +571,9 @@ b2sq_status validate_moe_layer(const char* fn, uint32_t tokens, uint32_t hidden,
     if (experts == 0 || experts > 1024) return fail(B2SQ_ERR_INVALID_ARG, "%s: experts must be in [1, 1024]", fn);
     if (topk == 0) return fail(B2SQ_ERR_INVALID_ARG, "%s: topk must be >= 1", fn);
     if (hidden == 0 || inter == 0) return fail(B2SQ_ERR_INVALID_ARG, "%s: hidden and inter must be >= 1", fn);
-    if (hidden % 16 || inter % 16 || hidden > kMaxMoeDepth || inter > kMaxMoeDepth)
-        return fail(B2SQ_ERR_UNSUPPORTED, "%s: hidden and inter must be multiples of 16 up to %u", fn, kMaxMoeDepth);
+    if (hidden % 16 || inter % 16 || hidden > kMaxMoeHidden || inter > kMaxMoeInter)
+        return fail(B2SQ_ERR_UNSUPPORTED, "%s: hidden and inter must be multiples of 16, up to %u and %u", fn,
+                    kMaxMoeHidden, kMaxMoeInter);
     if ((uint64_t)tokens * topk > kMaxMoeRoutes)
         return fail(B2SQ_ERR_UNSUPPORTED, "%s: tokens * topk above %u (use moe_sorting and gemm_i8_grouped)", fn,
                     kMaxMoeRoutes);

@@ -8,12 +8,29 @@
 //   out[t]  = sum over k of topk_w[t][k] * d, in slot order
 // A route whose id is outside [0, experts) adds nothing.
 //
-// Four plain kernels: quantise x, one warp per (route, gate and up row),
-// quantise h, one warp per (token, output).
+// What bounds it is reading the weights of the experts that were chosen, once.
+// Blocks of an expert's routes (up to 8 NT of them) meet its weight rows in
+// units of 16 rows; every block of the grid (one an SM) takes an equal run of
+// the units, which lie one after another in memory.  Weights stream through a
+// ring of cp.async stages in which each of the eight warps keeps its own
+// 16 x 128 byte tiles (every eighth of the unit's), so that no barrier stands
+// between loading and multiplying; the routes' int8 rows lie in shared memory.
+// mma.m16n8k32: weight rows are the 16, routes the 8 columns.  The warps' int32
+// sums meet in shared memory by integer adds, one barrier a unit.
+//
+//   moe_up_kernel    quantises x for its expert, multiplies gate and up rows
+//                    (8 + 8 a unit, so one thread has both), applies SwiGLU,
+//                    leaves h in fp32 and the largest |h| it saw of each route
+//   moe_down_kernel  starts streaming w2 before the first kernel is done, takes
+//                    the maxima, quantises its slice of h, multiplies; slices of
+//                    the inner dimension are added as integers (exact, any order)
+//   moe_sum_kernel   scales, weighs and adds the slots
 #include "common.cuh"
 #include "kernels.h"
 #include "sq_math.cuh"
 
+#include <algorithm>
+#include <atomic>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -21,154 +38,649 @@ namespace b2sq {
 
 namespace {
 
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kWarps = 8;
+constexpr uint32_t kThreads = kWarps * 32;
+constexpr uint32_t kTile = 2048;         // bytes of a warp's stage: 16 rows of 128
+constexpr uint32_t kSliceMost = 4096;    // inner elements of h that a block of the second kernel holds at a time
+constexpr uint32_t kSmemMost = 231424;   // dynamic shared memory: 227 KB, less 1 KB for what is static
 
-__device__ __forceinline__ float block_max(float v)
+struct Lists {
+    uint16_t *first, *block, *order;  // [E + 1] first route and first block of an expert, [R] routes by expert
+};
+
+struct Params {
+    MoeLayer m;
+    float* h;        // [R][inter]
+    float* part_max; // [blocks of the first kernel][R]
+    float* rs2;      // [R]
+    int32_t* acc;    // [R][hidden]
+    uint32_t grid1, slices, slice;  // of the second kernel: slices of `slice` inner elements
+};
+
+// Shared memory of both products: the ring, the routes' rows, the sums, the lists.
+template <int NT, int STAGES>
+struct Smem {
+    static constexpr uint32_t ring = kWarps * STAGES * kTile;
+    static constexpr uint32_t pitch = NT == 1 ? 8 : NT == 2 ? 24 : 40;  // ints of a row of sums: two-way bank conflicts at most
+    static constexpr uint32_t sums = 2 * 16 * pitch * 4;
+    __host__ __device__ static constexpr uint32_t row_pitch(uint32_t k) { return (k + 127) / 128 * 128 + 16; }
+    __host__ __device__ static constexpr uint32_t rows(uint32_t k) { return 8 * NT * row_pitch(k); }
+    __host__ __device__ static constexpr uint32_t lists(uint32_t experts, uint32_t routes)
+    {
+        return (2 * (experts + 1) + routes) * 2;
+    }
+    static constexpr uint64_t total(uint32_t k, uint32_t experts, uint32_t routes)
+    {
+        return (uint64_t)ring + rows(k) + sums + lists(experts, routes);
+    }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes)
 {
-    __shared__ float part[kThreads / 32];
-    for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x / 32] = v;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T>
+__device__ __forceinline__ float2 pair_to_f2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 pair_to_f2<__half>(uint32_t w)
+{
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 pair_to_f2<__nv_bfloat16>(uint32_t w)
+{
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Routes grouped by expert, in their own order, and blocks of at most `most`
+// routes; every block of both kernels computes the same lists.  `scratch`:
+// [R] uint16 and [E] uint32 of shared memory that is free until the next barrier.
+__device__ __forceinline__ void make_lists(const MoeLayer& m, uint32_t most, const Lists& l, uint32_t* scratch)
+{
+    __shared__ uint32_t warp_rows[kWarps], warp_blocks[kWarps];
+    const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31, routes = m.tokens * m.topk;
+    uint32_t* count = scratch;
+    uint16_t* rank = reinterpret_cast<uint16_t*>(scratch + m.experts);
+    for (uint32_t e = tid; e < m.experts; e += kThreads) count[e] = 0;
     __syncthreads();
-    v = part[0];
-    for (uint32_t i = 1; i < kThreads / 32; ++i) v = fmaxf(v, part[i]);
-    return v;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) moe_quant_x(MoeLayer m, int8_t* xq, float* rs)
-{
-    griddep_wait();
-    griddep_launch_dependents();
-    const uint32_t r = blockIdx.x;
-    const int32_t e = m.topk_ids[r];
-    if ((uint32_t)e >= m.experts) return;
-    const T* x = static_cast<const T*>(m.x) + (r / m.topk) * m.x_stride;
-    const float* s = m.smooth1 + (uint64_t)e * m.hidden;
-    float mx = 0.f;
-    for (uint32_t i = threadIdx.x; i < m.hidden; i += kThreads) mx = fmaxf(mx, fabsf(__fmul_rn((float)x[i], s[i])));
-    const float sc = row_scale_of(block_max(mx), m.qmax), inv = inv_scale_of(sc);
-    for (uint32_t i = threadIdx.x; i < m.hidden; i += kThreads)
-        xq[(uint64_t)r * m.hidden + i] = quant1(__fmul_rn((float)x[i], s[i]), inv, m.qmax);
-    if (threadIdx.x == 0) rs[r] = sc;
-}
-
-__device__ __forceinline__ int warp_dot(const int8_t* a, const int8_t* b, uint32_t k, uint32_t lane)
-{
-    int acc = 0;
-    const int4* av = reinterpret_cast<const int4*>(a);
-    const int4* bv = reinterpret_cast<const int4*>(b);
-    for (uint32_t i = lane; i < k / 16; i += 32) {
-        const int4 x = av[i], y = bv[i];
-        acc = __dp4a(x.x, y.x, acc);
-        acc = __dp4a(x.y, y.y, acc);
-        acc = __dp4a(x.z, y.z, acc);
-        acc = __dp4a(x.w, y.w, acc);
+    if (warp == 0)
+        for (uint32_t base = 0; base < routes; base += 32) {
+            const uint32_t r = base + lane;
+            const uint32_t e = r < routes ? (uint32_t)__ldg(m.topk_ids + r) : 0xffffffffu;
+            const bool valid = e < m.experts;
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            const uint32_t before = valid ? count[e] : 0;
+            __syncwarp();
+            if (valid) {
+                rank[r] = (uint16_t)(before + __popc(same & ((1u << lane) - 1)));
+                if (lane == __ffs(same) - 1) count[e] = before + __popc(same);
+            }
+            __syncwarp();
+        }
+    __syncthreads();
+    uint32_t row0 = 0, block0 = 0;
+    for (uint32_t base = 0; base < m.experts; base += kThreads) {
+        const uint32_t e = base + tid;
+        const uint32_t n = e < m.experts ? count[e] : 0, b = (n + most - 1) / most;
+        uint32_t ni = n, bi = b;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, ni, off), y = __shfl_up_sync(0xffffffffu, bi, off);
+            if (lane >= (uint32_t)off) {
+                ni += x;
+                bi += y;
+            }
+        }
+        if (lane == 31) {
+            warp_rows[warp] = ni;
+            warp_blocks[warp] = bi;
+        }
+        __syncthreads();
+        uint32_t rb = row0, bb = block0;
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            if (w < warp) {
+                rb += warp_rows[w];
+                bb += warp_blocks[w];
+            }
+            row0 += warp_rows[w];
+            block0 += warp_blocks[w];
+        }
+        if (e < m.experts) {
+            l.first[e] = (uint16_t)(rb + ni - n);
+            l.block[e] = (uint16_t)(bb + bi - b);
+        }
+        __syncthreads();
     }
-    for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-    return acc;
+    if (tid == 0) {
+        l.first[m.experts] = (uint16_t)row0;
+        l.block[m.experts] = (uint16_t)block0;
+    }
+    for (uint32_t r = tid; r < routes; r += kThreads) {
+        const uint32_t e = (uint32_t)__ldg(m.topk_ids + r);
+        if (e < m.experts) l.order[l.first[e] + rank[r]] = (uint16_t)r;
+    }
+    __syncthreads();
 }
 
-__global__ void __launch_bounds__(kThreads) moe_gate_up(MoeLayer m, const int8_t* xq, const float* rs, float* h)
+// The expert that block `b` belongs to.
+__device__ __forceinline__ uint32_t expert_of(const Lists& l, uint32_t experts, uint32_t b)
 {
+    uint32_t lo = 0, hi = experts;  // the last expert that starts at or before b
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (l.block[mid] <= b)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// Equal runs of `total` units for `blocks` blocks: the first `rest` get one more.
+struct Split {
+    uint32_t each, rest;
+    __device__ __forceinline__ Split(uint32_t total, uint32_t blocks) : each(total / blocks), rest(total % blocks) {}
+    __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * each + min(i, rest); }
+    __device__ __forceinline__ uint32_t block_of(uint32_t u) const
+    {
+        const uint32_t big = rest * (each + 1);
+        return u < big ? u / (each + 1) : rest + (u - big) / each;
+    }
+};
+
+// A warp's share of a unit: int32 products of 16 weight rows with the block's routes over its 128-byte pieces.
+template <int NT, int STAGES, typename Next>
+__device__ __forceinline__ void unit_product(uint32_t pieces, uint32_t live, uint32_t ring_base, uint32_t rows_base,
+                                             uint32_t row_pitch, uint32_t& slot, int (&acc)[NT][4], Next&& next)
+{
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const uint32_t arow = (lane & 7) + ((lane >> 3) & 1) * 8, asel = lane >> 4;
+    const uint32_t brow = rows_base + (lane & 7) * row_pitch + (lane >> 3) * 16;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[nt][i] = 0;
+    for (uint32_t p = warp; p < pieces; p += kWarps) {
+        cp_async_wait<STAGES - 2>();
+        __syncwarp();
+        // the slot that the last step freed takes the tile STAGES - 1 steps ahead
+        next();
+        const uint32_t a_at = ring_base + slot * kTile + arow * 128;
+        if (++slot == STAGES) slot = 0;
+        uint32_t a[4][4];
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q) ldsm4(a_at + (((q * 2 + asel) ^ (arow & 7)) * 16), a[q]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            if (nt == 0 || nt < live) {
+                const uint32_t b_at = brow + nt * 8 * row_pitch + p * 128;
+                uint32_t b[2][4];
+                ldsm4(b_at, b[0]);
+                ldsm4(b_at + 64, b[1]);
+                mma_s8(acc[nt], a[0], b[0][0], b[0][1]);
+                mma_s8(acc[nt], a[1], b[0][2], b[0][3]);
+                mma_s8(acc[nt], a[2], b[1][0], b[1][1]);
+                mma_s8(acc[nt], a[3], b[1][2], b[1][3]);
+            }
+    }
+}
+
+// Adds the warps' products into the unit's sums in shared memory (zero before).
+template <int NT, uint32_t PITCH>
+__device__ __forceinline__ void add_sums(int* sums, const int (&acc)[NT][4], uint32_t live)
+{
+    const uint32_t lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+        if (nt == 0 || nt < live) {
+            int* at = sums + g * PITCH + nt * 8 + 2 * tig;
+            atomicAdd(at, acc[nt][0]);
+            atomicAdd(at + 1, acc[nt][1]);
+            atomicAdd(at + 8 * PITCH, acc[nt][2]);
+            atomicAdd(at + 8 * PITCH + 1, acc[nt][3]);
+        }
+}
+
+// Gate and up rows.  Units: block of routes x 8 inner elements.
+template <typename T, int NT, int STAGES>
+__global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
+{
+    using S = Smem<NT, STAGES>;
+    extern __shared__ __align__(128) uint8_t moe_smem[];
+    __shared__ float rs1[8 * NT];
+    __shared__ uint32_t top[8 * NT];
+    __shared__ float warp_max[kWarps];
+    const MoeLayer& m = p.m;
+    const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const uint32_t routes = m.tokens * m.topk, H = m.hidden, I = m.inter;
+    const uint32_t row_pitch = S::row_pitch(H);
+    uint8_t* rows = moe_smem + S::ring;
+    int* sums = reinterpret_cast<int*>(rows + S::rows(H));
+    uint16_t* list = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(sums) + S::sums);
+    const Lists l{list, list + m.experts + 1, list + 2 * (m.experts + 1)};
+
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t r = blockIdx.y, j = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
-    const int32_t e = m.topk_ids[r];
-    if ((uint32_t)e >= m.experts || j >= m.inter) return;
-    const int8_t* w = m.w13 + (uint64_t)e * 2 * m.inter * m.hidden;
-    const int8_t* x = xq + (uint64_t)r * m.hidden;
-    const float* s = m.s13 + (uint64_t)e * 2 * m.inter;
-    const float g = (float)warp_dot(w + (uint64_t)j * m.hidden, x, m.hidden, lane) * (rs[r] * s[j]);
-    const float u = (float)warp_dot(w + (uint64_t)(m.inter + j) * m.hidden, x, m.hidden, lane) * (rs[r] * s[m.inter + j]);
-    if (lane == 0) h[(uint64_t)r * m.inter + j] = g / (1.f + expf(-g)) * u * m.smooth2[(uint64_t)e * m.inter + j];
+    make_lists(m, 8 * NT, l, reinterpret_cast<uint32_t*>(moe_smem));
+    if (p.slices > 1)  // the second kernel's sums start from zero
+        for (uint64_t i = (uint64_t)blockIdx.x * kThreads + tid; i < (uint64_t)routes * H / 4; i += (uint64_t)gridDim.x * kThreads)
+            reinterpret_cast<int4*>(p.acc)[i] = make_int4(0, 0, 0, 0);
+    for (uint32_t i = tid; i < 2 * 16 * S::pitch; i += kThreads) sums[i] = 0;
+
+    const uint32_t per_block = I / 8, total = l.block[m.experts] * per_block;
+    const Split split(total, gridDim.x);
+    const uint32_t begin = split.begin(blockIdx.x), end = split.begin(blockIdx.x + 1);
+    if (begin == end) return;
+
+    // producer: this warp's next tile (unit, piece) and its addresses
+    const uint32_t pieces = (H + 127) / 128;
+    const uint32_t ring_base = smem_u32(moe_smem) + warp * STAGES * kTile;
+    const uint32_t lrow = lane / 8, lchunk = lane & 7;
+    uint32_t pu = begin, pj = begin % per_block, pp = warp, pslot = 0;
+    const int8_t* src = nullptr;
+    auto place = [&]() {
+        const uint32_t e = expert_of(l, m.experts, pu / per_block);
+        src = m.w13 + ((uint64_t)e * 2 * I + pj * 8 + lrow) * H + lchunk * 16;
+    };
+    auto load = [&]() {
+        if (pu < end && pp < pieces) {
+            const uint32_t at = pp * 128 + lchunk * 16;
+            const uint32_t bytes = at < H ? 16u : 0u;
+            const uint32_t dst = ring_base + pslot * kTile;
+            const int8_t* s = src + pp * 128;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t r = i * 4 + lrow;  // 0..7 gate, 8..15 up
+                const int8_t* row = s + (uint64_t)((i & 1) * 4 + (i >> 1) * I) * H;
+                // (the last piece may reach past the row: nothing is read there)
+                cp_async16(dst + r * 128 + ((lchunk ^ (r & 7)) * 16), bytes ? row : m.w13, bytes);
+            }
+            pp += kWarps;
+            if (pp >= pieces) {
+                pp = warp;
+                ++pu;
+                if (++pj == per_block) pj = 0;
+                if (pu < end) {
+                    if (pj == 0)
+                        place();
+                    else
+                        src += (uint64_t)8 * H;
+                }
+            }
+        }
+        cp_async_commit();
+        if (++pslot == STAGES) pslot = 0;
+    };
+    place();
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) load();
+
+    uint32_t slot = 0, buf = 0;
+    uint32_t b = begin / per_block, j = begin % per_block;
+    for (uint32_t u = begin; u < end; ++b, j = 0) {
+        const uint32_t e = expert_of(l, m.experts, b);
+        const uint32_t r0 = l.first[e] + (b - l.block[e]) * 8 * NT;
+        const uint32_t count = min(8u * NT, (uint32_t)l.first[e + 1] - r0);
+        // quantise the block's tokens: 8, 4, 2 or 1 warps a token
+        {
+            const uint32_t wpt = count > 4 ? 1 : count > 2 ? 2 : count > 1 ? 4 : 8, per = kWarps / wpt;
+            const float* sm = m.smooth1 + (uint64_t)e * H;
+            for (uint32_t t0 = 0; t0 < count; t0 += per) {
+                const uint32_t t = t0 + warp / wpt;
+                const bool on = t < count;
+                const T* x = static_cast<const T*>(m.x) + (uint64_t)(on ? l.order[r0 + t] / m.topk : 0) * m.x_stride;
+                const uint32_t start = (warp % wpt) * 256 + lane * 8, stride = wpt * 256;
+                float mx = 0.f;
+                if (on)
+#pragma unroll 4
+                    for (uint32_t k = start; k < H; k += stride) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(x + k);
+                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 f = pair_to_f2<T>(ww[i]);
+                            mx = fmaxf(mx, fabsf(__fmul_rn(f.x, __ldg(sm + k + 2 * i))));
+                            mx = fmaxf(mx, fabsf(__fmul_rn(f.y, __ldg(sm + k + 2 * i + 1))));
+                        }
+                    }
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                __syncthreads();  // (also: the last block's rows, maxima and warp_max are read)
+                if (lane == 0) warp_max[warp] = mx;
+                __syncthreads();
+                for (uint32_t w = warp / wpt * wpt; w < warp / wpt * wpt + wpt; ++w) mx = fmaxf(mx, warp_max[w]);
+                const float rs = row_scale_of(mx, m.qmax), inv = inv_scale_of(rs);
+                if (on) {
+#pragma unroll 2
+                    for (uint32_t k = start; k < H; k += stride) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(x + k);
+                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+                        int8_t q[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 f = pair_to_f2<T>(ww[i]);
+                            q[2 * i] = quant1(__fmul_rn(f.x, __ldg(sm + k + 2 * i)), inv, m.qmax);
+                            q[2 * i + 1] = quant1(__fmul_rn(f.y, __ldg(sm + k + 2 * i + 1)), inv, m.qmax);
+                        }
+                        *reinterpret_cast<uint2*>(rows + t * row_pitch + k) =
+                            make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+                    }
+                    if (lane == 0 && warp % wpt == 0) {
+                        rs1[t] = rs;
+                        top[t] = 0;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        const uint32_t live = (count + 7) / 8;
+        const uint32_t tok = tid / 8, jj = tid & 7;  // of the epilogue
+        const bool mine = tok < count;
+        const uint32_t route = mine ? l.order[r0 + tok] : 0;
+        for (; j < per_block && u < end; ++j, ++u) {
+            float sg = 0.f, su = 0.f, s2 = 0.f;
+            if (mine) {
+                const uint64_t at = (uint64_t)e * 2 * I + j * 8 + jj;
+                sg = __ldg(m.s13 + at);
+                su = __ldg(m.s13 + at + I);
+                s2 = __ldg(m.smooth2 + (uint64_t)e * I + j * 8 + jj);
+            }
+            int acc[NT][4];
+            unit_product<NT, STAGES>(pieces, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
+            int* sum = sums + buf * 16 * S::pitch;
+            buf ^= 1;
+            add_sums<NT, S::pitch>(sum, acc, live);
+            __syncthreads();
+            // (the other buffer's readers are past this barrier too: it is free and zero again)
+            float hv = 0.f;
+            if (mine) {
+                int* at = sum + jj * S::pitch + tok;
+                const float g = __fmul_rn((float)at[0], __fmul_rn(rs1[tok], sg));
+                const float v = __fmul_rn((float)at[8 * S::pitch], __fmul_rn(rs1[tok], su));
+                hv = g / (1.f + expf(-g)) * v * s2;
+                p.h[(uint64_t)route * I + j * 8 + jj] = hv;
+            }
+            if (tid < 64 * live) {  // by the thread that read it
+                sum[jj * S::pitch + tok] = 0;
+                sum[(jj + 8) * S::pitch + tok] = 0;
+            }
+            float mx = fmaxf(fabsf(hv), 0.f);  // a NaN drops out, as in smoothquant
+#pragma unroll
+            for (int off = 4; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            if (mine && jj == 0) top[tok] = max(top[tok], __float_as_uint(mx));  // one thread a route
+        }
+        // (every thread reads back what it wrote itself)
+        if (mine && jj == 0) p.part_max[(uint64_t)blockIdx.x * routes + route] = __uint_as_float(top[tok]);
+    }
+    cp_async_wait<0>();
 }
 
-__global__ void __launch_bounds__(kThreads) moe_quant_h(MoeLayer m, const float* h, int8_t* hq, float* rs)
+// Down rows.  Units: (block of routes, slice of the inner dimension) x 16 rows.
+template <int NT, int STAGES>
+__global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
 {
+    using S = Smem<NT, STAGES>;
+    extern __shared__ __align__(128) uint8_t moe_smem[];
+    __shared__ float inv2[8 * NT];
+    const MoeLayer& m = p.m;
+    const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const uint32_t routes = m.tokens * m.topk, H = m.hidden, I = m.inter;
+    const uint32_t row_pitch = S::row_pitch(p.slice);
+    uint8_t* rows = moe_smem + S::ring;
+    int* sums = reinterpret_cast<int*>(rows + S::rows(p.slice));
+    uint16_t* list = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(sums) + S::sums);
+    const Lists l{list, list + m.experts + 1, list + 2 * (m.experts + 1)};
+
+    // before the wait: only what the layer's inputs say (the first kernel has waited for them)
+    make_lists(m, 8 * NT, l, reinterpret_cast<uint32_t*>(moe_smem));
+    for (uint32_t i = tid; i < 2 * 16 * S::pitch; i += kThreads) sums[i] = 0;
+    const uint32_t per_slice = H / 16, per_block = per_slice * p.slices;
+    const uint32_t total = l.block[m.experts] * per_block;
+    const Split split(total, gridDim.x);
+    const uint32_t begin = split.begin(blockIdx.x), end = split.begin(blockIdx.x + 1);
+
+    const uint32_t ring_base = smem_u32(moe_smem) + warp * STAGES * kTile;
+    const uint32_t lrow = lane / 8, lchunk = lane & 7;
+    uint32_t pu = begin, pr = begin % per_slice, pp = warp, pslot = 0;  // unit, row unit, piece
+    const int8_t* src = nullptr;
+    uint32_t left = 0, ppieces = 0;  // inner elements and pieces of the producer's slice
+    auto place = [&]() {
+        const uint32_t bs = pu / per_slice, e = expert_of(l, m.experts, bs / p.slices), k0 = bs % p.slices * p.slice;
+        left = min(p.slice, I - k0);
+        ppieces = (left + 127) / 128;
+        src = m.w2 + ((uint64_t)e * H + pr * 16 + lrow) * I + k0 + lchunk * 16;
+    };
+    auto advance = [&]() {
+        pp = warp;
+        ++pu;
+        if (++pr == per_slice) pr = 0;
+        if (pu < end) {
+            if (pr == 0)
+                place();
+            else
+                src += (uint64_t)16 * I;
+        }
+    };
+    auto load = [&]() {
+        if (pu < end) {
+            const uint32_t at = pp * 128 + lchunk * 16;
+            const uint32_t bytes = at < left ? 16u : 0u;
+            const uint32_t dst = ring_base + pslot * kTile;
+            const int8_t* s = src + pp * 128;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t r = i * 4 + lrow;
+                cp_async16(dst + r * 128 + ((lchunk ^ (r & 7)) * 16), bytes ? s + (uint64_t)i * 4 * I : m.w2, bytes);
+            }
+            pp += kWarps;
+            while (pu < end && pp >= ppieces) advance();
+        }
+        cp_async_commit();
+        if (++pslot == STAGES) pslot = 0;
+    };
+    if (begin < end) {
+        place();
+        while (pu < end && pp >= ppieces) advance();
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) load();
+    }
     griddep_wait();
     griddep_launch_dependents();
-    const uint64_t r = blockIdx.x;
-    if ((uint32_t)m.topk_ids[r] >= m.experts) return;
-    float mx = 0.f;
-    for (uint32_t i = threadIdx.x; i < m.inter; i += kThreads) mx = fmaxf(mx, fabsf(h[r * m.inter + i]));
-    const float sc = row_scale_of(block_max(mx), m.qmax), inv = inv_scale_of(sc);
-    for (uint32_t i = threadIdx.x; i < m.inter; i += kThreads) hq[r * m.inter + i] = quant1(h[r * m.inter + i], inv, m.qmax);
-    if (threadIdx.x == 0) rs[r] = sc;
+    if (begin == end) return;
+
+    const uint32_t up_units = I / 8;
+    const Split up(l.block[m.experts] * up_units, p.grid1);
+    uint32_t slot = 0, buf = 0;
+    uint32_t bs = begin / per_slice, ru = begin % per_slice;
+    for (uint32_t u = begin; u < end; ++bs, ru = 0) {
+        const uint32_t b = bs / p.slices, k0 = bs % p.slices * p.slice, depth = min(p.slice, I - k0);
+        const uint32_t e = expert_of(l, m.experts, b);
+        const uint32_t r0 = l.first[e] + (b - l.block[e]) * 8 * NT;
+        const uint32_t count = min(8u * NT, (uint32_t)l.first[e + 1] - r0);
+        __syncthreads();  // the last slice's rows are read
+        {  // the routes' scales: the largest of the maxima of the blocks that made them
+            const uint32_t c0 = up.block_of(b * up_units), c1 = up.block_of(b * up_units + up_units - 1);
+            for (uint32_t t = warp; t < count; t += kWarps) {
+                const uint32_t r = l.order[r0 + t];
+                float mx = 0.f;
+                for (uint32_t c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, p.part_max[(uint64_t)c * routes + r]);
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                const float rs = row_scale_of(mx, m.qmax);
+                if (lane == 0) {
+                    inv2[t] = inv_scale_of(rs);
+                    p.rs2[r] = rs;  // every block that needs it finds the same
+                }
+            }
+        }
+        __syncthreads();
+        {
+            const uint32_t quads = depth / 4;  // depth is a multiple of 16
+#pragma unroll 4
+            for (uint32_t i = tid; i < count * quads; i += kThreads) {
+                const uint32_t t = i / quads, k = (i - t * quads) * 4;
+                const float4 f = *reinterpret_cast<const float4*>(p.h + (uint64_t)l.order[r0 + t] * I + k0 + k);
+                const float inv = inv2[t];
+                *reinterpret_cast<uint32_t*>(rows + t * row_pitch + k) =
+                    pack4(quant1(f.x, inv, m.qmax), quant1(f.y, inv, m.qmax), quant1(f.z, inv, m.qmax),
+                          quant1(f.w, inv, m.qmax));
+            }
+        }
+        __syncthreads();
+        const uint32_t live = (count + 7) / 8, pieces = (depth + 127) / 128;
+        for (; ru < per_slice && u < end; ++ru, ++u) {
+            int acc[NT][4];
+            unit_product<NT, STAGES>(pieces, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
+            int* sum = sums + buf * 16 * S::pitch;
+            buf ^= 1;
+            add_sums<NT, S::pitch>(sum, acc, live);
+            __syncthreads();
+            for (uint32_t i = tid; i < 16 * 8 * live; i += kThreads) {
+                const uint32_t t = i / 16, row = i % 16;
+                const int v = sum[row * S::pitch + t];
+                sum[row * S::pitch + t] = 0;
+                if (t < count) {
+                    int32_t* at = p.acc + (uint64_t)l.order[r0 + t] * H + ru * 16 + row;
+                    if (p.slices > 1)
+                        atomicAdd(at, v);  // integers: exact in any order
+                    else
+                        *at = v;
+                }
+            }
+        }
+    }
+    cp_async_wait<0>();
 }
 
+// out[t][i] = sum over the slots of w * float(acc) * (rs2 * s2)
 template <typename T>
-__global__ void __launch_bounds__(kThreads) moe_down(MoeLayer m, const int8_t* hq, const float* rs)
+__global__ void __launch_bounds__(kThreads) moe_sum_kernel(Params p)
 {
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t t = blockIdx.y, i = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
+    const MoeLayer& m = p.m;
+    const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) * 2, t = blockIdx.y;
     if (i >= m.hidden) return;
-    float sum = 0.f;
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 4
     for (uint32_t k = 0; k < m.topk; ++k) {
-        const uint64_t r = (uint64_t)t * m.topk + k;
-        const int32_t e = m.topk_ids[r];
-        if ((uint32_t)e >= m.experts) continue;
-        const uint64_t row = (uint64_t)e * m.hidden + i;
-        const int acc = warp_dot(m.w2 + row * m.inter, hq + r * m.inter, m.inter, lane);
-        sum = fmaf(m.topk_w[r], (float)acc * (rs[r] * m.s2[row]), sum);
+        const uint32_t r = t * m.topk + k;
+        const uint32_t e = (uint32_t)__ldg(m.topk_ids + r);
+        if (e >= m.experts) continue;
+        const float w = __ldg(m.topk_w + r), rs = p.rs2[r];
+        const int2 a = *reinterpret_cast<const int2*>(p.acc + (uint64_t)r * m.hidden + i);
+        const float* s = m.s2 + (uint64_t)e * m.hidden + i;
+        sum.x = fmaf(w, __fmul_rn((float)a.x, __fmul_rn(rs, __ldg(s))), sum.x);
+        sum.y = fmaf(w, __fmul_rn((float)a.y, __fmul_rn(rs, __ldg(s + 1))), sum.y);
     }
-    if (lane == 0) static_cast<T*>(m.out)[(uint64_t)t * m.hidden + i] = (T)sum;
+    T* out = static_cast<T*>(m.out) + (uint64_t)t * m.hidden + i;
+    out[0] = (T)sum.x;
+    out[1] = (T)sum.y;
 }
 
 struct Ws {
-    float *h, *rs1, *rs2;
-    int8_t *xq, *hq;
-    size_t bytes;
+    size_t h, part_max, rs2, acc, bytes;
 };
-Ws carve(const MoeLayer& m, void* base)
+Ws layout(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t topk, uint32_t num_sms)
 {
-    const size_t r = (size_t)m.tokens * m.topk;
-    uint8_t* p = static_cast<uint8_t*>(base);
+    const size_t r = (size_t)tokens * topk;
     size_t at = 0;
     auto take = [&](size_t n) {
-        uint8_t* q = p + at;
+        const size_t here = at;
         at += (n + 255) / 256 * 256;
-        return q;
+        return here;
     };
     Ws w;
-    w.h = reinterpret_cast<float*>(take(r * m.inter * 4));
-    w.xq = reinterpret_cast<int8_t*>(take(r * m.hidden));
-    w.hq = reinterpret_cast<int8_t*>(take(r * m.inter));
-    w.rs1 = reinterpret_cast<float*>(take(r * 4));
-    w.rs2 = reinterpret_cast<float*>(take(r * 4));
+    w.h = take(r * inter * 4);
+    w.part_max = take(r * num_sms * 4);
+    w.rs2 = take(r * 4);
+    w.acc = take(r * hidden * 4);
     w.bytes = at;
     return w;
 }
 
-template <typename T>
-cudaError_t run(const MoeLayer& m, void* workspace, cudaStream_t st)
+template <typename T, int NT, int STAGES>
+cudaError_t run(Params& p, uint32_t num_sms, cudaStream_t st)
 {
-    const Ws w = carve(m, workspace);
-    const uint32_t r = m.tokens * m.topk;
-    constexpr uint32_t kWarps = kThreads / 32;
-    cudaError_t e = launch_pdl(moe_quant_x<T>, dim3(r), dim3(kThreads), 0, st, m, w.xq, w.rs1);
+    using S = Smem<NT, STAGES>;
+    const uint32_t routes = p.m.tokens * p.m.topk;
+    static std::atomic<uint64_t> done1{0}, done2{0};
+    cudaError_t e = allow_smem(moe_up_kernel<T, NT, STAGES>, kSmemMost, done1);
+    if (e == cudaSuccess) e = allow_smem(moe_down_kernel<NT, STAGES>, kSmemMost, done2);
     if (e == cudaSuccess)
-        e = launch_pdl(moe_gate_up, dim3((m.inter + kWarps - 1) / kWarps, r), dim3(kThreads), 0, st, m, (const int8_t*)w.xq,
-                       (const float*)w.rs1, w.h);
-    if (e == cudaSuccess) e = launch_pdl(moe_quant_h, dim3(r), dim3(kThreads), 0, st, m, (const float*)w.h, w.hq, w.rs2);
+        e = launch_pdl(moe_up_kernel<T, NT, STAGES>, dim3(num_sms), dim3(kThreads),
+                       (size_t)S::total(p.m.hidden, p.m.experts, routes), st, p);
     if (e == cudaSuccess)
-        e = launch_pdl(moe_down<T>, dim3((m.hidden + kWarps - 1) / kWarps, m.tokens), dim3(kThreads), 0, st, m,
-                       (const int8_t*)w.hq, (const float*)w.rs2);
+        e = launch_pdl(moe_down_kernel<NT, STAGES>, dim3(num_sms), dim3(kThreads),
+                       (size_t)S::total(p.slice, p.m.experts, routes), st, p);
+    if (e == cudaSuccess)
+        e = launch_pdl(moe_sum_kernel<T>, dim3((p.m.hidden / 2 + kThreads - 1) / kThreads, p.m.tokens), dim3(kThreads), 0,
+                       st, p);
     return e;
+}
+
+// The widest block of routes that the tokens call for and shared memory has room for, with eight stages or five:
+// a block too narrow for an expert's routes reads its weights again.
+template <typename T, int NT>
+cudaError_t pick(Params& p, uint32_t num_sms, cudaStream_t st)
+{
+    const uint32_t routes = p.m.tokens * p.m.topk, k = std::max(p.m.hidden, p.slice);
+    if (Smem<NT, 8>::total(k, p.m.experts, routes) <= kSmemMost) return run<T, NT, 8>(p, num_sms, st);
+    if (Smem<NT, 5>::total(k, p.m.experts, routes) <= kSmemMost) return run<T, NT, 5>(p, num_sms, st);
+    if constexpr (NT > 1) return pick<T, NT / 2>(p, num_sms, st);
+    return cudaErrorInvalidValue;
+}
+
+template <typename T>
+cudaError_t run_type(Params& p, uint32_t num_sms, cudaStream_t st)
+{
+    if (p.m.tokens <= 8) return pick<T, 1>(p, num_sms, st);
+    if (p.m.tokens <= 16) return pick<T, 2>(p, num_sms, st);
+    return pick<T, 4>(p, num_sms, st);
 }
 
 }  // namespace
 
-size_t moe_layer_workspace(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t experts, uint32_t topk, uint32_t)
+size_t moe_layer_workspace(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t, uint32_t topk, uint32_t num_sms)
 {
-    MoeLayer m{};
-    m.tokens = tokens, m.hidden = hidden, m.inter = inter, m.experts = experts, m.topk = topk;
-    return carve(m, nullptr).bytes;
+    return layout(tokens, hidden, inter, topk, num_sms).bytes;
 }
 
-cudaError_t launch_moe_layer(const MoeLayer& m, void* workspace, uint32_t, cudaStream_t st)
+cudaError_t launch_moe_layer(const MoeLayer& m, void* workspace, uint32_t num_sms, cudaStream_t st)
 {
-    return m.bf16 ? run<__nv_bfloat16>(m, workspace, st) : run<__half>(m, workspace, st);
+    const Ws w = layout(m.tokens, m.hidden, m.inter, m.topk, num_sms);
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    Params p{};
+    p.m = m;
+    p.h = reinterpret_cast<float*>(base + w.h);
+    p.part_max = reinterpret_cast<float*>(base + w.part_max);
+    p.rs2 = reinterpret_cast<float*>(base + w.rs2);
+    p.acc = reinterpret_cast<int32_t*>(base + w.acc);
+    p.grid1 = num_sms;
+    p.slices = (m.inter + kSliceMost - 1) / kSliceMost;
+    p.slice = ((m.inter + p.slices - 1) / p.slices + 127) / 128 * 128;
+    p.slices = (m.inter + p.slice - 1) / p.slice;
+    return m.bf16 ? run_type<__nv_bfloat16>(p, num_sms, st) : run_type<__half>(p, num_sms, st);
 }
 
 }  // namespace b2sq

@@ -22,7 +22,8 @@ def moe(**kw):
     (INVALID, dict(t=_lib.I32)), (INVALID, dict(t=9)), (INVALID, dict(qmax=0.0)), (INVALID, dict(qmax=128.0)),
     (INVALID, dict(qmax=float("nan"))), (INVALID, dict(experts=0)), (INVALID, dict(experts=1025)), (INVALID, dict(topk=0)),
     (INVALID, dict(hidden=0)), (INVALID, dict(inter=0)), (UNSUPPORTED, dict(hidden=72)), (UNSUPPORTED, dict(inter=40)),
-    (UNSUPPORTED, dict(hidden=131088, ldx=131088)), (UNSUPPORTED, dict(tokens=4096)), (OK, dict(tokens=0)),
+    (UNSUPPORTED, dict(hidden=131088, ldx=131088)), (UNSUPPORTED, dict(hidden=16400, ldx=16400)),
+    (UNSUPPORTED, dict(inter=131088)), (UNSUPPORTED, dict(tokens=4096)), (OK, dict(tokens=0)),
     (INVALID, dict(x=None)), (INVALID, dict(w13=None)), (INVALID, dict(out=None)), (INVALID, dict(s2=None)),
     (INVALID, dict(ldx=48)), (UNSUPPORTED, dict(ldx=68)), (UNSUPPORTED, dict(x=P + 2)), (UNSUPPORTED, dict(w2=P + 8)),
     (INVALID, dict(sm1=P + 2)),

@@ -100,6 +100,13 @@ def test_moe_layer(cuda_device, T, H, I, E, K, dtype):
     check(make(T, H, I, E, K, dtype, seed=T + H))
 
 
+@pytest.mark.parametrize("T,H,I,E,K", [(1, 16384, 32, 2, 2), (20, 16384, 16, 2, 1), (3, 32, 4112, 2, 2), (17, 80, 8208, 3, 2),
+                                       (512, 48, 32, 1024, 8), (9, 1040, 12400, 2, 1), (40, 8192, 144, 2, 2)])
+def test_moe_layer_far_sizes(cuda_device, T, H, I, E, K):
+    """The widest rows, several slices of the inner dimension with ragged ends, many experts, all 4096 routes."""
+    check(make(T, H, I, E, K, torch.bfloat16, seed=T + I))
+
+
 def test_all_tokens_to_one_expert(cuda_device):
     ids = torch.full((50, 1), 5, dtype=torch.int32, device=DEV)
     check(make(50, 320, 336, 7, 1, torch.bfloat16, ids=ids))
