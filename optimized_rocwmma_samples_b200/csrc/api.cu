@@ -649,8 +649,8 @@ b2sq_status b2sq_moe_layer(const void* x, b2sq_dtype x_type, uint32_t ldx, const
     if (!aligned(topk_weights, 4) || !aligned(topk_ids, 4) || !aligned(smooth1, 4) || !aligned(s13, 4) ||
         !aligned(smooth2, 4) || !aligned(s2, 4))
         return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: misaligned pointer");
-    if (!aligned(x, 16) || !aligned(w13, 16) || !aligned(w2, 16) || !aligned(out, 16) || ldx % 8)
-        return fail(B2SQ_ERR_UNSUPPORTED, "moe_layer: x, w13, w2, out 16-byte aligned and ldx a multiple of 8");
+    if (!aligned(x, 16) || !aligned(smooth1, 16) || !aligned(w13, 16) || !aligned(w2, 16) || !aligned(out, 16) || ldx % 8)
+        return fail(B2SQ_ERR_UNSUPPORTED, "moe_layer: x, smooth1, w13, w2, out 16-byte aligned and ldx a multiple of 8");
     uint32_t sms = 0;
     cudaError_t e = current_sm_count(&sms);
     if (e != cudaSuccess) return cuda_fail(e, "moe_layer: SM count");

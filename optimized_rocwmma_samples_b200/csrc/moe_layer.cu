@@ -41,6 +41,7 @@ namespace {
 constexpr uint32_t kWarps = 8;
 constexpr uint32_t kThreads = kWarps * 32;
 constexpr uint32_t kTile = 2048;         // bytes of a warp's stage: 16 rows of 128
+constexpr uint32_t kTilesMost = 2;
 constexpr uint32_t kSliceMost = 4096;    // inner elements of h that a block of the second kernel holds at a time
 constexpr uint32_t kSmemMost = 231424;   // dynamic shared memory: 227 KB, less 1 KB for what is static
 
@@ -55,6 +56,7 @@ struct Params {
     float* rs2;      // [R]
     int32_t* acc;    // [R][hidden]
     uint32_t grid1, slices, slice;  // of the second kernel: slices of `slice` inner elements
+    uint32_t tiles1, tiles2;        // row tiles of a unit: 2 where the pieces of one do not divide evenly among the warps
 };
 
 // Shared memory of both products: the ring, the routes' rows, the sums, the lists.
@@ -62,7 +64,7 @@ template <int NT, int STAGES>
 struct Smem {
     static constexpr uint32_t ring = kWarps * STAGES * kTile;
     static constexpr uint32_t pitch = NT == 1 ? 8 : NT == 2 ? 24 : 40;  // ints of a row of sums: two-way bank conflicts at most
-    static constexpr uint32_t sums = 2 * 16 * pitch * 4;
+    static constexpr uint32_t sums = 2 * kTilesMost * 16 * pitch * 4;  // two units
     __host__ __device__ static constexpr uint32_t row_pitch(uint32_t k) { return (k + 127) / 128 * 128 + 16; }
     __host__ __device__ static constexpr uint32_t rows(uint32_t k) { return 8 * NT * row_pitch(k); }
     __host__ __device__ static constexpr uint32_t lists(uint32_t experts, uint32_t routes)
@@ -110,6 +112,29 @@ template <>
 __device__ __forceinline__ float2 pair_to_f2<__nv_bfloat16>(uint32_t w)
 {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Loads that stay where they are written, ahead of the asynchronous copies behind them.
+__device__ __forceinline__ uint4 load16(const void* p)
+{
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float4 load16f(const float* p)
+{
+    float4 v;
+    asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
+
+// Eight activations times their smooth scales, in fp32 (smoothquant's first step).
+template <typename T>
+__device__ __forceinline__ void smoothed(const uint4& w, const float4& s0, const float4& s1, float (&f)[8])
+{
+    const float2 a = pair_to_f2<T>(w.x), b = pair_to_f2<T>(w.y), c = pair_to_f2<T>(w.z), d = pair_to_f2<T>(w.w);
+    f[0] = __fmul_rn(a.x, s0.x), f[1] = __fmul_rn(a.y, s0.y), f[2] = __fmul_rn(b.x, s0.z), f[3] = __fmul_rn(b.y, s0.w);
+    f[4] = __fmul_rn(c.x, s1.x), f[5] = __fmul_rn(c.y, s1.y), f[6] = __fmul_rn(d.x, s1.z), f[7] = __fmul_rn(d.y, s1.w);
 }
 
 // Routes grouped by expert, in their own order, and blocks of at most `most`
@@ -208,10 +233,17 @@ struct Split {
     }
 };
 
-// A warp's share of a unit: int32 products of 16 weight rows with the block's routes over its 128-byte pieces.
+// First of the 128-byte pieces of row tile `tile` that a warp takes: the unit's pieces, tile after tile, go round the warps.
+__device__ __forceinline__ uint32_t first_piece(uint32_t warp, uint32_t tile, uint32_t pieces)
+{
+    return (warp - tile * pieces) & (kWarps - 1);
+}
+
+// A warp's share of a row tile: int32 products of its 16 weight rows with the block's routes over its pieces.
 template <int NT, int STAGES, typename Next>
-__device__ __forceinline__ void unit_product(uint32_t pieces, uint32_t live, uint32_t ring_base, uint32_t rows_base,
-                                             uint32_t row_pitch, uint32_t& slot, int (&acc)[NT][4], Next&& next)
+__device__ __forceinline__ void tile_product(uint32_t tile, uint32_t pieces, uint32_t live, uint32_t ring_base,
+                                             uint32_t rows_base, uint32_t row_pitch, uint32_t& slot, int (&acc)[NT][4],
+                                             Next&& next)
 {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint32_t arow = (lane & 7) + ((lane >> 3) & 1) * 8, asel = lane >> 4;
@@ -220,7 +252,7 @@ __device__ __forceinline__ void unit_product(uint32_t pieces, uint32_t live, uin
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[nt][i] = 0;
-    for (uint32_t p = warp; p < pieces; p += kWarps) {
+    for (uint32_t p = first_piece(warp, tile, pieces); p < pieces; p += kWarps) {
         cp_async_wait<STAGES - 2>();
         __syncwarp();
         // the slot that the last step freed takes the tile STAGES - 1 steps ahead
@@ -285,25 +317,44 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
     if (p.slices > 1)  // the second kernel's sums start from zero
         for (uint64_t i = (uint64_t)blockIdx.x * kThreads + tid; i < (uint64_t)routes * H / 4; i += (uint64_t)gridDim.x * kThreads)
             reinterpret_cast<int4*>(p.acc)[i] = make_int4(0, 0, 0, 0);
-    for (uint32_t i = tid; i < 2 * 16 * S::pitch; i += kThreads) sums[i] = 0;
+    for (uint32_t i = tid; i < S::sums / 4; i += kThreads) sums[i] = 0;
 
-    const uint32_t per_block = I / 8, total = l.block[m.experts] * per_block;
+    const uint32_t tiles = p.tiles1;
+    const uint32_t per_block = (I / 8 + tiles - 1) / tiles, total = l.block[m.experts] * per_block;
     const Split split(total, gridDim.x);
     const uint32_t begin = split.begin(blockIdx.x), end = split.begin(blockIdx.x + 1);
     if (begin == end) return;
 
-    // producer: this warp's next tile (unit, piece) and its addresses
+    // producer: this warp's next piece (unit, row tile, piece) and its addresses
     const uint32_t pieces = (H + 127) / 128;
     const uint32_t ring_base = smem_u32(moe_smem) + warp * STAGES * kTile;
     const uint32_t lrow = lane / 8, lchunk = lane & 7;
-    uint32_t pu = begin, pj = begin % per_block, pp = warp, pslot = 0;
+    uint32_t pu = begin, pj = begin % per_block * tiles, pt = 0, pp = warp, pslot = 0;  // pj: row tile in the block
     const int8_t* src = nullptr;
     auto place = [&]() {
         const uint32_t e = expert_of(l, m.experts, pu / per_block);
         src = m.w13 + ((uint64_t)e * 2 * I + pj * 8 + lrow) * H + lchunk * 16;
     };
+    // to the next piece of this warp, over row tiles and units in which it has none
+    auto settle = [&]() {
+        while (pu < end && (pp >= pieces || pj * 8 >= I)) {
+            ++pj;
+            if (++pt == tiles) {
+                pt = 0;
+                ++pu;
+                if (pj * 8 >= I) pj = 0;
+            }
+            pp = first_piece(warp, pt, pieces);
+            if (pu < end) {
+                if (pj == 0)
+                    place();
+                else
+                    src += (uint64_t)8 * H;
+            }
+        }
+    };
     auto load = [&]() {
-        if (pu < end && pp < pieces) {
+        if (pu < end) {
             const uint32_t at = pp * 128 + lchunk * 16;
             const uint32_t bytes = at < H ? 16u : 0u;
             const uint32_t dst = ring_base + pslot * kTile;
@@ -316,79 +367,80 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
                 cp_async16(dst + r * 128 + ((lchunk ^ (r & 7)) * 16), bytes ? row : m.w13, bytes);
             }
             pp += kWarps;
-            if (pp >= pieces) {
-                pp = warp;
-                ++pu;
-                if (++pj == per_block) pj = 0;
-                if (pu < end) {
-                    if (pj == 0)
-                        place();
-                    else
-                        src += (uint64_t)8 * H;
-                }
-            }
+            settle();
         }
         cp_async_commit();
         if (++pslot == STAGES) pslot = 0;
     };
     place();
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) load();
+    settle();
 
+    bool primed = false;
     uint32_t slot = 0, buf = 0;
     uint32_t b = begin / per_block, j = begin % per_block;
     for (uint32_t u = begin; u < end; ++b, j = 0) {
         const uint32_t e = expert_of(l, m.experts, b);
         const uint32_t r0 = l.first[e] + (b - l.block[e]) * 8 * NT;
         const uint32_t count = min(8u * NT, (uint32_t)l.first[e + 1] - r0);
-        // quantise the block's tokens: 8, 4, 2 or 1 warps a token
+        // Quantise the block's tokens, wpt warps each, so that a lane holds at most 64 values: they are read once, all
+        // loads in flight together (behind the streaming weights a load takes microseconds), and for the first block
+        // ahead of the weights.
         {
-            const uint32_t wpt = count > 4 ? 1 : count > 2 ? 2 : count > 1 ? 4 : 8, per = kWarps / wpt;
+            uint32_t wpt = count > 4 ? 1 : count > 2 ? 2 : count > 1 ? 4 : 8;
+            while (wpt * 2048 < H) wpt *= 2;
+            const uint32_t per = kWarps / wpt;
             const float* sm = m.smooth1 + (uint64_t)e * H;
+            const uint32_t start = (warp & (wpt - 1)) * 256 + lane * 8, stride = wpt * 256;
             for (uint32_t t0 = 0; t0 < count; t0 += per) {
                 const uint32_t t = t0 + warp / wpt;
                 const bool on = t < count;
                 const T* x = static_cast<const T*>(m.x) + (uint64_t)(on ? l.order[r0 + t] / m.topk : 0) * m.x_stride;
-                const uint32_t start = (warp % wpt) * 256 + lane * 8, stride = wpt * 256;
-                float mx = 0.f;
-                if (on)
-#pragma unroll 4
-                    for (uint32_t k = start; k < H; k += stride) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(x + k);
-                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+                uint4 xw[8];
+                float4 sw[8][2];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 f = pair_to_f2<T>(ww[i]);
-                            mx = fmaxf(mx, fabsf(__fmul_rn(f.x, __ldg(sm + k + 2 * i))));
-                            mx = fmaxf(mx, fabsf(__fmul_rn(f.y, __ldg(sm + k + 2 * i + 1))));
-                        }
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const uint32_t k = start + i * stride;
+                    xw[i] = make_uint4(0, 0, 0, 0);
+                    sw[i][0] = sw[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (on && k < H) {
+                        xw[i] = load16(x + k);
+                        sw[i][0] = load16f(sm + k);
+                        sw[i][1] = load16f(sm + k + 4);
                     }
+                }
+                if (!primed) {
+                    primed = true;
+#pragma unroll 1
+                    for (int i = 0; i < STAGES - 1; ++i) load();
+                }
+                float f[8][8], mx = 0.f;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    smoothed<T>(xw[i], sw[i][0], sw[i][1], f[i]);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) mx = fmaxf(mx, fabsf(f[i][c]));
+                }
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
                 __syncthreads();  // (also: the last block's rows, maxima and warp_max are read)
                 if (lane == 0) warp_max[warp] = mx;
                 __syncthreads();
-                for (uint32_t w = warp / wpt * wpt; w < warp / wpt * wpt + wpt; ++w) mx = fmaxf(mx, warp_max[w]);
+                for (uint32_t w = warp & ~(wpt - 1); w < (warp & ~(wpt - 1)) + wpt; ++w) mx = fmaxf(mx, warp_max[w]);
                 const float rs = row_scale_of(mx, m.qmax), inv = inv_scale_of(rs);
-                if (on) {
-#pragma unroll 2
-                    for (uint32_t k = start; k < H; k += stride) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(x + k);
-                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const uint32_t k = start + i * stride;
+                    if (on && k < H) {
                         int8_t q[8];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 f = pair_to_f2<T>(ww[i]);
-                            q[2 * i] = quant1(__fmul_rn(f.x, __ldg(sm + k + 2 * i)), inv, m.qmax);
-                            q[2 * i + 1] = quant1(__fmul_rn(f.y, __ldg(sm + k + 2 * i + 1)), inv, m.qmax);
-                        }
+                        for (int c = 0; c < 8; ++c) q[c] = quant1(f[i][c], inv, m.qmax);
                         *reinterpret_cast<uint2*>(rows + t * row_pitch + k) =
                             make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
                     }
-                    if (lane == 0 && warp % wpt == 0) {
-                        rs1[t] = rs;
-                        top[t] = 0;
-                    }
+                }
+                if (on && lane == 0 && (warp & (wpt - 1)) == 0) {
+                    rs1[t] = rs;
+                    top[t] = 0;
                 }
             }
             __syncthreads();
@@ -398,36 +450,45 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
         const bool mine = tok < count;
         const uint32_t route = mine ? l.order[r0 + tok] : 0;
         for (; j < per_block && u < end; ++j, ++u) {
-            float sg = 0.f, su = 0.f, s2 = 0.f;
-            if (mine) {
-                const uint64_t at = (uint64_t)e * 2 * I + j * 8 + jj;
-                sg = __ldg(m.s13 + at);
-                su = __ldg(m.s13 + at + I);
-                s2 = __ldg(m.smooth2 + (uint64_t)e * I + j * 8 + jj);
-            }
-            int acc[NT][4];
-            unit_product<NT, STAGES>(pieces, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
-            int* sum = sums + buf * 16 * S::pitch;
+            const uint32_t here = min(tiles, I / 8 - j * tiles);  // row tiles of this unit
+            float sg[kTilesMost] = {}, su[kTilesMost] = {}, s2[kTilesMost] = {};
+#pragma unroll
+            for (uint32_t t = 0; t < kTilesMost; ++t)
+                if (mine && t < here) {
+                    const uint64_t at = (uint64_t)e * 2 * I + (j * tiles + t) * 8 + jj;
+                    sg[t] = __ldg(m.s13 + at);
+                    su[t] = __ldg(m.s13 + at + I);
+                    s2[t] = __ldg(m.smooth2 + (uint64_t)e * I + (j * tiles + t) * 8 + jj);
+                }
+            int* sum = sums + buf * kTilesMost * 16 * S::pitch;
             buf ^= 1;
-            add_sums<NT, S::pitch>(sum, acc, live);
+            for (uint32_t t = 0; t < here; ++t) {
+                int acc[NT][4];
+                tile_product<NT, STAGES>(t, pieces, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
+                add_sums<NT, S::pitch>(sum + t * 16 * S::pitch, acc, live);
+            }
             __syncthreads();
             // (the other buffer's readers are past this barrier too: it is free and zero again)
-            float hv = 0.f;
-            if (mine) {
-                int* at = sum + jj * S::pitch + tok;
-                const float g = __fmul_rn((float)at[0], __fmul_rn(rs1[tok], sg));
-                const float v = __fmul_rn((float)at[8 * S::pitch], __fmul_rn(rs1[tok], su));
-                hv = g / (1.f + expf(-g)) * v * s2;
-                p.h[(uint64_t)route * I + j * 8 + jj] = hv;
-            }
-            if (tid < 64 * live) {  // by the thread that read it
-                sum[jj * S::pitch + tok] = 0;
-                sum[(jj + 8) * S::pitch + tok] = 0;
-            }
-            float mx = fmaxf(fabsf(hv), 0.f);  // a NaN drops out, as in smoothquant
 #pragma unroll
-            for (int off = 4; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            if (mine && jj == 0) top[tok] = max(top[tok], __float_as_uint(mx));  // one thread a route
+            for (uint32_t t = 0; t < kTilesMost; ++t) {
+                if (t >= here) break;
+                int* at = sum + (t * 16 + jj) * S::pitch + tok;
+                float hv = 0.f;
+                if (mine) {
+                    const float g = __fmul_rn((float)at[0], __fmul_rn(rs1[tok], sg[t]));
+                    const float v = __fmul_rn((float)at[8 * S::pitch], __fmul_rn(rs1[tok], su[t]));
+                    hv = g / (1.f + expf(-g)) * v * s2[t];
+                    p.h[(uint64_t)route * I + (j * tiles + t) * 8 + jj] = hv;
+                }
+                if (tid < 64 * live) {  // cleared by the thread that read it
+                    at[0] = 0;
+                    at[8 * S::pitch] = 0;
+                }
+                float mx = fmaxf(fabsf(hv), 0.f);  // a NaN drops out, as in smoothquant
+#pragma unroll
+                for (int off = 4; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                if (mine && jj == 0) top[tok] = max(top[tok], __float_as_uint(mx));  // one thread a route
+            }
         }
         // (every thread reads back what it wrote itself)
         if (mine && jj == 0) p.part_max[(uint64_t)blockIdx.x * routes + route] = __uint_as_float(top[tok]);
@@ -453,15 +514,16 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
 
     // before the wait: only what the layer's inputs say (the first kernel has waited for them)
     make_lists(m, 8 * NT, l, reinterpret_cast<uint32_t*>(moe_smem));
-    for (uint32_t i = tid; i < 2 * 16 * S::pitch; i += kThreads) sums[i] = 0;
-    const uint32_t per_slice = H / 16, per_block = per_slice * p.slices;
+    for (uint32_t i = tid; i < S::sums / 4; i += kThreads) sums[i] = 0;
+    const uint32_t tiles = p.tiles2;
+    const uint32_t per_slice = (H / 16 + tiles - 1) / tiles, per_block = per_slice * p.slices;
     const uint32_t total = l.block[m.experts] * per_block;
     const Split split(total, gridDim.x);
     const uint32_t begin = split.begin(blockIdx.x), end = split.begin(blockIdx.x + 1);
 
     const uint32_t ring_base = smem_u32(moe_smem) + warp * STAGES * kTile;
     const uint32_t lrow = lane / 8, lchunk = lane & 7;
-    uint32_t pu = begin, pr = begin % per_slice, pp = warp, pslot = 0;  // unit, row unit, piece
+    uint32_t pu = begin, pr = begin % per_slice * tiles, pt = 0, pp = warp, pslot = 0;  // pr: row tile of the matrix
     const int8_t* src = nullptr;
     uint32_t left = 0, ppieces = 0;  // inner elements and pieces of the producer's slice
     auto place = [&]() {
@@ -470,15 +532,25 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
         ppieces = (left + 127) / 128;
         src = m.w2 + ((uint64_t)e * H + pr * 16 + lrow) * I + k0 + lchunk * 16;
     };
-    auto advance = [&]() {
-        pp = warp;
-        ++pu;
-        if (++pr == per_slice) pr = 0;
-        if (pu < end) {
-            if (pr == 0)
-                place();
-            else
-                src += (uint64_t)16 * I;
+    auto settle = [&]() {
+        while (pu < end && (pp >= ppieces || pr * 16 >= H)) {
+            ++pr;
+            bool fresh = false;
+            if (++pt == tiles) {
+                pt = 0;
+                ++pu;
+                if (pr * 16 >= H) {
+                    pr = 0;
+                    fresh = true;
+                }
+            }
+            if (pu < end) {
+                if (fresh)
+                    place();
+                else
+                    src += (uint64_t)16 * I;
+            }
+            pp = first_piece(warp, pt, ppieces);
         }
     };
     auto load = [&]() {
@@ -493,14 +565,14 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
                 cp_async16(dst + r * 128 + ((lchunk ^ (r & 7)) * 16), bytes ? s + (uint64_t)i * 4 * I : m.w2, bytes);
             }
             pp += kWarps;
-            while (pu < end && pp >= ppieces) advance();
+            settle();
         }
         cp_async_commit();
         if (++pslot == STAGES) pslot = 0;
     };
     if (begin < end) {
         place();
-        while (pu < end && pp >= ppieces) advance();
+        settle();
 #pragma unroll
         for (int i = 0; i < STAGES - 1; ++i) load();
     }
@@ -508,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
     griddep_launch_dependents();
     if (begin == end) return;
 
-    const uint32_t up_units = I / 8;
+    const uint32_t up_units = (I / 8 + p.tiles1 - 1) / p.tiles1;
     const Split up(l.block[m.experts] * up_units, p.grid1);
     uint32_t slot = 0, buf = 0;
     uint32_t bs = begin / per_slice, ru = begin % per_slice;
@@ -517,8 +589,23 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
         const uint32_t e = expert_of(l, m.experts, b);
         const uint32_t r0 = l.first[e] + (b - l.block[e]) * 8 * NT;
         const uint32_t count = min(8u * NT, (uint32_t)l.first[e + 1] - r0);
+        // the first 16 quads of h of each thread are in flight while the routes' scales are found
+        const uint32_t quads = depth / 4, all = count * quads;  // depth is a multiple of 16
+        float4 hv[16];
+        auto fetch = [&](uint32_t i0) {
+#pragma unroll
+            for (uint32_t n = 0; n < 16; ++n) {
+                const uint32_t i = i0 + n * kThreads;
+                hv[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < all) {
+                    const uint32_t t = i / quads;
+                    hv[n] = load16f(p.h + (uint64_t)l.order[r0 + t] * I + k0 + (i - t * quads) * 4);
+                }
+            }
+        };
+        fetch(tid);
         __syncthreads();  // the last slice's rows are read
-        {  // the routes' scales: the largest of the maxima of the blocks that made them
+        {  // the largest of the maxima of the blocks that made a route's h
             const uint32_t c0 = up.block_of(b * up_units), c1 = up.block_of(b * up_units + up_units - 1);
             for (uint32_t t = warp; t < count; t += kWarps) {
                 const uint32_t r = l.order[r0 + t];
@@ -534,33 +621,41 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
             }
         }
         __syncthreads();
-        {
-            const uint32_t quads = depth / 4;  // depth is a multiple of 16
-#pragma unroll 4
-            for (uint32_t i = tid; i < count * quads; i += kThreads) {
-                const uint32_t t = i / quads, k = (i - t * quads) * 4;
-                const float4 f = *reinterpret_cast<const float4*>(p.h + (uint64_t)l.order[r0 + t] * I + k0 + k);
-                const float inv = inv2[t];
-                *reinterpret_cast<uint32_t*>(rows + t * row_pitch + k) =
-                    pack4(quant1(f.x, inv, m.qmax), quant1(f.y, inv, m.qmax), quant1(f.z, inv, m.qmax),
-                          quant1(f.w, inv, m.qmax));
+        for (uint32_t i0 = tid;;) {
+#pragma unroll
+            for (uint32_t n = 0; n < 16; ++n) {
+                const uint32_t i = i0 + n * kThreads;
+                if (i < all) {
+                    const uint32_t t = i / quads;
+                    const float inv = inv2[t];
+                    *reinterpret_cast<uint32_t*>(rows + t * row_pitch + (i - t * quads) * 4) =
+                        pack4(quant1(hv[n].x, inv, m.qmax), quant1(hv[n].y, inv, m.qmax), quant1(hv[n].z, inv, m.qmax),
+                              quant1(hv[n].w, inv, m.qmax));
+                }
             }
+            i0 += 16 * kThreads;
+            if (i0 - tid >= all) break;
+            fetch(i0);
         }
         __syncthreads();
         const uint32_t live = (count + 7) / 8, pieces = (depth + 127) / 128;
         for (; ru < per_slice && u < end; ++ru, ++u) {
-            int acc[NT][4];
-            unit_product<NT, STAGES>(pieces, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
-            int* sum = sums + buf * 16 * S::pitch;
+            const uint32_t here = min(tiles, H / 16 - ru * tiles);
+            int* sum = sums + buf * kTilesMost * 16 * S::pitch;
             buf ^= 1;
-            add_sums<NT, S::pitch>(sum, acc, live);
+            for (uint32_t t = 0; t < here; ++t) {
+                int acc[NT][4];
+                tile_product<NT, STAGES>(t, pieces, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
+                add_sums<NT, S::pitch>(sum + t * 16 * S::pitch, acc, live);
+            }
             __syncthreads();
-            for (uint32_t i = tid; i < 16 * 8 * live; i += kThreads) {
-                const uint32_t t = i / 16, row = i % 16;
+            const uint32_t cells = 16 * here;
+            for (uint32_t i = tid; i < cells * 8 * live; i += kThreads) {
+                const uint32_t t = i / cells, row = i - t * cells;
                 const int v = sum[row * S::pitch + t];
                 sum[row * S::pitch + t] = 0;
                 if (t < count) {
-                    int32_t* at = p.acc + (uint64_t)l.order[r0 + t] * H + ru * 16 + row;
+                    int32_t* at = p.acc + (uint64_t)l.order[r0 + t] * H + ru * tiles * 16 + row;
                     if (p.slices > 1)
                         atomicAdd(at, v);  // integers: exact in any order
                     else
@@ -680,6 +775,8 @@ cudaError_t launch_moe_layer(const MoeLayer& m, void* workspace, uint32_t num_sm
     p.slices = (m.inter + kSliceMost - 1) / kSliceMost;
     p.slice = ((m.inter + p.slices - 1) / p.slices + 127) / 128 * 128;
     p.slices = (m.inter + p.slice - 1) / p.slice;
+    p.tiles1 = (m.hidden + 127) / 128 % kWarps == 0 ? 1 : 2;
+    p.tiles2 = p.slice / 128 % kWarps == 0 ? 1 : 2;
     return m.bf16 ? run_type<__nv_bfloat16>(p, num_sms, st) : run_type<__half>(p, num_sms, st);
 }
 
