@@ -625,10 +625,7 @@ b2sq_status b2sq_moe_layer_workspace_size(uint32_t tokens, uint32_t hidden, uint
     *bytes = 0;
     b2sq_status st = validate_moe_layer("moe_layer_workspace_size", tokens, hidden, inter, experts, topk);
     if (st != B2SQ_OK || tokens == 0) return st;
-    uint32_t sms = 0;
-    cudaError_t e = current_sm_count(&sms);
-    if (e != cudaSuccess) return cuda_fail(e, "moe_layer_workspace_size: SM count");
-    *bytes = b2sq::moe_layer_workspace(tokens, hidden, inter, experts, topk, sms);
+    *bytes = b2sq::moe_layer_workspace(tokens, hidden, inter, topk);
     return ok();
 }
 
@@ -651,13 +648,13 @@ b2sq_status b2sq_moe_layer(const void* x, b2sq_dtype x_type, uint32_t ldx, const
         return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: misaligned pointer");
     if (!aligned(x, 16) || !aligned(smooth1, 16) || !aligned(w13, 16) || !aligned(w2, 16) || !aligned(out, 16) || ldx % 8)
         return fail(B2SQ_ERR_UNSUPPORTED, "moe_layer: x, smooth1, w13, w2, out 16-byte aligned and ldx a multiple of 8");
-    uint32_t sms = 0;
-    cudaError_t e = current_sm_count(&sms);
-    if (e != cudaSuccess) return cuda_fail(e, "moe_layer: SM count");
-    const size_t need = b2sq::moe_layer_workspace(tokens, hidden, inter, experts, topk, sms);
+    const size_t need = b2sq::moe_layer_workspace(tokens, hidden, inter, topk);
     if (!workspace || workspace_bytes < need)
         return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: workspace of %zu bytes needed", need);
     if (!aligned(workspace, 256)) return fail(B2SQ_ERR_INVALID_ARG, "moe_layer: workspace must be 256-byte aligned");
+    uint32_t sms = 0;
+    cudaError_t e = current_sm_count(&sms);
+    if (e != cudaSuccess) return cuda_fail(e, "moe_layer: SM count");
     const b2sq::MoeLayer m{x,  x_type == B2SQ_BF16, ldx, topk_weights, topk_ids, smooth1, w13,  s13,      smooth2,
                            w2, s2,                  out, tokens,       hidden,   inter,   experts, topk, quant_max};
     e = b2sq::launch_moe_layer(m, workspace, sms, reinterpret_cast<cudaStream_t>(stream));

@@ -169,8 +169,7 @@ struct MoeLayer {
     uint32_t tokens, hidden, inter, experts, topk;
     float qmax;
 };
-size_t moe_layer_workspace(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t experts, uint32_t topk,
-                           uint32_t num_sms);
+size_t moe_layer_workspace(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t topk);
 cudaError_t launch_moe_layer(const MoeLayer& m, void* workspace, uint32_t num_sms, cudaStream_t st);
 
 // Debug: a kernel that waits for an mbarrier nobody arrives on, with a limit.

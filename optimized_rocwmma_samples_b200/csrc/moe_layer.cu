@@ -18,13 +18,17 @@
 // mma.m16n8k32: weight rows are the 16, routes the 8 columns.  The warps' int32
 // sums meet in shared memory by integer adds, one barrier a unit.
 //
-//   moe_up_kernel    quantises x for its expert, multiplies gate and up rows
-//                    (8 + 8 a unit, so one thread has both), applies SwiGLU,
-//                    leaves h in fp32 and the largest |h| it saw of each route
-//   moe_down_kernel  starts streaming w2 before the first kernel is done, takes
-//                    the maxima, quantises its slice of h, multiplies; slices of
-//                    the inner dimension are added as integers (exact, any order)
-//   moe_sum_kernel   scales, weighs and adds the slots
+//   moe_quant_x_kernel  smoothquant of each route's token; clears what the others add to
+//   moe_up_kernel       gate and up rows (8 + 8 a tile, so one thread has both), SwiGLU;
+//                       leaves h in fp32 and the largest |h| of each route
+//   moe_quant_h_kernel  h to int8
+//   moe_down_kernel     w2; slices of the inner dimension are added as integers
+//                       (exact, in any order)
+//   moe_sum_kernel      scales, weighs and adds the slots
+// The two products start to stream their weights before the kernel in front of
+// them is done (programmatic launch).  Quantising once in small kernels beats
+// doing it in the products, where every block repeats it for its experts behind
+// its own weight loads (16 tokens: 8 to 13 us a time; 4 us this way).
 #include "common.cuh"
 #include "kernels.h"
 #include "sq_math.cuh"
@@ -51,11 +55,12 @@ struct Lists {
 
 struct Params {
     MoeLayer m;
-    float* h;        // [R][inter]
-    float* part_max; // [blocks of the first kernel][R]
-    float* rs2;      // [R]
-    int32_t* acc;    // [R][hidden]
-    uint32_t grid1, slices, slice;  // of the second kernel: slices of `slice` inner elements
+    int8_t *xq, *hq;  // [R][hidden], [R][inter]
+    float* rs1;       // [R]
+    uint32_t* top;    // [R] largest |h|, as bits
+    float* h;         // [R][inter]
+    int32_t* acc;     // [R][hidden]
+    uint32_t slices, slice;  // of the second kernel: slices of `slice` inner elements
     uint32_t tiles1, tiles2;        // row tiles of a unit: 2 where the pieces of one do not divide evenly among the warps
 };
 
@@ -114,20 +119,6 @@ __device__ __forceinline__ float2 pair_to_f2<__nv_bfloat16>(uint32_t w)
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// Loads that stay where they are written, ahead of the asynchronous copies behind them.
-__device__ __forceinline__ uint4 load16(const void* p)
-{
-    uint4 v;
-    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ float4 load16f(const float* p)
-{
-    float4 v;
-    asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
-    return v;
-}
-
 // Eight activations times their smooth scales, in fp32 (smoothquant's first step).
 template <typename T>
 __device__ __forceinline__ void smoothed(const uint4& w, const float4& s0, const float4& s1, float (&f)[8])
@@ -135,6 +126,91 @@ __device__ __forceinline__ void smoothed(const uint4& w, const float4& s0, const
     const float2 a = pair_to_f2<T>(w.x), b = pair_to_f2<T>(w.y), c = pair_to_f2<T>(w.z), d = pair_to_f2<T>(w.w);
     f[0] = __fmul_rn(a.x, s0.x), f[1] = __fmul_rn(a.y, s0.y), f[2] = __fmul_rn(b.x, s0.z), f[3] = __fmul_rn(b.y, s0.w);
     f[4] = __fmul_rn(c.x, s1.x), f[5] = __fmul_rn(c.y, s1.y), f[6] = __fmul_rn(d.x, s1.z), f[7] = __fmul_rn(d.y, s1.w);
+}
+
+// The low byte of quant1's result; integral qmax takes the form without conversions.
+__device__ __forceinline__ uint32_t quant_byte(float xs, float inv, float qmax, bool whole)
+{
+    return whole ? quant_bits(xs, inv, qmax) : (uint32_t)(uint8_t)quant1(xs, inv, qmax);
+}
+__device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, float inv, float qmax, bool whole)
+{
+    return pack_low_bytes(quant_byte(a, inv, qmax, whole), quant_byte(b, inv, qmax, whole), quant_byte(c, inv, qmax, whole),
+                          quant_byte(d, inv, qmax, whole));
+}
+
+// A block a route: hidden <= 16384 is at most 64 values a thread, read once.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) moe_quant_x_kernel(Params p)
+{
+    __shared__ float warp_max[kWarps];
+    griddep_wait();
+    griddep_launch_dependents();
+    const MoeLayer& m = p.m;
+    const uint32_t r = blockIdx.x, tid = threadIdx.x, H = m.hidden;
+    const uint32_t e = (uint32_t)__ldg(m.topk_ids + r);
+    if (tid == 0) p.top[r] = 0;
+    if (e >= m.experts) return;
+    const T* x = static_cast<const T*>(m.x) + (uint64_t)(r / m.topk) * m.x_stride;
+    const float* sm = m.smooth1 + (uint64_t)e * H;
+    uint4 xw[8];
+    float4 sw[8][2];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t k = (i * kThreads + tid) * 8;
+        xw[i] = make_uint4(0, 0, 0, 0);
+        sw[i][0] = sw[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k < H) {
+            xw[i] = __ldg(reinterpret_cast<const uint4*>(x + k));
+            sw[i][0] = __ldg(reinterpret_cast<const float4*>(sm + k));
+            sw[i][1] = __ldg(reinterpret_cast<const float4*>(sm + k) + 1);
+        }
+    }
+    if (p.slices > 1)  // the down product adds its slices up from zero
+        for (uint32_t i = tid; i < H / 4; i += kThreads) reinterpret_cast<int4*>(p.acc + (uint64_t)r * H)[i] = make_int4(0, 0, 0, 0);
+    float f[8][8], mx = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        smoothed<T>(xw[i], sw[i][0], sw[i][1], f[i]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) mx = fmaxf(mx, fabsf(f[i][c]));
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    if ((tid & 31) == 0) warp_max[tid / 32] = mx;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) mx = fmaxf(mx, warp_max[w]);
+    const float rs = row_scale_of(mx, m.qmax), inv = inv_scale_of(rs);
+    const bool whole = m.qmax == rintf(m.qmax);
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t k = (i * kThreads + tid) * 8;
+        if (k < H)
+            *reinterpret_cast<uint2*>(p.xq + (uint64_t)r * H + k) =
+                make_uint2(quant4(f[i][0], f[i][1], f[i][2], f[i][3], inv, m.qmax, whole),
+                           quant4(f[i][4], f[i][5], f[i][6], f[i][7], inv, m.qmax, whole));
+    }
+    if (tid == 0) p.rs1[r] = rs;
+}
+
+// grid (pieces of 2048, routes)
+__global__ void __launch_bounds__(kThreads) moe_quant_h_kernel(Params p)
+{
+    // (the down product behind this kernel may start once the up product has: it touches only the layer's inputs
+    // until this kernel, which waits for the up product, is done)
+    griddep_launch_dependents();
+    const MoeLayer& m = p.m;
+    const uint32_t r = blockIdx.y, k = (blockIdx.x * kThreads + threadIdx.x) * 8;
+    const bool there = (uint32_t)__ldg(m.topk_ids + r) < m.experts && k < m.inter;
+    griddep_wait();
+    if (!there) return;
+    const float4* h = reinterpret_cast<const float4*>(p.h + (uint64_t)r * m.inter + k);
+    const float4 a = h[0], b = h[1];
+    const float inv = inv_scale_of(row_scale_of(__uint_as_float(p.top[r]), m.qmax));
+    const bool whole = m.qmax == rintf(m.qmax);
+    *reinterpret_cast<uint2*>(p.hq + (uint64_t)r * m.inter + k) =
+        make_uint2(quant4(a.x, a.y, a.z, a.w, inv, m.qmax, whole), quant4(b.x, b.y, b.z, b.w, inv, m.qmax, whole));
 }
 
 // Routes grouped by expert, in their own order, and blocks of at most `most`
@@ -226,12 +302,29 @@ struct Split {
     uint32_t each, rest;
     __device__ __forceinline__ Split(uint32_t total, uint32_t blocks) : each(total / blocks), rest(total % blocks) {}
     __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * each + min(i, rest); }
-    __device__ __forceinline__ uint32_t block_of(uint32_t u) const
-    {
-        const uint32_t big = rest * (each + 1);
-        return u < big ? u / (each + 1) : rest + (u - big) / each;
-    }
 };
+
+// The block's int8 rows (bytes k0 .. k0 + depth of rows of `width`) into shared memory.
+template <int NT>
+__device__ __forceinline__ void copy_rows(uint8_t* rows, uint32_t row_pitch, const int8_t* src, uint64_t width, uint32_t k0,
+                                          uint32_t depth, const uint16_t* order, uint32_t count)
+{
+    constexpr uint32_t FLY = 8;  // loads of a thread in flight
+    const uint32_t chunks = depth / 16, all = count * chunks;
+    for (uint32_t i0 = threadIdx.x; i0 < all; i0 += FLY * kThreads) {
+        uint4 v[FLY];
+#pragma unroll
+        for (uint32_t n = 0; n < FLY; ++n) {
+            const uint32_t i = i0 + n * kThreads, t = i / chunks;
+            if (i < all) v[n] = *reinterpret_cast<const uint4*>(src + order[t] * width + k0 + (i - t * chunks) * 16);
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < FLY; ++n) {
+            const uint32_t i = i0 + n * kThreads, t = i / chunks;
+            if (i < all) *reinterpret_cast<uint4*>(rows + t * row_pitch + (i - t * chunks) * 16) = v[n];
+        }
+    }
+}
 
 // First of the 128-byte pieces of row tile `tile` that a warp takes: the unit's pieces, tile after tile, go round the warps.
 __device__ __forceinline__ uint32_t first_piece(uint32_t warp, uint32_t tile, uint32_t pieces)
@@ -294,36 +387,30 @@ __device__ __forceinline__ void add_sums(int* sums, const int (&acc)[NT][4], uin
 }
 
 // Gate and up rows.  Units: block of routes x 8 inner elements.
-template <typename T, int NT, int STAGES>
+template <int NT, int STAGES>
 __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
 {
     using S = Smem<NT, STAGES>;
     extern __shared__ __align__(128) uint8_t moe_smem[];
     __shared__ float rs1[8 * NT];
     __shared__ uint32_t top[8 * NT];
-    __shared__ float warp_max[kWarps];
     const MoeLayer& m = p.m;
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    const uint32_t routes = m.tokens * m.topk, H = m.hidden, I = m.inter;
+    const uint32_t H = m.hidden, I = m.inter;
     const uint32_t row_pitch = S::row_pitch(H);
     uint8_t* rows = moe_smem + S::ring;
     int* sums = reinterpret_cast<int*>(rows + S::rows(H));
     uint16_t* list = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(sums) + S::sums);
     const Lists l{list, list + m.experts + 1, list + 2 * (m.experts + 1)};
 
-    griddep_wait();
-    griddep_launch_dependents();
+    // before the wait: only what the layer's inputs say (the first kernel has waited for them)
     make_lists(m, 8 * NT, l, reinterpret_cast<uint32_t*>(moe_smem));
-    if (p.slices > 1)  // the second kernel's sums start from zero
-        for (uint64_t i = (uint64_t)blockIdx.x * kThreads + tid; i < (uint64_t)routes * H / 4; i += (uint64_t)gridDim.x * kThreads)
-            reinterpret_cast<int4*>(p.acc)[i] = make_int4(0, 0, 0, 0);
     for (uint32_t i = tid; i < S::sums / 4; i += kThreads) sums[i] = 0;
 
     const uint32_t tiles = p.tiles1;
     const uint32_t per_block = (I / 8 + tiles - 1) / tiles, total = l.block[m.experts] * per_block;
     const Split split(total, gridDim.x);
     const uint32_t begin = split.begin(blockIdx.x), end = split.begin(blockIdx.x + 1);
-    if (begin == end) return;
 
     // producer: this warp's next piece (unit, row tile, piece) and its addresses
     const uint32_t pieces = (H + 127) / 128;
@@ -372,79 +459,29 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
         cp_async_commit();
         if (++pslot == STAGES) pslot = 0;
     };
-    place();
-    settle();
+    if (begin < end) {
+        place();
+        settle();
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) load();
+    }
+    griddep_wait();
+    griddep_launch_dependents();
+    if (begin == end) return;
 
-    bool primed = false;
     uint32_t slot = 0, buf = 0;
     uint32_t b = begin / per_block, j = begin % per_block;
     for (uint32_t u = begin; u < end; ++b, j = 0) {
         const uint32_t e = expert_of(l, m.experts, b);
         const uint32_t r0 = l.first[e] + (b - l.block[e]) * 8 * NT;
         const uint32_t count = min(8u * NT, (uint32_t)l.first[e + 1] - r0);
-        // Quantise the block's tokens, wpt warps each, so that a lane holds at most 64 values: they are read once, all
-        // loads in flight together (behind the streaming weights a load takes microseconds), and for the first block
-        // ahead of the weights.
-        {
-            uint32_t wpt = count > 4 ? 1 : count > 2 ? 2 : count > 1 ? 4 : 8;
-            while (wpt * 2048 < H) wpt *= 2;
-            const uint32_t per = kWarps / wpt;
-            const float* sm = m.smooth1 + (uint64_t)e * H;
-            const uint32_t start = (warp & (wpt - 1)) * 256 + lane * 8, stride = wpt * 256;
-            for (uint32_t t0 = 0; t0 < count; t0 += per) {
-                const uint32_t t = t0 + warp / wpt;
-                const bool on = t < count;
-                const T* x = static_cast<const T*>(m.x) + (uint64_t)(on ? l.order[r0 + t] / m.topk : 0) * m.x_stride;
-                uint4 xw[8];
-                float4 sw[8][2];
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    const uint32_t k = start + i * stride;
-                    xw[i] = make_uint4(0, 0, 0, 0);
-                    sw[i][0] = sw[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (on && k < H) {
-                        xw[i] = load16(x + k);
-                        sw[i][0] = load16f(sm + k);
-                        sw[i][1] = load16f(sm + k + 4);
-                    }
-                }
-                if (!primed) {
-                    primed = true;
-#pragma unroll 1
-                    for (int i = 0; i < STAGES - 1; ++i) load();
-                }
-                float f[8][8], mx = 0.f;
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    smoothed<T>(xw[i], sw[i][0], sw[i][1], f[i]);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) mx = fmaxf(mx, fabsf(f[i][c]));
-                }
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                __syncthreads();  // (also: the last block's rows, maxima and warp_max are read)
-                if (lane == 0) warp_max[warp] = mx;
-                __syncthreads();
-                for (uint32_t w = warp & ~(wpt - 1); w < (warp & ~(wpt - 1)) + wpt; ++w) mx = fmaxf(mx, warp_max[w]);
-                const float rs = row_scale_of(mx, m.qmax), inv = inv_scale_of(rs);
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    const uint32_t k = start + i * stride;
-                    if (on && k < H) {
-                        int8_t q[8];
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) q[c] = quant1(f[i][c], inv, m.qmax);
-                        *reinterpret_cast<uint2*>(rows + t * row_pitch + k) =
-                            make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
-                    }
-                }
-                if (on && lane == 0 && (warp & (wpt - 1)) == 0) {
-                    rs1[t] = rs;
-                    top[t] = 0;
-                }
-            }
-            __syncthreads();
+        __syncthreads();  // the last block's rows are read
+        copy_rows<NT>(rows, row_pitch, p.xq, H, 0, H, l.order + r0, count);
+        if (tid < count) {
+            rs1[tid] = p.rs1[l.order[r0 + tid]];
+            top[tid] = 0;
         }
+        __syncthreads();
         const uint32_t live = (count + 7) / 8;
         const uint32_t tok = tid / 8, jj = tid & 7;  // of the epilogue
         const bool mine = tok < count;
@@ -490,8 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
                 if (mine && jj == 0) top[tok] = max(top[tok], __float_as_uint(mx));  // one thread a route
             }
         }
-        // (every thread reads back what it wrote itself)
-        if (mine && jj == 0) p.part_max[(uint64_t)blockIdx.x * routes + route] = __uint_as_float(top[tok]);
+        if (mine && jj == 0) atomicMax(p.top + route, top[tok]);  // (this thread's own entry)
     }
     cp_async_wait<0>();
 }
@@ -502,10 +538,9 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
 {
     using S = Smem<NT, STAGES>;
     extern __shared__ __align__(128) uint8_t moe_smem[];
-    __shared__ float inv2[8 * NT];
     const MoeLayer& m = p.m;
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    const uint32_t routes = m.tokens * m.topk, H = m.hidden, I = m.inter;
+    const uint32_t H = m.hidden, I = m.inter;
     const uint32_t row_pitch = S::row_pitch(p.slice);
     uint8_t* rows = moe_smem + S::ring;
     int* sums = reinterpret_cast<int*>(rows + S::rows(p.slice));
@@ -580,8 +615,6 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
     griddep_launch_dependents();
     if (begin == end) return;
 
-    const uint32_t up_units = (I / 8 + p.tiles1 - 1) / p.tiles1;
-    const Split up(l.block[m.experts] * up_units, p.grid1);
     uint32_t slot = 0, buf = 0;
     uint32_t bs = begin / per_slice, ru = begin % per_slice;
     for (uint32_t u = begin; u < end; ++bs, ru = 0) {
@@ -589,54 +622,8 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
         const uint32_t e = expert_of(l, m.experts, b);
         const uint32_t r0 = l.first[e] + (b - l.block[e]) * 8 * NT;
         const uint32_t count = min(8u * NT, (uint32_t)l.first[e + 1] - r0);
-        // the first 16 quads of h of each thread are in flight while the routes' scales are found
-        const uint32_t quads = depth / 4, all = count * quads;  // depth is a multiple of 16
-        float4 hv[16];
-        auto fetch = [&](uint32_t i0) {
-#pragma unroll
-            for (uint32_t n = 0; n < 16; ++n) {
-                const uint32_t i = i0 + n * kThreads;
-                hv[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (i < all) {
-                    const uint32_t t = i / quads;
-                    hv[n] = load16f(p.h + (uint64_t)l.order[r0 + t] * I + k0 + (i - t * quads) * 4);
-                }
-            }
-        };
-        fetch(tid);
         __syncthreads();  // the last slice's rows are read
-        {  // the largest of the maxima of the blocks that made a route's h
-            const uint32_t c0 = up.block_of(b * up_units), c1 = up.block_of(b * up_units + up_units - 1);
-            for (uint32_t t = warp; t < count; t += kWarps) {
-                const uint32_t r = l.order[r0 + t];
-                float mx = 0.f;
-                for (uint32_t c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, p.part_max[(uint64_t)c * routes + r]);
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                const float rs = row_scale_of(mx, m.qmax);
-                if (lane == 0) {
-                    inv2[t] = inv_scale_of(rs);
-                    p.rs2[r] = rs;  // every block that needs it finds the same
-                }
-            }
-        }
-        __syncthreads();
-        for (uint32_t i0 = tid;;) {
-#pragma unroll
-            for (uint32_t n = 0; n < 16; ++n) {
-                const uint32_t i = i0 + n * kThreads;
-                if (i < all) {
-                    const uint32_t t = i / quads;
-                    const float inv = inv2[t];
-                    *reinterpret_cast<uint32_t*>(rows + t * row_pitch + (i - t * quads) * 4) =
-                        pack4(quant1(hv[n].x, inv, m.qmax), quant1(hv[n].y, inv, m.qmax), quant1(hv[n].z, inv, m.qmax),
-                              quant1(hv[n].w, inv, m.qmax));
-                }
-            }
-            i0 += 16 * kThreads;
-            if (i0 - tid >= all) break;
-            fetch(i0);
-        }
+        copy_rows<NT>(rows, row_pitch, p.hq, I, k0, depth, l.order + r0, count);
         __syncthreads();
         const uint32_t live = (count + 7) / 8, pieces = (depth + 127) / 128;
         for (; ru < per_slice && u < end; ++ru, ++u) {
@@ -682,7 +669,7 @@ __global__ void __launch_bounds__(kThreads) moe_sum_kernel(Params p)
         const uint32_t r = t * m.topk + k;
         const uint32_t e = (uint32_t)__ldg(m.topk_ids + r);
         if (e >= m.experts) continue;
-        const float w = __ldg(m.topk_w + r), rs = p.rs2[r];
+        const float w = __ldg(m.topk_w + r), rs = row_scale_of(__uint_as_float(p.top[r]), m.qmax);
         const int2 a = *reinterpret_cast<const int2*>(p.acc + (uint64_t)r * m.hidden + i);
         const float* s = m.s2 + (uint64_t)e * m.hidden + i;
         sum.x = fmaf(w, __fmul_rn((float)a.x, __fmul_rn(rs, __ldg(s))), sum.x);
@@ -694,9 +681,9 @@ __global__ void __launch_bounds__(kThreads) moe_sum_kernel(Params p)
 }
 
 struct Ws {
-    size_t h, part_max, rs2, acc, bytes;
+    size_t xq, hq, rs1, top, h, acc, bytes;
 };
-Ws layout(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t topk, uint32_t num_sms)
+Ws layout(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t topk)
 {
     const size_t r = (size_t)tokens * topk;
     size_t at = 0;
@@ -706,9 +693,11 @@ Ws layout(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t topk, uint3
         return here;
     };
     Ws w;
+    w.xq = take(r * hidden);
+    w.hq = take(r * inter);
+    w.rs1 = take(r * 4);
+    w.top = take(r * 4);
     w.h = take(r * inter * 4);
-    w.part_max = take(r * num_sms * 4);
-    w.rs2 = take(r * 4);
     w.acc = take(r * hidden * 4);
     w.bytes = at;
     return w;
@@ -720,11 +709,15 @@ cudaError_t run(Params& p, uint32_t num_sms, cudaStream_t st)
     using S = Smem<NT, STAGES>;
     const uint32_t routes = p.m.tokens * p.m.topk;
     static std::atomic<uint64_t> done1{0}, done2{0};
-    cudaError_t e = allow_smem(moe_up_kernel<T, NT, STAGES>, kSmemMost, done1);
+    cudaError_t e = allow_smem(moe_up_kernel<NT, STAGES>, kSmemMost, done1);
     if (e == cudaSuccess) e = allow_smem(moe_down_kernel<NT, STAGES>, kSmemMost, done2);
+    if (e == cudaSuccess) e = launch_pdl(moe_quant_x_kernel<T>, dim3(routes), dim3(kThreads), 0, st, p);
     if (e == cudaSuccess)
-        e = launch_pdl(moe_up_kernel<T, NT, STAGES>, dim3(num_sms), dim3(kThreads),
+        e = launch_pdl(moe_up_kernel<NT, STAGES>, dim3(num_sms), dim3(kThreads),
                        (size_t)S::total(p.m.hidden, p.m.experts, routes), st, p);
+    if (e == cudaSuccess)
+        e = launch_pdl(moe_quant_h_kernel, dim3((p.m.inter + 8 * kThreads - 1) / (8 * kThreads), routes), dim3(kThreads), 0, st,
+                       p);
     if (e == cudaSuccess)
         e = launch_pdl(moe_down_kernel<NT, STAGES>, dim3(num_sms), dim3(kThreads),
                        (size_t)S::total(p.slice, p.m.experts, routes), st, p);
@@ -756,22 +749,23 @@ cudaError_t run_type(Params& p, uint32_t num_sms, cudaStream_t st)
 
 }  // namespace
 
-size_t moe_layer_workspace(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t, uint32_t topk, uint32_t num_sms)
+size_t moe_layer_workspace(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t topk)
 {
-    return layout(tokens, hidden, inter, topk, num_sms).bytes;
+    return layout(tokens, hidden, inter, topk).bytes;
 }
 
 cudaError_t launch_moe_layer(const MoeLayer& m, void* workspace, uint32_t num_sms, cudaStream_t st)
 {
-    const Ws w = layout(m.tokens, m.hidden, m.inter, m.topk, num_sms);
+    const Ws w = layout(m.tokens, m.hidden, m.inter, m.topk);
     uint8_t* base = static_cast<uint8_t*>(workspace);
     Params p{};
     p.m = m;
+    p.xq = reinterpret_cast<int8_t*>(base + w.xq);
+    p.hq = reinterpret_cast<int8_t*>(base + w.hq);
+    p.rs1 = reinterpret_cast<float*>(base + w.rs1);
+    p.top = reinterpret_cast<uint32_t*>(base + w.top);
     p.h = reinterpret_cast<float*>(base + w.h);
-    p.part_max = reinterpret_cast<float*>(base + w.part_max);
-    p.rs2 = reinterpret_cast<float*>(base + w.rs2);
     p.acc = reinterpret_cast<int32_t*>(base + w.acc);
-    p.grid1 = num_sms;
     p.slices = (m.inter + kSliceMost - 1) / kSliceMost;
     p.slice = ((m.inter + p.slices - 1) / p.slices + 127) / 128 * 128;
     p.slices = (m.inter + p.slice - 1) / p.slice;
