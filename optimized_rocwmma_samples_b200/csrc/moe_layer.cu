@@ -68,7 +68,7 @@ template <int NT, int STAGES>
 struct Smem {
     static constexpr uint32_t ring = kWarps * STAGES * kTile;
     static constexpr uint32_t pitch = NT == 1 ? 8 : NT == 2 ? 24 : 40;  // ints of a row of sums: two-way bank conflicts at most
-    static constexpr uint32_t group = NT == 1 ? 4 : 2;              // row tiles between two barriers
+    static constexpr uint32_t group = NT == 4 ? 2 : 4;              // row tiles between two barriers
     static constexpr uint32_t sums = 2 * group * 16 * pitch * 4;    // of two groups
     __host__ __device__ static constexpr uint32_t row_pitch(uint32_t k) { return (k + 127) / 128 * 128 + 16; }
     __host__ __device__ static constexpr uint32_t rows(uint32_t k) { return 8 * NT * row_pitch(k); }
@@ -149,19 +149,22 @@ __global__ void __launch_bounds__(kThreads) moe_quant_x_kernel(Params p)
     const MoeLayer& m = p.m;
     const uint32_t r = blockIdx.x, tid = threadIdx.x, H = m.hidden;
     const uint32_t e = (uint32_t)__ldg(m.topk_ids + r);
-    if (tid == 0) p.top[r] = 0;
-    if (e >= m.experts) return;
     const T* x = static_cast<const T*>(m.x) + (uint64_t)(r / m.topk) * m.x_stride;
-    const float* sm = m.smooth1 + (uint64_t)e * H;
     uint4 xw[8];
     float4 sw[8][2];
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
         const uint32_t k = (i * kThreads + tid) * 8;
-        xw[i] = make_uint4(0, 0, 0, 0);
+        xw[i] = k < H ? __ldg(reinterpret_cast<const uint4*>(x + k)) : make_uint4(0, 0, 0, 0);
+    }
+    if (tid == 0) p.top[r] = 0;
+    if (e >= m.experts) return;
+    const float* sm = m.smooth1 + (uint64_t)e * H;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t k = (i * kThreads + tid) * 8;
         sw[i][0] = sw[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (k < H) {
-            xw[i] = __ldg(reinterpret_cast<const uint4*>(x + k));
             sw[i][0] = __ldg(reinterpret_cast<const float4*>(sm + k));
             sw[i][1] = __ldg(reinterpret_cast<const float4*>(sm + k) + 1);
         }
@@ -297,6 +300,19 @@ __device__ __forceinline__ uint32_t expert_of(const Lists& l, uint32_t experts, 
     return lo;
 }
 
+struct Block {
+    uint32_t expert, r0, count;  // routes order[r0 .. r0 + count)
+};
+template <int NT>
+__device__ __forceinline__ Block block_at(const Lists& l, uint32_t experts, uint32_t b)
+{
+    Block k;
+    k.expert = expert_of(l, experts, b);
+    k.r0 = l.first[k.expert] + (b - l.block[k.expert]) * 8 * NT;
+    k.count = min(8u * NT, (uint32_t)l.first[k.expert + 1] - k.r0);
+    return k;
+}
+
 // Equal runs of `total` units for `blocks` blocks: the first `rest` get one more.
 struct Split {
     uint32_t each, rest;
@@ -304,27 +320,42 @@ struct Split {
     __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * each + min(i, rest); }
 };
 
-// The block's int8 rows (bytes k0 .. k0 + depth of rows of `width`) into shared memory.
-template <int NT>
-__device__ __forceinline__ void copy_rows(uint8_t* rows, uint32_t row_pitch, const int8_t* src, uint64_t width, uint32_t k0,
-                                          uint32_t depth, const uint16_t* order, uint32_t count)
-{
-    constexpr uint32_t FLY = 8;  // loads of a thread in flight
-    const uint32_t chunks = depth / 16, all = count * chunks;
-    for (uint32_t i0 = threadIdx.x; i0 < all; i0 += FLY * kThreads) {
-        uint4 v[FLY];
+// The block's int8 rows (bytes k0 .. k0 + depth of rows of `width`) on their way into shared memory: the first
+// FLY x 16 bytes of each thread can be fetched early and stored when the rows before them are no longer read.
+struct RowCopy {
+    static constexpr uint32_t FLY = 8;
+    uint4 v[FLY];
+    template <typename F>
+    __device__ __forceinline__ void each(uint32_t i0, uint32_t depth, uint32_t count, F&& f)
+    {
+        const uint32_t chunks = depth / 16, all = count * chunks;
 #pragma unroll
         for (uint32_t n = 0; n < FLY; ++n) {
             const uint32_t i = i0 + n * kThreads, t = i / chunks;
-            if (i < all) v[n] = *reinterpret_cast<const uint4*>(src + order[t] * width + k0 + (i - t * chunks) * 16);
-        }
-#pragma unroll
-        for (uint32_t n = 0; n < FLY; ++n) {
-            const uint32_t i = i0 + n * kThreads, t = i / chunks;
-            if (i < all) *reinterpret_cast<uint4*>(rows + t * row_pitch + (i - t * chunks) * 16) = v[n];
+            if (i < all) f(v[n], t, (i - t * chunks) * 16);
         }
     }
-}
+    __device__ __forceinline__ void fetch(uint32_t i0, const int8_t* src, uint64_t width, uint32_t k0, uint32_t depth,
+                                          const uint16_t* order, uint32_t count)
+    {
+        each(i0, depth, count, [&](uint4& x, uint32_t t, uint32_t k) {
+            x = *reinterpret_cast<const uint4*>(src + order[t] * width + k0 + k);
+        });
+    }
+    // stores what was fetched from i0 = threadIdx.x on, then fetches and stores the rest
+    __device__ __forceinline__ void finish(uint8_t* rows, uint32_t row_pitch, const int8_t* src, uint64_t width, uint32_t k0,
+                                           uint32_t depth, const uint16_t* order, uint32_t count)
+    {
+        for (uint32_t i0 = threadIdx.x;;) {
+            each(i0, depth, count, [&](uint4& x, uint32_t t, uint32_t k) {
+                *reinterpret_cast<uint4*>(rows + t * row_pitch + k) = x;
+            });
+            i0 += FLY * kThreads;
+            if (i0 - threadIdx.x >= count * (depth / 16)) break;
+            fetch(i0, src, width, k0, depth, order, count);
+        }
+    }
+};
 
 // First of the 128-byte pieces of row tile `tile` of a group that a warp takes: the group's pieces go round the warps.
 __device__ __forceinline__ uint32_t first_piece(uint32_t warp, uint32_t tile, uint32_t pieces)
@@ -471,12 +502,13 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
 
     uint32_t slot = 0, buf = 0;
     uint32_t b = begin / per_block, j = begin % per_block;
+    RowCopy copy;
+    Block cur = block_at<NT>(l, m.experts, b);
+    copy.fetch(tid, p.xq, H, 0, H, l.order + cur.r0, cur.count);
     for (uint32_t u = begin; u < end;) {
-        const uint32_t e = expert_of(l, m.experts, b);
-        const uint32_t r0 = l.first[e] + (b - l.block[e]) * 8 * NT;
-        const uint32_t count = min(8u * NT, (uint32_t)l.first[e + 1] - r0);
+        const uint32_t e = cur.expert, r0 = cur.r0, count = cur.count;
         __syncthreads();  // the last block's rows are read
-        copy_rows<NT>(rows, row_pitch, p.xq, H, 0, H, l.order + r0, count);
+        copy.finish(rows, row_pitch, p.xq, H, 0, H, l.order + r0, count);
         if (tid < count) {
             rs1[tid] = p.rs1[l.order[r0 + tid]];
             top[tid] = 0;
@@ -498,6 +530,10 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
                     su[i] = __ldg(m.s13 + at + I);
                     s2[i] = __ldg(m.smooth2 + (uint64_t)e * I + (j + t) * 8 + (n & 7));
                 }
+            }
+            if (j + here == per_block && u + here < end) {  // the next block's rows, behind this group's products
+                cur = block_at<NT>(l, m.experts, b + 1);
+                copy.fetch(tid, p.xq, H, 0, H, l.order + cur.r0, cur.count);
             }
             int* sum = sums + buf * S::group * 16 * S::pitch;
             buf ^= 1;
@@ -616,17 +652,24 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
 
     uint32_t slot = 0, buf = 0;
     uint32_t bs = begin / per_slice, ru = begin % per_slice;
+    RowCopy copy;
+    Block cur = block_at<NT>(l, m.experts, bs / p.slices);
+    uint32_t k0 = bs % p.slices * p.slice, depth = min(p.slice, I - k0);
+    copy.fetch(tid, p.hq, I, k0, depth, l.order + cur.r0, cur.count);
     for (uint32_t u = begin; u < end;) {
-        const uint32_t b = bs / p.slices, k0 = bs % p.slices * p.slice, depth = min(p.slice, I - k0);
-        const uint32_t e = expert_of(l, m.experts, b);
-        const uint32_t r0 = l.first[e] + (b - l.block[e]) * 8 * NT;
-        const uint32_t count = min(8u * NT, (uint32_t)l.first[e + 1] - r0);
+        const uint32_t r0 = cur.r0, count = cur.count;
         __syncthreads();  // the last slice's rows are read
-        copy_rows<NT>(rows, row_pitch, p.hq, I, k0, depth, l.order + r0, count);
+        copy.finish(rows, row_pitch, p.hq, I, k0, depth, l.order + r0, count);
         __syncthreads();
         const uint32_t live = (count + 7) / 8, pieces = (depth + 127) / 128;
         while (ru < per_slice && u < end) {
             const uint32_t here = min(min((uint32_t)S::group, per_slice - ru), end - u);
+            if (ru + here == per_slice && u + here < end) {  // the next slice's rows, behind this group's products
+                cur = block_at<NT>(l, m.experts, (bs + 1) / p.slices);
+                k0 = (bs + 1) % p.slices * p.slice;
+                depth = min(p.slice, I - k0);
+                copy.fetch(tid, p.hq, I, k0, depth, l.order + cur.r0, cur.count);
+            }
             int* sum = sums + buf * S::group * 16 * S::pitch;
             buf ^= 1;
             for (uint32_t t = 0; t < here; ++t) {
@@ -657,26 +700,48 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
     cp_async_wait<0>();
 }
 
-// out[t][i] = sum over the slots of w * float(acc) * (rs2 * s2)
+// out[t][i] = sum over the slots of w * float(acc) * (rs2 * s2), two outputs a thread.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) moe_sum_kernel(Params p)
 {
-    griddep_wait();
     griddep_launch_dependents();
     const MoeLayer& m = p.m;
     const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) * 2, t = blockIdx.y;
-    if (i >= m.hidden) return;
+    const bool on = i < m.hidden;
+    constexpr uint32_t AHEAD = 8;
+    // All but the sums is there before the product in front of this kernel is done: the layer's inputs, and the routes'
+    // maxima, which that product waited for itself.
+    float w[AHEAD];
+    float2 sc[AHEAD];
+    auto scales = [&](uint32_t k0) {
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) {
+            w[k] = 0.f;
+            sc[k] = make_float2(0.f, 0.f);
+            if (!on || k0 + k >= m.topk) continue;
+            const uint32_t r = t * m.topk + k0 + k, e = (uint32_t)__ldg(m.topk_ids + r);
+            if (e >= m.experts) continue;
+            w[k] = __ldg(m.topk_w + r);
+            const float rs = row_scale_of(__uint_as_float(__ldcg(p.top + r)), m.qmax);
+            const float* s = m.s2 + (uint64_t)e * m.hidden + i;
+            sc[k] = make_float2(__fmul_rn(rs, __ldg(s)), __fmul_rn(rs, __ldg(s + 1)));
+        }
+    };
+    scales(0);
+    griddep_wait();
+    if (!on) return;
     float2 sum = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (uint32_t k = 0; k < m.topk; ++k) {
-        const uint32_t r = t * m.topk + k;
-        const uint32_t e = (uint32_t)__ldg(m.topk_ids + r);
-        if (e >= m.experts) continue;
-        const float w = __ldg(m.topk_w + r), rs = row_scale_of(__uint_as_float(p.top[r]), m.qmax);
-        const int2 a = *reinterpret_cast<const int2*>(p.acc + (uint64_t)r * m.hidden + i);
-        const float* s = m.s2 + (uint64_t)e * m.hidden + i;
-        sum.x = fmaf(w, __fmul_rn((float)a.x, __fmul_rn(rs, __ldg(s))), sum.x);
-        sum.y = fmaf(w, __fmul_rn((float)a.y, __fmul_rn(rs, __ldg(s + 1))), sum.y);
+    for (uint32_t k0 = 0; k0 < m.topk; k0 += AHEAD) {
+        if (k0 > 0) scales(k0);
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) {
+            if (k0 + k >= m.topk) break;
+            const uint32_t r = t * m.topk + k0 + k;
+            if ((uint32_t)__ldg(m.topk_ids + r) >= m.experts) continue;
+            const int2 a = __ldcg(reinterpret_cast<const int2*>(p.acc + (uint64_t)r * m.hidden + i));
+            sum.x = fmaf(w[k], __fmul_rn((float)a.x, sc[k].x), sum.x);
+            sum.y = fmaf(w[k], __fmul_rn((float)a.y, sc[k].y), sum.y);
+        }
     }
     T* out = static_cast<T*>(m.out) + (uint64_t)t * m.hidden + i;
     out[0] = (T)sum.x;
