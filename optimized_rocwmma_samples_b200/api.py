@@ -468,7 +468,10 @@ kernel_topk_softmax = topk_softmax
 # ----------------------------------------------------------------------------- decode step
 def _on(dev: torch.device):
     """The library launches on the current device: makes it the tensors' own."""
-    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+_HERE = nullcontext()
 
 
 def _new(make, shape, dtype: torch.dtype, dev: torch.device, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
@@ -493,10 +496,14 @@ def _scratch(given: Optional[torch.Tensor], nbytes: int, dev: torch.device, stre
 
 
 def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, dev: torch.device) -> int:
-    """Address of a contiguous tensor of this type, shape and device."""
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
+    """Address of a contiguous tensor of this type, shape and device (calls are short: every check counts)."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev.index:
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {dev}")
     return t.data_ptr()
+
+
+def _raw_stream(stream: Optional[torch.cuda.Stream], dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream.cuda_stream
 
 
 @functools.lru_cache(maxsize=1024)
@@ -535,7 +542,7 @@ def moe_layer(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tenso
     with _on(dev):
         ws, ws_bytes, hold = _scratch(workspace, _moe_layer_ws(dev.index, T, H, I, E, K), dev, stream)
         st = _lib.load().b2sq_moe_layer(x.data_ptr(), code, x.stride(0) if T > 1 else H, *args, T, H, I, E, K,
-                                        float(quant_max), ws, ws_bytes, _stream_ptr(stream, dev))
+                                        float(quant_max), ws, ws_bytes, _raw_stream(stream, dev))
     _lib.check(st, "b2sq_moe_layer")
     return out
 
@@ -583,9 +590,10 @@ class KV4Cache:
 
 def _kv4_rows(t: torch.Tensor, name: str, dev: torch.device):
     """(tokens, heads, token pitch) of a [tokens, heads, head_dim] tensor whose heads lie side by side."""
-    if t.dim() != 3 or t.device != dev or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or t.get_device() != dev.index or stride[2] != 1 or (shape[1] > 1 and stride[1] != shape[2]):
         raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous heads on {dev}")
-    return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1] * shape[2]
 
 
 def _kv4_seqs(page_table: torch.Tensor, seq_lens: torch.Tensor, token_start: Optional[torch.Tensor], dev: torch.device):
@@ -612,14 +620,14 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: KV4Cache, page_table: to
     T, heads, ks = _kv4_rows(k, "k", dev)
     _, _, vs = _kv4_rows(v, "v", dev)
     shape = (T, cache.kv_heads, cache.head_dim)
-    if tuple(k.shape) != shape or tuple(v.shape) != shape:
+    if k.shape != shape or v.shape != shape:
         raise ValueError(f"k and v must be {shape} for this cache")
     ko = None if k_out is None else _want(k_out, "k_out", k.dtype, shape, dev)
     vo = None if v_out is None else _want(v_out, "v_out", k.dtype, shape, dev)
     seqs = _kv4_seqs(page_table, seq_lens, token_start, dev)
     with _on(dev):
         st = _lib.load().b2sq_kv4_append(k.data_ptr(), v.data_ptr(), code, T, ks, vs, cache._ref, *seqs, ko, vo,
-                                         _stream_ptr(stream, dev))
+                                         _raw_stream(stream, dev))
     _lib.check(st, "b2sq_kv4_append")
 
 
@@ -650,7 +658,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, se
         raise ValueError("max_queries must not be negative")
     if out is None:
         out = _new(torch.zeros, q.shape, q.dtype, dev, stream)
-    o = _want(out, "out", q.dtype, tuple(q.shape), dev)
+    o = _want(out, "out", q.dtype, q.shape, dev)
     seqs = _kv4_seqs(page_table, seq_lens, token_start, dev)
     sc = cache.head_dim ** -0.5 if scale is None else float(scale)
     acc = int(accumulate_weight)
@@ -659,7 +667,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, se
                                  max_queries, acc)
         ws, ws_bytes, hold = _scratch(workspace, need, dev, stream)
         st = _lib.load().b2sq_kv4_attention(q.data_ptr(), code, T, heads, qs, cache._ref, *seqs, max_queries, sc, o, acc,
-                                            ws, ws_bytes, _stream_ptr(stream, dev))
+                                            ws, ws_bytes, _raw_stream(stream, dev))
     _lib.check(st, "b2sq_kv4_attention")
     return out
 
@@ -681,6 +689,6 @@ def kv4_evict(cache: KV4Cache, page_table: torch.Tensor, seq_lens: torch.Tensor,
     nl = _want(new_lens, "new_lens", torch.int32, (B,), dev)
     with _on(dev):
         st = _lib.load().b2sq_kv4_evict(cache._ref, table, B, P, lens, new_table, NP, budget, recent, nl,
-                                        _stream_ptr(stream, dev))
+                                        _raw_stream(stream, dev))
     _lib.check(st, "b2sq_kv4_evict")
     return new_lens
