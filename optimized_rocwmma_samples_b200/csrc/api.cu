@@ -612,7 +612,10 @@ b2sq_status validate_kv4_seqs(const char* fn, const int32_t* table, uint32_t bat
 
 b2sq::Kv4Cache kv4_cache_of(const b2sq_kv4_cache* c)
 {
-    return {c->k, c->v, c->k_scale, c->v_scale, c->weight, c->pages, c->kv_heads, c->page_size, c->head_dim};
+    int shift = 0;
+    while ((c->page_size >> shift) > 1) ++shift;
+    return {c->k, c->v, c->k_scale, c->v_scale, c->weight, c->pages, c->kv_heads, c->page_size, c->head_dim,
+            c->page_size == 1u << shift ? shift : -1};
 }
 }  // namespace
 
@@ -677,12 +680,15 @@ b2sq_status b2sq_kv4_append(const void* k, const void* v, b2sq_dtype type, uint3
     if (k_stride < row || v_stride < row) return fail(B2SQ_ERR_INVALID_ARG, "kv4_append: token pitch below kv_heads * head_dim");
     if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_out, 16) || !aligned(v_out, 16) || k_stride % 8 || v_stride % 8)
         return fail(B2SQ_ERR_UNSUPPORTED, "kv4_append: rows must be 16-byte aligned");
-    if (tokens > 0x7fffffffu || tokens * row / 2048 >= 0x7fffffffull)
-        return fail(B2SQ_ERR_INVALID_ARG, "kv4_append: too many tokens for one launch");
-    cudaError_t e = b2sq::launch_kv4_append(kv4_cache_of(cache),
-                                            {page_table, seq_lens, token_start, batch, max_pages, tokens}, k, v,
-                                            type == B2SQ_BF16, k_stride, v_stride, k_out, v_out,
-                                            reinterpret_cast<cudaStream_t>(stream));
+    if (tokens > 0x7fffffffu || row > 0x3fffffffu)
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_append: too many tokens or channels for one launch");
+    uint32_t sms = 0;
+    cudaError_t e = current_sm_count(&sms);
+    if (e != cudaSuccess) return cuda_fail(e, "kv4_append: SM count");
+    e = b2sq::launch_kv4_append(kv4_cache_of(cache),
+                                {page_table, seq_lens, token_start, batch, max_pages, tokens}, k, v,
+                                type == B2SQ_BF16, k_stride, v_stride, k_out, v_out, sms,
+                                reinterpret_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "kv4_append launch");
     return ok();
 }

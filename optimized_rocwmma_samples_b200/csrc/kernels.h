@@ -122,6 +122,7 @@ struct Kv4Cache {
     void *k_scale, *v_scale;  // fp16 pairs
     float* weight;            // nullable
     uint32_t pages, kv_heads, page_size, head_dim;
+    int page_shift;  // log2 of page_size, -1 where it is no power of two
 };
 struct Kv4Seqs {
     const int32_t* page_table;   // [batch][max_pages]
@@ -130,7 +131,8 @@ struct Kv4Seqs {
     uint32_t batch, max_pages, tokens;
 };
 cudaError_t launch_kv4_append(const Kv4Cache& c, const Kv4Seqs& s, const void* k, const void* v, bool bf16,
-                              uint64_t k_stride, uint64_t v_stride, void* k_out, void* v_out, cudaStream_t st);
+                              uint64_t k_stride, uint64_t v_stride, void* k_out, void* v_out, uint32_t num_sms,
+                              cudaStream_t st);
 
 struct Kv4Attention {
     Kv4Cache cache;

@@ -11,6 +11,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "sq_math.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -23,9 +24,10 @@ constexpr uint32_t kKv4Group = 64;
 __device__ __forceinline__ int64_t kv4_row(const Kv4Cache& c, const int32_t* __restrict__ table_row, uint32_t pos,
                                            uint32_t head)
 {
-    const int32_t page = __ldg(table_row + pos / c.page_size);
+    const uint32_t at = c.page_shift >= 0 ? pos >> c.page_shift : pos / c.page_size;
+    const int32_t page = __ldg(table_row + at);
     if ((uint32_t)page >= c.pages) return -1;
-    return ((int64_t)page * c.kv_heads + head) * c.page_size + pos % c.page_size;
+    return ((int64_t)page * c.kv_heads + head) * c.page_size + (pos - at * c.page_size);
 }
 
 // Length of sequence b (negative lengths count as 0); only its first kv4_cap tokens have a place in the table.
@@ -49,7 +51,9 @@ __device__ __forceinline__ float2 pair_to_f2(uint32_t w);
 template <>
 __device__ __forceinline__ float2 pair_to_f2<__half>(uint32_t w)
 {
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    float2 f;
+    h2_to_f2(w, f.x, f.y);
+    return f;
 }
 template <>
 __device__ __forceinline__ float2 pair_to_f2<__nv_bfloat16>(uint32_t w)

@@ -6,130 +6,188 @@
 // A NaN makes its group's s and z NaN, so it is not lost in the cache.
 //
 // Bound by HBM (2 bytes a channel in, 0.56 out, 2 more where the cached
-// values are asked for): eight lanes hold a group, one 16-byte load and one
-// 4-byte store of nibbles each, the extrema by three shuffles.  The quotient
-// is a product with 1 / s corrected by its exact remainder, since inputs of
-// 8 or 11 significant bits meet the border between two steps often.
+// values are asked for) as long as the arithmetic stays near ten instructions
+// a channel: eight lanes hold a group, one 16-byte load and one 4-byte store of
+// nibbles each; extrema in packed 16-bit operations and three shuffles; the
+// quotient as a saturated product with 1 / (15 s), whose exact remainder tells
+// whether it was rounded right.  Inputs of 8 or 11 significant bits meet the
+// border between two steps often, so those lanes decide it exactly.
 #include "kv4.cuh"
+
+#include <algorithm>
 
 namespace b2sq {
 
 namespace {
 
 constexpr uint32_t kAppendThreads = 256;
+constexpr uint32_t kAppendTokens = 8;  // tokens of a block at most
 constexpr float kHalfMax = 65504.f;
+constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, held in the low bits
 
+constexpr uint32_t kRoundBits = 0x3f400000u;  // sum of kRound's bits shifted left by 0, 4, ..., 28
+
+// Smaller and larger of packed pairs; a NaN wins.
+template <typename T>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b);
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t min2<__half>(uint32_t a, uint32_t b)
+{
+    uint32_t d;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+template <>
+__device__ __forceinline__ uint32_t max2<__half>(uint32_t a, uint32_t b)
+{
+    uint32_t d;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+template <>
+__device__ __forceinline__ uint32_t min2<__nv_bfloat16>(uint32_t a, uint32_t b)
+{
+    uint32_t d;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+template <>
+__device__ __forceinline__ uint32_t max2<__nv_bfloat16>(uint32_t a, uint32_t b)
+{
+    uint32_t d;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// A block takes a run of tokens: finds their places, then quantises their keys and values, eight channels a thread.
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads)
     kv4_append_kernel(Kv4Cache c, Kv4Seqs s, const T* __restrict__ k, const T* __restrict__ v, uint64_t k_stride,
-                      uint64_t v_stride, T* __restrict__ k_out, T* __restrict__ v_out)
+                      uint64_t v_stride, T* __restrict__ k_out, T* __restrict__ v_out, uint32_t tokens_each)
 {
+    __shared__ int64_t place[kAppendTokens];  // cache row of head 0, -1 for a token without a place
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t ng = c.head_dim / kKv4Group;
-    const uint32_t per_token = c.kv_heads * ng;  // groups
-    const uint64_t total = (uint64_t)s.tokens * per_token;
-    const uint64_t gi = ((uint64_t)blockIdx.x * kAppendThreads + threadIdx.x) / 8;
-    if (gi >= total) return;  // the eight lanes of a group leave together
-    const bool is_v = blockIdx.y != 0;
-    const uint32_t lane8 = threadIdx.x & 7;
-    const uint32_t mask = 0xffu << (threadIdx.x & 24);
-    const uint32_t token = (uint32_t)(gi / per_token), in_token = (uint32_t)(gi % per_token);
+    const uint32_t tid = threadIdx.x, token0 = blockIdx.x * tokens_each;
+    const uint32_t here = min(tokens_each, s.tokens - token0);
+    if (tid < here) {
+        const uint32_t token = token0 + tid;
+        // the sequence that holds this token: the last one starting at or before it
+        uint32_t lo = 0, hi = s.batch;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (__ldg(s.token_start + mid + 1) <= (int32_t)token)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        int64_t row = -1;
+        if (lo < s.batch) {
+            uint32_t start;
+            const uint32_t count = kv4_new_rows(s, lo, start);
+            // the new tokens are the sequence's last ones; what falls outside the table is not written
+            const int64_t p = (int64_t)kv4_len(s, lo) - count + ((int64_t)token - start);
+            if (token >= start && token - start < count && p >= 0 && p < (int64_t)kv4_cap(c, s))
+                row = kv4_row(c, s.page_table + (uint64_t)lo * s.max_pages, (uint32_t)p, 0);
+        }
+        place[tid] = row;
+    }
+    __syncthreads();
 
-    // the sequence that holds this token: the last one starting at or before it
-    uint32_t lo = 0, hi = s.batch;
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (__ldg(s.token_start + mid + 1) <= (int32_t)token)
-            lo = mid + 1;
-        else
-            hi = mid;
-    }
-    if (lo == s.batch) return;
-    uint32_t start;
-    const uint32_t count = kv4_new_rows(s, lo, start);
-    if (token < start || token - start >= count) return;
-    // the new tokens are the sequence's last ones; what falls outside the table is not written
-    const int64_t p = (int64_t)kv4_len(s, lo) - count + (token - start);
-    if (p < 0 || p >= (int64_t)kv4_cap(c, s)) return;
-    const uint32_t head = in_token / ng, g = in_token % ng;
-    const int64_t row = kv4_row(c, s.page_table + (uint64_t)lo * s.max_pages, (uint32_t)p, head);
-    if (row < 0) return;
-
-    const uint64_t ch = (uint64_t)in_token * kKv4Group + lane8 * 8;
-    const uint4 raw = *reinterpret_cast<const uint4*>((is_v ? v + token * v_stride : k + token * k_stride) + ch);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float f[8];
-    float mn = kHalfMax, mx = -kHalfMax;
-    bool nan = false;
+    const uint32_t ng = c.head_dim / kKv4Group, units = c.kv_heads * c.head_dim / 8;  // of keys, and of values
+    const uint32_t lane8 = tid & 7, mask = 0xffu << (tid & 24);
+    const uint32_t shift = __ffs(c.head_dim) - 1;
+    for (uint32_t t = 0; t < here; ++t) {
+        const int64_t row0 = place[t];
+        if (row0 < 0) continue;
+        const uint64_t token = token0 + t;
+        for (uint32_t u = tid; u < 2 * units; u += kAppendThreads) {  // whole groups of eight lanes: units is a multiple of 8
+            const bool is_v = u >= units;
+            const uint32_t ch = (is_v ? u - units : u) * 8;
+            const uint4 raw = *reinterpret_cast<const uint4*>((is_v ? v + token * v_stride : k + token * k_stride) + ch);
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            uint32_t lo2 = min2<T>(min2<T>(w[0], w[1]), min2<T>(w[2], w[3]));
+            uint32_t hi2 = max2<T>(max2<T>(w[0], w[1]), max2<T>(w[2], w[3]));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 t = pair_to_f2<T>(w[i]);
-        f[2 * i] = t.x;
-        f[2 * i + 1] = t.y;
-    }
+            for (int off = 4; off > 0; off >>= 1) {
+                lo2 = min2<T>(lo2, __shfl_xor_sync(mask, lo2, off));
+                hi2 = max2<T>(hi2, __shfl_xor_sync(mask, hi2, off));
+            }
+            const float2 lo = pair_to_f2<T>(lo2), hi = pair_to_f2<T>(hi2);
+            const bool nan = !(lo.x == lo.x && lo.y == lo.y);
+            const float mn = fminf(fmaxf(fminf(lo.x, lo.y), -kHalfMax), kHalfMax);
+            const float mx = fminf(fmaxf(fmaxf(hi.x, hi.y), -kHalfMax), kHalfMax);
+            const __half sh = __float2half_rn((mx - mn) / 15.f), zh = __float2half_rn(mn);
+            const float step = __half2float(sh), base = __half2float(zh), half_step = 0.5f * step;
+            const float inv15 = step > 0.f ? 1.f / (15.f * step) : 0.f;
+            float f[8], q[8], worst = 0.f;
+            uint32_t packed = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        nan |= f[i] != f[i];
-        f[i] = fminf(fmaxf(f[i], -kHalfMax), kHalfMax);
-        mn = fminf(mn, f[i]);
-        mx = fmaxf(mx, f[i]);
-    }
+            for (int i = 0; i < 4; ++i) {
+                const float2 x = pair_to_f2<T>(w[i]);
+                f[2 * i] = x.x;
+                f[2 * i + 1] = x.y;
+            }
 #pragma unroll
-    for (int off = 4; off > 0; off >>= 1) {
-        mn = fminf(mn, __shfl_xor_sync(mask, mn, off));
-        mx = fmaxf(mx, __shfl_xor_sync(mask, mx, off));
-    }
-    nan = __any_sync(mask, nan);
-    const __half sh = __float2half_rn((mx - mn) / 15.f), zh = __float2half_rn(mn);
-    const float step = __half2float(sh), base = __half2float(zh);
-    const float inv = step > 0.f ? 1.f / step : 0.f;
-    uint32_t packed = 0;
-    float back[8];
+            for (int i = 0; i < 8; ++i) {
+                const float d = f[i] - base;
+                const float r = fmaf(__saturatef(d * inv15), 15.f, kRound);
+                q[i] = r - kRound;
+                worst = fmaxf(worst, fabsf(fmaf(-q[i], step, d)));  // the remainder, exactly
+                packed += __float_as_uint(r) << (4 * i);
+            }
+            packed -= kRoundBits;
+            if (worst >= half_step && step > 0.f) {  // a border, a quotient rounded wrong, or a value that saturates
+                packed = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float t = f[i] - base;
-        float q = rintf(t * inv);
-        const float r2 = 2.f * fmaf(-q, step, t);  // twice the exact remainder
-        const bool odd = ((int)q & 1) != 0;
-        if (r2 > step || (r2 == step && odd)) q += 1.f;
-        if (r2 < -step || (r2 == -step && odd)) q -= 1.f;
-        q = step > 0.f ? fminf(fmaxf(q, 0.f), 15.f) : 0.f;
-        packed |= (uint32_t)q << (4 * i);
-        back[i] = nan ? __int_as_float(0x7fffffff) : fmaf(q, step, base);
-    }
-    uint8_t* data = (is_v ? c.v : c.k) + row * (c.head_dim / 2);
-    reinterpret_cast<uint32_t*>(data)[g * 8 + lane8] = packed;
-    if (lane8 == 0) {
-        const uint32_t sz = nan ? 0x7fff7fffu : (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(zh) << 16);
-        reinterpret_cast<uint32_t*>(is_v ? c.v_scale : c.k_scale)[row * ng + g] = sz;
-        if (!is_v && g == 0 && c.weight) c.weight[row] = 0.f;
-    }
-    T* out = is_v ? v_out : k_out;
-    if (out) {
-        uint4 o;
-        o.x = f2_to_pair<T>(back[0], back[1]);
-        o.y = f2_to_pair<T>(back[2], back[3]);
-        o.z = f2_to_pair<T>(back[4], back[5]);
-        o.w = f2_to_pair<T>(back[6], back[7]);
-        *reinterpret_cast<uint4*>(out + (uint64_t)token * c.kv_heads * c.head_dim + ch) = o;
+                for (int i = 0; i < 8; ++i) {
+                    const float d = f[i] - base, r2 = 2.f * fmaf(-q[i], step, d);
+                    const bool odd = ((int)q[i] & 1) != 0;
+                    if (r2 > step || (r2 == step && odd)) q[i] = fminf(q[i] + 1.f, 15.f);
+                    if (r2 < -step || (r2 == -step && odd)) q[i] = fmaxf(q[i] - 1.f, 0.f);
+                    packed |= (uint32_t)q[i] << (4 * i);
+                }
+            }
+            const uint32_t head = ch >> shift, in_head = ch & (c.head_dim - 1);
+            const int64_t row = row0 + (int64_t)head * c.page_size;
+            reinterpret_cast<uint32_t*>(is_v ? c.v : c.k)[row * (c.head_dim / 8) + in_head / 8] = packed;
+            if (lane8 == 0) {
+                const uint32_t g = in_head / kKv4Group;
+                const uint32_t sz = nan ? 0x7fff7fffu : (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(zh) << 16);
+                reinterpret_cast<uint32_t*>(is_v ? c.v_scale : c.k_scale)[row * ng + g] = sz;
+                if (!is_v && g == 0 && c.weight) c.weight[row] = 0.f;
+            }
+            T* out = is_v ? v_out : k_out;
+            if (out) {
+                const float b0 = nan ? __int_as_float(0x7fffffff) : base;
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o[i] = f2_to_pair<T>(fmaf(q[2 * i], step, b0), fmaf(q[2 * i + 1], step, b0));
+                *reinterpret_cast<uint4*>(out + token * c.kv_heads * c.head_dim + ch) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
     }
 }
 
 }  // namespace
 
 cudaError_t launch_kv4_append(const Kv4Cache& c, const Kv4Seqs& s, const void* k, const void* v, bool bf16,
-                              uint64_t k_stride, uint64_t v_stride, void* k_out, void* v_out, cudaStream_t st)
+                              uint64_t k_stride, uint64_t v_stride, void* k_out, void* v_out, uint32_t num_sms,
+                              cudaStream_t st)
 {
-    const uint64_t groups = (uint64_t)s.tokens * c.kv_heads * (c.head_dim / kKv4Group);
-    const dim3 grid((uint32_t)((groups * 8 + kAppendThreads - 1) / kAppendThreads), 2);
+    // a token a block until every SM has several, then runs of them
+    const uint32_t each = std::max(1u, std::min(kAppendTokens, s.tokens / (8 * num_sms)));
+    const dim3 grid((s.tokens + each - 1) / each);
     if (bf16)
         return launch_pdl(kv4_append_kernel<__nv_bfloat16>, grid, dim3(kAppendThreads), 0, st, c, s,
                           static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), k_stride,
-                          v_stride, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out));
+                          v_stride, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), each);
     return launch_pdl(kv4_append_kernel<__half>, grid, dim3(kAppendThreads), 0, st, c, s,
                       static_cast<const __half*>(k), static_cast<const __half*>(v), k_stride, v_stride,
-                      static_cast<__half*>(k_out), static_cast<__half*>(v_out));
+                      static_cast<__half*>(k_out), static_cast<__half*>(v_out), each);
 }
 
 }  // namespace b2sq

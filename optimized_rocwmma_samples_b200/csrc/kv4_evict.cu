@@ -23,7 +23,8 @@ namespace {
 constexpr uint32_t kEvictThreads = 512;
 constexpr uint32_t kEvictWarps = kEvictThreads / 32;
 constexpr uint32_t kEvictKeys = 40960;  // keys held in shared memory (160 KB); longer sequences re-read theirs
-constexpr uint32_t kEvictRows = 4096;   // kept rows one block lists at a time
+constexpr uint32_t kEvictRows = 1024;   // kept rows one block lists at a time
+constexpr uint32_t kEvictFly = 4;       // copies of a thread in flight
 
 // Bits that order as the weights do; -0 equals +0, NaN is above infinity.
 __device__ __forceinline__ uint32_t weight_key(float w)
@@ -39,9 +40,10 @@ __global__ void __launch_bounds__(kEvictThreads)
                      uint32_t new_max_pages, uint32_t budget, uint32_t recent, int32_t* __restrict__ new_lens,
                      uint32_t key_slots, uint32_t row_slots)
 {
-    extern __shared__ uint32_t ev_smem[];
+    extern __shared__ __align__(16) uint32_t ev_smem[];
     uint32_t* keys = ev_smem;              // [key_slots]
-    uint32_t* rows = ev_smem + key_slots;  // [row_slots]
+    uint32_t* rows = ev_smem + key_slots;  // [row_slots] positions of kept tokens
+    longlong2* at = reinterpret_cast<longlong2*>(rows + row_slots);  // [row_slots] cache rows they come from and go to
     __shared__ uint32_t hist[256];
     __shared__ uint32_t warp_gt[kEvictWarps], warp_eq[kEvictWarps];
     __shared__ uint32_t sel_digit, sel_above;
@@ -70,8 +72,21 @@ __global__ void __launch_bounds__(kEvictThreads)
         return r < 0 ? 0u : weight_key(c.weight[r]);
     };
     const bool held = old <= key_slots;
-    if (held)
-        for (uint32_t i = tid; i < old; i += kEvictThreads) keys[i] = key_of(i);
+    if (held) {
+        constexpr uint32_t FLY = 8;
+        for (uint32_t i0 = tid; i0 < old; i0 += FLY * kEvictThreads) {
+            int64_t r[FLY];
+            float w[FLY];
+#pragma unroll
+            for (uint32_t n = 0; n < FLY; ++n)
+                r[n] = i0 + n * kEvictThreads < old ? kv4_row(c, table, i0 + n * kEvictThreads, head) : -1;
+#pragma unroll
+            for (uint32_t n = 0; n < FLY; ++n) w[n] = r[n] >= 0 ? c.weight[r[n]] : 0.f;
+#pragma unroll
+            for (uint32_t n = 0; n < FLY; ++n)
+                if (i0 + n * kEvictThreads < old) keys[i0 + n * kEvictThreads] = r[n] >= 0 ? weight_key(w[n]) : 0u;
+        }
+    }
     auto key_at = [&](uint32_t i) { return held ? keys[i] : key_of(i); };
 
     // the want-th largest key: `prefix` gathers its digits, `above` counts larger ones
@@ -143,6 +158,7 @@ __global__ void __launch_bounds__(kEvictThreads)
 
     const uint32_t ng = c.head_dim / kKv4Group;
     const uint32_t quads = c.head_dim / 32;  // 16-byte pieces of a row's keys (and of its values)
+    const uint32_t gshift = __ffs(ng) - 1, qshift = __ffs(quads) - 1;
     for (uint32_t r0 = d0; r0 < d1; r0 += row_slots) {
         const uint32_t r1 = min(r0 + row_slots, d1);
         if (!take_none) {
@@ -164,25 +180,48 @@ __global__ void __launch_bounds__(kEvictThreads)
         }
         for (uint32_t to = max(r0, want) + tid; to < r1; to += kEvictThreads) rows[to - r0] = all ? to : n - kept + to;
         __syncthreads();
-        for (uint32_t u = tid; u < (r1 - r0) * 2 * quads; u += kEvictThreads) {
-            const uint32_t j = u / (2 * quads), piece = u % (2 * quads);
+        for (uint32_t j = tid; j < r1 - r0; j += kEvictThreads) {
             const int64_t src = kv4_row(c, table, rows[j], head), dst = kv4_row(c, dst_table, r0 + j, head);
-            if (src < 0 || dst < 0) continue;
-            uint8_t* base = piece < quads ? c.k : c.v;
-            const uint32_t q = piece < quads ? piece : piece - quads;
-            reinterpret_cast<uint4*>(base)[dst * quads + q] = reinterpret_cast<const uint4*>(base)[src * quads + q];
+            at[j] = src < 0 || dst < 0 ? make_longlong2(-1, -1) : make_longlong2(src, dst);
+            if (src >= 0 && dst >= 0) c.weight[dst] = c.weight[src];
         }
-        for (uint32_t u = tid; u < (r1 - r0) * (2 * ng + 1); u += kEvictThreads) {
-            const uint32_t j = u / (2 * ng + 1), piece = u % (2 * ng + 1);
-            const int64_t src = kv4_row(c, table, rows[j], head), dst = kv4_row(c, dst_table, r0 + j, head);
-            if (src < 0 || dst < 0) continue;
-            if (piece == 2 * ng) {
-                c.weight[dst] = c.weight[src];
-            } else {
-                uint32_t* base = static_cast<uint32_t*>(piece < ng ? c.k_scale : c.v_scale);
-                const uint32_t q = piece < ng ? piece : piece - ng;
-                base[dst * ng + q] = base[src * ng + q];
+        __syncthreads();
+        // 16-byte pieces of keys, then values; then the steps and bases, word by word
+        const uint32_t pieces = (r1 - r0) * 2 * quads;
+        for (uint32_t u0 = tid; u0 < pieces; u0 += kEvictFly * kEvictThreads) {
+            uint4 v[kEvictFly];
+            uint4* to[kEvictFly];
+#pragma unroll
+            for (uint32_t n = 0; n < kEvictFly; ++n) {
+                const uint32_t u = u0 + n * kEvictThreads, j = u >> (qshift + 1), piece = u & (2 * quads - 1);
+                to[n] = nullptr;
+                if (u < pieces && at[j].x >= 0) {
+                    uint4* base = reinterpret_cast<uint4*>(piece < quads ? c.k : c.v) + (piece & (quads - 1));
+                    v[n] = base[at[j].x << qshift];
+                    to[n] = base + (at[j].y << qshift);
+                }
             }
+#pragma unroll
+            for (uint32_t n = 0; n < kEvictFly; ++n)
+                if (to[n]) *to[n] = v[n];
+        }
+        const uint32_t words = (r1 - r0) * 2 * ng;
+        for (uint32_t u0 = tid; u0 < words; u0 += kEvictFly * kEvictThreads) {
+            uint32_t v[kEvictFly];
+            uint32_t* to[kEvictFly];
+#pragma unroll
+            for (uint32_t n = 0; n < kEvictFly; ++n) {
+                const uint32_t u = u0 + n * kEvictThreads, j = u >> (gshift + 1), piece = u & (2 * ng - 1);
+                to[n] = nullptr;
+                if (u < words && at[j].x >= 0) {
+                    uint32_t* base = static_cast<uint32_t*>(piece < ng ? c.k_scale : c.v_scale) + (piece & (ng - 1));
+                    v[n] = base[at[j].x << gshift];
+                    to[n] = base + (at[j].y << gshift);
+                }
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < kEvictFly; ++n)
+                if (to[n]) *to[n] = v[n];
         }
         __syncthreads();
     }
@@ -200,10 +239,10 @@ cudaError_t launch_kv4_evict(const Kv4Cache& c, const int32_t* page_table, uint3
         1, std::min<uint64_t>((2 * num_sms + heads - 1) / heads, std::min<uint64_t>(16, (budget + 63) / 64)));
     const uint32_t cap = max_pages * c.page_size;
     const uint32_t key_slots = cap <= kEvictKeys ? (cap + 3) / 4 * 4 : 0;
-    const uint32_t row_slots = std::min(kEvictRows, (budget + split - 1) / split + 1);
-    const size_t smem = (size_t)(key_slots + row_slots) * 4;
+    const uint32_t row_slots = (std::min(kEvictRows, (budget + split - 1) / split + 1) + 3) / 4 * 4;
+    const size_t smem = (size_t)key_slots * 4 + (size_t)row_slots * 20;
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = allow_smem(kv4_evict_kernel, (kEvictKeys + kEvictRows) * 4, done);
+    const cudaError_t e = allow_smem(kv4_evict_kernel, kEvictKeys * 4 + kEvictRows * 20, done);
     if (e != cudaSuccess) return e;
     return launch_pdl(kv4_evict_kernel, dim3(split, c.kv_heads, batch), dim3(kEvictThreads), smem, st, c, page_table,
                       max_pages, seq_lens, new_table, new_max_pages, budget, recent, new_lens, key_slots, row_slots);
