@@ -27,6 +27,15 @@ constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an inte
 
 constexpr uint32_t kRoundBits = 0x3f400000u;  // sum of kRound's bits shifted left by 0, 4, ..., 28
 
+constexpr float kFifteenth = 1.f / 15.f;
+
+__device__ __forceinline__ float approx_rcp(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Smaller and larger of packed pairs; a NaN wins.
 template <typename T>
 __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b);
@@ -96,18 +105,30 @@ __global__ void __launch_bounds__(kAppendThreads)
     }
     __syncthreads();
 
-    const uint32_t ng = c.head_dim / kKv4Group, units = c.kv_heads * c.head_dim / 8;  // of keys, and of values
+    const uint32_t units = c.kv_heads * c.head_dim / 8;  // of keys, and of values
     const uint32_t lane8 = tid & 7, mask = 0xffu << (tid & 24);
-    const uint32_t shift = __ffs(c.head_dim) - 1;
-    for (uint32_t t = 0; t < here; ++t) {
-        const int64_t row0 = place[t];
-        if (row0 < 0) continue;
-        const uint64_t token = token0 + t;
-        for (uint32_t u = tid; u < 2 * units; u += kAppendThreads) {  // whole groups of eight lanes: units is a multiple of 8
-            const bool is_v = u >= units;
-            const uint32_t ch = (is_v ? u - units : u) * 8;
-            const uint4 raw = *reinterpret_cast<const uint4*>((is_v ? v + token * v_stride : k + token * k_stride) + ch);
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    const uint32_t dshift = __ffs(c.head_dim) - 1, gshift = dshift - 6;
+    for (uint32_t u = tid; u < 2 * units; u += kAppendThreads) {  // whole groups of eight lanes: units is a multiple of 8
+        const bool is_v = u >= units;
+        const uint32_t ch = (is_v ? u - units : u) * 8, head = ch >> dshift, in_head = ch & (c.head_dim - 1);
+        const uint64_t stride = is_v ? v_stride : k_stride, out_stride = (uint64_t)units * 8;
+        const T* src = (is_v ? v : k) + token0 * stride + ch;
+        T* out = is_v ? v_out : k_out;
+        if (out) out += token0 * out_stride + ch;
+        // of head 0's row in the cache: this head's nibbles and group
+        uint32_t* data = reinterpret_cast<uint32_t*>(is_v ? c.v : c.k) + ((uint64_t)head * c.page_size << (dshift - 3)) + in_head / 8;
+        uint32_t* scale = reinterpret_cast<uint32_t*>(is_v ? c.v_scale : c.k_scale) +
+                          ((uint64_t)head * c.page_size << gshift) + in_head / kKv4Group;
+        float* weight = !is_v && in_head == 0 && c.weight ? c.weight + (uint64_t)head * c.page_size : nullptr;
+        uint4 next = place[0] >= 0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+        for (uint32_t t = 0; t < here; ++t) {
+            const uint32_t w[4] = {next.x, next.y, next.z, next.w};
+            const int64_t row0 = place[t];
+            src += stride;
+            if (t + 1 < here && place[t + 1] >= 0) next = *reinterpret_cast<const uint4*>(src);
+            T* to = out;
+            if (out) out += out_stride;
+            if (row0 < 0) continue;
             uint32_t lo2 = min2<T>(min2<T>(w[0], w[1]), min2<T>(w[2], w[3]));
             uint32_t hi2 = max2<T>(max2<T>(w[0], w[1]), max2<T>(w[2], w[3]));
 #pragma unroll
@@ -119,54 +140,50 @@ __global__ void __launch_bounds__(kAppendThreads)
             const bool nan = !(lo.x == lo.x && lo.y == lo.y);
             const float mn = fminf(fmaxf(fminf(lo.x, lo.y), -kHalfMax), kHalfMax);
             const float mx = fminf(fmaxf(fmaxf(hi.x, hi.y), -kHalfMax), kHalfMax);
-            const __half sh = __float2half_rn((mx - mn) / 15.f), zh = __float2half_rn(mn);
+            // (mx - mn) / 15, the product with 1 / 15 and one Newton correction by its exact remainder
+            const float range = mx - mn, s0 = range * kFifteenth, s1 = fmaf(fmaf(-s0, 15.f, range), kFifteenth, s0);
+            const __half sh = __float2half_rn(s1), zh = __float2half_rn(mn);
             const float step = __half2float(sh), base = __half2float(zh), half_step = 0.5f * step;
-            const float inv15 = step > 0.f ? 1.f / (15.f * step) : 0.f;
+            const float inv15 = step > 0.f ? approx_rcp(15.f * step) : 0.f;  // (its errors are mended below)
             float f[8], q[8], worst = 0.f;
-            uint32_t packed = 0;
+            uint32_t packed = 0u - kRoundBits;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float2 x = pair_to_f2<T>(w[i]);
-                f[2 * i] = x.x;
-                f[2 * i + 1] = x.y;
+                f[2 * i] = x.x - base;
+                f[2 * i + 1] = x.y - base;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float d = f[i] - base;
-                const float r = fmaf(__saturatef(d * inv15), 15.f, kRound);
+                const float r = fmaf(__saturatef(f[i] * inv15), 15.f, kRound);
                 q[i] = r - kRound;
-                worst = fmaxf(worst, fabsf(fmaf(-q[i], step, d)));  // the remainder, exactly
+                worst = fmaxf(worst, fabsf(fmaf(-q[i], step, f[i])));  // the remainder, exactly
                 packed += __float_as_uint(r) << (4 * i);
             }
-            packed -= kRoundBits;
             if (worst >= half_step && step > 0.f) {  // a border, a quotient rounded wrong, or a value that saturates
                 packed = 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float d = f[i] - base, r2 = 2.f * fmaf(-q[i], step, d);
+                    const float r2 = 2.f * fmaf(-q[i], step, f[i]);
                     const bool odd = ((int)q[i] & 1) != 0;
                     if (r2 > step || (r2 == step && odd)) q[i] = fminf(q[i] + 1.f, 15.f);
                     if (r2 < -step || (r2 == -step && odd)) q[i] = fmaxf(q[i] - 1.f, 0.f);
                     packed |= (uint32_t)q[i] << (4 * i);
                 }
             }
-            const uint32_t head = ch >> shift, in_head = ch & (c.head_dim - 1);
-            const int64_t row = row0 + (int64_t)head * c.page_size;
-            reinterpret_cast<uint32_t*>(is_v ? c.v : c.k)[row * (c.head_dim / 8) + in_head / 8] = packed;
+            data[row0 << (dshift - 3)] = packed;
             if (lane8 == 0) {
-                const uint32_t g = in_head / kKv4Group;
-                const uint32_t sz = nan ? 0x7fff7fffu : (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(zh) << 16);
-                reinterpret_cast<uint32_t*>(is_v ? c.v_scale : c.k_scale)[row * ng + g] = sz;
-                if (!is_v && g == 0 && c.weight) c.weight[row] = 0.f;
+                scale[row0 << gshift] =
+                    nan ? 0x7fff7fffu : (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(zh) << 16);
+                if (weight) weight[row0] = 0.f;
             }
-            T* out = is_v ? v_out : k_out;
-            if (out) {
+            if (to) {
                 const float b0 = nan ? __int_as_float(0x7fffffff) : base;
                 uint32_t o[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     o[i] = f2_to_pair<T>(fmaf(q[2 * i], step, b0), fmaf(q[2 * i + 1], step, b0));
-                *reinterpret_cast<uint4*>(out + token * c.kv_heads * c.head_dim + ch) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(to) = make_uint4(o[0], o[1], o[2], o[3]);
             }
         }
     }

@@ -8,8 +8,8 @@
 // whole.
 //
 // The threshold is found by a radix search over the weights' sortable bits
-// (four passes of 8 bits over keys in shared memory), places by ballots and
-// one prefix sum over the warps.  Every block of a head repeats that search
+// (four passes of 8 bits over keys in shared memory), places by prefix sums
+// within and over the warps.  Every block of a head repeats that search
 // and copies its own share of the kept rows, so no block waits for another.
 #include "kv4.cuh"
 
@@ -87,7 +87,16 @@ __global__ void __launch_bounds__(kEvictThreads)
                 if (i0 + n * kEvictThreads < old) keys[i0 + n * kEvictThreads] = r[n] >= 0 ? weight_key(w[n]) : 0u;
         }
     }
-    auto key_at = [&](uint32_t i) { return held ? keys[i] : key_of(i); };
+    // keys of positions i .. i + 3 (i a multiple of 4); past the candidates: anything
+    auto keys_at = [&](uint32_t i, uint32_t (&k)[4]) {
+        if (held) {
+            const uint4 v = *reinterpret_cast<const uint4*>(keys + i);
+            k[0] = v.x, k[1] = v.y, k[2] = v.z, k[3] = v.w;
+        } else {
+#pragma unroll
+            for (uint32_t n = 0; n < 4; ++n) k[n] = i + n < old ? key_of(i + n) : 0;
+        }
+    };
 
     // the want-th largest key: `prefix` gathers its digits, `above` counts larger ones
     uint32_t prefix = 0, above = 0;
@@ -95,13 +104,13 @@ __global__ void __launch_bounds__(kEvictThreads)
         for (int shift = 24; shift >= 0; shift -= 8) {
             for (uint32_t i = tid; i < 256; i += kEvictThreads) hist[i] = 0;
             __syncthreads();
-            for (uint32_t i = tid; i < (old + 31) / 32 * 32; i += kEvictThreads) {  // whole warps
-                const uint32_t key = i < old ? key_at(i) : 0;
-                const bool mine = i < old && (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
-                const uint32_t digit = mine ? (key >> shift) & 255u : 256u;
-                // lanes of the same digit add once (weights of one size share their upper digits)
-                const uint32_t same = __match_any_sync(0xffffffffu, digit);
-                if (mine && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+            for (uint32_t i = tid * 4; i < old; i += 4 * kEvictThreads) {
+                uint32_t k[4];
+                keys_at(i, k);
+#pragma unroll
+                for (uint32_t n = 0; n < 4; ++n)
+                    if (i + n < old && (shift == 24 || ((k[n] ^ prefix) >> (shift + 8)) == 0))
+                        atomicAdd(&hist[(k[n] >> shift) & 255u], 1u);
             }
             __syncthreads();
             if (warp == 0) {
@@ -135,16 +144,31 @@ __global__ void __launch_bounds__(kEvictThreads)
     const uint32_t ties = want - above;  // of the keys equal to `prefix`, the first ones
     const bool take_all_old = want == old, take_none = want == 0;
 
-    // each warp walks a run of positions: first its counts, then the places
-    const uint32_t run = (old + kEvictWarps * 32 - 1) / (kEvictWarps * 32) * 32;
+    // each warp walks a run of positions, four a lane: first its counts, then the places.  Larger ones are counted in
+    // the lower half of a word, equal ones in the upper (a run of 128 positions a step, so a step's sums fit).
+    const uint32_t run = (old + kEvictWarps * 128 - 1) / (kEvictWarps * 128) * 128;
     const uint32_t w0 = min(warp * run, old), w1 = min(w0 + run, old);
+    auto marks = [&](uint32_t i, uint32_t n, uint32_t key) -> uint32_t {  // 1: larger, 1 << 16: equal
+        if (i + n >= w1) return 0u;
+        if (take_all_old || key > prefix) return 1u;
+        return key == prefix ? 1u << 16 : 0u;
+    };
     uint32_t gt = 0, eq = 0;
     if (!take_none)
-        for (uint32_t i = w0 + lane; i < w0 + run; i += 32) {
-            const uint32_t key = i < w1 ? key_at(i) : 0;
-            gt += __popc(__ballot_sync(0xffffffffu, i < w1 && (take_all_old || key > prefix)));
-            eq += __popc(__ballot_sync(0xffffffffu, i < w1 && !take_all_old && key == prefix));
+        for (uint32_t i = w0 + lane * 4; i < w1; i += 128) {
+            uint32_t k[4];
+            keys_at(i, k);
+            uint32_t both = 0;
+#pragma unroll
+            for (uint32_t n = 0; n < 4; ++n) both += marks(i, n, k[n]);
+            gt += both & 0xffffu;
+            eq += both >> 16;
         }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        gt += __shfl_xor_sync(0xffffffffu, gt, off);
+        eq += __shfl_xor_sync(0xffffffffu, eq, off);
+    }
     if (lane == 0) {
         warp_gt[warp] = gt;
         warp_eq[warp] = eq;
@@ -162,20 +186,36 @@ __global__ void __launch_bounds__(kEvictThreads)
     for (uint32_t r0 = d0; r0 < d1; r0 += row_slots) {
         const uint32_t r1 = min(r0 + row_slots, d1);
         if (!take_none) {
-            uint32_t g = gt0, e = eq0;
-            for (uint32_t i = w0 + lane; i < w0 + run; i += 32) {
-                const uint32_t key = i < w1 ? key_at(i) : 0;
-                const bool is_gt = i < w1 && (take_all_old || key > prefix);
-                const bool is_eq = i < w1 && !take_all_old && key == prefix;
-                const uint32_t mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
-                const uint32_t below = (1u << lane) - 1;
-                const uint32_t eq_rank = e + __popc(me & below);
-                if (is_gt || (is_eq && eq_rank < ties)) {
-                    const uint32_t to = g + __popc(mg & below) + min(eq_rank, ties);
-                    if (to >= r0 && to < r1) rows[to - r0] = i;
+            uint32_t g = gt0, e = eq0;  // before this step
+            for (uint32_t base = w0; base < w1; base += 128) {
+                const uint32_t i = base + lane * 4;
+                uint32_t k[4] = {}, mine[4], sum = 0;
+                if (i < w1) keys_at(i, k);
+#pragma unroll
+                for (uint32_t n = 0; n < 4; ++n) {
+                    mine[n] = marks(i, n, k[n]);
+                    sum += mine[n];
                 }
-                g += __popc(mg);
-                e += __popc(me);
+                uint32_t incl = sum;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const uint32_t t = __shfl_up_sync(0xffffffffu, incl, off);
+                    if (lane >= (uint32_t)off) incl += t;
+                }
+                uint32_t lg = g + ((incl - sum) & 0xffffu), le = e + ((incl - sum) >> 16);
+#pragma unroll
+                for (uint32_t n = 0; n < 4; ++n) {
+                    const bool is_gt = mine[n] == 1u, is_eq = mine[n] > 1u;
+                    if (is_gt || (is_eq && le < ties)) {
+                        const uint32_t to = lg + min(le, ties);
+                        if (to >= r0 && to < r1) rows[to - r0] = i + n;
+                    }
+                    lg += is_gt;
+                    le += is_eq;
+                }
+                const uint32_t all_sum = __shfl_sync(0xffffffffu, incl, 31);
+                g += all_sum & 0xffffu;
+                e += all_sum >> 16;
             }
         }
         for (uint32_t to = max(r0, want) + tid; to < r1; to += kEvictThreads) rows[to - r0] = all ? to : n - kept + to;
