@@ -23,7 +23,7 @@ namespace {
 constexpr uint32_t kEvictThreads = 512;
 constexpr uint32_t kEvictWarps = kEvictThreads / 32;
 constexpr uint32_t kEvictKeys = 40960;  // keys held in shared memory (160 KB); longer sequences re-read theirs
-constexpr uint32_t kEvictRows = 1024;   // kept rows one block lists at a time
+constexpr uint32_t kEvictRows = 2048;   // kept rows one block lists at a time
 constexpr uint32_t kEvictFly = 4;       // copies of a thread in flight
 
 // Bits that order as the weights do; -0 equals +0, NaN is above infinity.
@@ -34,7 +34,45 @@ __device__ __forceinline__ uint32_t weight_key(float w)
     return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kEvictThreads)
+template <uint32_t NG>
+struct ScaleWord;  // a row's steps and bases of its keys, or values
+template <>
+struct ScaleWord<1> {
+    using type = uint32_t;
+};
+template <>
+struct ScaleWord<2> {
+    using type = uint2;
+};
+template <>
+struct ScaleWord<4> {
+    using type = uint4;
+};
+
+// Rows turn, turn + STEP, ... of `count`: one word of rows of PITCH words each.
+template <uint32_t STEP, uint32_t PITCH, typename W>
+__device__ __forceinline__ void copy_rows(W* base, const longlong2* at, uint32_t turn, uint32_t count)
+{
+    for (uint32_t j0 = turn; j0 < count; j0 += kEvictFly * STEP) {
+        W v[kEvictFly];
+        int64_t to[kEvictFly];
+#pragma unroll
+        for (uint32_t n = 0; n < kEvictFly; ++n) {
+            to[n] = -1;
+            if (j0 + n * STEP < count) {
+                const longlong2 a = at[j0 + n * STEP];
+                to[n] = a.y;
+                if (a.y >= 0) v[n] = base[a.x * PITCH];
+            }
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < kEvictFly; ++n)
+            if (to[n] >= 0) base[to[n] * PITCH] = v[n];
+    }
+}
+
+template <uint32_t NG>  // groups of 64 channels
+__global__ void __launch_bounds__(kEvictThreads, 2)
     kv4_evict_kernel(Kv4Cache c, const int32_t* __restrict__ page_table, uint32_t max_pages,
                      const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ new_table,
                      uint32_t new_max_pages, uint32_t budget, uint32_t recent, int32_t* __restrict__ new_lens,
@@ -180,9 +218,12 @@ __global__ void __launch_bounds__(kEvictThreads)
         eq0 += warp_eq[i];
     }
 
-    const uint32_t ng = c.head_dim / kKv4Group;
-    const uint32_t quads = c.head_dim / 32;  // 16-byte pieces of a row's keys (and of its values)
-    const uint32_t gshift = __ffs(ng) - 1, qshift = __ffs(quads) - 1;
+    // a thread copies the same 16-byte piece of every row that is its turn: keys, then values
+    constexpr uint32_t PIECES = 4 * NG, ROWS = kEvictThreads / PIECES;
+    const uint32_t piece = tid % PIECES, turn = tid / PIECES;
+    uint4* const data = reinterpret_cast<uint4*>(piece < PIECES / 2 ? c.k : c.v) + piece % (PIECES / 2);
+    using Scale = typename ScaleWord<NG>::type;
+    Scale* const scale = static_cast<Scale*>(tid & 1 ? c.v_scale : c.k_scale);
     for (uint32_t r0 = d0; r0 < d1; r0 += row_slots) {
         const uint32_t r1 = min(r0 + row_slots, d1);
         if (!take_none) {
@@ -226,43 +267,8 @@ __global__ void __launch_bounds__(kEvictThreads)
             if (src >= 0 && dst >= 0) c.weight[dst] = c.weight[src];
         }
         __syncthreads();
-        // 16-byte pieces of keys, then values; then the steps and bases, word by word
-        const uint32_t pieces = (r1 - r0) * 2 * quads;
-        for (uint32_t u0 = tid; u0 < pieces; u0 += kEvictFly * kEvictThreads) {
-            uint4 v[kEvictFly];
-            uint4* to[kEvictFly];
-#pragma unroll
-            for (uint32_t n = 0; n < kEvictFly; ++n) {
-                const uint32_t u = u0 + n * kEvictThreads, j = u >> (qshift + 1), piece = u & (2 * quads - 1);
-                to[n] = nullptr;
-                if (u < pieces && at[j].x >= 0) {
-                    uint4* base = reinterpret_cast<uint4*>(piece < quads ? c.k : c.v) + (piece & (quads - 1));
-                    v[n] = base[at[j].x << qshift];
-                    to[n] = base + (at[j].y << qshift);
-                }
-            }
-#pragma unroll
-            for (uint32_t n = 0; n < kEvictFly; ++n)
-                if (to[n]) *to[n] = v[n];
-        }
-        const uint32_t words = (r1 - r0) * 2 * ng;
-        for (uint32_t u0 = tid; u0 < words; u0 += kEvictFly * kEvictThreads) {
-            uint32_t v[kEvictFly];
-            uint32_t* to[kEvictFly];
-#pragma unroll
-            for (uint32_t n = 0; n < kEvictFly; ++n) {
-                const uint32_t u = u0 + n * kEvictThreads, j = u >> (gshift + 1), piece = u & (2 * ng - 1);
-                to[n] = nullptr;
-                if (u < words && at[j].x >= 0) {
-                    uint32_t* base = static_cast<uint32_t*>(piece < ng ? c.k_scale : c.v_scale) + (piece & (ng - 1));
-                    v[n] = base[at[j].x << gshift];
-                    to[n] = base + (at[j].y << gshift);
-                }
-            }
-#pragma unroll
-            for (uint32_t n = 0; n < kEvictFly; ++n)
-                if (to[n]) *to[n] = v[n];
-        }
+        copy_rows<ROWS, PIECES / 2>(data, at, turn, r1 - r0);
+        copy_rows<kEvictThreads / 2, 1>(scale, at, tid / 2, r1 - r0);
         __syncthreads();
     }
 }
@@ -274,18 +280,26 @@ cudaError_t launch_kv4_evict(const Kv4Cache& c, const int32_t* page_table, uint3
                              uint32_t recent, int32_t* new_lens, uint32_t num_sms, cudaStream_t st)
 {
     const uint64_t heads = (uint64_t)batch * c.kv_heads;
-    // about two blocks an SM; a block copies at least 64 rows
+    // a block for every SM; each copies at least 64 rows (twice as many took 64 us instead of 54 at 32 x 8192 tokens and
+    // 8 heads: the search is repeated)
     const uint32_t split = (uint32_t)std::max<uint64_t>(
-        1, std::min<uint64_t>((2 * num_sms + heads - 1) / heads, std::min<uint64_t>(16, (budget + 63) / 64)));
+        1, std::min<uint64_t>((num_sms + heads - 1) / heads, std::min<uint64_t>(16, (budget + 63) / 64)));
     const uint32_t cap = max_pages * c.page_size;
     const uint32_t key_slots = cap <= kEvictKeys ? (cap + 3) / 4 * 4 : 0;
     const uint32_t row_slots = (std::min(kEvictRows, (budget + split - 1) / split + 1) + 3) / 4 * 4;
     const size_t smem = (size_t)key_slots * 4 + (size_t)row_slots * 20;
-    static std::atomic<uint64_t> done{0};
-    const cudaError_t e = allow_smem(kv4_evict_kernel, kEvictKeys * 4 + kEvictRows * 20, done);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(kv4_evict_kernel, dim3(split, c.kv_heads, batch), dim3(kEvictThreads), smem, st, c, page_table,
-                      max_pages, seq_lens, new_table, new_max_pages, budget, recent, new_lens, key_slots, row_slots);
+    auto launch = [&](auto kernel, std::atomic<uint64_t>& done) {
+        const cudaError_t e = allow_smem(kernel, kEvictKeys * 4 + kEvictRows * 20, done);
+        if (e != cudaSuccess) return e;
+        return launch_pdl(kernel, dim3(split, c.kv_heads, batch), dim3(kEvictThreads), smem, st, c, page_table, max_pages,
+                          seq_lens, new_table, new_max_pages, budget, recent, new_lens, key_slots, row_slots);
+    };
+    static std::atomic<uint64_t> done[3];
+    switch (c.head_dim) {
+        case 64: return launch(kv4_evict_kernel<1>, done[0]);
+        case 128: return launch(kv4_evict_kernel<2>, done[1]);
+        default: return launch(kv4_evict_kernel<4>, done[2]);
+    }
 }
 
 }  // namespace b2sq
