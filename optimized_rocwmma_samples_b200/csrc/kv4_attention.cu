@@ -882,22 +882,51 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, ui
                                          : make_float2(0.f, 0.f);
             }
             __syncthreads();
-#pragma unroll 4
-            for (uint32_t t = p0 + tid; t < p1; t += kJoinThreads) {
-                const int64_t at = kv4_row(a.c, table, t, head);
-                const float* sp = scores + (uint64_t)t * a.row_pad + r0;
-                float sum = 0.f;
-                for (uint32_t r = 0; r < rows; r += 4) {  // row_pad is a multiple of 4
-                    const float4 s = *reinterpret_cast<const float4*>(sp + r);
-                    const float sv[4] = {s.x, s.y, s.z, s.w};
+            auto add = [&](auto quads_tag) {  // quads_tag: groups of four rows held in registers, 0: any number
+                constexpr uint32_t QUADS = decltype(quads_tag)::value, FLY = QUADS == 1 ? 8 : QUADS == 2 ? 4 : 1;
+                float2 ml[QUADS ? QUADS * 4 : 1];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 ml = row_ml[r + i];
-                        if (r + i < rows) sum = fmaf(ex2(sv[i] - ml.x), ml.y, sum);
+                for (uint32_t r = 0; r < QUADS * 4; ++r) ml[r] = row_ml[r];
+                for (uint32_t t0 = p0 + tid; t0 < p1; t0 += FLY * kJoinThreads) {
+                    int64_t at[FLY];
+                    float sum[FLY];
+                    float4 sv[FLY][QUADS ? QUADS : 1];
+#pragma unroll
+                    for (uint32_t n = 0; n < FLY; ++n) {
+                        const uint32_t t = t0 + n * kJoinThreads;
+                        at[n] = t < p1 ? kv4_row(a.c, table, t, head) : -1;
+#pragma unroll
+                        for (uint32_t q = 0; q < QUADS; ++q)
+                            if (t < p1) sv[n][q] = reinterpret_cast<const float4*>(scores + (uint64_t)t * a.row_pad + r0)[q];
+                    }
+#pragma unroll
+                    for (uint32_t n = 0; n < FLY; ++n) sum[n] = at[n] >= 0 ? a.c.weight[at[n]] : 0.f;
+#pragma unroll
+                    for (uint32_t n = 0; n < FLY; ++n) {
+                        float more = 0.f;
+                        auto quad = [&](const float4& s4, const float2* m4) {  // (rows that are not there have a factor of 0)
+                            more = fmaf(ex2(s4.x - m4[0].x), m4[0].y, more);
+                            more = fmaf(ex2(s4.y - m4[1].x), m4[1].y, more);
+                            more = fmaf(ex2(s4.z - m4[2].x), m4[2].y, more);
+                            more = fmaf(ex2(s4.w - m4[3].x), m4[3].y, more);
+                        };
+                        if constexpr (QUADS > 0) {
+#pragma unroll
+                            for (uint32_t q = 0; q < QUADS; ++q) quad(sv[n][q], ml + 4 * q);
+                        } else if (at[n] >= 0) {
+                            const float4* sp = reinterpret_cast<const float4*>(scores + (uint64_t)t0 * a.row_pad + r0);
+                            for (uint32_t q = 0; q * 4 < rows; ++q) quad(sp[q], row_ml + 4 * q);
+                        }
+                        if (at[n] >= 0) a.c.weight[at[n]] = sum[n] + more;
                     }
                 }
-                if (at >= 0) a.c.weight[at] += sum;
-            }
+            };
+            if (rows <= 4)
+                add(std::integral_constant<uint32_t, 1>());
+            else if (rows <= 8)
+                add(std::integral_constant<uint32_t, 2>());
+            else
+                add(std::integral_constant<uint32_t, 0>());
         }
         unit += u1 - u0;
     }
