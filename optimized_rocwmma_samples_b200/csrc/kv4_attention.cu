@@ -69,8 +69,8 @@ constexpr uint32_t attn_warps()
 template <int D, int NT, int CH>
 constexpr uint32_t attn_blocks()
 {
-    if (CH == 2) return D == 64 ? 5 : 3;
-    return D == 64 ? (NT == 1 ? 6 : NT == 2 ? 4 : 3) : D == 128 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (NT == 1 ? 3 : 2);
+    if (CH == 2) return D == 64 ? 4 : 3;
+    return D == 64 ? (NT == 1 ? 5 : NT == 2 ? 4 : 3) : D == 128 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (NT == 1 ? 3 : 2);
 }
 constexpr uint32_t kMaxBlocks = 6;
 
@@ -81,12 +81,14 @@ struct AttnSmem {
     static constexpr uint32_t data = CH * 16 * D / 2;               // a chunk's key nibbles
     static constexpr uint32_t scales = CH * 16 * (D / 64) * 4;      // and their steps and bases
     static constexpr uint32_t stage = 2 * (data + scales);
-    static constexpr uint32_t stages = D == 64 ? (CH == 2 ? 4 : 6) : D == 128 ? (CH == 2 ? 3 : 4) : 3;
+    static constexpr uint32_t stages = D == 64 ? (CH == 2 ? 3 : 5) : 3;
     static constexpr uint32_t ring = warps * stages * stage;
     static constexpr uint32_t q = rows * D * 2;
-    static constexpr uint32_t pitch = D + 2;  // of a row in the join of the warps, which uses the drained ring
-    static_assert(warps * 8 * pitch * 4 <= ring, "ring too small for the join");
-    static constexpr uint32_t fixed = ring + q;
+    static constexpr uint32_t pitch = D + 2;  // of a row in the join of the warps
+    static constexpr uint32_t merge = warps * 8 * pitch * 4;
+    static constexpr bool early = D < 256;  // room for the join beside the ring, so that the next piece's loads need not wait
+    static_assert(early || merge <= ring, "ring too small for the join");
+    static constexpr uint32_t fixed = ring + q + (early ? merge : 0);
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src)
@@ -173,6 +175,16 @@ __device__ __forceinline__ SeqShape seq_shape(const AttnParams& a, uint32_t b, u
     s.blocks = (min(s.n, a.max_queries) * a.group + rows - 1) / rows;
     return s;
 }
+// For the values, two operands a byte: nibble 0 (J even), and the byte itself, nibble 0 + 16 nibble 1 (J odd): the sums
+// over nibble 1 come from the difference in the end, which saves a mask.  `hi`: the upper bytes of w's halves.
+template <int J>
+__device__ __forceinline__ uint32_t value_bits(uint32_t w, uint32_t hi)
+{
+    if constexpr (J == 0) return w & 0x000f000fu;
+    if constexpr (J == 1) return w & 0x00ff00ffu;
+    if constexpr (J == 2) return hi & 0x000f000fu;
+    return hi;
+}
 
 // Equal pieces of `total` chunks for `blocks` blocks: the first `rest` get one more.
 struct Split {
@@ -248,7 +260,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
     extern __shared__ __align__(16) uint8_t at_smem[];
     uint8_t* ring = at_smem;
     __half* q_frag = reinterpret_cast<__half*>(at_smem + S::ring);  // [NT][NG][2][32 lanes] x 16 bytes
-    float* merge = reinterpret_cast<float*>(ring);  // [kWarps][8][pitch]
+    float* merge = reinterpret_cast<float*>(S::early ? at_smem + S::ring + S::q : ring);  // [kWarps][8][pitch]
     uint32_t* ustart = reinterpret_cast<uint32_t*>(at_smem + S::fixed);  // [batch + 1]
     __shared__ float row_mul[ROWS], row_sum[ROWS][NG];
     __shared__ int row_vis[ROWS];
@@ -267,79 +279,115 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
 
     const uint32_t page_chunks = a.c.page_size / CHUNK;
     const uint32_t ring_base = smem_u32(ring) + warp * STAGES * S::stage;
-    uint32_t unit = begin;
-    uint32_t b = seq_of(ustart, a.s.batch, unit);
-    while (unit < end) {
-        while (ustart[b + 1] <= unit) ++b;
-        const SeqShape sh = seq_shape(a, b, ROWS);
-        const uint32_t in_seq = unit - ustart[b];
-        const uint32_t item = in_seq / sh.chunks, c0 = in_seq % sh.chunks;
-        const uint32_t head = item / sh.blocks, block = item % sh.blocks;
-        const uint32_t c1 = min(sh.chunks, c0 + (end - unit));
-        const bool whole = c0 == 0 && c1 == sh.chunks;
-        const int32_t* table = a.s.page_table + (uint64_t)b * a.s.max_pages;
-        const uint32_t all_rows = min(sh.n, a.max_queries) * a.group;
-
-        // this warp's chunks: an even share of the block's, one after another
-        const uint32_t wc0 = c0 + (uint32_t)((uint64_t)(c1 - c0) * warp / kWarps);
-        const uint32_t wc1 = c0 + (uint32_t)((uint64_t)(c1 - c0) * (warp + 1) / kWarps);
-        // loads run ahead of the computation by STAGES - 1 chunks, and page ids by one page
-        uint32_t lc = wc0, lslot = 0, left = 0;  // next chunk, its ring slot, chunks left on its page
-        uint32_t valid = 0;                      // bit i: the chunk loaded i loads ago has a page
-        uint32_t page_at = wc0 / page_chunks;
-        const uint32_t page_end = sh.vis == 0 ? 0 : (sh.vis - 1) / a.c.page_size + 1;
-        int32_t page = page_at < page_end ? __ldg(table + page_at) : -1, next_page = page;
-        const uint8_t *kp = nullptr, *vp = nullptr, *sp = nullptr;
-        auto load = [&]() {
-            valid <<= 1;
-            if (lc < wc1) {
-                if (left == 0) {
-                    const uint32_t skip = lc == wc0 ? wc0 % page_chunks : 0;
-                    left = page_chunks - skip;
-                    page = next_page;
-                    ++page_at;
-                    next_page = page_at < page_end ? __ldg(table + page_at) : -1;
-                    const int64_t row = ((int64_t)page * a.c.kv_heads + head) * a.c.page_size + skip * CHUNK;
-                    kp = a.c.k + row * (D / 2) + lane * 16;
-                    vp = a.c.v + row * (D / 2) + lane * 16;
-                    sp = static_cast<const uint8_t*>(lane < SC ? a.c.k_scale : a.c.v_scale) + row * (NG * 4) +
-                         (lane < SC ? lane : lane - SC) * 16;
-                }
-                if ((uint32_t)page < a.c.pages) {
-                    valid |= 1;
-                    const uint32_t dst = ring_base + lslot * S::stage;
+    // A piece of an item: what of it is this block's, and of that this warp's (an even share, one chunk after another).
+    struct Piece {
+        SeqShape sh;
+        uint32_t b, head, block, c0, c1, wc0, wc1, all_rows;
+    };
+    uint32_t seq = seq_of(ustart, a.s.batch, begin);
+    auto piece_at = [&](uint32_t unit) {
+        while (ustart[seq + 1] <= unit) ++seq;
+        Piece p;
+        p.b = seq;
+        p.sh = seq_shape(a, seq, ROWS);
+        const uint32_t in_seq = unit - ustart[seq], item = in_seq / p.sh.chunks;
+        p.c0 = in_seq - item * p.sh.chunks;
+        p.head = item / p.sh.blocks;
+        p.block = item - p.head * p.sh.blocks;
+        p.c1 = min(p.sh.chunks, p.c0 + (end - unit));
+        p.all_rows = min(p.sh.n, a.max_queries) * a.group;
+        p.wc0 = p.c0 + (p.c1 - p.c0) * warp / kWarps;
+        p.wc1 = p.c0 + (p.c1 - p.c0) * (warp + 1) / kWarps;
+        return p;
+    };
+    // this warp's query rows of a piece, on their way (ahead of the piece's keys: behind them a load takes long)
+    constexpr uint32_t QROWS = ROWS / kWarps;
+    T qv[QROWS][D / 32];
+    auto fetch_rows = [&](const Piece& p) {
 #pragma unroll
-                    for (uint32_t i = 0; i < S::data / 512; ++i) {
-                        const uint32_t u = i * 32 + lane, r = u / CPR, ch = u % CPR;
-                        const uint32_t to = r * CPR + (ch ^ ((r / (8 / CPR)) & (CPR - 1)));
-                        cp_async16(dst + to * 16, kp + i * 512);
-                        cp_async16(dst + S::data + to * 16, vp + i * 512);
-                    }
-                    if (lane < 2 * SC) cp_async16(dst + 2 * S::data + lane * 16, sp);
-                }
-                kp += S::data;
-                vp += S::data;
-                sp += S::scales;
-                --left;
-                ++lc;
+        for (uint32_t i = 0; i < QROWS; ++i) {
+            const uint32_t row = p.block * ROWS + warp + i * kWarps;
+            const uint32_t qi = row / a.group, qh = p.head * a.group + row % a.group;
+            const T* src = static_cast<const T*>(a.q) + (uint64_t)(p.sh.start + qi) * a.q_stride + (uint64_t)qh * D;
+#pragma unroll
+            for (uint32_t j = 0; j < D / 32; ++j) qv[i][j] = row < p.all_rows ? src[lane + 32 * j] : T(0.f);
+        }
+    };
+    // loads run ahead of the computation by STAGES - 1 chunks, and page ids by one page
+    uint32_t lc = 0, lend = 0, lslot = 0, left = 0;  // next chunk, the last one, its ring slot, chunks left on its page
+    uint32_t valid = 0;                              // bit i: the chunk loaded i loads ago has a page
+    uint32_t page_at = 0, page_end = 0, lskip = 0;
+    int32_t page = -1, next_page = -1;
+    const int32_t* ltable = nullptr;
+    const uint8_t *kp = nullptr, *vp = nullptr, *sp = nullptr;
+    uint64_t head_row = 0;
+    auto load = [&]() {
+        valid <<= 1;
+        if (lc < lend) {
+            if (left == 0) {
+                left = page_chunks - lskip;
+                page = next_page;
+                ++page_at;
+                next_page = page_at < page_end ? __ldg(ltable + page_at) : -1;
+                const uint64_t row = (uint64_t)(uint32_t)page * a.c.kv_heads * a.c.page_size + head_row + lskip * CHUNK;
+                lskip = 0;
+                kp = a.c.k + row * (D / 2) + lane * 16;
+                vp = a.c.v + row * (D / 2) + lane * 16;
+                sp = static_cast<const uint8_t*>(lane < SC ? a.c.k_scale : a.c.v_scale) + row * (NG * 4) +
+                     (lane < SC ? lane : lane - SC) * 16;
             }
-            cp_async_commit();
-            if (++lslot == STAGES) lslot = 0;
-        };
+            if ((uint32_t)page < a.c.pages) {
+                valid |= 1;
+                const uint32_t dst = ring_base + lslot * S::stage;
 #pragma unroll
+                for (uint32_t i = 0; i < S::data / 512; ++i) {
+                    const uint32_t u = i * 32 + lane, r = u / CPR, ch = u % CPR;
+                    const uint32_t to = r * CPR + (ch ^ ((r / (8 / CPR)) & (CPR - 1)));
+                    cp_async16(dst + to * 16, kp + i * 512);
+                    cp_async16(dst + S::data + to * 16, vp + i * 512);
+                }
+                if (lane < 2 * SC) cp_async16(dst + 2 * S::data + lane * 16, sp);
+            }
+            kp += S::data;
+            vp += S::data;
+            sp += S::scales;
+            --left;
+            ++lc;
+        }
+        cp_async_commit();
+        if (++lslot == STAGES) lslot = 0;
+    };
+    auto begin_loads = [&](const Piece& p) {
+        lc = p.wc0;
+        lend = p.wc1;
+        left = 0;
+        page_at = lc / page_chunks;
+        lskip = lc - page_at * page_chunks;
+        page_end = p.sh.vis == 0 ? 0 : (p.sh.vis - 1) / a.c.page_size + 1;
+        ltable = a.s.page_table + (uint64_t)p.b * a.s.max_pages;
+        head_row = (uint64_t)p.head * a.c.page_size;
+        next_page = page_at < page_end ? __ldg(ltable + page_at) : -1;
+#pragma unroll 1
         for (uint32_t i = 0; i < STAGES - 1; ++i) load();
+    };
 
-        // the item's query rows, as operands
-        for (uint32_t r = warp; r < ROWS; r += kWarps) {
-            const uint32_t row = block * ROWS + r;
-            float v[D / 32], mx = 0.f;
-            const bool there = row < all_rows;
-            const uint32_t qi = row / a.group, qh = head * a.group + row % a.group;
-            const T* src = static_cast<const T*>(a.q) + (uint64_t)(sh.start + qi) * a.q_stride + (uint64_t)qh * D;
+    Piece cur = piece_at(begin);
+    fetch_rows(cur);
+    uint32_t slot = lslot;
+    begin_loads(cur);
+    for (uint32_t unit = begin;;) {
+        const SeqShape sh = cur.sh;
+        const uint32_t b = cur.b, head = cur.head, block = cur.block, all_rows = cur.all_rows, wc0 = cur.wc0, wc1 = cur.wc1;
+        const bool whole = cur.c0 == 0 && cur.c1 == sh.chunks;
+        // the rows become operands (the last piece's are no longer read: the warps have met since)
 #pragma unroll
-            for (uint32_t i = 0; i < D / 32; ++i) {
-                v[i] = there ? (float)src[lane + 32 * i] : 0.f;
-                mx = fmaxf(mx, fabsf(v[i]));
+        for (uint32_t i = 0; i < QROWS; ++i) {
+            const uint32_t r = warp + i * kWarps, row = block * ROWS + r;
+            float v[D / 32], mx = 0.f;
+#pragma unroll
+            for (uint32_t j = 0; j < D / 32; ++j) {
+                v[j] = (float)qv[i][j];
+                mx = fmaxf(mx, fabsf(v[j]));
             }
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
@@ -348,11 +396,11 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
             const int shift = (ex == 0 || ex == 255) ? 0 : min(max(136 - ex, -100), 100);
             const float f = __uint_as_float((uint32_t)(127 + shift) << 23);
 #pragma unroll
-            for (uint32_t i = 0; i < D / 32; ++i) {
-                // channel 32 i + lane: word position j, k half, operand register and lane
-                const uint32_t gr = i / 2, cb = i & 1, t4 = lane / 8, y = lane & 7, j = y & 3, hi = y >> 2;
+            for (uint32_t c = 0; c < D / 32; ++c) {
+                // channel 32 c + lane: word position j, k half, operand register and lane
+                const uint32_t gr = c / 2, cb = c & 1, t4 = lane / 8, y = lane & 7, j = y & 3, hi = y >> 2;
                 const uint32_t at = ((((r / 8) * NG + gr) * 2 + j / 2) * 32 + (r & 7) * 4 + t4) * 8 + (j & 1) * 4 + cb * 2 + hi;
-                q_frag[at] = __float2half_rn(v[i] * ((j & 1) ? f * 0.0625f : f));
+                q_frag[at] = __float2half_rn(v[c] * ((j & 1) ? f * 0.0625f : f));
             }
 #pragma unroll
             for (uint32_t gr = 0; gr < NG; ++gr) {
@@ -364,13 +412,14 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
             if (lane == 0) {
                 row_mul[r] = a.scale_log2 * (16777216.f / f);
                 // rows that are not there see everything (their columns are not used), so that they mask nothing
-                row_vis[r] = there ? (int)max((int64_t)0, min((int64_t)sh.vis, (int64_t)sh.len - sh.n + qi + 1)) : (int)sh.vis;
+                row_vis[r] = row < all_rows
+                                 ? (int)max((int64_t)0, min((int64_t)sh.vis, (int64_t)sh.len - sh.n + row / a.group + 1))
+                                 : (int)sh.vis;
             }
         }
         __syncthreads();
         float mul[NT][2], qsum[NT][2][NG];
         int vis[NT][2];
-        int least = 0x7fffffff;  // positions that all rows see
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -381,7 +430,8 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
 #pragma unroll
                 for (uint32_t gr = 0; gr < NG; ++gr) qsum[nt][x][gr] = row_sum[r][gr];
             }
-        for (uint32_t r = 0; r < ROWS; ++r) least = min(least, row_vis[r]);
+        // positions that all rows see
+        const int least = __reduce_min_sync(0xffffffffu, lane < ROWS ? row_vis[lane % ROWS] : 0x7fffffff);
 
         float o[NG][4][NT][4] = {};
         float m[NT][2], l[NT][2], zs[NT][2][NG];  // m: 0 until the row has seen a token
@@ -591,10 +641,13 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                 for (uint32_t gr = 0; gr < NG; ++gr) {
                     uint32_t w[4];
                     ldsm4_trans(base + S::data + ch * 8 * D + ((gr * 2 + (lane >> 4)) ^ sw) * 16, w);
+                    uint32_t hi[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) hi[i] = __byte_perm(w[i], 0u, 0x4341);
                     auto word = [&](auto j_tag) {
                         constexpr int J = decltype(j_tag)::value;
-                        const uint32_t a0 = nibbles<J>(w[0]), a1 = nibbles<J>(w[2]), a2 = nibbles<J>(w[1]),
-                                       a3 = nibbles<J>(w[3]);
+                        const uint32_t a0 = value_bits<J>(w[0], hi[0]), a1 = value_bits<J>(w[2], hi[2]),
+                                       a2 = value_bits<J>(w[1], hi[1]), a3 = value_bits<J>(w[3], hi[3]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             mma_f16(o[gr][J][nt], a0, a1, a2, a3, pb[gr][nt][0], pb[gr][nt][1]);
@@ -609,7 +662,6 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
             }
         };
 
-        uint32_t slot = 0;
         for (uint32_t c = wc0; c < wc1; ++c) {
             __syncwarp();
             load();
@@ -628,7 +680,24 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
             if (score_at) score_at += CHUNK * a.row_pad;
             if (++slot == STAGES) slot = 0;
         }
-        cp_async_wait<0>();
+        // the next piece's rows and first chunks, behind this one's join (which needs the ring itself where shared memory
+        // has no room for both)
+        const uint32_t next_unit = unit + (cur.c1 - cur.c0);
+        if (S::early && next_unit < end) {
+            cur = piece_at(next_unit);
+            if (NT == 1) fetch_rows(cur);  // (more rows would not fit beside the sums)
+            slot = lslot;
+            begin_loads(cur);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (uint32_t gr = 0; gr < NG; ++gr)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[gr][1][nt][i] -= o[gr][0][nt][i];  // nibbles 1 and 3 from their bytes
+                    o[gr][3][nt][i] -= o[gr][2][nt][i];
+                }
 
         // the warps' sums become the block's
 #pragma unroll
@@ -645,7 +714,8 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                 if (!((seen >> (nt * 2 + x)) & 1)) m[nt][x] = -INFINITY;
                 if (g == 0) warp_ml[warp][nt * 8 + 2 * tig + x] = make_float2(m[nt][x], l[nt][x]);
             }
-        __syncthreads();  // every warp's ring is drained, its maxima and sums are there
+        if (!S::early) cp_async_wait<0>();
+        __syncthreads();  // every warp is through its chunks, its maxima and sums are there
         const uint32_t seg = unit == begin ? 0 : 1;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -710,9 +780,17 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                 }
             }
         }
-        __syncthreads();
-        unit += c1 - c0;
+        if (next_unit >= end) break;
+        unit = next_unit;
+        if (!S::early) {
+            __syncthreads();
+            cur = piece_at(unit);
+            slot = lslot;
+            begin_loads(cur);
+        }
+        if (!S::early || NT > 1) fetch_rows(cur);
     }
+    cp_async_wait<0>();
 }
 
 // Pieces of an item that blocks left in the workspace: slots of blocks `first` .. `last`.
