@@ -203,17 +203,20 @@ struct Split {
     }
 };
 
-// First chunk of every sequence on the line, into shared memory [batch + 1]; all threads of the block.
+// First chunk of every sequence on the line, into shared memory [batch + 1] (and, where asked, the chunks of its items
+// [batch]); all threads of the block.
 template <uint32_t THREADS>
-__device__ __forceinline__ void lay_out(const AttnParams& a, uint32_t rows, uint32_t* ustart, uint32_t* part)
+__device__ __forceinline__ void lay_out(const AttnParams& a, uint32_t rows, uint32_t* ustart, uint32_t* part,
+                                        uint32_t* chunks = nullptr)
 {
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     uint32_t carry = 0;
     for (uint32_t base = 0; base < a.s.batch; base += THREADS) {
         const uint32_t b = base + tid;
-        uint32_t v = 0;
+        uint32_t v = 0, here = 1;
         if (b < a.s.batch) {
             const SeqShape sh = seq_shape(a, b, rows);
+            here = sh.chunks;
             v = sh.chunks * sh.blocks * a.c.kv_heads;
         }
         uint32_t incl = v;
@@ -229,7 +232,10 @@ __device__ __forceinline__ void lay_out(const AttnParams& a, uint32_t rows, uint
             if (w < warp) before += part[w];
             carry += part[w];
         }
-        if (b < a.s.batch) ustart[b] = before + incl - v;
+        if (b < a.s.batch) {
+            ustart[b] = before + incl - v;
+            if (chunks) chunks[b] = here;
+        }
         __syncthreads();
     }
     if (tid == 0) ustart[a.s.batch] = carry;
@@ -807,23 +813,28 @@ struct Pieces {
 };
 
 constexpr uint32_t kJoinThreads = 256;
+constexpr uint32_t kJoinGroup = 4;  // warps that join one row
 
-// Blocks below join_blocks: WPR warps a query row join the pieces of its item.
-// The others: weights of an equal piece of all positions, from the scores.
-// What depends on the call's inputs alone is worked out before the wait for
-// the first kernel, which has waited for the inputs itself.
-template <typename T, int D, uint32_t WPR>
-__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, uint32_t rows_per_item, uint32_t grid1,
-                                                                uint32_t join_blocks)
+// The first join_blocks blocks join the items that lie in several blocks' shares, four warps a row; the others add up the
+// weights, each of an equal piece of all positions, from the scores.  Every boundary between two shares stands for the
+// item it cuts, if it is the first to do so: there are at most as many such items as blocks, however many rows the call
+// has, and they are found in shared memory alone.  What depends on the call's inputs is worked out before the wait for
+// the first kernel, which has waited for the inputs itself.  It does not let its dependents start early: blocks of the
+// next attention that come into registers freed piecemeal leave holes that their last ones do not fit (they then ran
+// after the others: 48 x 8192 tokens 128 us instead of 100).
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a, uint32_t rows_per_item, uint32_t grid1,
+                                                                   uint32_t join_blocks)
 {
-    constexpr uint32_t WARPS = kJoinThreads / 32, V = D / 64;  // V: pairs of channels a lane holds
-    extern __shared__ uint32_t ustart[];
+    constexpr uint32_t WARPS = kJoinThreads / 32, GROUPS = WARPS / kJoinGroup, V = D / 64;  // V: pairs of channels a lane holds
+    extern __shared__ uint32_t ustart[];  // [batch + 1], then the chunks of a sequence's items [batch]
     __shared__ float2 row_ml[kJoinThreads];
-    __shared__ float2 part[WPR > 1 ? WARPS : 1][V * 32];
+    __shared__ float2 part[WARPS][V * 32];
     __shared__ float part_l[WARPS];
     __shared__ uint32_t scan_part[WARPS];
+    const uint32_t* seq_chunks = ustart + a.s.batch + 1;
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    lay_out<kJoinThreads>(a, rows_per_item, ustart, scan_part);
+    lay_out<kJoinThreads>(a, rows_per_item, ustart, scan_part, ustart + a.s.batch + 1);
     const uint32_t total = ustart[a.s.batch];
     if (total == 0) {
         griddep_wait();
@@ -831,88 +842,89 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, ui
     }
     const Split split(total, grid1, a.chunk);
     if (blockIdx.x < join_blocks) {
-        const uint64_t id = (uint64_t)blockIdx.x * (WARPS / WPR) + warp / WPR;
-        const uint32_t token = (uint32_t)min(id / a.heads, (uint64_t)a.s.tokens), qh = (uint32_t)(id % a.heads);
-        uint32_t lo = 0, hi = a.s.batch;
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (__ldg(a.s.token_start + mid + 1) <= (int32_t)token)
-                lo = mid + 1;
-            else
-                hi = mid;
-        }
-        bool mine = token < a.s.tokens && lo < a.s.batch;
-        uint32_t count = 0, r = 0;
-        Pieces p(split, 0, 1);
-        if (mine) {
-            const SeqShape sh = seq_shape(a, lo, rows_per_item);
-            mine = token >= sh.start && token - sh.start < min(sh.n, a.max_queries);
-            if (mine) {
-                const uint32_t head = qh / a.group, row = (token - sh.start) * a.group + qh % a.group;
-                r = row % rows_per_item;
-                p = Pieces(split, ustart[lo] + (head * sh.blocks + row / rows_per_item) * sh.chunks, sh.chunks);
-                count = p.count();
-                mine = count > 1;  // otherwise written whole
+        const uint32_t in_group = warp % kJoinGroup, group = warp / kJoinGroup;
+        const uint32_t most_rows = min(rows_per_item, a.group * a.max_queries), units = (split.blocks - 1) * most_rows;
+        bool waited = false;
+        for (uint32_t x = blockIdx.x * GROUPS + group; x < units; x += join_blocks * GROUPS) {
+            const uint32_t r = x % most_rows, cut = split.begin(x / most_rows + 1);
+            const uint32_t b = seq_of(ustart, a.s.batch, cut), chunks = seq_chunks[b];
+            const uint32_t item = (cut - ustart[b]) / chunks, unit0 = ustart[b] + item * chunks;
+            if (unit0 == cut || split.block_of(unit0) != x / most_rows) continue;  // cuts no item, or not as the first
+            const Pieces p(split, unit0, chunks);
+            const SeqShape sh = seq_shape(a, b, rows_per_item);
+            const uint32_t head = item / sh.blocks, row = item % sh.blocks * rows_per_item + r;
+            if (row >= min(sh.n, a.max_queries) * a.group) continue;
+            if (!waited) {
+                waited = true;
+                griddep_wait();
             }
-        }
-        griddep_wait();
-        griddep_launch_dependents();
-        float top = -INFINITY;
-        if (mine)
+            const uint32_t count = p.count();
+            float top = -INFINITY;
             for (uint32_t i = lane; i < count; i += 32)
                 top = fmaxf(top, a.part_ml[(uint64_t)p.slot(i) * rows_per_item + r].x);
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        float2 o[V] = {};
-        float sum = 0.f;
-        // this warp's pieces: every WPR-th
-        if (mine)
-            for (uint32_t i0 = warp % WPR; i0 < count; i0 += 32 * WPR) {
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            float2 o[V] = {};
+            float sum = 0.f;
+            // this warp's pieces: every fourth
+            for (uint32_t i0 = in_group; i0 < count; i0 += 32 * kJoinGroup) {
                 float f = 0.f;
-                const uint32_t i_lane = i0 + lane * WPR;
+                const uint32_t i_lane = i0 + lane * kJoinGroup;
                 if (i_lane < count) {
                     const float2 ml = a.part_ml[(uint64_t)p.slot(i_lane) * rows_per_item + r];
                     f = ml.x == -INFINITY ? 0.f : ml.x == top ? 1.f : ex2(ml.x - top);
                     sum += ml.x == -INFINITY ? ml.y : ml.y * f;  // a NaN stays
                 }
-                const uint32_t here = min(32u, (count - i0 + WPR - 1) / WPR);
-#pragma unroll 8
-                for (uint32_t i = 0; i < here; ++i) {
-                    const float fi = __shfl_sync(0xffffffffu, f, i);
-                    const float* src = a.part_o + ((uint64_t)p.slot(i0 + i * WPR) * rows_per_item + r) * D;
+                const uint32_t here = min(32u, (count - i0 + kJoinGroup - 1) / kJoinGroup);
+                constexpr uint32_t FLY = V == 4 ? 4 : 8;  // pieces in flight, the last ones too
+                for (uint32_t i = 0; i < here; i += FLY) {
+                    float2 y[FLY][V];
 #pragma unroll
-                    for (uint32_t v = 0; v < V; ++v) {
-                        const float2 x = *reinterpret_cast<const float2*>(src + v * 64 + lane * 2);
-                        o[v].x = fmaf(x.x, fi, o[v].x);
-                        o[v].y = fmaf(x.y, fi, o[v].y);
+                    for (uint32_t n = 0; n < FLY; ++n) {
+                        const uint32_t k = min(i + n, here - 1);
+                        const float* src = a.part_o + ((uint64_t)p.slot(i0 + k * kJoinGroup) * rows_per_item + r) * D;
+#pragma unroll
+                        for (uint32_t v = 0; v < V; ++v) y[n][v] = *reinterpret_cast<const float2*>(src + v * 64 + lane * 2);
+                    }
+#pragma unroll
+                    for (uint32_t n = 0; n < FLY; ++n) {
+                        const float fi = i + n < here ? __shfl_sync(0xffffffffu, f, (i + n) & 31) : 0.f;
+                        if (i + n < here) {
+#pragma unroll
+                            for (uint32_t v = 0; v < V; ++v) {
+                                o[v].x = fmaf(y[n][v].x, fi, o[v].x);
+                                o[v].y = fmaf(y[n][v].y, fi, o[v].y);
+                            }
+                        }
                     }
                 }
             }
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if constexpr (WPR > 1) {
+            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            named_bar_sync(1 + group, kJoinGroup * 32);  // (the last row's sums are read)
 #pragma unroll
             for (uint32_t v = 0; v < V; ++v) part[warp][v * 32 + lane] = o[v];
             if (lane == 0) part_l[warp] = sum;
-            __syncthreads();
-            if (warp % WPR != 0) return;
+            named_bar_sync(1 + group, kJoinGroup * 32);
+            if (in_group != 0) continue;
 #pragma unroll
-            for (uint32_t w = 1; w < WPR; ++w) {
+            for (uint32_t w = 1; w < kJoinGroup; ++w) {
                 sum += part_l[warp + w];
 #pragma unroll
                 for (uint32_t v = 0; v < V; ++v) {
-                    const float2 x = part[warp + w][v * 32 + lane];
-                    o[v].x += x.x;
-                    o[v].y += x.y;
+                    const float2 y = part[warp + w][v * 32 + lane];
+                    o[v].x += y.x;
+                    o[v].y += y.y;
                 }
             }
-        }
-        if (!mine) return;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        T* dst = static_cast<T*>(a.out) + ((uint64_t)token * a.heads + qh) * D;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T* dst = static_cast<T*>(a.out) +
+                     ((uint64_t)(sh.start + row / a.group) * a.heads + head * a.group + row % a.group) * D;
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v)
-            *reinterpret_cast<uint32_t*>(dst + v * 64 + lane * 2) = f2_to_pair<T>(o[v].x * inv, o[v].y * inv);
+            for (uint32_t v = 0; v < V; ++v)
+                *reinterpret_cast<uint32_t*>(dst + v * 64 + lane * 2) = f2_to_pair<T>(o[v].x * inv, o[v].y * inv);
+        }
+        if (!waited) griddep_wait();
         return;
     }
     // weights: the line again; a head's row blocks make one run of blocks * chunks units, over which its positions
@@ -921,7 +933,6 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, ui
     const uint32_t begin = (uint32_t)((uint64_t)total * wb / wblocks), end = (uint32_t)((uint64_t)total * (wb + 1) / wblocks);
     uint32_t unit = begin, b = seq_of(ustart, a.s.batch, unit);
     griddep_wait();
-    griddep_launch_dependents();
     while (unit < end) {
         while (ustart[b + 1] <= unit) ++b;
         const SeqShape sh = seq_shape(a, b, rows_per_item);
@@ -961,7 +972,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnParams a, ui
             }
             __syncthreads();
             auto add = [&](auto quads_tag) {  // quads_tag: groups of four rows held in registers, 0: any number
-                constexpr uint32_t QUADS = decltype(quads_tag)::value, FLY = QUADS == 1 ? 8 : QUADS == 2 ? 4 : 1;
+                constexpr uint32_t QUADS = decltype(quads_tag)::value, FLY = QUADS == 1 ? 4 : QUADS == 2 ? 2 : 1;
                 float2 ml[QUADS ? QUADS * 4 : 1];
 #pragma unroll
                 for (uint32_t r = 0; r < QUADS * 4; ++r) ml[r] = row_ml[r];
@@ -1051,16 +1062,14 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
     const uint32_t line = (p.s.batch + 1) * 4;
     e = launch_pdl(kv4_attention_kernel<T, D, NT, CH>, dim3(grid), dim3(S::warps * 32), S::fixed + line, st, p);
     if (e != cudaSuccess) return e;
-    const uint64_t rows = (uint64_t)p.s.tokens * p.heads;
-    const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 4 * num_sms) : 0;
-    constexpr uint32_t kJoinWarps = kJoinThreads / 32;
-    // few rows: four warps each, for the latency; many: one
-    if (rows <= 16 * num_sms) {
-        const uint32_t join = (uint32_t)((rows * 4 + kJoinWarps - 1) / kJoinWarps);
-        return launch_pdl(kv4_join_kernel<T, D, 4>, dim3(join + weights), dim3(kJoinThreads), line, st, p, 8u * NT, grid, join);
-    }
-    const uint32_t join = (uint32_t)((rows + kJoinWarps - 1) / kJoinWarps);
-    return launch_pdl(kv4_join_kernel<T, D, 1>, dim3(join + weights), dim3(kJoinThreads), line, st, p, 8u * NT, grid, join);
+    // The second kernel is one wave of three blocks an SM: one for the rows of cut items, two for the weights (a block
+    // takes a few microseconds to its first row; four waves of them took 36 us where one takes 20).
+    constexpr uint32_t kGroups = kJoinThreads / 32 / kJoinGroup;
+    const uint64_t rows = (uint64_t)(grid - 1) * std::min(8u * NT, p.group * p.max_queries);
+    const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 2 * num_sms) : 0;
+    const uint32_t join = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((rows + kGroups - 1) / kGroups, (accumulate ? 1 : 3) * num_sms));
+    return launch_pdl(kv4_join_kernel<T, D>, dim3(join + weights), dim3(kJoinThreads), line + p.s.batch * 4, st, p, 8u * NT,
+                      grid, join);
 }
 
 template <typename T, int D>
