@@ -815,25 +815,98 @@ struct Pieces {
 constexpr uint32_t kJoinThreads = 256;
 constexpr uint32_t kJoinGroup = 4;  // warps that join one row
 
+// Joins one row of an item from its pieces, four warps together (all of them call it); the first of them stores it.
+template <typename T, int D>
+__device__ __forceinline__ void join_row(const AttnParams& a, const Pieces& p, uint32_t rows_per_item, uint32_t r, T* dst,
+                                         float2 (*part)[D / 2], float* part_l)
+{
+    constexpr uint32_t V = D / 64;  // pairs of channels a lane holds
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, in_group = warp % kJoinGroup, group = warp / kJoinGroup;
+    const uint32_t count = p.count();
+    float top = -INFINITY;
+    for (uint32_t i = lane; i < count; i += 32)
+        top = fmaxf(top, a.part_ml[(uint64_t)p.slot(i) * rows_per_item + r].x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    float2 o[V] = {};
+    float sum = 0.f;
+    // this warp's pieces: every fourth
+    for (uint32_t i0 = in_group; i0 < count; i0 += 32 * kJoinGroup) {
+        float f = 0.f;
+        const uint32_t i_lane = i0 + lane * kJoinGroup;
+        if (i_lane < count) {
+            const float2 ml = a.part_ml[(uint64_t)p.slot(i_lane) * rows_per_item + r];
+            f = ml.x == -INFINITY ? 0.f : ml.x == top ? 1.f : ex2(ml.x - top);
+            sum += ml.x == -INFINITY ? ml.y : ml.y * f;  // a NaN stays
+        }
+        const uint32_t here = min(32u, (count - i0 + kJoinGroup - 1) / kJoinGroup);
+        constexpr uint32_t FLY = V == 4 ? 4 : 8;  // pieces in flight, the last ones too
+        for (uint32_t i = 0; i < here; i += FLY) {
+            float2 y[FLY][V];
+#pragma unroll
+            for (uint32_t n = 0; n < FLY; ++n) {
+                const uint32_t k = min(i + n, here - 1);
+                const float* src = a.part_o + ((uint64_t)p.slot(i0 + k * kJoinGroup) * rows_per_item + r) * D;
+#pragma unroll
+                for (uint32_t v = 0; v < V; ++v) y[n][v] = *reinterpret_cast<const float2*>(src + v * 64 + lane * 2);
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < FLY; ++n) {
+                const float fi = i + n < here ? __shfl_sync(0xffffffffu, f, (i + n) & 31) : 0.f;
+                if (i + n < here) {
+#pragma unroll
+                    for (uint32_t v = 0; v < V; ++v) {
+                        o[v].x = fmaf(y[n][v].x, fi, o[v].x);
+                        o[v].y = fmaf(y[n][v].y, fi, o[v].y);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    named_bar_sync(1 + group, kJoinGroup * 32);  // (the last row's sums are read)
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v) part[warp][v * 32 + lane] = o[v];
+    if (lane == 0) part_l[warp] = sum;
+    named_bar_sync(1 + group, kJoinGroup * 32);
+    if (in_group != 0) return;
+#pragma unroll
+    for (uint32_t w = 1; w < kJoinGroup; ++w) {
+        sum += part_l[warp + w];
+#pragma unroll
+        for (uint32_t v = 0; v < V; ++v) {
+            const float2 y = part[warp + w][v * 32 + lane];
+            o[v].x += y.x;
+            o[v].y += y.y;
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v)
+        *reinterpret_cast<uint32_t*>(dst + v * 64 + lane * 2) = f2_to_pair<T>(o[v].x * inv, o[v].y * inv);
+}
+
 // The first join_blocks blocks join the items that lie in several blocks' shares, four warps a row; the others add up the
-// weights, each of an equal piece of all positions, from the scores.  Every boundary between two shares stands for the
-// item it cuts, if it is the first to do so: there are at most as many such items as blocks, however many rows the call
-// has, and they are found in shared memory alone.  What depends on the call's inputs is worked out before the wait for
-// the first kernel, which has waited for the inputs itself.  It does not let its dependents start early: blocks of the
-// next attention that come into registers freed piecemeal leave holes that their last ones do not fit (they then ran
-// after the others: 48 x 8192 tokens 128 us instead of 100).
+// weights, each of an equal piece of all positions, from the scores.  With few query rows (`by_rows`) every row looks for
+// its own item.  With many, every boundary between two shares stands for the item it cuts, if it is the first to do so:
+// there are at most as many such items as blocks, and they are found in shared memory alone.  What depends on the call's
+// inputs is worked out before the wait for the first kernel, which has waited for the inputs itself.
+// With weights, the kernel does not let its dependents start early: blocks of the next attention that come into registers
+// freed piecemeal leave holes that its last ones do not fit (they then ran after the others: 48 x 8192 tokens 128 us, not
+// 100).
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a, uint32_t rows_per_item, uint32_t grid1,
-                                                                   uint32_t join_blocks)
+                                                                   uint32_t join_blocks, bool by_rows)
 {
-    constexpr uint32_t WARPS = kJoinThreads / 32, GROUPS = WARPS / kJoinGroup, V = D / 64;  // V: pairs of channels a lane holds
+    constexpr uint32_t WARPS = kJoinThreads / 32, GROUPS = WARPS / kJoinGroup;
     extern __shared__ uint32_t ustart[];  // [batch + 1], then the chunks of a sequence's items [batch]
     __shared__ float2 row_ml[kJoinThreads];
-    __shared__ float2 part[WARPS][V * 32];
+    __shared__ float2 part[WARPS][D / 2];
     __shared__ float part_l[WARPS];
     __shared__ uint32_t scan_part[WARPS];
     const uint32_t* seq_chunks = ustart + a.s.batch + 1;
-    const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const uint32_t tid = threadIdx.x, warp = tid / 32;
     lay_out<kJoinThreads>(a, rows_per_item, ustart, scan_part, ustart + a.s.batch + 1);
     const uint32_t total = ustart[a.s.batch];
     if (total == 0) {
@@ -842,89 +915,54 @@ __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a,
     }
     const Split split(total, grid1, a.chunk);
     if (blockIdx.x < join_blocks) {
-        const uint32_t in_group = warp % kJoinGroup, group = warp / kJoinGroup;
-        const uint32_t most_rows = min(rows_per_item, a.group * a.max_queries), units = (split.blocks - 1) * most_rows;
         bool waited = false;
-        for (uint32_t x = blockIdx.x * GROUPS + group; x < units; x += join_blocks * GROUPS) {
-            const uint32_t r = x % most_rows, cut = split.begin(x / most_rows + 1);
-            const uint32_t b = seq_of(ustart, a.s.batch, cut), chunks = seq_chunks[b];
-            const uint32_t item = (cut - ustart[b]) / chunks, unit0 = ustart[b] + item * chunks;
-            if (unit0 == cut || split.block_of(unit0) != x / most_rows) continue;  // cuts no item, or not as the first
-            const Pieces p(split, unit0, chunks);
-            const SeqShape sh = seq_shape(a, b, rows_per_item);
-            const uint32_t head = item / sh.blocks, row = item % sh.blocks * rows_per_item + r;
-            if (row >= min(sh.n, a.max_queries) * a.group) continue;
-            if (!waited) {
-                waited = true;
-                griddep_wait();
-            }
-            const uint32_t count = p.count();
-            float top = -INFINITY;
-            for (uint32_t i = lane; i < count; i += 32)
-                top = fmaxf(top, a.part_ml[(uint64_t)p.slot(i) * rows_per_item + r].x);
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            float2 o[V] = {};
-            float sum = 0.f;
-            // this warp's pieces: every fourth
-            for (uint32_t i0 = in_group; i0 < count; i0 += 32 * kJoinGroup) {
-                float f = 0.f;
-                const uint32_t i_lane = i0 + lane * kJoinGroup;
-                if (i_lane < count) {
-                    const float2 ml = a.part_ml[(uint64_t)p.slot(i_lane) * rows_per_item + r];
-                    f = ml.x == -INFINITY ? 0.f : ml.x == top ? 1.f : ex2(ml.x - top);
-                    sum += ml.x == -INFINITY ? ml.y : ml.y * f;  // a NaN stays
+        auto wait = [&]() {
+            if (waited) return;
+            waited = true;
+            griddep_wait();
+            if (!a.scores) griddep_launch_dependents();
+        };
+        const uint32_t most_rows = min(rows_per_item, a.group * a.max_queries);
+        const uint64_t units = by_rows ? (uint64_t)a.s.tokens * a.heads : (uint64_t)(split.blocks - 1) * most_rows;
+        for (uint64_t x = blockIdx.x * GROUPS + warp / kJoinGroup; x < units; x += join_blocks * GROUPS) {
+            uint32_t b, head, row, unit0;  // sequence, key head, row of its rows, the item's first chunk on the line
+            SeqShape sh;
+            if (by_rows) {
+                const uint32_t token = (uint32_t)(x / a.heads), qh = (uint32_t)(x % a.heads);
+                uint32_t hi = a.s.batch;
+                b = 0;
+                while (b < hi) {
+                    const uint32_t mid = (b + hi) / 2;
+                    if (__ldg(a.s.token_start + mid + 1) <= (int32_t)token)
+                        b = mid + 1;
+                    else
+                        hi = mid;
                 }
-                const uint32_t here = min(32u, (count - i0 + kJoinGroup - 1) / kJoinGroup);
-                constexpr uint32_t FLY = V == 4 ? 4 : 8;  // pieces in flight, the last ones too
-                for (uint32_t i = 0; i < here; i += FLY) {
-                    float2 y[FLY][V];
-#pragma unroll
-                    for (uint32_t n = 0; n < FLY; ++n) {
-                        const uint32_t k = min(i + n, here - 1);
-                        const float* src = a.part_o + ((uint64_t)p.slot(i0 + k * kJoinGroup) * rows_per_item + r) * D;
-#pragma unroll
-                        for (uint32_t v = 0; v < V; ++v) y[n][v] = *reinterpret_cast<const float2*>(src + v * 64 + lane * 2);
-                    }
-#pragma unroll
-                    for (uint32_t n = 0; n < FLY; ++n) {
-                        const float fi = i + n < here ? __shfl_sync(0xffffffffu, f, (i + n) & 31) : 0.f;
-                        if (i + n < here) {
-#pragma unroll
-                            for (uint32_t v = 0; v < V; ++v) {
-                                o[v].x = fmaf(y[n][v].x, fi, o[v].x);
-                                o[v].y = fmaf(y[n][v].y, fi, o[v].y);
-                            }
-                        }
-                    }
-                }
+                if (b == a.s.batch) continue;
+                sh = seq_shape(a, b, rows_per_item);
+                if (token < sh.start || token - sh.start >= min(sh.n, a.max_queries)) continue;
+                head = qh / a.group;
+                row = (token - sh.start) * a.group + qh % a.group;
+                unit0 = ustart[b] + (head * sh.blocks + row / rows_per_item) * sh.chunks;
+            } else {
+                const uint32_t at = (uint32_t)(x / most_rows), cut = split.begin(at + 1);
+                b = seq_of(ustart, a.s.batch, cut);
+                const uint32_t item = (cut - ustart[b]) / seq_chunks[b];
+                unit0 = ustart[b] + item * seq_chunks[b];
+                if (unit0 == cut || split.block_of(unit0) != at) continue;  // cuts no item, or not as the first
+                sh = seq_shape(a, b, rows_per_item);
+                head = item / sh.blocks;
+                row = item % sh.blocks * rows_per_item + (uint32_t)(x % most_rows);
+                if (row >= min(sh.n, a.max_queries) * a.group) continue;
             }
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            named_bar_sync(1 + group, kJoinGroup * 32);  // (the last row's sums are read)
-#pragma unroll
-            for (uint32_t v = 0; v < V; ++v) part[warp][v * 32 + lane] = o[v];
-            if (lane == 0) part_l[warp] = sum;
-            named_bar_sync(1 + group, kJoinGroup * 32);
-            if (in_group != 0) continue;
-#pragma unroll
-            for (uint32_t w = 1; w < kJoinGroup; ++w) {
-                sum += part_l[warp + w];
-#pragma unroll
-                for (uint32_t v = 0; v < V; ++v) {
-                    const float2 y = part[warp + w][v * 32 + lane];
-                    o[v].x += y.x;
-                    o[v].y += y.y;
-                }
-            }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const Pieces p(split, unit0, sh.chunks);
+            if (p.first == p.last) continue;  // written whole
+            wait();
             T* dst = static_cast<T*>(a.out) +
                      ((uint64_t)(sh.start + row / a.group) * a.heads + head * a.group + row % a.group) * D;
-#pragma unroll
-            for (uint32_t v = 0; v < V; ++v)
-                *reinterpret_cast<uint32_t*>(dst + v * 64 + lane * 2) = f2_to_pair<T>(o[v].x * inv, o[v].y * inv);
+            join_row<T, D>(a, p, rows_per_item, row % rows_per_item, dst, part, part_l);
         }
-        if (!waited) griddep_wait();
+        wait();
         return;
     }
     // weights: the line again; a head's row blocks make one run of blocks * chunks units, over which its positions
@@ -1062,14 +1100,17 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
     const uint32_t line = (p.s.batch + 1) * 4;
     e = launch_pdl(kv4_attention_kernel<T, D, NT, CH>, dim3(grid), dim3(S::warps * 32), S::fixed + line, st, p);
     if (e != cudaSuccess) return e;
-    // The second kernel is one wave of three blocks an SM: one for the rows of cut items, two for the weights (a block
-    // takes a few microseconds to its first row; four waves of them took 36 us where one takes 20).
+    // The second kernel is one wave of three blocks an SM, with weights one for the rows and two for the weights (a block
+    // takes a few microseconds to its first row; four waves of them took 36 us where one takes 20).  Few rows look for
+    // their items themselves (16 x 4000 tokens, 512 rows: 22.8 us, by cuts 25.2), many are found by the cuts.
     constexpr uint32_t kGroups = kJoinThreads / 32 / kJoinGroup;
-    const uint64_t rows = (uint64_t)(grid - 1) * std::min(8u * NT, p.group * p.max_queries);
+    const uint64_t all_rows = (uint64_t)p.s.tokens * p.heads;
+    const bool by_rows = all_rows <= 4 * num_sms;
+    const uint64_t rows = by_rows ? all_rows : (uint64_t)(grid - 1) * std::min(8u * NT, p.group * p.max_queries);
     const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 2 * num_sms) : 0;
     const uint32_t join = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((rows + kGroups - 1) / kGroups, (accumulate ? 1 : 3) * num_sms));
     return launch_pdl(kv4_join_kernel<T, D>, dim3(join + weights), dim3(kJoinThreads), line + p.s.batch * 4, st, p, 8u * NT,
-                      grid, join);
+                      grid, join, by_rows);
 }
 
 template <typename T, int D>
