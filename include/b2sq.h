@@ -456,7 +456,8 @@ typedef struct {
  *   to +-65504;  q = clamp(rint((v - z) / s), 0, 15), ties to even (0 if s = 0)
  * and sets their weight to 0.  A NaN makes s and z of its group NaN.
  * k_out / v_out (nullable, contiguous, same type) receive the values that the
- * cache now stands for.  A token without a place in the table is skipped.
+ * cache now stands for.  A token without a place in the table is skipped; no
+ * two tokens of a call may have the same place.
  * Requirements (else UNSUPPORTED): 16-byte aligned rows (pitches multiples of 8).
  */
 B2SQ_API b2sq_status b2sq_kv4_append(const void* k, const void* v, b2sq_dtype type, uint32_t tokens,

@@ -654,8 +654,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, se
     T, heads, qs = _kv4_rows(q, "q", dev)
     if q.shape[2] != cache.head_dim:
         raise ValueError(f"q must have head_dim {cache.head_dim}")
-    if max_queries < 0:
-        raise ValueError("max_queries must not be negative")
+    if not 0 <= max_queries < 2 ** 31:
+        raise ValueError("max_queries must be in [0, 2^31)")
     if out is None:
         out = _new(torch.zeros, q.shape, q.dtype, dev, stream)
     o = _want(out, "out", q.dtype, q.shape, dev)
@@ -682,6 +682,7 @@ def kv4_evict(cache: KV4Cache, page_table: torch.Tensor, seq_lens: torch.Tensor,
     table, B, P, lens = _kv4_seqs(page_table, seq_lens, None, dev)
     if new_page_table.dim() != 2 or budget < 0 or recent < 0:
         raise ValueError("new_page_table must be int32 [batch, pages], budget and recent must not be negative")
+    budget, recent = min(budget, 2 ** 31 - 1), min(recent, 2 ** 31 - 1)  # more than any table holds
     NP = new_page_table.shape[1]
     new_table = _want(new_page_table, "new_page_table", torch.int32, (B, NP), dev)
     if new_lens is None:

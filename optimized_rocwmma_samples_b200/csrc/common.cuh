@@ -253,7 +253,11 @@ __device__ __forceinline__ void griddep_launch_dependents() { asm volatile("grid
 // cannot start before the kernel before it has completed (the fused
 // smoothquant -> GEMM entry prefetches weights ahead of its own wait).  What
 // overlaps is the launch and the CTAs' start-up, which otherwise leave the
-// GPU idle for a couple of microseconds between two short kernels.
+// GPU idle for a couple of microseconds between two short kernels.  Inside one
+// entry point the kernels behind the first may read the call's inputs before
+// their own wait (the first one has waited for them before it released them);
+// a kernel that writes nothing before its wait may also release its dependents
+// ahead of it, since they still wait for its completion.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                               Args&&... args)

@@ -279,12 +279,13 @@ cudaError_t launch_kv4_evict(const Kv4Cache& c, const int32_t* page_table, uint3
                              const int32_t* new_table, uint32_t new_max_pages, uint32_t batch, uint32_t budget,
                              uint32_t recent, int32_t* new_lens, uint32_t num_sms, cudaStream_t st)
 {
+    const uint32_t cap = max_pages * c.page_size;
+    budget = std::min(budget, std::min(cap, new_max_pages * c.page_size));  // (no more tokens fit either table)
     const uint64_t heads = (uint64_t)batch * c.kv_heads;
     // a block for every SM; each copies at least 64 rows (twice as many took 64 us instead of 54 at 32 x 8192 tokens and
     // 8 heads: the search is repeated)
     const uint32_t split = (uint32_t)std::max<uint64_t>(
         1, std::min<uint64_t>((num_sms + heads - 1) / heads, std::min<uint64_t>(16, (budget + 63) / 64)));
-    const uint32_t cap = max_pages * c.page_size;
     const uint32_t key_slots = cap <= kEvictKeys ? (cap + 3) / 4 * 4 : 0;
     const uint32_t row_slots = (std::min(kEvictRows, (budget + split - 1) / split + 1) + 3) / 4 * 4;
     const size_t smem = (size_t)key_slots * 4 + (size_t)row_slots * 20;

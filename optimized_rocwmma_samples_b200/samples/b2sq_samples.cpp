@@ -7,6 +7,8 @@
 //   rocwmma_moe_sorting.cpp:141-208      [MoE Sorting] tokens=.. experts=.. topk=.. unit=..  X ms  Y GB/s
 //   rocwmma_topk_softmax.cpp:197-256     [TopK-Softmax] tokens=.. experts=.. topk=..  X ms  Y GB/s
 //
+//   (no counterpart)                    [KV4-Append] [KV4-Attention] [KV4-Evict] [MoE-Layer] ...  X ms  Y GB/s
+//
 // so output parsers written for the reference (benchmark.sh:177-188) read it
 // unchanged.  Inputs are the reference drivers' constants (x = 0.5, smooth = 1,
 // A = B = 1 as int8 standing in for fp8(0.1)); timing: warm-up launches, then
@@ -14,11 +16,12 @@
 // sample also checks the known answer its constant inputs imply and exits
 // non-zero on a mismatch (the reference checks nothing here).
 //
-//   b2sq_samples [smoothquant|moe|gemm|sorting|topk|all] [M N]
+//   b2sq_samples [smoothquant|moe|gemm|sorting|topk|kv4|moe_layer|all] [M N]
 #include "../../include/b2sq.h"
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
@@ -360,6 +363,148 @@ static void test_topk_softmax(uint32_t tokens, uint32_t experts, uint32_t topk)
     CHECK_CUDA(cudaFree(dI));
 }
 
+// A decode step of a batch over the 4-bit cache: append, attention with weights, eviction to a quarter.  Keys and values
+// are the constant 0.5, so every group has step 0 and base 0.5.  Known answers: the values read back and the outputs are
+// 0.5, every token gathers heads / kv_heads / len of weight, and eviction keeps the lowest positions (all weights equal).
+static void test_kv4(uint32_t batch, uint32_t len, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t page)
+{
+    const uint32_t per_seq = (len + page - 1) / page, budget = len / 4, new_per_seq = (budget + page - 1) / page;
+    const uint32_t pages = batch * (per_seq + new_per_seq);
+    const uint64_t tokens = (uint64_t)batch * len, slots = (uint64_t)pages * kv_heads * page;
+    const size_t row = (size_t)kv_heads * dim;
+    std::vector<uint16_t> hK(tokens * row, half_of(0.5f));
+    std::vector<int32_t> hTable(batch * per_seq), hNew(batch * new_per_seq), hLens(batch, (int32_t)len), hAll(batch + 1),
+        hOne(batch + 1);
+    for (uint32_t i = 0; i < hTable.size(); ++i) hTable[i] = (int32_t)i;
+    for (uint32_t i = 0; i < hNew.size(); ++i) hNew[i] = (int32_t)(hTable.size() + i);
+    for (uint32_t b = 0; b <= batch; ++b) hAll[b] = (int32_t)(b * len), hOne[b] = (int32_t)b;
+    auto upload = [](const void* src, size_t n) {
+        void* d;
+        CHECK_CUDA(cudaMalloc(&d, n));
+        CHECK_CUDA(cudaMemcpy(d, src, n, cudaMemcpyHostToDevice));
+        return d;
+    };
+    auto room = [](size_t n) {
+        void* d;
+        CHECK_CUDA(cudaMalloc(&d, n));
+        CHECK_CUDA(cudaMemset(d, 0, n));
+        return d;
+    };
+    void* dK = upload(hK.data(), hK.size() * 2);
+    void* dOut = room(hK.size() * 2);
+    auto* dTable = (int32_t*)upload(hTable.data(), hTable.size() * 4);
+    auto* dNew = (int32_t*)upload(hNew.data(), hNew.size() * 4);
+    auto* dLens = (int32_t*)upload(hLens.data(), hLens.size() * 4);
+    auto* dAll = (int32_t*)upload(hAll.data(), hAll.size() * 4);
+    auto* dOne = (int32_t*)upload(hOne.data(), hOne.size() * 4);
+    auto* dNewLens = (int32_t*)room(batch * 4);
+    const b2sq_kv4_cache cache = {(uint8_t*)room(slots * dim / 2), (uint8_t*)room(slots * dim / 2), room(slots * dim / 64 * 4),
+                                  room(slots * dim / 64 * 4), (float*)room(slots * 4), pages, kv_heads, page, dim};
+    const double held = (double)dim / 2 + dim / 64 * 4;  // bytes of a token's keys, or values, in one head
+    const double append_ms = bench([&] {
+        CHECK_B2SQ(b2sq_kv4_append(dK, dK, B2SQ_F16, (uint32_t)tokens, (uint32_t)row, (uint32_t)row, &cache, dTable, batch,
+                                   per_seq, dLens, dAll, dOut, nullptr, nullptr));
+    });
+    std::printf("[KV4-Append] tokens=%llu kv_heads=%u dim=%u  %g ms  %g GB/s\n", (unsigned long long)tokens, kv_heads, dim,
+                append_ms, tokens * kv_heads * (2 * held + 6.0 * dim) / (append_ms * 1e-3) / 1e9);
+    size_t ws_bytes = 0;
+    CHECK_B2SQ(b2sq_kv4_attention_workspace_size(batch, heads, kv_heads, dim, page, per_seq, 1, 1, &ws_bytes));
+    void* ws = room(ws_bytes);
+    void* dQ = upload(hK.data(), (size_t)batch * heads * dim * 2);
+    void* dO = room((size_t)batch * heads * dim * 2);
+    auto attend = [&](int weights) {
+        CHECK_B2SQ(b2sq_kv4_attention(dQ, B2SQ_F16, batch, heads, heads * dim, &cache, dTable, batch, per_seq, dLens, dOne, 1,
+                                      1.f / std::sqrt((float)dim), dO, weights, ws, ws_bytes, nullptr));
+    };
+    const double attend_ms = bench([&] { attend(0); });
+    std::printf("[KV4-Attention] batch=%u len=%u heads=%u kv_heads=%u dim=%u  %g ms  %g GB/s\n", batch, len, heads, kv_heads,
+                dim, attend_ms, tokens * kv_heads * 2 * held / (attend_ms * 1e-3) / 1e9);
+    attend(1);
+    const double evict_ms = bench([&] {
+        CHECK_B2SQ(b2sq_kv4_evict(&cache, dTable, batch, per_seq, dLens, dNew, new_per_seq, budget, budget / 8, dNewLens,
+                                  nullptr));
+    });
+    std::printf("[KV4-Evict] batch=%u len=%u budget=%u kv_heads=%u dim=%u  %g ms  %g GB/s\n", batch, len, budget, kv_heads,
+                dim, evict_ms, (tokens * kv_heads * 4.0 + (double)batch * budget * kv_heads * (4 * held + 4)) / (evict_ms * 1e-3) / 1e9);
+    std::vector<uint16_t> hOut(hK.size()), hO((size_t)batch * heads * dim);
+    std::vector<float> hW(slots);
+    std::vector<int32_t> hNewLens(batch);
+    CHECK_CUDA(cudaMemcpy(hOut.data(), dOut, hOut.size() * 2, cudaMemcpyDeviceToHost));
+    CHECK_CUDA(cudaMemcpy(hO.data(), dO, hO.size() * 2, cudaMemcpyDeviceToHost));
+    CHECK_CUDA(cudaMemcpy(hW.data(), cache.weight, slots * 4, cudaMemcpyDeviceToHost));
+    CHECK_CUDA(cudaMemcpy(hNewLens.data(), dNewLens, batch * 4, cudaMemcpyDeviceToHost));
+    bool ok = true;
+    for (uint16_t v : hOut) ok = ok && v == half_of(0.5f);
+    for (uint16_t v : hO) ok = ok && v == half_of(0.5f);
+    for (int32_t v : hNewLens) ok = ok && v == (int32_t)budget;
+    const float share = (float)(heads / kv_heads) / len;
+    for (uint32_t b = 0; b < batch && ok; ++b)
+        for (uint32_t h = 0; h < kv_heads; ++h)
+            for (uint32_t t = 0; t < budget; ++t) {  // copied with the tokens
+                const float w = hW[((uint64_t)hNew[b * new_per_seq + t / page] * kv_heads + h) * page + t % page];
+                ok = ok && std::fabs(w - share) <= share * 1e-5f;
+            }
+    if (!ok) {
+        std::printf("[KV4] known answer FAILED\n");
+        ++g_failures;
+    }
+    for (void* d : {dK, dOut, (void*)dTable, (void*)dNew, (void*)dLens, (void*)dAll, (void*)dOne, (void*)dNewLens, ws, dQ, dO,
+                    (void*)cache.k, (void*)cache.v, cache.k_scale, cache.v_scale, (void*)cache.weight})
+        CHECK_CUDA(cudaFree(d));
+}
+
+// A whole mixture-of-experts layer for a few tokens.  x = 0.5, smooth = 1 and weights of 1 with steps 2 / hidden and
+// 1 / inter make gate = up = 1 in every expert.  Known answer: silu(1) = 0.7311 (weights of the slots add up to 1).
+static void test_moe_layer(uint32_t tokens, uint32_t hidden, uint32_t inter, uint32_t experts, uint32_t topk)
+{
+    std::vector<uint16_t> hX((size_t)tokens * hidden, half_of(0.5f));
+    std::vector<float> hOnes((size_t)experts * std::max(hidden, inter), 1.f), hS13((size_t)experts * 2 * inter, 2.f / hidden),
+        hS2((size_t)experts * hidden, 1.f / inter), hW((size_t)tokens * topk, 1.f / topk);
+    std::vector<int32_t> hIds((size_t)tokens * topk);
+    for (uint32_t t = 0; t < tokens; ++t)
+        for (uint32_t k = 0; k < topk; ++k) hIds[t * topk + k] = (int32_t)((t * topk + k) % experts);
+    auto upload = [](const void* src, size_t n) {
+        void* d;
+        CHECK_CUDA(cudaMalloc(&d, n));
+        CHECK_CUDA(cudaMemcpy(d, src, n, cudaMemcpyHostToDevice));
+        return d;
+    };
+    void* dX = upload(hX.data(), hX.size() * 2);
+    auto* dOnes = (float*)upload(hOnes.data(), hOnes.size() * 4);
+    auto* dS13 = (float*)upload(hS13.data(), hS13.size() * 4);
+    auto* dS2 = (float*)upload(hS2.data(), hS2.size() * 4);
+    auto* dW = (float*)upload(hW.data(), hW.size() * 4);
+    auto* dIds = (int32_t*)upload(hIds.data(), hIds.size() * 4);
+    int8_t *d13, *d2;
+    void *dOut, *ws;
+    const size_t n13 = (size_t)experts * 2 * inter * hidden;
+    CHECK_CUDA(cudaMalloc(&d13, n13));
+    CHECK_CUDA(cudaMalloc(&d2, n13 / 2));
+    CHECK_CUDA(cudaMemset(d13, 1, n13));
+    CHECK_CUDA(cudaMemset(d2, 1, n13 / 2));
+    CHECK_CUDA(cudaMalloc(&dOut, hX.size() * 2));
+    size_t ws_bytes = 0;
+    CHECK_B2SQ(b2sq_moe_layer_workspace_size(tokens, hidden, inter, experts, topk, &ws_bytes));
+    CHECK_CUDA(cudaMalloc(&ws, ws_bytes));
+    const double ms = bench([&] {
+        CHECK_B2SQ(b2sq_moe_layer(dX, B2SQ_F16, hidden, dW, dIds, dOnes, d13, dS13, dOnes, d2, dS2, dOut, tokens, hidden, inter,
+                                  experts, topk, 127.f, ws, ws_bytes, nullptr));
+    });
+    const double used = std::min<double>(experts, (double)tokens * topk);  // experts chosen, each read once
+    std::printf("[MoE-Layer] tokens=%u hidden=%u inter=%u experts=%u topk=%u  %g ms  %g GB/s\n", tokens, hidden, inter, experts,
+                topk, ms, used * 3 * hidden * inter / (ms * 1e-3) / 1e9);
+    std::vector<uint16_t> hOut(hX.size());
+    CHECK_CUDA(cudaMemcpy(hOut.data(), dOut, hOut.size() * 2, cudaMemcpyDeviceToHost));
+    bool ok = true;
+    for (uint16_t v : hOut) ok = ok && v >= 0x39d8 && v <= 0x39da;  // 0.7311 is 0x39d9 in fp16, a step either way
+    if (!ok) {
+        std::printf("[MoE-Layer] known answer FAILED\n");
+        ++g_failures;
+    }
+    for (void* d : {dX, (void*)dOnes, (void*)dS13, (void*)dS2, (void*)dW, (void*)dIds, (void*)d13, (void*)d2, dOut, ws})
+        CHECK_CUDA(cudaFree(d));
+}
+
 int main(int argc, char** argv)
 {
     cudaDeviceProp prop;
@@ -399,6 +544,16 @@ int main(int argc, char** argv)
         test_topk_softmax(128, 8, 4);
         for (auto ek : {std::pair<uint32_t, uint32_t>{8, 2}, {16, 2}, {32, 5}, {64, 5}})
             test_topk_softmax(3328, ek.first, ek.second);
+    }
+    if (what == "kv4" || what == "all") {
+        std::printf("=== 4-bit key/value cache (b2sq, sm_100a) ===\n");
+        test_kv4(16, 4096, 32, 8, 128, 64);
+        test_kv4(3, 1000, 8, 8, 64, 16);
+    }
+    if (what == "moe_layer" || what == "all") {
+        std::printf("=== MoE layer for a few tokens (b2sq, sm_100a) ===\n");
+        test_moe_layer(1, 4096, 14336, 8, 2);
+        test_moe_layer(16, 4096, 14336, 8, 2);
     }
     return g_failures ? 1 : 0;
 }

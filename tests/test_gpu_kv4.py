@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import kv4_ref as R
-from optimized_rocwmma_samples_b200 import api
+from optimized_rocwmma_samples_b200 import _lib, api
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -381,6 +381,22 @@ def test_evict_bad_pages_and_short_table(cuda_device):
     w = torch.cat([keep["weight"][0, 0], keep["weight"][1, 0]])
     pos = torch.tensor(R.kept(w, 32, 16, 2), device=DEV)
     assert torch.equal(cache.weight[6, 0], w[pos])
+
+
+@pytest.mark.parametrize("budget", [2 ** 31 - 1, 2 ** 32 - 1, 2 ** 40])
+def test_evict_without_a_bound(cuda_device, budget):
+    """Budgets that no table reaches keep everything."""
+    lens, size = [70, 5], 16
+    table, pages = R.tables(lens, size, 20, DEV)
+    cache = R.random_cache(api, pages + 6, 1, size, 64, True, 25, DEV)
+    check_evict(cache, lens, size, budget, 3, table, pages)
+    new = torch.zeros(2, dtype=torch.int32, device=DEV)
+    fresh, _ = R.tables(lens, size, 22, DEV, first=pages)
+    ln = ints(*lens)
+    seqs = (table.data_ptr(), 2, table.shape[1], ln.data_ptr(), fresh.data_ptr(), fresh.shape[1])
+    st = _lib.load().b2sq_kv4_evict(cache._ref, *seqs, budget & 0xffffffff, 0, new.data_ptr(), None)
+    torch.cuda.synchronize()
+    assert st == 0 and (budget & 0xffffffff == 0 or new.tolist() == lens)
 
 
 # ------------------------------------------------------------ all together
