@@ -813,15 +813,15 @@ struct Pieces {
 };
 
 constexpr uint32_t kJoinThreads = 256;
-constexpr uint32_t kJoinGroup = 4;  // warps that join one row
+constexpr uint32_t kJoinGroup = 4;  // warps that join one row, where there are few
 
-// Joins one row of an item from its pieces, four warps together (all of them call it); the first of them stores it.
-template <typename T, int D>
+// Joins one row of an item from its pieces, GROUP warps together (all of them call it); the first of them stores it.
+template <typename T, int D, uint32_t GROUP>
 __device__ __forceinline__ void join_row(const AttnParams& a, const Pieces& p, uint32_t rows_per_item, uint32_t r, T* dst,
                                          float2 (*part)[D / 2], float* part_l)
 {
     constexpr uint32_t V = D / 64;  // pairs of channels a lane holds
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, in_group = warp % kJoinGroup, group = warp / kJoinGroup;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, in_group = warp % GROUP, group = warp / GROUP;
     const uint32_t count = p.count();
     float top = -INFINITY;
     for (uint32_t i = lane; i < count; i += 32)
@@ -830,23 +830,23 @@ __device__ __forceinline__ void join_row(const AttnParams& a, const Pieces& p, u
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     float2 o[V] = {};
     float sum = 0.f;
-    // this warp's pieces: every fourth
-    for (uint32_t i0 = in_group; i0 < count; i0 += 32 * kJoinGroup) {
+    // this warp's pieces: every GROUP-th
+    for (uint32_t i0 = in_group; i0 < count; i0 += 32 * GROUP) {
         float f = 0.f;
-        const uint32_t i_lane = i0 + lane * kJoinGroup;
+        const uint32_t i_lane = i0 + lane * GROUP;
         if (i_lane < count) {
             const float2 ml = a.part_ml[(uint64_t)p.slot(i_lane) * rows_per_item + r];
             f = ml.x == -INFINITY ? 0.f : ml.x == top ? 1.f : ex2(ml.x - top);
             sum += ml.x == -INFINITY ? ml.y : ml.y * f;  // a NaN stays
         }
-        const uint32_t here = min(32u, (count - i0 + kJoinGroup - 1) / kJoinGroup);
+        const uint32_t here = min(32u, (count - i0 + GROUP - 1) / GROUP);
         constexpr uint32_t FLY = V == 4 ? 4 : 8;  // pieces in flight, the last ones too
         for (uint32_t i = 0; i < here; i += FLY) {
             float2 y[FLY][V];
 #pragma unroll
             for (uint32_t n = 0; n < FLY; ++n) {
                 const uint32_t k = min(i + n, here - 1);
-                const float* src = a.part_o + ((uint64_t)p.slot(i0 + k * kJoinGroup) * rows_per_item + r) * D;
+                const float* src = a.part_o + ((uint64_t)p.slot(i0 + k * GROUP) * rows_per_item + r) * D;
 #pragma unroll
                 for (uint32_t v = 0; v < V; ++v) y[n][v] = *reinterpret_cast<const float2*>(src + v * 64 + lane * 2);
             }
@@ -865,20 +865,22 @@ __device__ __forceinline__ void join_row(const AttnParams& a, const Pieces& p, u
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    named_bar_sync(1 + group, kJoinGroup * 32);  // (the last row's sums are read)
+    if constexpr (GROUP > 1) {
+        named_bar_sync(1 + group, GROUP * 32);  // (the last row's sums are read)
 #pragma unroll
-    for (uint32_t v = 0; v < V; ++v) part[warp][v * 32 + lane] = o[v];
-    if (lane == 0) part_l[warp] = sum;
-    named_bar_sync(1 + group, kJoinGroup * 32);
-    if (in_group != 0) return;
+        for (uint32_t v = 0; v < V; ++v) part[warp][v * 32 + lane] = o[v];
+        if (lane == 0) part_l[warp] = sum;
+        named_bar_sync(1 + group, GROUP * 32);
+        if (in_group != 0) return;
 #pragma unroll
-    for (uint32_t w = 1; w < kJoinGroup; ++w) {
-        sum += part_l[warp + w];
+        for (uint32_t w = 1; w < GROUP; ++w) {
+            sum += part_l[warp + w];
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) {
-            const float2 y = part[warp + w][v * 32 + lane];
-            o[v].x += y.x;
-            o[v].y += y.y;
+            for (uint32_t v = 0; v < V; ++v) {
+                const float2 y = part[warp + w][v * 32 + lane];
+                o[v].x += y.x;
+                o[v].y += y.y;
+            }
         }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -887,9 +889,9 @@ __device__ __forceinline__ void join_row(const AttnParams& a, const Pieces& p, u
         *reinterpret_cast<uint32_t*>(dst + v * 64 + lane * 2) = f2_to_pair<T>(o[v].x * inv, o[v].y * inv);
 }
 
-// The first join_blocks blocks join the items that lie in several blocks' shares, four warps a row; the others add up the
-// weights, each of an equal piece of all positions, from the scores.  With few query rows (`by_rows`) every row looks for
-// its own item.  With many, every boundary between two shares stands for the item it cuts, if it is the first to do so:
+// The first join_blocks blocks join the items that lie in several blocks' shares; the others add up the weights, each of an
+// equal piece of all positions, from the scores.  With few query rows (`by_rows`) every row looks for its own item, four
+// warps a row.  With many, a warp a row, every boundary between two shares stands for the item it cuts, if it is the first to do so:
 // there are at most as many such items as blocks, and they are found in shared memory alone.  What depends on the call's
 // inputs is worked out before the wait for the first kernel, which has waited for the inputs itself.
 // With weights, the kernel does not let its dependents start early: blocks of the next attention that come into registers
@@ -899,7 +901,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a, uint32_t rows_per_item, uint32_t grid1,
                                                                    uint32_t join_blocks, bool by_rows)
 {
-    constexpr uint32_t WARPS = kJoinThreads / 32, GROUPS = WARPS / kJoinGroup;
+    constexpr uint32_t WARPS = kJoinThreads / 32;
     extern __shared__ uint32_t ustart[];  // [batch + 1], then the chunks of a sequence's items [batch]
     __shared__ float2 row_ml[kJoinThreads];
     __shared__ float2 part[WARPS][D / 2];
@@ -924,7 +926,8 @@ __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a,
         };
         const uint32_t most_rows = min(rows_per_item, a.group * a.max_queries);
         const uint64_t units = by_rows ? (uint64_t)a.s.tokens * a.heads : (uint64_t)(split.blocks - 1) * most_rows;
-        for (uint64_t x = blockIdx.x * GROUPS + warp / kJoinGroup; x < units; x += join_blocks * GROUPS) {
+        const uint32_t group = by_rows ? kJoinGroup : 1, groups = WARPS / group;
+        for (uint64_t x = blockIdx.x * groups + warp / group; x < units; x += join_blocks * groups) {
             uint32_t b, head, row, unit0;  // sequence, key head, row of its rows, the item's first chunk on the line
             SeqShape sh;
             if (by_rows) {
@@ -960,7 +963,10 @@ __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a,
             wait();
             T* dst = static_cast<T*>(a.out) +
                      ((uint64_t)(sh.start + row / a.group) * a.heads + head * a.group + row % a.group) * D;
-            join_row<T, D>(a, p, rows_per_item, row % rows_per_item, dst, part, part_l);
+            if (by_rows)
+                join_row<T, D, kJoinGroup>(a, p, rows_per_item, row % rows_per_item, dst, part, part_l);
+            else
+                join_row<T, D, 1>(a, p, rows_per_item, row % rows_per_item, dst, part, part_l);
         }
         wait();
         return;
@@ -1103,12 +1109,12 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
     // The second kernel is one wave of three blocks an SM, with weights one for the rows and two for the weights (a block
     // takes a few microseconds to its first row; four waves of them took 36 us where one takes 20).  Few rows look for
     // their items themselves (16 x 4000 tokens, 512 rows: 22.8 us, by cuts 25.2), many are found by the cuts.
-    constexpr uint32_t kGroups = kJoinThreads / 32 / kJoinGroup;
     const uint64_t all_rows = (uint64_t)p.s.tokens * p.heads;
     const bool by_rows = all_rows <= 4 * num_sms;
+    const uint32_t groups = kJoinThreads / 32 / (by_rows ? kJoinGroup : 1);
     const uint64_t rows = by_rows ? all_rows : (uint64_t)(grid - 1) * std::min(8u * NT, p.group * p.max_queries);
     const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 2 * num_sms) : 0;
-    const uint32_t join = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((rows + kGroups - 1) / kGroups, (accumulate ? 1 : 3) * num_sms));
+    const uint32_t join = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((rows + groups - 1) / groups, (accumulate ? 1 : 3) * num_sms));
     return launch_pdl(kv4_join_kernel<T, D>, dim3(join + weights), dim3(kJoinThreads), line + p.s.batch * 4, st, p, 8u * NT,
                       grid, join, by_rows);
 }
