@@ -42,7 +42,9 @@ namespace b2sq {
 
 namespace {
 
-constexpr uint32_t kMinTokens = 64;  // of a block's share: fewer leave too little to do between its start and its join
+// Tokens of a block's share: fewer leave too little to do between its start and its join.  Shorter items have a block
+// each while there are blocks (4 x 7 tokens, 4 key heads: one after another they took 27 us, side by side 9).
+constexpr uint32_t kMinTokens = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -54,6 +56,7 @@ struct AttnParams {
     uint32_t heads, group, max_queries, row_pad;  // row_pad: group * max_queries rounded up to 4
     float scale_log2;
     uint32_t chunk;  // tokens a warp takes at a time: 16 or 32
+    uint32_t items;  // (sequence, head, row block) at most
     float2* stats;         // [batch * kv_heads][row_pad] (max, sum) of items that one block did whole
     float* part_o;         // [2 * blocks][8 NT][D]
     float2* part_ml;       // [2 * blocks][8 NT]
@@ -70,9 +73,9 @@ template <int D, int NT, int CH>
 constexpr uint32_t attn_blocks()
 {
     if (CH == 2) return D == 64 ? 4 : 3;
-    return D == 64 ? (NT == 1 ? 5 : NT == 2 ? 4 : 3) : D == 128 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (NT == 1 ? 3 : 2);
+    return D == 64 ? (NT == 1 ? 5 : 4) : D == 128 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2);
 }
-constexpr uint32_t kMaxBlocks = 6;
+constexpr uint32_t kMaxBlocks = 5;
 
 template <int D, int NT, int CH>
 struct AttnSmem {
@@ -189,9 +192,9 @@ __device__ __forceinline__ uint32_t value_bits(uint32_t w, uint32_t hi)
 // Equal pieces of `total` chunks for `blocks` blocks: the first `rest` get one more.
 struct Split {
     uint32_t blocks, each, rest;
-    __device__ __forceinline__ Split(uint32_t total, uint32_t grid, uint32_t chunk)
+    __device__ __forceinline__ Split(uint32_t total, uint32_t grid, uint32_t chunk, uint32_t items)
     {
-        blocks = max(1u, min(grid, total / (kMinTokens / chunk)));
+        blocks = max(1u, min(grid, max(total / (kMinTokens / chunk), min(total, items))));
         each = total / blocks;
         rest = total - each * blocks;
     }
@@ -279,7 +282,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
 
     lay_out<kThreads>(a, ROWS, ustart, scan_part);
     const uint32_t total = ustart[a.s.batch];
-    const Split split(total, gridDim.x, CHUNK);
+    const Split split(total, gridDim.x, CHUNK, a.items);
     if (blockIdx.x >= split.blocks || total == 0) return;
     const uint32_t begin = split.begin(blockIdx.x), end = split.begin(blockIdx.x + 1);
 
@@ -915,7 +918,7 @@ __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a,
         griddep_wait();
         return;
     }
-    const Split split(total, grid1, a.chunk);
+    const Split split(total, grid1, a.chunk, a.items);
     if (blockIdx.x < join_blocks) {
         bool waited = false;
         auto wait = [&]() {
@@ -1068,14 +1071,17 @@ __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a,
 struct AttnWs {
     size_t stats, part_o, part_ml, scores, bytes;
 };
-uint32_t tiles_of(uint32_t rows, uint32_t dim) { return rows <= 8 ? 1 : rows <= 16 || dim == 256 ? 2 : 4; }
+// Tiles of 8 rows a block takes.  Blocks of 4 tiles read the cache once for 32 rows, but their sums leave the registers
+// and their code the instruction cache: 72 us for 32 rows of 128 channels at 4 x 40000 tokens, two blocks of 2 tiles 63,
+// and 52 against 40 at 16 x 4000.
+uint32_t tiles_of(uint32_t rows) { return rows <= 8 ? 1 : 2; }
 
 AttnWs layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t max_queries, uint32_t max_len,
               bool accumulate, uint32_t num_sms)
 {
     const uint64_t rows = (uint64_t)(heads / kv_heads) * max_queries;
     const uint64_t pad = (rows + 3) / 4 * 4;
-    const uint64_t slots = 2ull * num_sms * kMaxBlocks * 8 * tiles_of((uint32_t)std::min<uint64_t>(rows, 1u << 20), dim);
+    const uint64_t slots = 2ull * num_sms * kMaxBlocks * 8 * tiles_of((uint32_t)std::min<uint64_t>(rows, 1u << 20));
     AttnWs w;
     size_t at = 0;
     auto take = [&](uint64_t n) {
@@ -1095,13 +1101,15 @@ template <typename T, int D, int NT, int CH>
 cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t st)
 {
     using S = AttnSmem<D, NT, CH>;
+    static_assert(attn_blocks<D, NT, CH>() <= kMaxBlocks, "workspace too small");
     p.chunk = 16 * CH;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(kv4_attention_kernel<T, D, NT, CH>, S::fixed + (kMaxAttnBatch + 1) * 4, done);
     if (e != cudaSuccess) return e;
     // no more blocks than the page tables have room for chunks
     const uint64_t items = (uint64_t)p.s.batch * p.c.kv_heads * ((p.group * p.max_queries + 8 * NT - 1) / (8 * NT));
-    const uint64_t most = items * ((uint64_t)p.s.max_pages * p.c.page_size + p.chunk) / kMinTokens + 1;
+    p.items = (uint32_t)std::min<uint64_t>(items, UINT32_MAX);
+    const uint64_t most = std::max(items, items * ((uint64_t)p.s.max_pages * p.c.page_size + p.chunk) / kMinTokens + 1);
     const uint32_t grid = (uint32_t)std::min<uint64_t>(most, num_sms * attn_blocks<D, NT, CH>());
     const uint32_t line = (p.s.batch + 1) * 4;
     e = launch_pdl(kv4_attention_kernel<T, D, NT, CH>, dim3(grid), dim3(S::warps * 32), S::fixed + line, st, p);
@@ -1122,17 +1130,11 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
 template <typename T, int D>
 cudaError_t run_dim(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t st)
 {
-    switch (tiles_of(std::min(p.group * p.max_queries, 1u << 20), D)) {
-        case 1:
-            // chunks of 32 tokens, where pages hold whole ones: half the steps, and two chains of products to overlap
-            if constexpr (D < 256)
-                if (p.c.page_size % 32 == 0) return run<T, D, 1, 2>(p, accumulate, num_sms, st);
-            return run<T, D, 1, 1>(p, accumulate, num_sms, st);
-        case 2: return run<T, D, 2, 1>(p, accumulate, num_sms, st);
-        default:
-            if constexpr (D < 256) return run<T, D, 4, 1>(p, accumulate, num_sms, st);
-            return cudaErrorInvalidValue;
-    }
+    if (tiles_of(std::min(p.group * p.max_queries, 1u << 20)) == 2) return run<T, D, 2, 1>(p, accumulate, num_sms, st);
+    // chunks of 32 tokens, where pages hold whole ones: half the steps, and two chains of products to overlap
+    if constexpr (D < 256)
+        if (p.c.page_size % 32 == 0) return run<T, D, 1, 2>(p, accumulate, num_sms, st);
+    return run<T, D, 1, 1>(p, accumulate, num_sms, st);
 }
 
 }  // namespace

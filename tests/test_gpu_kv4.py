@@ -145,6 +145,9 @@ SHAPES = [  # D, heads, kv_heads, page, lengths, query counts
     (128, 64, 8, 64, [5003], [1]),
     (128, 4, 2, 16, [70, 0, 20], [0, 0, 0]),
     (128, 5, 1, 16, [4], [9]),  # more queries than tokens: the first ones see nothing
+    (64, 8, 2, 16, [(7 * i) % 61 for i in range(150)], [i % 4 for i in range(150)]),  # items shorter than a block's share
+    (128, 16, 2, 32, [5, 40, 33, 0, 7], [5, 3, 8, 1, 2]),
+    (128, 24, 8, 64, [(29 * i) % 200 + 1 for i in range(97)], [1] * 97),  # more items than blocks
 ]
 
 
