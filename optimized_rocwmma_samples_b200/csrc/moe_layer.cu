@@ -226,11 +226,14 @@ __device__ __forceinline__ void make_lists(const MoeLayer& m, uint32_t most, con
     uint32_t* count = scratch;
     uint16_t* rank = reinterpret_cast<uint16_t*>(scratch + m.experts);
     for (uint32_t e = tid; e < m.experts; e += kThreads) count[e] = 0;
+    // the ranks' places hold the experts first: one trip to memory for all of them
+    for (uint32_t r = tid; r < routes; r += kThreads)
+        rank[r] = (uint16_t)min((uint32_t)__ldg(m.topk_ids + r), m.experts);
     __syncthreads();
     if (warp == 0)
         for (uint32_t base = 0; base < routes; base += 32) {
             const uint32_t r = base + lane;
-            const uint32_t e = r < routes ? (uint32_t)__ldg(m.topk_ids + r) : 0xffffffffu;
+            const uint32_t e = r < routes ? rank[r] : m.experts;
             const bool valid = e < m.experts;
             const uint32_t same = __match_any_sync(0xffffffffu, e);
             const uint32_t before = valid ? count[e] : 0;
