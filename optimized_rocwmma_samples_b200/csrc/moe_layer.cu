@@ -10,13 +10,22 @@
 //
 // What bounds it is reading the weights of the experts that were chosen, once.
 // Blocks of an expert's routes (up to 8 NT of them) meet its weight rows in
-// units of 16 rows; every block of the grid (one an SM) takes an equal run of
-// the units, which lie one after another in memory.  Weights stream through a
-// ring of cp.async stages in which each of the eight warps keeps its own
-// 16 x 128 byte tiles (every eighth of the unit's), so that no barrier stands
-// between loading and multiplying; the routes' int8 rows lie in shared memory.
-// mma.m16n8k32: weight rows are the 16, routes the 8 columns.  The warps' int32
-// sums meet in shared memory by integer adds, one barrier a unit.
+// tiles of 16 rows; every block of the grid (one an SM) takes an equal run of
+// the tiles, which lie one after another in memory, and each of its eight warps
+// an equal run of their 128-byte pieces.  Weights stream through a ring of
+// cp.async stages of the warp's own, so that no barrier stands between loading
+// and multiplying; the routes' int8 rows lie in shared memory.
+// mma.m16n8k32: weight rows are the 16, routes the 8 columns.  A warp has most
+// tiles to itself and ends them in registers; the tiles between two warps' runs
+// meet in shared memory by integer adds.  (Eight warps on every tile, an eighth
+// of its columns each, add and wait 16 times as often: 64 tokens, 8 experts,
+// 2 slots, 4096 x 14336: 337 us, 295 this way; 58 tokens, 128 experts, 3 slots,
+// 4832 x 336: 102 and 76; but 16 tokens, where few sums wait and each weight row
+// is read in longer pieces, 222 and 227.)
+//
+// 1 token, 8 experts, 2 slots, 4096 x 14336: 64 us (353 MB: 5.5 TB/s of the 6.6
+// that a copy moves); 16 tokens: 227 us (6.2); 24 tokens, 32 experts, 5 slots,
+// 4096 x 1456: 94 us (6.0).
 //
 //   moe_quant_x_kernel  smoothquant of each route's token; clears what the others add to
 //   moe_up_kernel       gate and up rows (8 + 8 a tile, so one thread has both), SwiGLU;
@@ -67,9 +76,9 @@ struct Params {
 template <int NT, int STAGES>
 struct Smem {
     static constexpr uint32_t ring = kWarps * STAGES * kTile;
-    static constexpr uint32_t pitch = NT == 1 ? 8 : NT == 2 ? 24 : 40;  // ints of a row of sums: two-way bank conflicts at most
-    static constexpr uint32_t group = NT == 4 ? 2 : 4;              // row tiles between two barriers
-    static constexpr uint32_t sums = 2 * group * 16 * pitch * 4;    // of two groups
+    static constexpr uint32_t pitch = NT == 1 ? 8 : NT == 2 ? 24 : 36;  // ints of a row of sums: two-way bank conflicts at most
+    static constexpr uint32_t tile_sums = 16 * pitch;
+    static constexpr uint32_t sums = (kWarps - 1) * tile_sums * 4;      // of the tiles between two warps' runs
     __host__ __device__ static constexpr uint32_t row_pitch(uint32_t k) { return (k + 127) / 128 * 128 + 16; }
     __host__ __device__ static constexpr uint32_t rows(uint32_t k) { return 8 * NT * row_pitch(k); }
     __host__ __device__ static constexpr uint32_t lists(uint32_t experts, uint32_t routes)
@@ -82,9 +91,10 @@ struct Smem {
     }
 };
 
+// (256 bytes a trip to memory: with 128, 24 tokens over 32 experts took 99 us, with 256 they take 94)
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes)
 {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -360,30 +370,49 @@ struct RowCopy {
     }
 };
 
-// First of the 128-byte pieces of row tile `tile` of a group that a warp takes: the group's pieces go round the warps.
-__device__ __forceinline__ uint32_t first_piece(uint32_t warp, uint32_t tile, uint32_t pieces)
-{
-    return (warp - tile * pieces) & (kWarps - 1);
-}
+// The pieces of a block's row tiles, one tile's 128-byte pieces after another's, in equal runs for the warps.
+struct Runs {
+    uint32_t total, pieces;
+    __device__ __forceinline__ Runs(uint32_t tiles, uint32_t pieces_) : total(tiles * pieces_), pieces(pieces_) {}
+    __device__ __forceinline__ uint32_t begin(uint32_t w) const
+    {
+        return total / kWarps * w + total % kWarps * w / kWarps;
+    }
+    // Warp w's run begins inside a tile, and is the first to: that tile (its sums meet in place w - 1), else ~0.
+    __device__ __forceinline__ uint32_t cut_tile(uint32_t w) const
+    {
+        if (w == 0) return ~0u;
+        const uint32_t q = begin(w), t = q / pieces;
+        return q == t * pieces || begin(w - 1) > t * pieces ? ~0u : t;
+    }
+    // The place of a cut tile's sums, for a warp whose run begins in it or before it.
+    __device__ __forceinline__ uint32_t place_of(uint32_t w, uint32_t t) const
+    {
+        if (begin(w) <= t * pieces) ++w;
+        while (w > 1 && begin(w - 1) > t * pieces) --w;
+        return w - 1;
+    }
+};
 
-// A warp's share of a row tile: int32 products of its 16 weight rows with the block's routes over its pieces.
+// int32 products of a tile's 16 weight rows with the block's routes, over `count` of its pieces from p0 on.
 template <int NT, int STAGES, typename Next>
-__device__ __forceinline__ void tile_product(uint32_t tile, uint32_t pieces, uint32_t live, uint32_t ring_base,
+__device__ __forceinline__ void tile_product(uint32_t p0, uint32_t count, uint32_t live, uint32_t ring_base,
                                              uint32_t rows_base, uint32_t row_pitch, uint32_t& slot, int (&acc)[NT][4],
                                              Next&& next)
 {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const uint32_t lane = threadIdx.x & 31;
     const uint32_t arow = (lane & 7) + ((lane >> 3) & 1) * 8, asel = lane >> 4;
-    const uint32_t brow = rows_base + (lane & 7) * row_pitch + (lane >> 3) * 16;
+    uint32_t brow = rows_base + (lane & 7) * row_pitch + (lane >> 3) * 16 + p0 * 128;
     int odd[NT][4];  // a second chain of products: one waits half as long for its own
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[nt][i] = odd[nt][i] = 0;
-    for (uint32_t p = first_piece(warp, tile, pieces); p < pieces; p += kWarps) {
+#pragma unroll 1
+    for (uint32_t n = 0; n < count; ++n, brow += 128) {
         cp_async_wait<STAGES - 2>();
         __syncwarp();
-        // the slot that the last step freed takes the tile STAGES - 1 steps ahead
+        // the slot that the last step freed takes the piece STAGES - 1 steps ahead
         next();
         const uint32_t a_at = ring_base + slot * kTile + arow * 128;
         if (++slot == STAGES) slot = 0;
@@ -393,7 +422,7 @@ __device__ __forceinline__ void tile_product(uint32_t tile, uint32_t pieces, uin
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             if (nt == 0 || nt < live) {
-                const uint32_t b_at = brow + nt * 8 * row_pitch + p * 128;
+                const uint32_t b_at = brow + nt * 8 * row_pitch;
                 uint32_t b[2][4];
                 ldsm4(b_at, b[0]);
                 ldsm4(b_at + 64, b[1]);
@@ -409,19 +438,28 @@ __device__ __forceinline__ void tile_product(uint32_t tile, uint32_t pieces, uin
         for (int i = 0; i < 4; ++i) acc[nt][i] += odd[nt][i];
 }
 
-// Adds the warps' products into a tile's sums in shared memory (zero before).
+// Adds a warp's products into a cut tile's sums in shared memory (zero before), and takes them out again.
 template <int NT, uint32_t PITCH>
 __device__ __forceinline__ void add_sums(int* sums, const int (&acc)[NT][4], uint32_t live)
 {
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
-        if (nt == 0 || nt < live) {
-            int* at = sums + g * PITCH + nt * 8 + 2 * tig;
-            atomicAdd(at, acc[nt][0]);
-            atomicAdd(at + 1, acc[nt][1]);
-            atomicAdd(at + 8 * PITCH, acc[nt][2]);
-            atomicAdd(at + 8 * PITCH + 1, acc[nt][3]);
+        if (nt == 0 || nt < live)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) atomicAdd(sums + (g + i / 2 * 8) * PITCH + nt * 8 + 2 * tig + (i & 1), acc[nt][i]);
+}
+template <int NT, uint32_t PITCH>
+__device__ __forceinline__ void take_sums(int* sums, int (&acc)[NT][4])
+{
+    const uint32_t lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int* at = sums + (g + i / 2 * 8) * PITCH + nt * 8 + 2 * tig + (i & 1);
+            acc[nt][i] = *at;
+            *at = 0;
         }
 }
 
@@ -450,32 +488,26 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
     const Split split(total, gridDim.x);
     const uint32_t begin = split.begin(blockIdx.x), end = split.begin(blockIdx.x + 1);
 
-    // producer: this warp's next piece (row tile, piece) and its addresses; pt: place of the tile in its group
+    // producer: this warp's next piece pq of its run in the units pu .. pu + pn of one block of routes, and its address
     const uint32_t pieces = (H + 127) / 128;
     const uint32_t ring_base = smem_u32(moe_smem) + warp * STAGES * kTile;
     const uint32_t lrow = lane / 8, lchunk = lane & 7;
-    uint32_t pu = begin, pj = begin % per_block, pt = 0, pp = warp, pslot = 0;
+    uint32_t pu = begin, pn = 0, pq = 0, pend = 0, pp = 0, pslot = 0;
     const int8_t* src = nullptr;
-    auto place = [&]() {
-        const uint32_t e = expert_of(l, m.experts, pu / per_block);
-        src = m.w13 + ((uint64_t)e * 2 * I + pj * 8 + lrow) * H + lchunk * 16;
-    };
-    auto settle = [&]() {  // over tiles in which the warp has no piece
-        while (pu < end && pp >= pieces) {
-            ++pu;
-            if (++pt == S::group) pt = 0;
-            if (++pj == per_block) pj = pt = 0;
-            pp = first_piece(warp, pt, pieces);
-            if (pu < end) {
-                if (pj == 0)
-                    place();
-                else
-                    src += (uint64_t)8 * H;
-            }
+    auto settle = [&]() {  // on to the next run that is not empty
+        while (pq == pend && (pu += pn) < end) {
+            const uint32_t pb = pu / per_block, pj = pu - pb * per_block;
+            pn = min(per_block - pj, end - pu);
+            const Runs runs(pn, pieces);
+            pq = runs.begin(warp);
+            pend = runs.begin(warp + 1);
+            const uint32_t t = pq / pieces;
+            pp = pq - t * pieces;
+            src = m.w13 + ((uint64_t)expert_of(l, m.experts, pb) * 2 * I + (pj + t) * 8 + lrow) * H + lchunk * 16;
         }
     };
     auto load = [&]() {
-        if (pu < end) {
+        if (pq < pend) {
             const uint32_t at = pp * 128 + lchunk * 16;
             const uint32_t bytes = at < H ? 16u : 0u;
             const uint32_t dst = ring_base + pslot * kTile;
@@ -487,14 +519,16 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
                 // (the last piece may reach past the row: nothing is read there)
                 cp_async16(dst + r * 128 + ((lchunk ^ (r & 7)) * 16), bytes ? row : m.w13, bytes);
             }
-            pp += kWarps;
-            settle();
+            if (++pp == pieces) {
+                pp = 0;
+                src += (uint64_t)8 * H;
+            }
+            if (++pq == pend) settle();
         }
         cp_async_commit();
         if (++pslot == STAGES) pslot = 0;
     };
     if (begin < end) {
-        place();
         settle();
 #pragma unroll 1
         for (int i = 0; i < STAGES - 1; ++i) load();
@@ -503,75 +537,86 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
     griddep_launch_dependents();
     if (begin == end) return;
 
-    uint32_t slot = 0, buf = 0;
+    uint32_t slot = 0;
     uint32_t b = begin / per_block, j = begin % per_block;
     RowCopy copy;
     Block cur = block_at<NT>(l, m.experts, b);
     copy.fetch(tid, p.xq, H, 0, H, l.order + cur.r0, cur.count);
+    const uint32_t g = lane >> 2, tig = lane & 3;
     for (uint32_t u = begin; u < end;) {
         const uint32_t e = cur.expert, r0 = cur.r0, count = cur.count;
-        __syncthreads();  // the last block's rows are read
         copy.finish(rows, row_pitch, p.xq, H, 0, H, l.order + r0, count);
         if (tid < count) {
             rs1[tid] = p.rs1[l.order[r0 + tid]];
             top[tid] = 0;
         }
         __syncthreads();
-        const uint32_t live = (count + 7) / 8;
-        constexpr uint32_t CELLS = 64 * NT, EACH = (S::group * CELLS + kThreads - 1) / kThreads;
-        while (j < per_block && u < end) {
-            const uint32_t here = min(min((uint32_t)S::group, per_block - j), end - u);  // row tiles of this group
-            // the epilogue's share of a thread: tile n / CELLS, route n / 8 % (8 NT), inner element n % 8 of the tile
-            float sg[EACH], su[EACH], s2[EACH];
-#pragma unroll
-            for (uint32_t i = 0; i < EACH; ++i) {
-                const uint32_t n = tid + i * kThreads, t = n / CELLS;
-                sg[i] = su[i] = s2[i] = 0.f;
-                if (t < here && n / 8 % (8 * NT) < count) {
-                    const uint64_t at = (uint64_t)e * 2 * I + (j + t) * 8 + (n & 7);
-                    sg[i] = __ldg(m.s13 + at);
-                    su[i] = __ldg(m.s13 + at + I);
-                    s2[i] = __ldg(m.smooth2 + (uint64_t)e * I + (j + t) * 8 + (n & 7));
-                }
-            }
-            if (j + here == per_block && u + here < end) {  // the next block's rows, behind this group's products
-                cur = block_at<NT>(l, m.experts, b + 1);
-                copy.fetch(tid, p.xq, H, 0, H, l.order + cur.r0, cur.count);
-            }
-            int* sum = sums + buf * S::group * 16 * S::pitch;
-            buf ^= 1;
-            for (uint32_t t = 0; t < here; ++t) {
-                int acc[NT][4];
-                tile_product<NT, STAGES>(t, pieces, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
-                add_sums<NT, S::pitch>(sum + t * 16 * S::pitch, acc, live);
-            }
-            __syncthreads();
-            // (the other buffer's readers are past this barrier too: it is free and zero again)
-#pragma unroll
-            for (uint32_t i = 0; i < EACH; ++i) {
-                const uint32_t n = tid + i * kThreads, t = n / CELLS, tok = n / 8 % (8 * NT), jj = n & 7;
-                float hv = 0.f;
-                if (t < here && tok < 8 * live) {
-                    int* at = sum + (t * 16 + jj) * S::pitch + tok;
-                    if (tok < count) {
-                        const float g = __fmul_rn((float)at[0], __fmul_rn(rs1[tok], sg[i]));
-                        const float v = __fmul_rn((float)at[8 * S::pitch], __fmul_rn(rs1[tok], su[i]));
-                        hv = g / (1.f + expf(-g)) * v * s2[i];
-                        p.h[(uint64_t)l.order[r0 + tok] * I + (j + t) * 8 + jj] = hv;
-                    }
-                    at[0] = 0;
-                    at[8 * S::pitch] = 0;
-                }
-                float mx = fmaxf(fabsf(hv), 0.f);  // a NaN drops out, as in smoothquant
-#pragma unroll
-                for (int off = 4; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                if (jj == 0 && t < here && tok < count) atomicMax(top + tok, __float_as_uint(mx));
-            }
-            j += here;
-            u += here;
+        const uint32_t live = (count + 7) / 8, here = min(per_block - j, end - u);
+        if (u + here < end) {  // the next block's rows, behind this one's products
+            cur = block_at<NT>(l, m.experts, b + 1);
+            copy.fetch(tid, p.xq, H, 0, H, l.order + cur.r0, cur.count);
         }
+        float mx[NT][2] = {};
+        struct Scales {
+            float gate, up, smooth;
+        };
+        auto scales = [&](uint32_t t) {  // of the thread's inner element of tile t
+            const uint32_t at = (j + t) * 8 + g;
+            const float* s = m.s13 + (uint64_t)e * 2 * I + at;
+            return Scales{__ldg(s), __ldg(s + I), __ldg(m.smooth2 + (uint64_t)e * I + at)};
+        };
+        auto finish = [&](uint32_t t, const int (&acc)[NT][4], const Scales& s) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t tok = nt * 8 + 2 * tig + c;
+                    if (tok >= count) continue;
+                    const float gv = __fmul_rn((float)acc[nt][c], __fmul_rn(rs1[tok], s.gate));
+                    const float uv = __fmul_rn((float)acc[nt][2 + c], __fmul_rn(rs1[tok], s.up));
+                    const float hv = gv / (1.f + expf(-gv)) * uv * s.smooth;
+                    p.h[(uint64_t)l.order[r0 + tok] * I + (j + t) * 8 + g] = hv;
+                    mx[nt][c] = fmaxf(mx[nt][c], fabsf(hv));  // a NaN drops out, as in smoothquant
+                }
+        };
+        const Runs runs(here, pieces);
+        uint32_t q = runs.begin(warp), t = q / pieces, p0 = q - t * pieces;
+        const uint32_t qe = runs.begin(warp + 1);
+        Scales sc = q < qe ? scales(t) : Scales{};
+        int acc[NT][4];
+        while (q < qe) {
+            const uint32_t n = min(pieces - p0, qe - q);
+            const Scales ahead = q + n < qe ? scales(t + 1) : Scales{};
+            tile_product<NT, STAGES>(p0, n, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
+            if (n == pieces)
+                finish(t, acc, sc);
+            else
+                add_sums<NT, S::pitch>(sums + runs.place_of(warp, t) * S::tile_sums, acc, live);
+            sc = ahead;
+            q += n;
+            p0 = 0;
+            ++t;
+        }
+        // the tiles between two runs, a warp each
+        const uint32_t cut = runs.cut_tile(warp);
+        if (cut != ~0u) sc = scales(cut);
         __syncthreads();
+        if (cut != ~0u) {
+            take_sums<NT, S::pitch>(sums + (warp - 1) * S::tile_sums, acc);
+            finish(cut, acc, sc);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) mx[nt][c] = fmaxf(mx[nt][c], __shfl_xor_sync(0xffffffffu, mx[nt][c], off));
+                const uint32_t tok = nt * 8 + 2 * tig + c;
+                if (g == 0 && tok < count) atomicMax(top + tok, __float_as_uint(mx[nt][c]));
+            }
+        __syncthreads();  // (and the rows are read, and the sums are zero)
         if (tid < count) atomicMax(p.top + l.order[r0 + tid], top[tid]);
+        u += here;
         ++b;
         j = 0;
     }
@@ -603,31 +648,25 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
 
     const uint32_t ring_base = smem_u32(moe_smem) + warp * STAGES * kTile;
     const uint32_t lrow = lane / 8, lchunk = lane & 7;
-    uint32_t pu = begin, pr = begin % per_slice, pt = 0, pp = warp, pslot = 0;  // pr: row tile of the matrix
+    uint32_t pu = begin, pn = 0, pq = 0, pend = 0, pp = 0, ppieces = 0, pslot = 0;
+    uint32_t left = 0;  // inner elements of the producer's slice
     const int8_t* src = nullptr;
-    uint32_t left = 0, ppieces = 0;  // inner elements and pieces of the producer's slice
-    auto place = [&]() {
-        const uint32_t bs = pu / per_slice, e = expert_of(l, m.experts, bs / p.slices), k0 = bs % p.slices * p.slice;
-        left = min(p.slice, I - k0);
-        ppieces = (left + 127) / 128;
-        src = m.w2 + ((uint64_t)e * H + pr * 16 + lrow) * I + k0 + lchunk * 16;
-    };
     auto settle = [&]() {
-        while (pu < end && pp >= ppieces) {
-            ++pu;
-            if (++pt == S::group) pt = 0;
-            if (++pr == per_slice) pr = pt = 0;
-            if (pu < end) {
-                if (pr == 0)
-                    place();
-                else
-                    src += (uint64_t)16 * I;
-            }
-            pp = first_piece(warp, pt, ppieces);
+        while (pq == pend && (pu += pn) < end) {
+            const uint32_t bs = pu / per_slice, pr = pu - bs * per_slice, k0 = bs % p.slices * p.slice;
+            left = min(p.slice, I - k0);
+            ppieces = (left + 127) / 128;
+            pn = min(per_slice - pr, end - pu);
+            const Runs runs(pn, ppieces);
+            pq = runs.begin(warp);
+            pend = runs.begin(warp + 1);
+            const uint32_t t = pq / ppieces;
+            pp = pq - t * ppieces;
+            src = m.w2 + ((uint64_t)expert_of(l, m.experts, bs / p.slices) * H + (pr + t) * 16 + lrow) * I + k0 + lchunk * 16;
         }
     };
     auto load = [&]() {
-        if (pu < end) {
+        if (pq < pend) {
             const uint32_t at = pp * 128 + lchunk * 16;
             const uint32_t bytes = at < left ? 16u : 0u;
             const uint32_t dst = ring_base + pslot * kTile;
@@ -637,14 +676,16 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
                 const uint32_t r = i * 4 + lrow;
                 cp_async16(dst + r * 128 + ((lchunk ^ (r & 7)) * 16), bytes ? s + (uint64_t)i * 4 * I : m.w2, bytes);
             }
-            pp += kWarps;
-            settle();
+            if (++pp == ppieces) {
+                pp = 0;
+                src += (uint64_t)16 * I;
+            }
+            if (++pq == pend) settle();
         }
         cp_async_commit();
         if (++pslot == STAGES) pslot = 0;
     };
     if (begin < end) {
-        place();
         settle();
 #pragma unroll 1
         for (int i = 0; i < STAGES - 1; ++i) load();
@@ -653,50 +694,64 @@ __global__ void __launch_bounds__(kThreads, 1) moe_down_kernel(Params p)
     griddep_launch_dependents();
     if (begin == end) return;
 
-    uint32_t slot = 0, buf = 0;
+    uint32_t slot = 0;
     uint32_t bs = begin / per_slice, ru = begin % per_slice;
     RowCopy copy;
     Block cur = block_at<NT>(l, m.experts, bs / p.slices);
     uint32_t k0 = bs % p.slices * p.slice, depth = min(p.slice, I - k0);
     copy.fetch(tid, p.hq, I, k0, depth, l.order + cur.r0, cur.count);
+    const uint32_t g = lane >> 2, tig = lane & 3;
     for (uint32_t u = begin; u < end;) {
         const uint32_t r0 = cur.r0, count = cur.count;
-        __syncthreads();  // the last slice's rows are read
         copy.finish(rows, row_pitch, p.hq, I, k0, depth, l.order + r0, count);
         __syncthreads();
-        const uint32_t live = (count + 7) / 8, pieces = (depth + 127) / 128;
-        while (ru < per_slice && u < end) {
-            const uint32_t here = min(min((uint32_t)S::group, per_slice - ru), end - u);
-            if (ru + here == per_slice && u + here < end) {  // the next slice's rows, behind this group's products
-                cur = block_at<NT>(l, m.experts, (bs + 1) / p.slices);
-                k0 = (bs + 1) % p.slices * p.slice;
-                depth = min(p.slice, I - k0);
-                copy.fetch(tid, p.hq, I, k0, depth, l.order + cur.r0, cur.count);
-            }
-            int* sum = sums + buf * S::group * 16 * S::pitch;
-            buf ^= 1;
-            for (uint32_t t = 0; t < here; ++t) {
-                int acc[NT][4];
-                tile_product<NT, STAGES>(t, pieces, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
-                add_sums<NT, S::pitch>(sum + t * 16 * S::pitch, acc, live);
-            }
-            __syncthreads();
-            for (uint32_t i = tid; i < here * 128 * live; i += kThreads) {
-                const uint32_t row = i % 16, x = i / 16, t = x % here, tok = x / here;
-                int* from = sum + (t * 16 + row) * S::pitch + tok;
-                const int v = *from;
-                *from = 0;
-                if (tok < count) {
-                    int32_t* at = p.acc + (uint64_t)l.order[r0 + tok] * H + (ru + t) * 16 + row;
-                    if (p.slices > 1)
-                        atomicAdd(at, v);  // integers: exact in any order
-                    else
-                        *at = v;
-                }
-            }
-            ru += here;
-            u += here;
+        const uint32_t live = (count + 7) / 8, pieces = (depth + 127) / 128, here = min(per_slice - ru, end - u);
+        if (u + here < end) {  // the next slice's rows, behind this one's products
+            cur = block_at<NT>(l, m.experts, (bs + 1) / p.slices);
+            k0 = (bs + 1) % p.slices * p.slice;
+            depth = min(p.slice, I - k0);
+            copy.fetch(tid, p.hq, I, k0, depth, l.order + cur.r0, cur.count);
         }
+        auto finish = [&](uint32_t t, const int (&acc)[NT][4]) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t tok = nt * 8 + 2 * tig + c;
+                    if (tok >= count) continue;
+                    int32_t* at = p.acc + (uint64_t)l.order[r0 + tok] * H + (ru + t) * 16 + g;
+                    if (p.slices > 1) {  // integers: exact in any order
+                        atomicAdd(at, acc[nt][c]);
+                        atomicAdd(at + 8, acc[nt][2 + c]);
+                    } else {
+                        at[0] = acc[nt][c];
+                        at[8] = acc[nt][2 + c];
+                    }
+                }
+        };
+        const Runs runs(here, pieces);
+        uint32_t q = runs.begin(warp), t = q / pieces, p0 = q - t * pieces;
+        const uint32_t qe = runs.begin(warp + 1);
+        int acc[NT][4];
+        while (q < qe) {
+            const uint32_t n = min(pieces - p0, qe - q);
+            tile_product<NT, STAGES>(p0, n, live, ring_base, smem_u32(rows), row_pitch, slot, acc, load);
+            if (n == pieces)
+                finish(t, acc);
+            else
+                add_sums<NT, S::pitch>(sums + runs.place_of(warp, t) * S::tile_sums, acc, live);
+            q += n;
+            p0 = 0;
+            ++t;
+        }
+        __syncthreads();
+        const uint32_t cut = runs.cut_tile(warp);  // the tiles between two runs, a warp each
+        if (cut != ~0u) {
+            take_sums<NT, S::pitch>(sums + (warp - 1) * S::tile_sums, acc);
+            finish(cut, acc);
+        }
+        // (the rows are read; the sums are zero before the next adds: the barrier behind the next rows)
+        u += here;
         ++bs;
         ru = 0;
     }
@@ -798,12 +853,16 @@ cudaError_t run(Params& p, uint32_t num_sms, cudaStream_t st)
     return e;
 }
 
-// The widest block of routes that the tokens call for and shared memory has room for, with eight stages or five:
-// a block too narrow for an expert's routes reads its weights again.
+// The widest block of routes that the tokens call for and shared memory has room for, with as many stages as fit:
+// a block too narrow for an expert's routes reads its weights again.  Narrow blocks gain from eleven stages (1 token:
+// 64.1 us, with eight 65.7), wider ones do not.  Three stages under blocks of 32 lose more than reading twice (48 tokens,
+// 32 experts, 8 slots, hidden 5120: 491 us against 433).
 template <typename T, int NT>
 cudaError_t pick(Params& p, uint32_t num_sms, cudaStream_t st)
 {
     const uint32_t routes = p.m.tokens * p.m.topk, k = std::max(p.m.hidden, p.slice);
+    if constexpr (NT == 1)
+        if (Smem<NT, 11>::total(k, p.m.experts, routes) <= kSmemMost) return run<T, NT, 11>(p, num_sms, st);
     if (Smem<NT, 8>::total(k, p.m.experts, routes) <= kSmemMost) return run<T, NT, 8>(p, num_sms, st);
     if (Smem<NT, 5>::total(k, p.m.experts, routes) <= kSmemMost) return run<T, NT, 5>(p, num_sms, st);
     if constexpr (NT > 1) return pick<T, NT / 2>(p, num_sms, st);
@@ -812,7 +871,7 @@ cudaError_t pick(Params& p, uint32_t num_sms, cudaStream_t st)
 
 // Routes of an expert at an even spread are about routes / experts; a block takes three standard deviations more (and no
 // expert has more than the tokens, unless a token names it twice).  Narrow blocks leave room for a deeper ring: 24 tokens
-// over 32 experts ran 123 us with blocks of 32 and five stages, 110 us with blocks of 16 and eight.
+// over 32 experts ran 107 us with blocks of 32 and five stages, 97 us with blocks of 16 and eight.
 template <typename T>
 cudaError_t run_type(Params& p, uint32_t num_sms, cudaStream_t st)
 {
