@@ -541,7 +541,7 @@ def moe_layer(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tenso
             _want(out, "out", x.dtype, (T, H), dev))
     with _on(dev):
         ws, ws_bytes, hold = _scratch(workspace, _moe_layer_ws(dev.index, T, H, I, E, K), dev, stream)
-        st = _lib.load().b2sq_moe_layer(x.data_ptr(), code, x.stride(0) if T > 1 else H, *args, T, H, I, E, K,
+        st = _lib.load().b2sq_moe_layer(x.data_ptr(), code, _pitch(x.stride(0), "x") if T > 1 else H, *args, T, H, I, E, K,
                                         float(quant_max), ws, ws_bytes, _raw_stream(stream, dev))
     _lib.check(st, "b2sq_moe_layer")
     return out
@@ -588,12 +588,19 @@ class KV4Cache:
         return cls(*data, *scale, w)
 
 
+def _pitch(elements: int, name: str) -> int:
+    """A token pitch as the library takes it, in 32 bits (a longer one would be cut off on its way there)."""
+    if elements >> 32:
+        raise ValueError(f"{name}: tokens must lie less than 2^32 elements apart")
+    return elements
+
+
 def _kv4_rows(t: torch.Tensor, name: str, dev: torch.device):
     """(tokens, heads, token pitch) of a [tokens, heads, head_dim] tensor whose heads lie side by side."""
     shape, stride = t.shape, t.stride()
     if len(shape) != 3 or t.get_device() != dev.index or stride[2] != 1 or (shape[1] > 1 and stride[1] != shape[2]):
         raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous heads on {dev}")
-    return shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1] * shape[2]
+    return shape[0], shape[1], _pitch(stride[0], name) if shape[0] > 1 else shape[1] * shape[2]
 
 
 def _kv4_seqs(page_table: torch.Tensor, seq_lens: torch.Tensor, token_start: Optional[torch.Tensor], dev: torch.device):

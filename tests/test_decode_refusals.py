@@ -134,3 +134,23 @@ def test_python_refuses_host_tensors():
         api.moe_layer(x, *([x] * 8))
     with pytest.raises(ValueError):
         api.moe_layer(x.float(), *([x] * 8))
+
+
+def test_pitches_past_32_bits():
+    """The library takes pitches in 32 bits; longer ones are refused, not cut off."""
+    class Rows:  # a view that no test could hold in memory
+        shape = (2, 8, 64)
+
+        def __init__(self, pitch):
+            self.pitch = pitch
+
+        def stride(self):
+            return (self.pitch, 64, 1)
+
+        def get_device(self):
+            return 0
+
+    dev = torch.device("cuda", 0)
+    assert api._kv4_rows(Rows(2 ** 32 - 8), "q", dev) == (2, 8, 2 ** 32 - 8)
+    with pytest.raises(ValueError, match="2\\^32"):
+        api._kv4_rows(Rows(2 ** 32 + 512), "q", dev)
