@@ -5,13 +5,16 @@
 //   q = clamp(rint((v - z) / s), 0, 15), ties to even; s = 0 gives q = 0
 // A NaN makes its group's s and z NaN, so it is not lost in the cache.
 //
-// Bound by HBM (2 bytes a channel in, 0.56 out, 2 more where the cached
-// values are asked for) as long as the arithmetic stays near ten instructions
-// a channel: eight lanes hold a group, one 16-byte load and one 4-byte store of
+// HBM would bound it (2 bytes a channel in, 0.56 out, 2 more where the cached
+// values are asked for) with fewer than ten instructions a channel; it takes 15,
+// and the issue slots do: eight lanes hold a group, one 16-byte load and one 4-byte store of
 // nibbles each; extrema in packed 16-bit operations and three shuffles; the
 // quotient as a saturated product with 1 / (15 s), whose exact remainder tells
 // whether it was rounded right.  Inputs of 8 or 11 significant bits meet the
 // border between two steps often, so those lanes decide it exactly.
+//
+// 7 x 4001 tokens, 8 heads of 128 channels: 41 us (173 MB, 4.2 TB/s); 16 tokens
+// 2.7 us.
 #include "kv4.cuh"
 
 #include <algorithm>

