@@ -8,13 +8,14 @@
 // whole.
 //
 // The threshold is found by a radix search over the weights' sortable bits
-// (four passes of 8 bits over keys in shared memory), places by prefix sums
-// within and over the warps.  Every block of a head repeats that search
+// (four passes of 8 bits over keys in shared memory, of long sequences as many
+// as fit: 1 x 60785 tokens, one head, 130 us, with none of them 245), places by
+// prefix sums within and over the warps.  Every block of a head repeats that search
 // and copies its own share of the kept rows, so no block waits for another.
 //
 // The copy is bound by HBM, the search by the latency of its passes: 32 x 8192
-// tokens, 8 heads of 128 channels, down to 2048: 52 us (158 MB, 3.1 TB/s);
-// 1 x 1040 down to 1024: 7.8 us.
+// tokens, 8 heads of 128 channels, down to 2048: 51 us (159 MB, 3.1 TB/s);
+// 1 x 1040 down to 1024: 7.4 us.
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -26,7 +27,7 @@ namespace {
 
 constexpr uint32_t kEvictThreads = 512;
 constexpr uint32_t kEvictWarps = kEvictThreads / 32;
-constexpr uint32_t kEvictKeys = 40960;  // keys held in shared memory (160 KB); longer sequences re-read theirs
+constexpr uint32_t kEvictKeys = 40960;  // keys held in shared memory (160 KB); longer sequences re-read the others
 constexpr uint32_t kEvictRows = 2048;   // kept rows one block lists at a time
 constexpr uint32_t kEvictFly = 4;       // copies of a thread in flight
 
@@ -109,34 +110,30 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
     const uint32_t old = all ? 0 : n - newest;      // candidates
     const uint32_t want = all ? 0 : kept - newest;  // of them kept
 
-    auto key_of = [&](uint32_t i) -> uint32_t {
-        const int64_t r = kv4_row(c, table, i, head);
-        return r < 0 ? 0u : weight_key(c.weight[r]);
+    // keys of positions i .. i + 3 (i a multiple of 4, so they are neighbours on one page); past the candidates: anything
+    auto read_keys = [&](uint32_t i, uint32_t (&k)[4]) {
+        const int64_t r = i < old ? kv4_row(c, table, i, head) : -1;
+        const float4 w = r < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldg(reinterpret_cast<const float4*>(c.weight + r));
+        k[0] = weight_key(w.x), k[1] = weight_key(w.y), k[2] = weight_key(w.z), k[3] = weight_key(w.w);
+        if (r < 0) k[0] = k[1] = k[2] = k[3] = 0;
     };
-    const bool held = old <= key_slots;
-    if (held) {
-        constexpr uint32_t FLY = 8;
-        for (uint32_t i0 = tid; i0 < old; i0 += FLY * kEvictThreads) {
-            int64_t r[FLY];
-            float w[FLY];
+    const uint32_t held = min(old, key_slots);  // (key_slots is a multiple of 4)
+    constexpr uint32_t FLY = 2, STRIDE = 4 * kEvictThreads;
+    for (uint32_t i0 = tid * 4; i0 < held; i0 += FLY * STRIDE) {
+        uint32_t k[FLY][4];
 #pragma unroll
-            for (uint32_t n = 0; n < FLY; ++n)
-                r[n] = i0 + n * kEvictThreads < old ? kv4_row(c, table, i0 + n * kEvictThreads, head) : -1;
+        for (uint32_t n = 0; n < FLY; ++n) read_keys(i0 + n * STRIDE, k[n]);
 #pragma unroll
-            for (uint32_t n = 0; n < FLY; ++n) w[n] = r[n] >= 0 ? c.weight[r[n]] : 0.f;
-#pragma unroll
-            for (uint32_t n = 0; n < FLY; ++n)
-                if (i0 + n * kEvictThreads < old) keys[i0 + n * kEvictThreads] = r[n] >= 0 ? weight_key(w[n]) : 0u;
-        }
+        for (uint32_t n = 0; n < FLY; ++n)
+            if (i0 + n * STRIDE < held)
+                *reinterpret_cast<uint4*>(keys + i0 + n * STRIDE) = make_uint4(k[n][0], k[n][1], k[n][2], k[n][3]);
     }
-    // keys of positions i .. i + 3 (i a multiple of 4); past the candidates: anything
     auto keys_at = [&](uint32_t i, uint32_t (&k)[4]) {
-        if (held) {
+        if (i < held) {
             const uint4 v = *reinterpret_cast<const uint4*>(keys + i);
             k[0] = v.x, k[1] = v.y, k[2] = v.z, k[3] = v.w;
         } else {
-#pragma unroll
-            for (uint32_t n = 0; n < 4; ++n) k[n] = i + n < old ? key_of(i + n) : 0;
+            read_keys(i, k);
         }
     };
 
@@ -146,13 +143,24 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
         for (int shift = 24; shift >= 0; shift -= 8) {
             for (uint32_t i = tid; i < 256; i += kEvictThreads) hist[i] = 0;
             __syncthreads();
-            for (uint32_t i = tid * 4; i < old; i += 4 * kEvictThreads) {
-                uint32_t k[4];
-                keys_at(i, k);
+            auto count = [&](uint32_t i, const uint32_t (&k)[4]) {
 #pragma unroll
                 for (uint32_t n = 0; n < 4; ++n)
                     if (i + n < old && (shift == 24 || ((k[n] ^ prefix) >> (shift + 8)) == 0))
                         atomicAdd(&hist[(k[n] >> shift) & 255u], 1u);
+            };
+            uint32_t i = tid * 4;
+            for (; i < held; i += STRIDE) {
+                uint32_t k[4];
+                keys_at(i, k);
+                count(i, k);
+            }
+            for (; i < old; i += FLY * STRIDE) {
+                uint32_t k[FLY][4];
+#pragma unroll
+                for (uint32_t n = 0; n < FLY; ++n) read_keys(i + n * STRIDE, k[n]);
+#pragma unroll
+                for (uint32_t n = 0; n < FLY; ++n) count(i + n * STRIDE, k[n]);
             }
             __syncthreads();
             if (warp == 0) {
@@ -197,12 +205,14 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
     };
     uint32_t gt = 0, eq = 0;
     if (!take_none)
-        for (uint32_t i = w0 + lane * 4; i < w1; i += 128) {
-            uint32_t k[4];
-            keys_at(i, k);
-            uint32_t both = 0;
+        for (uint32_t i0 = w0 + lane * 4; i0 < w1; i0 += FLY * 128) {
+            uint32_t k[FLY][4], both = 0;
 #pragma unroll
-            for (uint32_t n = 0; n < 4; ++n) both += marks(i, n, k[n]);
+            for (uint32_t f = 0; f < FLY; ++f) keys_at(i0 + f * 128, k[f]);
+#pragma unroll
+            for (uint32_t f = 0; f < FLY; ++f)
+#pragma unroll
+                for (uint32_t n = 0; n < 4; ++n) both += marks(i0 + f * 128, n, k[f][n]);
             gt += both & 0xffffu;
             eq += both >> 16;
         }
@@ -221,6 +231,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
         gt0 += warp_gt[i];
         eq0 += warp_eq[i];
     }
+    // places of the warp's kept tokens
+    const uint32_t to0 = gt0 + min(eq0, ties), to1 = gt0 + gt + min(eq0 + eq, ties);
 
     // a thread copies the same 16-byte piece of every row that is its turn: keys, then values
     constexpr uint32_t PIECES = 4 * NG, ROWS = kEvictThreads / PIECES;
@@ -230,16 +242,19 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
     Scale* const scale = static_cast<Scale*>(tid & 1 ? c.v_scale : c.k_scale);
     for (uint32_t r0 = d0; r0 < d1; r0 += row_slots) {
         const uint32_t r1 = min(r0 + row_slots, d1);
-        if (!take_none) {
+        if (to0 < r1 && to1 > r0) {
             uint32_t g = gt0, e = eq0;  // before this step
+            uint32_t k[4], next[4];
+            keys_at(w0 + lane * 4, k);
             for (uint32_t base = w0; base < w1; base += 128) {
                 const uint32_t i = base + lane * 4;
-                uint32_t k[4] = {}, mine[4], sum = 0;
-                if (i < w1) keys_at(i, k);
+                uint32_t mine[4], sum = 0;
+                keys_at(i + 128, next);  // (on their way behind this step's)
 #pragma unroll
                 for (uint32_t n = 0; n < 4; ++n) {
                     mine[n] = marks(i, n, k[n]);
                     sum += mine[n];
+                    k[n] = next[n];
                 }
                 uint32_t incl = sum;
 #pragma unroll
@@ -288,9 +303,11 @@ cudaError_t launch_kv4_evict(const Kv4Cache& c, const int32_t* page_table, uint3
     const uint64_t heads = (uint64_t)batch * c.kv_heads;
     // a block for every SM; each copies at least 64 rows (twice as many took 64 us instead of 54 at 32 x 8192 tokens and
     // 8 heads: the search is repeated)
+    const uint32_t key_slots = std::min(cap, kEvictKeys);
+    // where two do not fit on one SM, no more than there are SMs (2 x 131000 tokens to 60000, 8 heads: 521 us; 812 with twelve blocks left for a second turn)
+    const bool two = (key_slots * 4 + kEvictRows * 20) * 2 <= 225 * 1024;
     const uint32_t split = (uint32_t)std::max<uint64_t>(
-        1, std::min<uint64_t>((num_sms + heads - 1) / heads, std::min<uint64_t>(16, (budget + 63) / 64)));
-    const uint32_t key_slots = cap <= kEvictKeys ? (cap + 3) / 4 * 4 : 0;
+        1, std::min<uint64_t>((num_sms + (two ? heads - 1 : 0)) / heads, std::min<uint64_t>(16, (budget + 63) / 64)));
     const uint32_t row_slots = (std::min(kEvictRows, (budget + split - 1) / split + 1) + 3) / 4 * 4;
     const size_t smem = (size_t)key_slots * 4 + (size_t)row_slots * 20;
     auto launch = [&](auto kernel, std::atomic<uint64_t>& done) {
