@@ -336,6 +336,8 @@ def check_evict(cache, lens, size, budget, recent, table, first, new_lens_cap=No
     (128, 2, 16, [64, 10], 0, 0),
     (64, 1, 64, [50000, 41000], 5000, 100),
     (64, 2, 64, [6000], 5999, 7),
+    (64, 1, 64, [50000, 300, 0], 40000, 100),  # more rows a block than it lists at a time, short ones in a wide table
+    (128, 1, 32, [44000], 36000, 0),
 ])
 def test_evict(cuda_device, D, kv, size, lens, budget, recent):
     table, pages = R.tables(lens, size, 20, DEV, spare=1)
