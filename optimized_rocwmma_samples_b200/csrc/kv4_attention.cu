@@ -23,6 +23,14 @@
 //    probabilities, times the token's step over a running power of two of the
 //    group, are rounded to fp16 (11 bits; the result has 8 or 11) and turned
 //    into the other operand by movmatrix.  sum(p z) is kept apart in fp32.
+//  * The matrix unit cuts its fp32 sums off instead of rounding them, and nibbles
+//    are never negative: left alone the sums shrink by about 2^-23 a product,
+//    and sum(p z), of the other sign, leaves that a large part of the result.
+//    So every 32 products an amount known exactly, close to 8 steps times the
+//    sum of p, moves from the sums to sum(p z): they stay about their centre,
+//    where what is cut off cancels (64 x 131072 tokens, fp16: off by 2.2e-4 of
+//    the result, 2.1e-3 without; rounding the result is 2.2e-4.  It takes 2 to
+//    3% of the time; 8 steps taken off by a product of their own took 14%).
 //
 // Work is split evenly over the grid in chunks of 16 tokens, whatever the
 // lengths: the (sequence, head, row block) items lie one after another on a
@@ -52,6 +60,8 @@ namespace {
 // each while there are blocks (4 x 7 tokens, 4 key heads: one after another they took 27 us, side by side 9).
 constexpr uint32_t kMinTokens = 64;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kRun = 32;           // products between two centrings of the sums (16 gave the same error)
+constexpr float kSample = 1.f / 256.f;  // keeps a sample's sum in fp16: 32 products, 8 lanes, p times step at most 2^15
 
 struct AttnParams {
     Kv4Cache c;
@@ -451,6 +461,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
         float o[NG][4][NT][4] = {};
         float m[NT][2], l[NT][2], zs[NT][2][NG];  // m: 0 until the row has seen a token
         float ref[NG];                            // 2^8 / the power of two that a group's steps are taken over
+        __half2 part_p[NG][NT], last_p[NG][NT];   // half of the tokens' p times step since the last centring, and before it
         uint32_t seen = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -462,7 +473,11 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                 for (uint32_t gr = 0; gr < NG; ++gr) zs[nt][x][gr] = 0.f;
             }
 #pragma unroll
-        for (uint32_t gr = 0; gr < NG; ++gr) ref[gr] = 4294967296.f;
+        for (uint32_t gr = 0; gr < NG; ++gr) {
+            ref[gr] = 4294967296.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) part_p[gr][nt] = last_p[gr][nt] = __half2(0.f, 0.f);
+        }
 
         const uint32_t tok = (lane & 7) + ((lane >> 3) & 1) * 8;  // ldmatrix row of this lane
         const uint32_t sw = (tok / (8 / CPR)) & (CPR - 1);
@@ -576,6 +591,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
 #pragma unroll
                             for (uint32_t gr = 0; gr < NG; ++gr) {
                                 zs[nt][x][gr] *= f;
+                                part_p[gr][nt] = last_p[gr][nt] = __half2(0.f, 0.f);
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) {
                                     o[gr][j][nt][x] *= f;
@@ -600,6 +616,8 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                         const float fresh = __uint_as_float((262u - (__float_as_uint(mx) >> 23)) << 23);
                         const float f = fresh / ref[gr];
                         ref[gr] = fresh;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) part_p[gr][nt] = last_p[gr][nt] = __half2(0.f, 0.f);
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -644,6 +662,8 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                         for (int h = 0; h < 2; ++h) {
                             const uint32_t w = f2_to_pair<__half>(pv[2 * h], pv[2 * h + 1]);
                             pb[gr][nt][h] = movmatrix(w);
+                            if (h == (ch & 1))
+                                part_p[gr][nt] = __hfma2(*reinterpret_cast<const __half2*>(&w), __half2(kSample, kSample), part_p[gr][nt]);
                             if constexpr (SPLIT) {
                                 const float2 r = pair_to_f2<__half>(w);
                                 pb2[gr][nt][h] = movmatrix(f2_to_pair<__half>(pv[2 * h] - r.x, pv[2 * h + 1] - r.y));
@@ -677,6 +697,35 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
             }
         };
 
+        // Takes 8 steps a nibble out of the run's sums, by twice the sample, and half of that again, less the half taken
+        // before: the next run's sums start about as far below their centre as they end above it.  The sample need not be
+        // exact, nor does it grow with what a new maximum rescales: what leaves the sums enters zs.
+        auto centre = [&]() {
+#pragma unroll
+            for (uint32_t gr = 0; gr < NG; ++gr) {
+                const float back = __uint_as_float((254u << 23) - __float_as_uint(ref[gr])) * (0.25f / kSample);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    __half2 v = part_p[gr][nt];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) v = __hadd2(v, __shfl_xor_sync(0xffffffffu, v, off));
+                    const float2 now = __half22float2(v), then = __half22float2(last_p[gr][nt]);
+                    last_p[gr][nt] = v;
+                    part_p[gr][nt] = __half2(0.f, 0.f);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float out = x ? fmaf(12.f, now.y, -4.f * then.y) : fmaf(12.f, now.x, -4.f * then.x);
+                        zs[nt][x][gr] = fmaf(out, back, zs[nt][x][gr]);  // (an eighth in each of the lanes that are added up)
+                        const float even = out * (2.f / kSample / 16777216.f), odd = 17.f * even;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            o[gr][j][nt][x] -= (j & 1) ? odd : even;
+                            o[gr][j][nt][2 + x] -= (j & 1) ? odd : even;
+                        }
+                    }
+                }
+            }
+        };
         for (uint32_t c = wc0; c < wc1; ++c) {
             __syncwarp();
             load();
@@ -687,6 +736,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                     step(c, slot, std::true_type());
                 else
                     step(c, slot, std::false_type());
+                if ((c - wc0) % (kRun / CH) == kRun / CH - 1) centre();
             } else if (score_at) {  // no such page: nothing of this chunk is seen
                 const uint32_t rows = min(ROWS, a.row_pad - block * ROWS);
                 for (uint32_t i = lane; i < CHUNK * rows && c * CHUNK + i / rows < sh.vis; i += 32)
