@@ -17,7 +17,9 @@
 //    to the sums: q.K over a group = s * sum(q4 q) + z * sum(q).
 //  * Scores: K is the 16 x 16 operand (16 tokens, 16 channels of one word
 //    position), the query rows are the 8 columns, prepared once in that order
-//    as fp16 scaled by a power of two to [2^9, 2^10) (exact for both types).
+//    as fp16 scaled by a power of two that brings the row's largest to [2^9, 2^10)
+//    (exact, but for channels below 2^-20 (fp16) or 2^-23 (bf16) of the largest,
+//    which are off by up to 2^-30 of it).
 //  * Output: V^T is the 16 x 16 operand; ldmatrix.trans moves whole 16-bit
 //    words (4 channels of a token), which is the transposition needed.  The
 //    probabilities, times the token's step over a running power of two of the
@@ -70,7 +72,7 @@ struct AttnParams {
     void* out;
     uint64_t q_stride;
     uint32_t heads, group, max_queries, row_pad;  // row_pad: group * max_queries rounded up to 4
-    float scale_log2;
+    float scale;
     uint32_t chunk;  // tokens a warp takes at a time: 16 or 32
     uint32_t items;  // (sequence, head, row block) at most
     float2* stats;         // [batch * kv_heads][row_pad] (max, sum) of items that one block did whole
@@ -416,10 +418,12 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
             }
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            // 2^(9 - exponent of the largest); none for rows of zeros or with an infinity
+            // 2^(9 - exponent of the largest), 2^127 at most; none for rows with an infinity
             const int ex = (int)(__float_as_uint(mx) >> 23);
-            const int shift = (ex == 0 || ex == 255) ? 0 : min(max(136 - ex, -100), 100);
-            const float f = __uint_as_float((uint32_t)(127 + shift) << 23);
+            const float f = __uint_as_float((uint32_t)(127 + (ex == 255 ? 0 : min(136 - ex, 127))) << 23);
+            // What brings the row's products back, below 2^76: there a softmax is 0 or 1, since products that differ do so
+            // by 2^-48 or more, and the scores stay finite.
+            const float mul = fminf(fmaxf(a.scale / f * kLog2e, -7.55578637e22f), 7.55578637e22f);
 #pragma unroll
             for (uint32_t c = 0; c < D / 32; ++c) {
                 // channel 32 c + lane: word position j, k half, operand register and lane
@@ -429,13 +433,13 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
             }
 #pragma unroll
             for (uint32_t gr = 0; gr < NG; ++gr) {
-                float sum = v[2 * gr] + v[2 * gr + 1];
+                float sum = v[2 * gr] * f + v[2 * gr + 1] * f;
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                if (lane == 0) row_sum[r][gr] = sum * a.scale_log2;
+                if (lane == 0) row_sum[r][gr] = sum * mul;
             }
             if (lane == 0) {
-                row_mul[r] = a.scale_log2 * (16777216.f / f);
+                row_mul[r] = mul * 16777216.f;
                 // rows that are not there see everything (their columns are not used), so that they mask nothing
                 row_vis[r] = row < all_rows
                                  ? (int)max((int64_t)0, min((int64_t)sh.vis, (int64_t)sh.len - sh.n + row / a.group + 1))
@@ -1217,7 +1221,7 @@ cudaError_t launch_kv4_attention(const Kv4Attention& a, void* workspace, uint32_
     p.group = a.heads / a.cache.kv_heads;
     p.max_queries = a.max_queries;
     p.row_pad = (p.group * a.max_queries + 3) / 4 * 4;
-    p.scale_log2 = a.scale * kLog2e;
+    p.scale = a.scale;
     p.stats = reinterpret_cast<float2*>(base + w.stats);
     p.part_o = reinterpret_cast<float*>(base + w.part_o);
     p.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
