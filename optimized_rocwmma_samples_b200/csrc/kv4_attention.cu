@@ -753,6 +753,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
         // has no room for both)
         const uint32_t next_unit = unit + (cur.c1 - cur.c0);
         if (S::early && next_unit < end) {
+            __syncwarp();  // the first load takes the slot of the last chunk, which every lane has read
             cur = piece_at(next_unit);
             if (NT == 1) fetch_rows(cur);  // (more rows would not fit beside the sums)
             slot = lslot;
