@@ -500,8 +500,8 @@ B2SQ_API b2sq_status b2sq_kv4_attention_workspace_size(uint32_t batch, uint32_t 
  * (equal weights: the lower position; -0 equals 0; a NaN counts as the
  * largest); a shorter one keeps all.  Kept tokens are copied in order, with
  * their weights, to positions 0, 1, ... of new_page_table, and new_lens[b]
- * receives their number, min(seq_lens[b], budget) (less where the new table
- * holds fewer).  The old pages are only read: they may be shared with other
+ * receives their number, min(seq_lens[b], budget) (less where either table
+ * holds fewer); new_lens may be seq_lens itself, but not overlap it otherwise.  The old pages are only read: they may be shared with other
  * sequences, but no page may stand in both tables.  recent <= budget; the
  * cache keeps weights; budget 0 empties every sequence.
  */

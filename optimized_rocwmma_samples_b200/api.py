@@ -684,7 +684,8 @@ def kv4_evict(cache: KV4Cache, page_table: torch.Tensor, seq_lens: torch.Tensor,
               stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """Thins each sequence out to ``budget`` tokens: in every key head the newest ``recent`` ones and those that
     gathered the most attention weight, copied in order to the pages of new_page_table (pages that page_table does not
-    name).  Returns the new lengths int32 [batch]; the old pages are left as they are."""
+    name).  Returns the new lengths int32 [batch] (``new_lens`` may be ``seq_lens`` itself); the old pages are left as they
+    are."""
     dev = cache.device
     table, B, P, lens = _kv4_seqs(page_table, seq_lens, None, dev)
     if new_page_table.dim() != 2 or budget < 0 or recent < 0:

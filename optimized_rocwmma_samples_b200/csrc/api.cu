@@ -777,6 +777,9 @@ b2sq_status b2sq_kv4_evict(const b2sq_kv4_cache* cache, const int32_t* page_tabl
         return fail(B2SQ_ERR_INVALID_ARG, "kv4_evict: misaligned pointer");
     if (new_page_table && new_page_table == page_table)
         return fail(B2SQ_ERR_INVALID_ARG, "kv4_evict: the new table must name other pages than the old one");
+    const uintptr_t was = (uintptr_t)seq_lens, is = (uintptr_t)new_lens, bytes = (uintptr_t)batch * 4;
+    if (was != is && was < is + bytes && is < was + bytes)
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_evict: new_lens overlaps seq_lens without being it");
     uint32_t sms = 0;
     cudaError_t e = current_sm_count(&sms);
     if (e != cudaSuccess) return cuda_fail(e, "kv4_evict: SM count");

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
     const int32_t* dst_table = new_table + (uint64_t)b * new_max_pages;
     const uint32_t n = min((uint32_t)max(__ldg(seq_lens + b), 0), max_pages * c.page_size);
     const uint32_t kept = min(min(n, budget), new_max_pages * c.page_size);
-    if (blockIdx.x == 0 && head == 0 && tid == 0) new_lens[b] = (int32_t)kept;
+    if (new_lens && blockIdx.x == 0 && head == 0 && tid == 0) new_lens[b] = (int32_t)kept;
     // this block's share of the kept rows
     const uint32_t d0 = (uint32_t)((uint64_t)kept * blockIdx.x / gridDim.x);
     const uint32_t d1 = (uint32_t)((uint64_t)kept * (blockIdx.x + 1) / gridDim.x);
@@ -292,6 +292,15 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
     }
 }
 
+// New lengths in the place of the old ones, once no block of the eviction reads them any more.
+__global__ void kv4_lens_kernel(int32_t* lens, uint32_t batch, uint32_t cap, uint32_t budget)
+{
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint32_t b = blockIdx.x * blockDim.x + threadIdx.x;
+    if (b < batch) lens[b] = (int32_t)min(min((uint32_t)max(lens[b], 0), cap), budget);
+}
+
 }  // namespace
 
 cudaError_t launch_kv4_evict(const Kv4Cache& c, const int32_t* page_table, uint32_t max_pages, const int32_t* seq_lens,
@@ -310,11 +319,16 @@ cudaError_t launch_kv4_evict(const Kv4Cache& c, const int32_t* page_table, uint3
         1, std::min<uint64_t>((num_sms + (two ? heads - 1 : 0)) / heads, std::min<uint64_t>(16, (budget + 63) / 64)));
     const uint32_t row_slots = (std::min(kEvictRows, (budget + split - 1) / split + 1) + 3) / 4 * 4;
     const size_t smem = (size_t)key_slots * 4 + (size_t)row_slots * 20;
+    const bool in_place = new_lens == seq_lens;
+    int32_t* const lens = in_place ? nullptr : new_lens;
     auto launch = [&](auto kernel, std::atomic<uint64_t>& done) {
-        const cudaError_t e = allow_smem(kernel, kEvictKeys * 4 + kEvictRows * 20, done);
-        if (e != cudaSuccess) return e;
-        return launch_pdl(kernel, dim3(split, c.kv_heads, batch), dim3(kEvictThreads), smem, st, c, page_table, max_pages,
-                          seq_lens, new_table, new_max_pages, budget, recent, new_lens, key_slots, row_slots);
+        cudaError_t e = allow_smem(kernel, kEvictKeys * 4 + kEvictRows * 20, done);
+        if (e == cudaSuccess)
+            e = launch_pdl(kernel, dim3(split, c.kv_heads, batch), dim3(kEvictThreads), smem, st, c, page_table, max_pages,
+                           seq_lens, new_table, new_max_pages, budget, recent, lens, key_slots, row_slots);
+        if (e == cudaSuccess && in_place)
+            e = launch_pdl(kv4_lens_kernel, dim3((batch + 255) / 256), dim3(256), 0, st, new_lens, batch, cap, budget);
+        return e;
     };
     static std::atomic<uint64_t> done[3];
     switch (c.head_dim) {
