@@ -454,6 +454,7 @@ typedef struct {
  * token pitch k_stride / v_stride elements, heads contiguous) into the cache:
  *   z = fp16(min), s = fp16((max - min) / 15) over the group, inputs saturated
  *   to +-65504;  q = clamp(rint((v - z) / s), 0, 15), ties to even (0 if s = 0)
+ *   (s through an fp32 difference and quotient; q as the exact quotient rounds)
  * and sets their weight to 0.  A NaN makes s and z of its group NaN.
  * k_out / v_out (nullable, contiguous, same type) receive the values that the
  * cache now stands for.  A token without a place in the table is skipped; no
