@@ -390,7 +390,9 @@ B2SQ_API b2sq_status b2sq_gemm_i8_grouped(uint32_t groups, uint32_t rows, uint32
  *   d        = float(w2[e] hq) * (rs2 * s2[e])
  *   out[t]   = cvt_rn(sum over k of topk_weights[t*topk+k] * d)   fp32, in slot order
  * A slot whose id is outside [0, experts) adds nothing; an expert may be named
- * twice by one token.  Everything between the int8 products is fp32.
+ * twice by one token.  Everything between the int8 products is fp32.  Unlike in
+ * b2sq_smoothquant, a NaN or an infinity in x[t] * smooth1[e] or in h makes all
+ * of out[t] NaN.
  *   x        fp16 or bf16 (x_type) [tokens, hidden], row pitch ldx elements
  *   smooth1  [experts, hidden], smooth2 [experts, inter]
  *   w13      int8 [experts][2 * inter][hidden]: gate rows, then up rows

@@ -522,7 +522,8 @@ def moe_layer(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tenso
 
     x fp16 / bf16 [T, H]; topk_weights fp32 and topk_ids int32 [T, topk]; smooth1 fp32 [E, H]; w13 int8 [E, 2I, H]
     (gate rows, then up rows) with s13 fp32 [E, 2I]; smooth2 fp32 [E, I]; w2 int8 [E, H, I] with s2 fp32 [E, H].
-    Returns out [T, H] in x's type.  T * topk <= 4096; H and I multiples of 16."""
+    Returns out [T, H] in x's type.  T * topk <= 4096; H and I multiples of 16.  A NaN or an infinity in a token makes all
+    of its output NaN."""
     code = _DTYPE_CODE.get(x.dtype)
     if code is None or x.dtype == torch.int32 or x.dim() != 2 or x.stride(1) != 1:
         raise ValueError("x must be a row-major fp16 or bf16 [tokens, hidden] tensor")

@@ -6,7 +6,9 @@
 //   h       = g / (1 + exp(-g)) * u * smooth2[e];  hq, rs2 = its quantisation
 //   d       = float(w2[e] hq) * (rs2 * s2[e])
 //   out[t]  = sum over k of topk_w[t][k] * d, in slot order
-// A route whose id is outside [0, experts) adds nothing.
+// A route whose id is outside [0, experts) adds nothing.  A NaN or an infinity
+// among xs or h makes the token's whole output NaN (smoothquant by itself would
+// drop it from the maximum and go on with a wrong row).
 //
 // What bounds it is reading the weights of the experts that were chosen, once.
 // Blocks of an expert's routes (up to 8 NT of them) meet its weight rows in
@@ -149,11 +151,19 @@ __device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, f
                           quant_byte(d, inv, qmax, whole));
 }
 
+// The scale of a row whose largest magnitude has these bits.  Magnitudes are compared as integers, which order as the
+// floats do with a NaN above infinity: a row that holds either has a NaN for its scale, and so for everything after it.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ float scale_of(uint32_t top, float qmax)
+{
+    return top < 0x7f800000u ? row_scale_of(__uint_as_float(top), qmax) : __uint_as_float(0x7fffffffu);
+}
+
 // A block a route: hidden <= 16384 is at most 64 values a thread, read once.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) moe_quant_x_kernel(Params p)
 {
-    __shared__ float warp_max[kWarps];
+    __shared__ uint32_t warp_max[kWarps];
     griddep_wait();
     griddep_launch_dependents();
     const MoeLayer& m = p.m;
@@ -181,20 +191,20 @@ __global__ void __launch_bounds__(kThreads) moe_quant_x_kernel(Params p)
     }
     if (p.slices > 1)  // the down product adds its slices up from zero
         for (uint32_t i = tid; i < H / 4; i += kThreads) reinterpret_cast<int4*>(p.acc + (uint64_t)r * H)[i] = make_int4(0, 0, 0, 0);
-    float f[8][8], mx = 0.f;
+    float f[8][8];
+    uint32_t mx = 0;
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
         smoothed<T>(xw[i], sw[i][0], sw[i][1], f[i]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) mx = fmaxf(mx, fabsf(f[i][c]));
+        for (int c = 0; c < 8; ++c) mx = max(mx, magnitude(f[i][c]));
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    mx = __reduce_max_sync(0xffffffffu, mx);
     if ((tid & 31) == 0) warp_max[tid / 32] = mx;
     __syncthreads();
 #pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) mx = fmaxf(mx, warp_max[w]);
-    const float rs = row_scale_of(mx, m.qmax), inv = inv_scale_of(rs);
+    for (uint32_t w = 0; w < kWarps; ++w) mx = max(mx, warp_max[w]);
+    const float rs = scale_of(mx, m.qmax), inv = inv_scale_of(rs);
     const bool whole = m.qmax == rintf(m.qmax);
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
@@ -220,7 +230,7 @@ __global__ void __launch_bounds__(kThreads) moe_quant_h_kernel(Params p)
     if (!there) return;
     const float4* h = reinterpret_cast<const float4*>(p.h + (uint64_t)r * m.inter + k);
     const float4 a = h[0], b = h[1];
-    const float inv = inv_scale_of(row_scale_of(__uint_as_float(p.top[r]), m.qmax));
+    const float inv = inv_scale_of(scale_of(p.top[r], m.qmax));
     const bool whole = m.qmax == rintf(m.qmax);
     *reinterpret_cast<uint2*>(p.hq + (uint64_t)r * m.inter + k) =
         make_uint2(quant4(a.x, a.y, a.z, a.w, inv, m.qmax, whole), quant4(b.x, b.y, b.z, b.w, inv, m.qmax, whole));
@@ -556,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
             cur = block_at<NT>(l, m.experts, b + 1);
             copy.fetch(tid, p.xq, H, 0, H, l.order + cur.r0, cur.count);
         }
-        float mx[NT][2] = {};
+        uint32_t mx[NT][2] = {};
         struct Scales {
             float gate, up, smooth;
         };
@@ -576,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
                     const float uv = __fmul_rn((float)acc[nt][2 + c], __fmul_rn(rs1[tok], s.up));
                     const float hv = gv / (1.f + expf(-gv)) * uv * s.smooth;
                     p.h[(uint64_t)l.order[r0 + tok] * I + (j + t) * 8 + g] = hv;
-                    mx[nt][c] = fmaxf(mx[nt][c], fabsf(hv));  // a NaN drops out, as in smoothquant
+                    mx[nt][c] = max(mx[nt][c], magnitude(hv));
                 }
         };
         const Runs runs(here, pieces);
@@ -610,9 +620,9 @@ __global__ void __launch_bounds__(kThreads, 1) moe_up_kernel(Params p)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                for (int off = 4; off < 32; off <<= 1) mx[nt][c] = fmaxf(mx[nt][c], __shfl_xor_sync(0xffffffffu, mx[nt][c], off));
+                for (int off = 4; off < 32; off <<= 1) mx[nt][c] = max(mx[nt][c], __shfl_xor_sync(0xffffffffu, mx[nt][c], off));
                 const uint32_t tok = nt * 8 + 2 * tig + c;
-                if (g == 0 && tok < count) atomicMax(top + tok, __float_as_uint(mx[nt][c]));
+                if (g == 0 && tok < count) atomicMax(top + tok, mx[nt][c]);
             }
         __syncthreads();  // (and the rows are read, and the sums are zero)
         if (tid < count) atomicMax(p.top + l.order[r0 + tid], top[tid]);
@@ -780,7 +790,7 @@ __global__ void __launch_bounds__(kThreads) moe_sum_kernel(Params p)
             const uint32_t r = t * m.topk + k0 + k, e = (uint32_t)__ldg(m.topk_ids + r);
             if (e >= m.experts) continue;
             w[k] = __ldg(m.topk_w + r);
-            const float rs = row_scale_of(__uint_as_float(__ldcg(p.top + r)), m.qmax);
+            const float rs = scale_of(__ldcg(p.top + r), m.qmax);
             const float* s = m.s2 + (uint64_t)e * m.hidden + i;
             sc[k] = make_float2(__fmul_rn(rs, __ldg(s)), __fmul_rn(rs, __ldg(s + 1)));
         }
