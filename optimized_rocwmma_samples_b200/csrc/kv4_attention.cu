@@ -420,10 +420,12 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
             for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
             // 2^(9 - exponent of the largest), 2^127 at most; none for rows with an infinity
             const int ex = (int)(__float_as_uint(mx) >> 23);
-            const float f = __uint_as_float((uint32_t)(127 + (ex == 255 ? 0 : min(136 - ex, 127))) << 23);
+            const int shift = ex == 255 ? 0 : min(136 - ex, 127);
+            const float f = __uint_as_float((uint32_t)(127 + shift) << 23);
+            const float back = __uint_as_float(shift == 127 ? 1u << 22 : (uint32_t)(127 - shift) << 23);  // 1 / f
             // What brings the row's products back, below 2^76: there a softmax is 0 or 1, since products that differ do so
             // by 2^-48 or more, and the scores stay finite.
-            const float mul = fminf(fmaxf(a.scale / f * kLog2e, -7.55578637e22f), 7.55578637e22f);
+            const float mul = fminf(fmaxf(a.scale * back * kLog2e, -7.55578637e22f), 7.55578637e22f);
 #pragma unroll
             for (uint32_t c = 0; c < D / 32; ++c) {
                 // channel 32 c + lane: word position j, k half, operand register and lane
