@@ -483,7 +483,11 @@ B2SQ_API b2sq_status b2sq_kv4_append(const void* k, const void* v, b2sq_dtype ty
  * sequences of the call share would be added to by both at once, so it must
  * belong to one.
  * workspace: b2sq_kv4_attention_workspace_size bytes, 256-byte aligned, contents
- * arbitrary and not kept; calls that may overlap need separate ones.
+ * arbitrary and not kept; calls that may overlap need separate ones.  With
+ * accumulate_weight it holds an fp32 score for each of the table's positions and
+ * key heads and each of their query rows: batch * kv_heads * max_pages *
+ * page_size * 4 bytes times heads / kv_heads (rounded up to 4) for one query a
+ * sequence.  Of more queries as many are taken at a time as fit 256 MiB (or one).
  */
 B2SQ_API b2sq_status b2sq_kv4_attention(const void* q, b2sq_dtype type, uint32_t tokens, uint32_t heads,
                                         uint32_t q_stride, const b2sq_kv4_cache* cache,

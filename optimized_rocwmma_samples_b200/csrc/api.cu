@@ -738,12 +738,8 @@ b2sq_status b2sq_kv4_attention(const void* q, b2sq_dtype type, uint32_t tokens, 
         return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: batch must be <= %u", b2sq::kMaxAttnBatch);
     if (tokens > 0x7fffffffu || (uint64_t)max_queries * heads > 0x7fffffffull || (uint64_t)tokens * heads > 0x3ffffffffull)
         return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: too many query rows for one launch");
-    // chunks of 16 tokens are counted in 32 bits, over all key heads and blocks of at least 8 rows
-    const uint64_t row_blocks = (uint64_t)heads / cache->kv_heads * max_queries / 8 + 1;
-    const uint64_t chunks = (uint64_t)max_pages * cache->page_size / 16 + 1;
-    if (row_blocks * batch * cache->kv_heads >= 0x100000000ull ||
-        row_blocks * batch * cache->kv_heads * chunks >= 0x100000000ull)
-        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: batch * heads * queries * max_pages too large for one launch");
+    if (!b2sq::kv4_attention_fits(batch, heads, cache->kv_heads, max_queries, max_pages * cache->page_size, accumulate_weight != 0))
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: batch * heads * max_pages too large for one launch");
     uint32_t sms = 0;
     cudaError_t e = current_sm_count(&sms);
     if (e != cudaSuccess) return cuda_fail(e, "kv4_attention: SM count");

@@ -146,6 +146,8 @@ struct Kv4Attention {
     bool accumulate;
 };
 constexpr uint32_t kMaxAttnBatch = 4096;  // sequences of one call: their chunk offsets lie in shared memory
+bool kv4_attention_fits(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t max_queries, uint32_t max_len,
+                        bool accumulate);  // 32-bit counts of a launch
 size_t kv4_attention_workspace(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                                uint32_t max_queries, uint32_t max_len, bool accumulate, uint32_t num_sms);
 cudaError_t launch_kv4_attention(const Kv4Attention& a, void* workspace, uint32_t num_sms, cudaStream_t st);

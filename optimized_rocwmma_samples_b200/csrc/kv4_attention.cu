@@ -71,7 +71,9 @@ struct AttnParams {
     const void* q;
     void* out;
     uint64_t q_stride;
-    uint32_t heads, group, max_queries, row_pad;  // row_pad: group * max_queries rounded up to 4
+    uint32_t heads, group;
+    uint32_t first_query, max_queries, all_queries;  // of a sequence's: the first and the number of this launch, the call's
+    uint32_t row_pad;                                // group * max_queries rounded up to 4
     float scale;
     uint32_t chunk;  // tokens a warp takes at a time: 16 or 32
     uint32_t items;  // (sequence, head, row block) at most
@@ -183,17 +185,20 @@ __device__ __forceinline__ uint32_t nibbles(uint32_t w)
 }
 
 struct SeqShape {
-    uint32_t len, n, start, vis, chunks, blocks;
+    uint32_t len, n, start, queries, vis, chunks, blocks;
 };
-// vis: positions with a place in the table; an empty sequence has one chunk in which nothing is seen
+// start, queries: the rows of this launch; vis: positions with a place in the table; an empty sequence has one chunk in which nothing is seen
 __device__ __forceinline__ SeqShape seq_shape(const AttnParams& a, uint32_t b, uint32_t rows)
 {
     SeqShape s;
     s.len = kv4_len(a.s, b);
     s.n = kv4_new_rows(a.s, b, s.start);
+    s.start += a.first_query;
+    const uint32_t upto = min(s.n, a.all_queries);
+    s.queries = upto > a.first_query ? min(upto - a.first_query, a.max_queries) : 0;
     s.vis = min(s.len, kv4_cap(a.c, a.s));
     s.chunks = max(1u, (s.vis + a.chunk - 1) / a.chunk);
-    s.blocks = (min(s.n, a.max_queries) * a.group + rows - 1) / rows;
+    s.blocks = (s.queries * a.group + rows - 1) / rows;
     return s;
 }
 // For the values, two operands a byte: nibble 0 (J even), and the byte itself, nibble 0 + 16 nibble 1 (J odd): the sums
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
         p.head = item / p.sh.blocks;
         p.block = item - p.head * p.sh.blocks;
         p.c1 = min(p.sh.chunks, p.c0 + (end - unit));
-        p.all_rows = min(p.sh.n, a.max_queries) * a.group;
+        p.all_rows = p.sh.queries * a.group;
         p.wc0 = p.c0 + (p.c1 - p.c0) * warp / kWarps;
         p.wc1 = p.c0 + (p.c1 - p.c0) * (warp + 1) / kWarps;
         return p;
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                 row_mul[r] = mul * 16777216.f;
                 // rows that are not there see everything (their columns are not used), so that they mask nothing
                 row_vis[r] = row < all_rows
-                                 ? (int)max((int64_t)0, min((int64_t)sh.vis, (int64_t)sh.len - sh.n + row / a.group + 1))
+                                 ? (int)max((int64_t)0, min((int64_t)sh.vis, (int64_t)sh.len - sh.n + a.first_query + row / a.group + 1))
                                  : (int)sh.vis;
             }
         }
@@ -1009,7 +1014,7 @@ __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a,
                 }
                 if (b == a.s.batch) continue;
                 sh = seq_shape(a, b, rows_per_item);
-                if (token < sh.start || token - sh.start >= min(sh.n, a.max_queries)) continue;
+                if (token < sh.start || token - sh.start >= sh.queries) continue;
                 head = qh / a.group;
                 row = (token - sh.start) * a.group + qh % a.group;
                 unit0 = ustart[b] + (head * sh.blocks + row / rows_per_item) * sh.chunks;
@@ -1022,7 +1027,7 @@ __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a,
                 sh = seq_shape(a, b, rows_per_item);
                 head = item / sh.blocks;
                 row = item % sh.blocks * rows_per_item + (uint32_t)(x % most_rows);
-                if (row >= min(sh.n, a.max_queries) * a.group) continue;
+                if (row >= sh.queries * a.group) continue;
             }
             const Pieces p(split, unit0, sh.chunks);
             if (p.first == p.last) continue;  // written whole
@@ -1049,7 +1054,7 @@ __global__ void __launch_bounds__(kJoinThreads, 3) kv4_join_kernel(AttnParams a,
         const uint32_t in_seq = unit - ustart[b];
         const uint32_t run = sh.blocks * sh.chunks, head = in_seq / run, u0 = in_seq % run, u1 = min(run, u0 + (end - unit));
         const uint32_t p0 = (uint32_t)((uint64_t)sh.vis * u0 / run), p1 = (uint32_t)((uint64_t)sh.vis * u1 / run);
-        const uint32_t all_rows = min(sh.n, a.max_queries) * a.group;
+        const uint32_t all_rows = sh.queries * a.group;
         const float* scores = a.scores + ((uint64_t)b * a.c.kv_heads + head) * kv4_cap(a.c, a.s) * a.row_pad;
         const int32_t* table = a.s.page_table + (uint64_t)b * a.s.max_pages;
         for (uint32_t r0 = 0; r0 < all_rows; r0 += kJoinThreads) {
@@ -1139,10 +1144,30 @@ struct AttnWs {
 // and 52 against 40 at 16 x 4000.
 uint32_t tiles_of(uint32_t rows) { return rows <= 8 ? 1 : 2; }
 
+// Queries of a sequence that one pair of launches takes.  With weights, their scores over the whole table have to fit
+// kScoreBytes (one query's have room in any case): a prompt of 8192 tokens, 32 heads over 8, would ask for 8.6 GB of them.
+// And a launch counts its chunks of 16 tokens, over all key heads and blocks of at least 8 rows, in 32 bits.  0: not even
+// one query's.
+constexpr uint64_t kScoreBytes = 256ull << 20;
+uint32_t queries_of(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t max_queries, uint32_t max_len, bool accumulate)
+{
+    const uint64_t group = heads / kv_heads, per_row = (uint64_t)batch * kv_heads * max_len * 4;
+    const uint64_t chunks = (uint64_t)batch * kv_heads * (max_len / 16 + 1);
+    uint64_t n = max_queries;
+    if (accumulate && per_row > 0) n = std::min(n, std::max<uint64_t>(1, kScoreBytes / per_row / 4 * 4 / group));
+    if (chunks > 0) {
+        const uint64_t blocks = UINT32_MAX / chunks;  // rows / 8 + 1 of them
+        if (blocks <= group / 8) return 0;
+        n = std::min(n, ((blocks - 1) * 8 + 7) / group);
+    }
+    if (n < max_queries && n * group >= 16) n = std::max<uint64_t>(1, n * group / 16 * 16 / group);  // whole blocks of rows
+    return (uint32_t)n;
+}
+
 AttnWs layout(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t max_queries, uint32_t max_len,
               bool accumulate, uint32_t num_sms)
 {
-    const uint64_t rows = (uint64_t)(heads / kv_heads) * max_queries;
+    const uint64_t rows = (uint64_t)(heads / kv_heads) * queries_of(batch, heads, kv_heads, max_queries, max_len, accumulate);
     const uint64_t pad = (rows + 3) / 4 * 4;
     const uint64_t slots = 2ull * num_sms * kMaxBlocks * 8 * tiles_of((uint32_t)std::min<uint64_t>(rows, 1u << 20));
     AttnWs w;
@@ -1175,8 +1200,6 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
     const uint64_t most = std::max(items, items * ((uint64_t)p.s.max_pages * p.c.page_size + p.chunk) / kMinTokens + 1);
     const uint32_t grid = (uint32_t)std::min<uint64_t>(most, num_sms * attn_blocks<D, NT, CH>());
     const uint32_t line = (p.s.batch + 1) * 4;
-    e = launch_pdl(kv4_attention_kernel<T, D, NT, CH>, dim3(grid), dim3(S::warps * 32), S::fixed + line, st, p);
-    if (e != cudaSuccess) return e;
     // The second kernel is one wave of three blocks an SM, with weights one for the rows and two for the weights (a block
     // takes a few microseconds to its first row; four waves of them took 36 us where one takes 20).  Few rows look for
     // their items themselves (16 x 4000 tokens, 512 rows: 22.8 us, by cuts 25.2), many are found by the cuts.
@@ -1186,8 +1209,13 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
     const uint64_t rows = by_rows ? all_rows : (uint64_t)(grid - 1) * std::min(8u * NT, p.group * p.max_queries);
     const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 2 * num_sms) : 0;
     const uint32_t join = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((rows + groups - 1) / groups, (accumulate ? 1 : 3) * num_sms));
-    return launch_pdl(kv4_join_kernel<T, D>, dim3(join + weights), dim3(kJoinThreads), line + p.s.batch * 4, st, p, 8u * NT,
-                      grid, join, by_rows);
+    for (p.first_query = 0; e == cudaSuccess && p.first_query < p.all_queries; p.first_query += p.max_queries) {
+        e = launch_pdl(kv4_attention_kernel<T, D, NT, CH>, dim3(grid), dim3(S::warps * 32), S::fixed + line, st, p);
+        if (e == cudaSuccess)
+            e = launch_pdl(kv4_join_kernel<T, D>, dim3(join + weights), dim3(kJoinThreads), line + p.s.batch * 4, st, p,
+                           8u * NT, grid, join, by_rows);
+    }
+    return e;
 }
 
 template <typename T, int D>
@@ -1201,6 +1229,12 @@ cudaError_t run_dim(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream
 }
 
 }  // namespace
+
+bool kv4_attention_fits(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t max_queries, uint32_t max_len,
+                        bool accumulate)
+{
+    return max_queries == 0 || queries_of(batch, heads, kv_heads, max_queries, max_len, accumulate) > 0;
+}
 
 size_t kv4_attention_workspace(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                                uint32_t max_queries, uint32_t max_len, bool accumulate, uint32_t num_sms)
@@ -1222,8 +1256,9 @@ cudaError_t launch_kv4_attention(const Kv4Attention& a, void* workspace, uint32_
     p.q_stride = a.q_stride;
     p.heads = a.heads;
     p.group = a.heads / a.cache.kv_heads;
-    p.max_queries = a.max_queries;
-    p.row_pad = (p.group * a.max_queries + 3) / 4 * 4;
+    p.all_queries = std::min(a.max_queries, a.seqs.tokens);
+    p.max_queries = queries_of(a.seqs.batch, a.heads, a.cache.kv_heads, a.max_queries, cap, a.accumulate);
+    p.row_pad = (p.group * p.max_queries + 3) / 4 * 4;
     p.scale = a.scale;
     p.stats = reinterpret_cast<float2*>(base + w.stats);
     p.part_o = reinterpret_cast<float*>(base + w.part_o);
