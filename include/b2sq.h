@@ -477,7 +477,8 @@ B2SQ_API b2sq_status b2sq_kv4_append(const void* k, const void* v, b2sq_dtype ty
  * heads a multiple of kv_heads (query head j reads key head j / (heads /
  * kv_heads)).  out: the same type, contiguous.  A query that sees nothing gives
  * 0.  No sequence has more than max_queries rows (rows past it are not
- * written).  Statistics and sums are fp32.
+ * written).  Statistics and sums are fp32.  batch at most 4096, max_queries *
+ * heads below 2^31.
  * accumulate_weight: adds to cache->weight, for every key head and position, the
  * sum of p over the head's query heads and the call's queries; a page that two
  * sequences of the call share would be added to by both at once, so it must

@@ -580,17 +580,23 @@ b2sq_status validate_moe_layer(const char* fn, uint32_t tokens, uint32_t hidden,
     return ok();
 }
 
+b2sq_status validate_kv4_sizes(const char* fn, uint32_t kv_heads, uint32_t head_dim, uint32_t page_size,
+                               uint32_t max_pages)
+{
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return fail(B2SQ_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256", fn);
+    if (page_size == 0 || page_size % 16) return fail(B2SQ_ERR_UNSUPPORTED, "%s: page_size must be a multiple of 16", fn);
+    if (kv_heads == 0 || kv_heads > 65535) return fail(B2SQ_ERR_INVALID_ARG, "%s: kv_heads must be in [1, 65535]", fn);
+    if ((uint64_t)max_pages * page_size > 0x7fffffffull)
+        return fail(B2SQ_ERR_INVALID_ARG, "%s: max_pages * page_size overflows 31 bits", fn);
+    return ok();
+}
+
 b2sq_status validate_kv4_cache(const char* fn, const b2sq_kv4_cache* c, uint32_t max_pages)
 {
     if (!c) return fail(B2SQ_ERR_INVALID_ARG, "%s: cache is null", fn);
-    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
-        return fail(B2SQ_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256", fn);
-    if (c->page_size == 0 || c->page_size % 16)
-        return fail(B2SQ_ERR_UNSUPPORTED, "%s: page_size must be a multiple of 16", fn);
-    if (c->kv_heads == 0 || c->kv_heads > 65535)
-        return fail(B2SQ_ERR_INVALID_ARG, "%s: kv_heads must be in [1, 65535]", fn);
-    if ((uint64_t)max_pages * c->page_size > 0x7fffffffull)
-        return fail(B2SQ_ERR_INVALID_ARG, "%s: max_pages * page_size overflows 31 bits", fn);
+    const b2sq_status st = validate_kv4_sizes(fn, c->kv_heads, c->head_dim, c->page_size, max_pages);
+    if (st != B2SQ_OK) return st;
     if (c->pages > 0x7fffffffu) return fail(B2SQ_ERR_INVALID_ARG, "%s: too many pages", fn);
     if (c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale))
         return fail(B2SQ_ERR_INVALID_ARG, "%s: null cache buffer", fn);
@@ -607,6 +613,21 @@ b2sq_status validate_kv4_seqs(const char* fn, const int32_t* table, uint32_t bat
     if ((max_pages > 0 && !table) || !lens || !start) return fail(B2SQ_ERR_INVALID_ARG, "%s: null pointer", fn);
     if (!aligned(table, 4) || !aligned(lens, 4) || !aligned(start, 4))
         return fail(B2SQ_ERR_INVALID_ARG, "%s: misaligned pointer", fn);
+    return ok();
+}
+
+// What attention and its workspace size take of a batch.
+b2sq_status validate_kv4_attention(const char* fn, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t positions,
+                                   uint32_t max_queries, int accumulate_weight)
+{
+    if (heads == 0 || heads % kv_heads)
+        return fail(B2SQ_ERR_INVALID_ARG, "%s: heads (%u) must be a multiple of kv_heads (%u)", fn, heads, kv_heads);
+    if (batch > b2sq::kMaxAttnBatch)
+        return fail(B2SQ_ERR_INVALID_ARG, "%s: batch must be <= %u", fn, b2sq::kMaxAttnBatch);
+    if ((uint64_t)max_queries * heads > 0x7fffffffull)
+        return fail(B2SQ_ERR_INVALID_ARG, "%s: too many query rows for one launch", fn);
+    if (!b2sq::kv4_attention_fits(batch, heads, kv_heads, max_queries, positions, accumulate_weight != 0))
+        return fail(B2SQ_ERR_INVALID_ARG, "%s: batch * heads * max_pages too large for one launch", fn);
     return ok();
 }
 
@@ -699,10 +720,11 @@ b2sq_status b2sq_kv4_attention_workspace_size(uint32_t batch, uint32_t heads, ui
 {
     if (!bytes) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention_workspace_size: bytes is null");
     *bytes = 0;
-    if (kv_heads == 0 || heads == 0 || heads % kv_heads)
-        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention_workspace_size: heads must be a multiple of kv_heads");
-    if ((uint64_t)max_pages * page_size > 0x7fffffffull)
-        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention_workspace_size: max_pages * page_size overflows 31 bits");
+    b2sq_status st = validate_kv4_sizes("kv4_attention_workspace_size", kv_heads, head_dim, page_size, max_pages);
+    if (st == B2SQ_OK)
+        st = validate_kv4_attention("kv4_attention_workspace_size", batch, heads, kv_heads, max_pages * page_size, max_queries,
+                                    accumulate_weight);
+    if (st != B2SQ_OK) return st;
     uint32_t sms = 0;
     cudaError_t e = current_sm_count(&sms);
     if (e != cudaSuccess) return cuda_fail(e, "kv4_attention_workspace_size: SM count");
@@ -721,12 +743,13 @@ b2sq_status b2sq_kv4_attention(const void* q, b2sq_dtype type, uint32_t tokens, 
     if (!std::isfinite(scale)) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: scale must be finite");
     b2sq_status st = validate_kv4_cache("kv4_attention", cache, max_pages);
     if (st != B2SQ_OK) return st;
-    if (heads == 0 || heads % cache->kv_heads)
-        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: heads (%u) must be a multiple of kv_heads (%u)", heads,
-                    cache->kv_heads);
+    const bool nothing = tokens == 0 || batch == 0 || max_queries == 0;
+    st = validate_kv4_attention("kv4_attention", nothing ? 0 : batch, heads, cache->kv_heads, max_pages * cache->page_size,
+                                nothing ? 0 : max_queries, accumulate_weight);
+    if (st != B2SQ_OK) return st;
     if (accumulate_weight && !cache->weight)
         return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: the cache keeps no weights");
-    if (tokens == 0 || batch == 0 || max_queries == 0) return ok();
+    if (nothing) return ok();
     st = validate_kv4_seqs("kv4_attention", page_table, batch, max_pages, seq_lens, token_start);
     if (st != B2SQ_OK) return st;
     if (!q || !out) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: null pointer");
@@ -734,12 +757,8 @@ b2sq_status b2sq_kv4_attention(const void* q, b2sq_dtype type, uint32_t tokens, 
     if (q_stride < row) return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: token pitch below heads * head_dim");
     if (!aligned(q, 16) || !aligned(out, 16) || q_stride % 8)
         return fail(B2SQ_ERR_UNSUPPORTED, "kv4_attention: q and out rows must be 16-byte aligned");
-    if (batch > b2sq::kMaxAttnBatch)
-        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: batch must be <= %u", b2sq::kMaxAttnBatch);
-    if (tokens > 0x7fffffffu || (uint64_t)max_queries * heads > 0x7fffffffull || (uint64_t)tokens * heads > 0x3ffffffffull)
+    if (tokens > 0x7fffffffu || (uint64_t)tokens * heads > 0x3ffffffffull)
         return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: too many query rows for one launch");
-    if (!b2sq::kv4_attention_fits(batch, heads, cache->kv_heads, max_queries, max_pages * cache->page_size, accumulate_weight != 0))
-        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: batch * heads * max_pages too large for one launch");
     uint32_t sms = 0;
     cudaError_t e = current_sm_count(&sms);
     if (e != cudaSuccess) return cuda_fail(e, "kv4_attention: SM count");
