@@ -647,14 +647,16 @@ def _kv4_attention_ws(device: int, *sizes: int) -> int:
 
 
 def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, seq_lens: torch.Tensor,
-                  token_start: torch.Tensor, max_queries: int = 1, scale: Optional[float] = None,
+                  token_start: torch.Tensor, max_queries: Optional[int] = None, scale: Optional[float] = None,
                   out: Optional[torch.Tensor] = None, accumulate_weight: bool = False,
                   workspace: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """Attention of new query tokens over the 4-bit cache; q fp16 / bf16 [tokens, heads, head_dim], heads a multiple of
-    the cache's.  Rows token_start[b] .. token_start[b+1] - 1 (at most max_queries) are the last tokens of sequence b,
-    and each sees itself and what came before it.  scale defaults to head_dim ** -0.5.  accumulate_weight adds the
-    softmax weights each cached token received to cache.weight.  Rows of a new ``out`` that belong to no sequence are
-    zero; those of a given one are left as they were."""
+    the cache's.  Rows token_start[b] .. token_start[b+1] - 1 are the last tokens of sequence b, and each sees itself and
+    what came before it.  max_queries: no sequence has more rows (those past it are not computed); by default 1 where q has
+    no more rows than there are sequences, one token of each, and else the number of rows, which a
+    prompt may have (the longest prompt's own number takes less workspace and time).  scale defaults to head_dim ** -0.5.
+    accumulate_weight adds the softmax weights each cached token received to cache.weight.  Rows of a new ``out`` that
+    belong to no sequence are zero; those of a given one are left as they were."""
     dev = cache.device
     code = _DTYPE_CODE.get(q.dtype)
     if code is None or q.dtype == torch.int32:
@@ -662,12 +664,14 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, se
     T, heads, qs = _kv4_rows(q, "q", dev)
     if q.shape[2] != cache.head_dim:
         raise ValueError(f"q must have head_dim {cache.head_dim}")
+    seqs = _kv4_seqs(page_table, seq_lens, token_start, dev)
+    if max_queries is None:
+        max_queries = 1 if T <= seqs[1] else T
     if not 0 <= max_queries < 2 ** 31:
         raise ValueError("max_queries must be in [0, 2^31)")
     if out is None:
         out = _new(torch.zeros, q.shape, q.dtype, dev, stream)
     o = _want(out, "out", q.dtype, q.shape, dev)
-    seqs = _kv4_seqs(page_table, seq_lens, token_start, dev)
     sc = cache.head_dim ** -0.5 if scale is None else float(scale)
     acc = int(accumulate_weight)
     with _on(dev):

@@ -64,3 +64,24 @@ def test_prompt_then_decode(cuda_device):
         ln, st = torch.tensor([length], dtype=torch.int32, device=DEV), R.starts([count], DEV)
         api.kv4_append(k, v, cache, table, ln, st)
         run_attention(cache, table, [length], [count], heads, D, torch.float16, True, extra=0, q=q)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("lens,counts", [([40], [33]), ([9, 50, 20], [1, 30, 7]), ([20, 30], [1, 1])])
+def test_all_rows_by_default(cuda_device, lens, counts, accumulate):
+    """Without max_queries no row of a prompt is left out."""
+    heads, kv, D, page = 8, 2, 64, 16
+    table, pages = R.tables(lens, page, 5, DEV)
+    q = torch.randn((sum(counts), heads, D), device=DEV).half()
+    ln, st = torch.tensor(lens, dtype=torch.int32, device=DEV), R.starts(counts, DEV)
+    got, weights = [], []
+    for kw in ({}, dict(max_queries=max(counts))):
+        cache = R.random_cache(api, pages, kv, page, D, accumulate, 7, DEV)
+        got.append(api.kv4_attention(q, cache, table, ln, st, accumulate_weight=accumulate, **kw))
+        weights.append(cache.weight)
+    torch.cuda.synchronize()
+    want, _, tol, _ = R.attention(q, cache, table, ln, st, D ** -0.5)
+    for out in got:
+        assert torch.all((out.double() - want).abs() <= tol)
+    if accumulate:  # sums of at most 50 scores' exponentials in another order: 50 * 2^-24 of them
+        assert torch.all((weights[0] - weights[1]).abs() <= 2.0 ** -18 * weights[1])
