@@ -459,8 +459,9 @@ typedef struct {
  *   (s through an fp32 difference and quotient; q as the exact quotient rounds)
  * and sets their weight to 0.  A NaN makes s and z of its group NaN.
  * k_out / v_out (nullable, contiguous, same type) receive the values that the
- * cache now stands for.  A token without a place in the table is skipped; no
- * two tokens of a call may have the same place.
+ * cache now stands for; they may be k and v themselves where these are
+ * contiguous, and overlap nothing else.  A token without a place in the table is
+ * skipped; no two tokens of a call may have the same place.
  * Requirements (else UNSUPPORTED): 16-byte aligned rows (pitches multiples of 8).
  */
 B2SQ_API b2sq_status b2sq_kv4_append(const void* k, const void* v, b2sq_dtype type, uint32_t tokens,
@@ -475,14 +476,15 @@ B2SQ_API b2sq_status b2sq_kv4_append(const void* k, const void* v, b2sq_dtype ty
  *   s = scale * q . K,  p = softmax(s),  out = p V
  * q: [tokens, heads, head_dim] fp16 or bf16, token pitch q_stride elements;
  * heads a multiple of kv_heads (query head j reads key head j / (heads /
- * kv_heads)).  out: the same type, contiguous.  A query that sees nothing gives
- * 0.  No sequence has more than max_queries rows (rows past it are not
- * written).  Statistics and sums are fp32.  batch at most 4096, max_queries *
- * heads below 2^31.
+ * kv_heads)).  out: the same type, contiguous; it may be q itself where that is
+ * contiguous, but not overlap it otherwise.  A query that sees nothing gives 0.
+ * No sequence has more than max_queries rows (rows past it are not written).
+ * Statistics and sums are fp32.  batch at most 4096, max_queries * heads below
+ * 2^31.
  * accumulate_weight: adds to cache->weight, for every key head and position, the
- * sum of p over the head's query heads and the call's queries; a page that two
- * sequences of the call share would be added to by both at once, so it must
- * belong to one.
+ * sum of p over the head's query heads and the call's queries; a page that the
+ * call's tables name twice would be added to by both at once, so each stands
+ * there once.
  * workspace: b2sq_kv4_attention_workspace_size bytes, 256-byte aligned, contents
  * arbitrary and not kept; calls that may overlap need separate ones.  With
  * accumulate_weight it holds an fp32 score for each of the table's positions and

@@ -580,6 +580,14 @@ b2sq_status validate_moe_layer(const char* fn, uint32_t tokens, uint32_t hidden,
     return ok();
 }
 
+// `out` (dense rows) meets `in` (rows of `row` bytes, `pitch` apart) in another way than row for row in the same place.
+bool overlaps(const void* out, const void* in, uint64_t rows, uint64_t row, uint64_t pitch)
+{
+    if (!out || !in || rows == 0 || (out == in && (pitch == row || rows == 1))) return false;
+    const uintptr_t o = (uintptr_t)out, i = (uintptr_t)in;
+    return o < i + (rows - 1) * pitch + row && i < o + rows * row;
+}
+
 b2sq_status validate_kv4_sizes(const char* fn, uint32_t kv_heads, uint32_t head_dim, uint32_t page_size,
                                uint32_t max_pages)
 {
@@ -703,6 +711,10 @@ b2sq_status b2sq_kv4_append(const void* k, const void* v, b2sq_dtype type, uint3
         return fail(B2SQ_ERR_UNSUPPORTED, "kv4_append: rows must be 16-byte aligned");
     if (tokens > 0x7fffffffu || row > 0x3fffffffu)
         return fail(B2SQ_ERR_INVALID_ARG, "kv4_append: too many tokens or channels for one launch");
+    if (overlaps(k_out, k, tokens, row * 2, k_stride * 2ull) || overlaps(v_out, v, tokens, row * 2, v_stride * 2ull) ||
+        overlaps(k_out, v, tokens, row * 2, v_stride * 2ull) || overlaps(v_out, k, tokens, row * 2, k_stride * 2ull) ||
+        (k_out && (k_out == v || k_out == v_out)) || (v_out && v_out == k) || overlaps(k_out, v_out, tokens, row * 2, row * 2))
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_append: k_out and v_out may be k and v, but overlap nothing else");
     uint32_t sms = 0;
     cudaError_t e = current_sm_count(&sms);
     if (e != cudaSuccess) return cuda_fail(e, "kv4_append: SM count");
@@ -759,6 +771,8 @@ b2sq_status b2sq_kv4_attention(const void* q, b2sq_dtype type, uint32_t tokens, 
         return fail(B2SQ_ERR_UNSUPPORTED, "kv4_attention: q and out rows must be 16-byte aligned");
     if (tokens > 0x7fffffffu || (uint64_t)tokens * heads > 0x3ffffffffull)
         return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: too many query rows for one launch");
+    if (overlaps(out, q, tokens, row * 2, q_stride * 2ull))
+        return fail(B2SQ_ERR_INVALID_ARG, "kv4_attention: out may be q, but not overlap it otherwise");
     uint32_t sms = 0;
     cudaError_t e = current_sm_count(&sms);
     if (e != cudaSuccess) return cuda_fail(e, "kv4_attention: SM count");

@@ -1,4 +1,4 @@
-"""Eviction that writes the new lengths over the old ones."""
+"""Calls that write over their inputs: eviction its lengths, append its keys and values, attention its queries."""
 import pytest
 import torch
 
@@ -60,3 +60,35 @@ def test_evict_in_place_captured(cuda_device):
     assert ln.tolist() == [64, 50]
     want, _, tol, _ = R.attention(q, cache, fresh, ln, st, D ** -0.5)
     assert torch.all((out.double() - want).abs() <= tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [700, 30, 2900]])
+def test_append_in_place(cuda_device, counts, dtype):
+    kv, D, size = 4, 128, 32
+    table, pages = R.tables(counts, size, 2, DEV)
+    st, ln = R.starts(counts, DEV), ints(*counts)
+    k, v = (torch.randn((sum(counts), kv, D), device=DEV).to(dtype) for _ in range(2))
+    k[0, 0, :64] = torch.linspace(-7.5, 7.5, 64, device=DEV).to(dtype)
+    k[0, 0, 3] = 2.0 ** -24
+    one, two = (api.KV4Cache.empty(pages, kv, size, D, device=DEV) for _ in range(2))
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    api.kv4_append(k, v, one, table, ln, st, k_out=ko, v_out=vo)
+    api.kv4_append(k, v, two, table, ln, st, k_out=k, v_out=v)
+    torch.cuda.synchronize()
+    assert torch.equal(k, ko) and torch.equal(v, vo)
+    for n in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(one, n), getattr(two, n)), n
+
+
+@pytest.mark.parametrize("D,heads,kv,lens,counts", [(64, 8, 8, [9, 700], [1, 1]), (128, 32, 8, [3000, 20, 41], [1, 1, 1]),
+                                                    (128, 16, 2, [600, 90], [40, 7]), (256, 8, 2, [500], [30])])
+def test_attention_in_place(cuda_device, D, heads, kv, lens, counts):
+    table, pages = R.tables(lens, 32, 2, DEV)
+    cache = R.random_cache(api, pages, kv, 32, D, False, 3, DEV)
+    q = torch.randn((sum(counts), heads, D), device=DEV).half()
+    st, ln = R.starts(counts, DEV), ints(*lens)
+    apart = api.kv4_attention(q, cache, table, ln, st, max_queries=max(counts))
+    assert api.kv4_attention(q, cache, table, ln, st, max_queries=max(counts), out=q) is q
+    torch.cuda.synchronize()
+    assert torch.equal(q, apart)
