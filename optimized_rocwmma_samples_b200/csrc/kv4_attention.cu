@@ -1202,9 +1202,10 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
     const uint32_t line = (p.s.batch + 1) * 4;
     // The second kernel is one wave of three blocks an SM, with weights one for the rows and two for the weights (a block
     // takes a few microseconds to its first row; four waves of them took 36 us where one takes 20).  Few rows look for
-    // their items themselves (16 x 4000 tokens, 512 rows: 22.8 us, by cuts 25.2), many are found by the cuts.
+    // their items themselves, many are found by the cuts (lengths up to 4000, 32 heads over 8 of 128 channels: 128 rows
+    // 15.3 us, by cuts 16.6; 256 rows 18.3 and 18.9; 384 rows 22.0 and 22.0; 512 rows 24.9 and 24.3; 2048 rows 72 and 59).
     const uint64_t all_rows = (uint64_t)p.s.tokens * p.heads;
-    const bool by_rows = all_rows <= 4 * num_sms;
+    const bool by_rows = all_rows <= 2 * num_sms;
     const uint32_t groups = kJoinThreads / 32 / (by_rows ? kJoinGroup : 1);
     const uint64_t rows = by_rows ? all_rows : (uint64_t)(grid - 1) * std::min(8u * NT, p.group * p.max_queries);
     const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 2 * num_sms) : 0;
