@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
         float o[NG][4][NT][4] = {};
         float m[NT][2], l[NT][2], zs[NT][2][NG];  // m: 0 until the row has seen a token
         float ref[NG];                            // 2^8 / the power of two that a group's steps are taken over
-        __half2 part_p[NG][NT], last_p[NG][NT];   // half of the tokens' p times step since the last centring, and before it
+        __half2 part_p[NG][NT];                   // half of the tokens' p times step since the last centring
         uint32_t seen = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
         for (uint32_t gr = 0; gr < NG; ++gr) {
             ref[gr] = 4294967296.f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) part_p[gr][nt] = last_p[gr][nt] = __half2(0.f, 0.f);
+            for (int nt = 0; nt < NT; ++nt) part_p[gr][nt] = __half2(0.f, 0.f);
         }
 
         const uint32_t tok = (lane & 7) + ((lane >> 3) & 1) * 8;  // ldmatrix row of this lane
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
 #pragma unroll
                             for (uint32_t gr = 0; gr < NG; ++gr) {
                                 zs[nt][x][gr] *= f;
-                                part_p[gr][nt] = last_p[gr][nt] = __half2(0.f, 0.f);
+                                part_p[gr][nt] = __half2(0.f, 0.f);
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) {
                                     o[gr][j][nt][x] *= f;
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                         const float f = fresh / ref[gr];
                         ref[gr] = fresh;
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) part_p[gr][nt] = last_p[gr][nt] = __half2(0.f, 0.f);
+                        for (int nt = 0; nt < NT; ++nt) part_p[gr][nt] = __half2(0.f, 0.f);
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -708,10 +708,10 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
             }
         };
 
-        // Takes 8 steps a nibble out of the run's sums, by twice the sample, and half of that again, less the half taken
-        // before: the next run's sums start about as far below their centre as they end above it.  The sample need not be
-        // exact, nor does it grow with what a new maximum rescales: what leaves the sums enters zs.
-        auto centre = [&]() {
+        // Takes 8 steps a nibble out of the run's sums, by twice the sample, and the first time half as much again: every
+        // run's sums then start about as far below their centre as they end above it.  The sample need not be exact, nor
+        // does it follow what a new maximum rescales: what leaves the sums enters zs.
+        auto centre = [&](float steps) {
 #pragma unroll
             for (uint32_t gr = 0; gr < NG; ++gr) {
                 const float back = __uint_as_float((254u << 23) - __float_as_uint(ref[gr])) * (0.25f / kSample);
@@ -720,12 +720,11 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                     __half2 v = part_p[gr][nt];
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) v = __hadd2(v, __shfl_xor_sync(0xffffffffu, v, off));
-                    const float2 now = __half22float2(v), then = __half22float2(last_p[gr][nt]);
-                    last_p[gr][nt] = v;
+                    const float2 now = __half22float2(v);
                     part_p[gr][nt] = __half2(0.f, 0.f);
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const float out = x ? fmaf(12.f, now.y, -4.f * then.y) : fmaf(12.f, now.x, -4.f * then.x);
+                        const float out = steps * (x ? now.y : now.x);
                         zs[nt][x][gr] = fmaf(out, back, zs[nt][x][gr]);  // (an eighth in each of the lanes that are added up)
                         const float even = out * (2.f / kSample / 16777216.f), odd = 17.f * even;
 #pragma unroll
@@ -747,7 +746,7 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                     step(c, slot, std::true_type());
                 else
                     step(c, slot, std::false_type());
-                if ((c - wc0) % (kRun / CH) == kRun / CH - 1) centre();
+                if ((c - wc0) % (kRun / CH) == kRun / CH - 1) centre(c - wc0 < kRun / CH ? 12.f : 8.f);
             } else if (score_at) {  // no such page: nothing of this chunk is seen
                 const uint32_t rows = min(ROWS, a.row_pad - block * ROWS);
                 for (uint32_t i = lane; i < CHUNK * rows && c * CHUNK + i / rows < sh.vis; i += 32)
@@ -1202,10 +1201,12 @@ cudaError_t run(AttnParams& p, bool accumulate, uint32_t num_sms, cudaStream_t s
     const uint32_t line = (p.s.batch + 1) * 4;
     // The second kernel is one wave of three blocks an SM, with weights one for the rows and two for the weights (a block
     // takes a few microseconds to its first row; four waves of them took 36 us where one takes 20).  Few rows look for
-    // their items themselves, many are found by the cuts (lengths up to 4000, 32 heads over 8 of 128 channels: 128 rows
-    // 15.3 us, by cuts 16.6; 256 rows 18.3 and 18.9; 384 rows 22.0 and 22.0; 512 rows 24.9 and 24.3; 2048 rows 72 and 59).
+    // their items themselves, many are found by the cuts.  Where the two meet depends on the pieces a row has: lengths up to
+    // 4000, 32 heads over 8 of 128 channels, 128 rows 15.3 us, by cuts 16.6, 384 rows 22.0 and 22.0, 576 rows 26.6 and 26.2,
+    // 2048 rows 72 and 59; 40000 tokens, 4 queries, 512 rows 62.6 and 67.2, 640 rows 61.4 and 65.9 (64 channels), 1024 rows
+    // of one query 108 and 106.
     const uint64_t all_rows = (uint64_t)p.s.tokens * p.heads;
-    const bool by_rows = all_rows <= 2 * num_sms;
+    const bool by_rows = all_rows <= 4 * num_sms;
     const uint32_t groups = kJoinThreads / 32 / (by_rows ? kJoinGroup : 1);
     const uint64_t rows = by_rows ? all_rows : (uint64_t)(grid - 1) * std::min(8u * NT, p.group * p.max_queries);
     const uint32_t weights = accumulate ? (uint32_t)std::min<uint64_t>(most, 2 * num_sms) : 0;
