@@ -401,8 +401,10 @@ B2SQ_API b2sq_status b2sq_gemm_i8_grouped(uint32_t groups, uint32_t rows, uint32
  *   out      x_type [tokens, hidden], contiguous
  * Requirements (else UNSUPPORTED): hidden and inter multiples of 16 and at
  * most 16384 and 131072, x, smooth1, w13, w2 and out 16-byte aligned, ldx a
- * multiple of 8, tokens * topk <= 4096 (larger batches: b2sq_moe_sorting and
- * b2sq_gemm_i8_grouped).  experts <= 1024.
+ * multiple of 8, tokens * topk <= 4096 (larger batches: tokens do not depend on
+ * one another, so in slices; or b2sq_moe_sorting, b2sq_moe_smoothquant and
+ * b2sq_gemm_i8_grouped, which leave the activation, the second quantisation and
+ * the weighted sum to the caller).  experts <= 1024.
  * workspace: b2sq_moe_layer_workspace_size bytes, 256-byte aligned, contents
  * arbitrary and not kept; calls that may overlap need separate ones.
  */

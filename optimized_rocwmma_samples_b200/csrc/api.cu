@@ -575,7 +575,7 @@ b2sq_status validate_moe_layer(const char* fn, uint32_t tokens, uint32_t hidden,
         return fail(B2SQ_ERR_UNSUPPORTED, "%s: hidden and inter must be multiples of 16, up to %u and %u", fn,
                     kMaxMoeHidden, kMaxMoeInter);
     if ((uint64_t)tokens * topk > kMaxMoeRoutes)
-        return fail(B2SQ_ERR_UNSUPPORTED, "%s: tokens * topk above %u (use moe_sorting and gemm_i8_grouped)", fn,
+        return fail(B2SQ_ERR_UNSUPPORTED, "%s: tokens * topk above %u (pass the tokens in slices)", fn,
                     kMaxMoeRoutes);
     return ok();
 }

@@ -6,16 +6,17 @@
 // A NaN makes its group's s and z NaN, so it is not lost in the cache.
 //
 // HBM would bound it (2 bytes a channel in, 0.56 out, 2 more where the cached
-// values are asked for) with fewer than ten instructions a channel; it takes 15,
-// and the issue slots do: eight lanes hold a group, one 16-byte load and one 4-byte store of
-// nibbles each; extrema in packed 16-bit operations and three shuffles; the
+// values are asked for) with fewer than 18 instructions a channel at the rate they
+// issue here; it takes 28, and the issue slots (75% full) and the wait for a
+// block's places in front of its first loads do.  Eight lanes hold a group, one
+// 16-byte load and one 4-byte store of nibbles each; extrema in packed 16-bit operations and three shuffles; the
 // quotient as a saturated product with 1 / (15 s), whose exact remainder tells
 // whether it was rounded right.  Inputs of 8 or 11 significant bits meet the
 // border between two steps often, so those lanes decide it exactly, with what
 // the difference v - z has beyond fp32.
 //
-// 7 x 4001 tokens, 8 heads of 128 channels: 41 us (173 MB, 4.2 TB/s); 16 tokens
-// 2.7 us.
+// 7 prompts of up to 4001 tokens, 8 heads of 128 channels: 42 us (173 MB, 4.1
+// TB/s); 16 tokens 2.9 us.
 #include "kv4.cuh"
 
 #include <algorithm>

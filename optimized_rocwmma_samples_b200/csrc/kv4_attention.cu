@@ -32,7 +32,7 @@
 //    sum of p, moves from the sums to sum(p z): they stay about their centre,
 //    where what is cut off cancels (64 x 131072 tokens, fp16: off by 2.2e-4 of
 //    the result, 2.1e-3 without; rounding the result is 2.2e-4.  It takes 2 to
-//    3% of the time; 8 steps taken off by a product of their own took 14%).
+//    5% of the time; 8 steps taken off by a product of their own took 14%).
 //
 // Work is split evenly over the grid in chunks of 16 tokens, whatever the
 // lengths: the (sequence, head, row block) items lie one after another on a
@@ -43,11 +43,13 @@
 // streams its own chunks through a ring of cp.async stages, with no barrier
 // until the item's end.
 //
-// 2 x 100001 tokens, 64 heads over 8 of 128 channels: 54 us (221 MB, 4.1 TB/s),
-// with about 270 warp instructions for 16 tokens of a head, 80 of them masks,
-// beside the bytes; 16 x 4000, 32 heads: 23.5 us, 15 of which do not depend on
-// the lengths (start, joins, second kernel); 48 x 8192 with weights 99 us, 25 of
-// them the second kernel's reading of the scores; 1 x 257: 11.6 us.
+// 2 x 100001 tokens, 64 heads over 8 of 128 channels: 56 us (221 MB, 3.9 TB/s),
+// with about 290 warp instructions for 16 tokens of a head, 80 of them masks,
+// beside the bytes; neither is full (0.54 instructions a cycle): with three warps
+// a scheduler the latencies of masks and products show.  16 x 4000, 32 heads: 24
+// us, 15 of which do not depend on the lengths (start, joins, second kernel); 48
+// x 8192 with weights 100 us, 25 of them the second kernel's reading of the
+// scores; 1 x 257: 11.8 us.
 #include "kv4.cuh"
 #include "sq_math.cuh"
 
