@@ -748,12 +748,12 @@ __global__ void __launch_bounds__(attn_warps<D, NT, CH>() * 32, attn_blocks<D, N
                     step(c, slot, std::true_type());
                 else
                     step(c, slot, std::false_type());
-                if ((c - wc0) % (kRun / CH) == kRun / CH - 1) centre(c - wc0 < kRun / CH ? 12.f : 8.f);
             } else if (score_at) {  // no such page: nothing of this chunk is seen
                 const uint32_t rows = min(ROWS, a.row_pad - block * ROWS);
                 for (uint32_t i = lane; i < CHUNK * rows && c * CHUNK + i / rows < sh.vis; i += 32)
                     score_at[((int64_t)(i / rows) - g) * a.row_pad + (int64_t)(i % rows) - 2 * tig] = -INFINITY;
             }
+            if ((c - wc0) % (kRun / CH) == kRun / CH - 1) centre(c - wc0 < kRun / CH ? 12.f : 8.f);
             if (score_at) score_at += CHUNK * a.row_pad;
             if (++slot == STAGES) slot = 0;
         }

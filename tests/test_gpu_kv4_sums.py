@@ -40,6 +40,27 @@ def test_long_sums(cuda_device, dtype, D, kv, group, size, pages):
     assert err <= 1.25 * rounding, f"{err} against {rounding}"
 
 
+@pytest.mark.parametrize("every", [2, 16, 32])
+def test_long_sums_with_holes(cuda_device, every):
+    """The same where each second, 16th or 32nd page is missing: what is set aside for the sums' centre does not pile up."""
+    batch, pages, size, D, kv, group = 64, 64, 32, 128, 8, 4
+    cache = R.random_cache(api, pages, kv, size, D, False, 8, DEV)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+    q = (torch.randn((batch, kv * group, D), generator=g, device=DEV) * 0.1).half()
+    row = torch.arange(131072 // size, dtype=torch.int32, device=DEV)
+    row = torch.where(row % every == every - 1, -1, row % pages).to(torch.int32)
+    out = api.kv4_attention(q, cache, row.expand(batch, -1).contiguous(),
+                            torch.full((batch,), 131072, dtype=torch.int32, device=DEV),
+                            torch.arange(batch + 1, dtype=torch.int32, device=DEV))
+    k, v = (x.transpose(0, 1).flatten(1, 2) for x in R.values(cache))
+    there = (torch.arange(pages, device=DEV) % every != every - 1).repeat_interleave(size)
+    p = torch.softmax(torch.einsum("bhgd,hnd->bhgn", q.double().view(batch, kv, group, D), k[:, there]) * D ** -0.5, -1)
+    want = torch.einsum("bhgn,hnd->bhgd", p, v[:, there]).reshape(batch, kv * group, D)
+    err, rounding = norms(out, want)
+    assert err <= 1.25 * rounding, f"{err} against {rounding}"
+
+
 def test_fp16_keeps_its_probabilities(cuda_device):
     """Few tokens, fp16: the probabilities that meet the nibbles hold more bits than fp16 has, or the result loses some.
 
